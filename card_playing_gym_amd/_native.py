@@ -23,12 +23,14 @@ CG_OK, CG_ERR_INVALID, CG_ERR_UNSUPPORTED, CG_ERR_RANGE, CG_ERR_HIP = 0, 1, 2, 3
 CG_F32, CG_BF16, CG_F16 = 0, 1, 2
 CG_ACT_NONE, CG_ACT_GELU = 0, 1
 CG_COPY_AUTO, CG_COPY_ORDERED = 0, 1
+CG_CLIP_NONE, CG_CLIP_OWN_NORM, CG_CLIP_GIVEN_NORM = 0, 1, 2
 CG_TRUNK_STATIC_WORKSPACE = 64 << 20
 
 c_int32 = ctypes.c_int32
 c_int64 = ctypes.c_int64
 c_void_p = ctypes.c_void_p
 c_float = ctypes.c_float
+c_double = ctypes.c_double
 c_size_t = ctypes.c_size_t
 
 
@@ -124,6 +126,18 @@ class TrainBlockGrads(ctypes.Structure):
 
 class TrainGrads(ctypes.Structure):
     _fields_ = [("blocks", ctypes.POINTER(TrainBlockGrads)), ("final_dw", c_void_p), ("final_db", c_void_p)]
+
+
+class AdamWTensor(ctypes.Structure):
+    _fields_ = [(name, c_void_p) for name in ("param", "exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale",
+                                              "step")] + [("n", c_int64)]
+
+
+class AdamWConfig(ctypes.Structure):
+    _fields_ = [(name, c_double) for name in ("lr", "beta1", "beta2", "eps", "weight_decay", "max_norm")] + [
+        ("lr_device", c_void_p), ("seed", ctypes.c_uint32), ("first", c_int32), ("dtype", c_int32),
+        ("state_bits", c_int32), ("clip", c_int32),
+    ]
 
 
 class LayerParams(ctypes.Structure):
@@ -280,6 +294,15 @@ _SIGNATURES = {
          P(TrainGrads), c_void_p, c_void_p, c_void_p, c_void_p],
     ),
     "cg_attn_train_bwd": (c_int32, [P(AttnTrain), c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "cg_grad_norm_workspace_size": (c_size_t, [c_int32]),
+    "cg_grad_norm": (
+        c_int32, [c_void_p, c_void_p, c_void_p, c_int32, c_void_p, c_void_p, c_size_t, c_void_p],
+    ),
+    "cg_adamw_workspace_size": (c_size_t, [c_int32]),
+    "cg_adamw_step": (
+        c_int32, [c_void_p, c_void_p, c_int32, P(AdamWConfig), c_void_p, c_void_p, c_size_t, c_void_p],
+    ),
+    "cg_moment_values": (c_int32, [c_void_p, c_void_p, c_int32, c_void_p, c_int64, c_void_p]),
     "cg_piquet_destroy": (c_int32, [c_void_p]),
     "cg_piquet_embed": (
         c_int32, [c_void_p, c_void_p, c_int64, c_int32, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p],

@@ -540,6 +540,65 @@ int cg_trunk_train_backward(const cg_train_config *c, const cg_train_block *bloc
                             size_t saved_size, void *scratch, size_t scratch_size, const cg_train_grads *grads,
                             float *dx, float *dple, float *dvalues, void *stream);
 
+/* ---- the optimiser step ------------------------------------------------------------------
+ * What follows the training backward in an update: the gradients' global norm and one AdamW
+ * step over many tensors (decoupled weight decay, bias-corrected moments), the work of
+ * torch.nn.utils.clip_grad_norm_ and a fused torch.optim.AdamW.  Per element, with t the
+ * tensor's step count after this step and c the clipping factor,
+ *   g = c * grad;  m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2;
+ *   p -= lr wd p + lr / (1 - beta1^t) * m / (sqrt(v / (1 - beta2^t)) + eps)
+ * in fp32 and rounded once to the parameter's type. */
+
+/* The Euclidean norm of the gradients together, in fp64 (0 for none): grads host [n] of device
+ * pointers (NULL: skipped), sizes and dtypes (CG_F32 / CG_BF16 / CG_F16) host [n]; norm and
+ * workspace on the device, the workspace 8-byte aligned. */
+size_t cg_grad_norm_workspace_size(int32_t n);
+int cg_grad_norm(const void *const *grads, const int64_t *sizes, const int32_t *dtypes, int32_t n, double *norm,
+                 void *workspace, size_t workspace_size, void *stream);
+
+/* One tensor of a step.  state_bits 32: exp_avg / exp_avg_sq are float [n], the scales unused.
+ * state_bits 8: uint8 codes [n] and a float scale for each 256 elements, [ceil(n / 256)].  A
+ * code q stands for f(q) * scale: f(0) = 0, else f(q) = (1 + (u mod 8) / 8) 2^(u div 8 - 127)
+ * with u = 889 + q for exp_avg (q up to 127, bit 7 the sign) and u = 761 + q for exp_avg_sq (q
+ * up to 255), so 1 is the largest code's.  New codes are rounded up with the probability of
+ * what is cut off, by 16-bit random numbers hashed from (seed, t, first + the tensor's index,
+ * the element's index).  A gradient that is not finite makes its block of 256 not finite. */
+typedef struct {
+  void *param;
+  void *exp_avg, *exp_avg_sq;
+  float *exp_avg_scale, *exp_avg_sq_scale;
+  float *step; /* the count of steps taken; this one adds 1 */
+  int64_t n;
+} cg_adamw_tensor;
+
+#define CG_CLIP_NONE 0
+#define CG_CLIP_OWN_NORM 1   /* the norm of this call's gradients, which is written to norm */
+#define CG_CLIP_GIVEN_NORM 2 /* the norm that norm holds */
+
+typedef struct {
+  double lr, beta1, beta2, eps, weight_decay;
+  double max_norm;        /* c = min(1, max_norm / (norm + 1e-6)); a NaN norm gives NaN */
+  const float *lr_device; /* NULL, or a device scalar in lr's place */
+  uint32_t seed;
+  int32_t first;
+  int32_t dtype;      /* of parameters and gradients: CG_F32, CG_BF16 or CG_F16 */
+  int32_t state_bits; /* 32 or 8 */
+  int32_t clip;       /* CG_CLIP_... */
+} cg_adamw_config;
+
+/* tensors and grads are host arrays [n] (read before the call returns); a tensor with a NULL
+ * gradient, or of size 0, keeps its parameter, state and count.  Tensors must not overlap.  A
+ * captured step reads lr_device and the counts at every replay, and lr, the betas, eps and
+ * weight_decay as captured.  norm (device) may be NULL without clipping.  workspace: device,
+ * 16-byte aligned, of this call alone until the step has run. */
+size_t cg_adamw_workspace_size(int32_t n);
+int cg_adamw_step(const cg_adamw_tensor *tensors, const void *const *grads, int32_t n, const cg_adamw_config *config,
+                  double *norm, void *workspace, size_t workspace_size, void *stream);
+
+/* values[i] = what codes[i] stands for, in fp32 (is_signed: exp_avg's codes; else exp_avg_sq's). */
+int cg_moment_values(const uint8_t *codes, const float *scales, int32_t is_signed, float *values, int64_t n,
+                     void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,500 @@
+"""The optimiser step on the GPU (csrc/optim.hip, nn/optim.py) against float64.
+
+Bars, with u = 2^-24 (half an fp32 step): m and v are sums of two products whose factors (the clipping
+factor, the gradient times it, 1 - beta) are rounded, at most 6 roundings of their magnitudes; the
+update divides m by a root (9 more) and by factors rounded once; p takes one rounding of its type.
+With 8-bit moments m and v are formed in fp64 and their codes have to be equal."""
+
+from __future__ import annotations
+
+import copy
+import pickle
+
+import numpy as np
+import pytest
+import torch
+
+from card_playing_gym_amd.nn import AdamW, AdamWPlan, grad_norm, moment_values
+from card_playing_gym_amd.nn.optim import moment_blocks
+from oracle import optim as ref
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0**-24
+HALF_STEP = {torch.float32: U, torch.bfloat16: 2.0**-8, torch.float16: 2.0**-11}
+OPTIONS = {"lr": 3e-3, "betas": (0.9, 0.99), "eps": 1e-8, "weight_decay": 0.1}
+
+
+class Case:
+    """Parameters, gradients and state in numpy beside their device twins."""
+
+    def __init__(self, device, sizes, dtype, bits, seed, offset=0, first=0):
+        rng = np.random.default_rng(seed)
+        self.sizes, self.dtype, self.bits, self.device, self.seed, self.first = sizes, dtype, bits, device, seed, first
+        self.rng, self.offset = rng, offset
+        self.p = [self.put(rng.normal(size=n) * 0.1, dtype) for n in sizes]
+        if bits == 32:
+            self.m = [self.put(rng.normal(size=n) * 0.01, torch.float32) for n in sizes]
+            self.v = [self.put(rng.random(n) ** 2 * 1e-3, torch.float32) for n in sizes]
+            self.scales = None
+        else:
+            self.m = [self.put(rng.integers(0, 256, n), torch.uint8) for n in sizes]
+            self.v = [self.put(rng.integers(0, 256, n), torch.uint8) for n in sizes]
+            self.scales = [[self.put(rng.random(moment_blocks(n)) * s + 1e-9, torch.float32) for n in sizes]
+                           for s in (0.1, 1e-2)]
+        self.steps = [torch.tensor(float(t % 7), device=device) for t in range(len(sizes))]
+        scales = {} if bits == 32 else dict(zip(("exp_avg_scales", "exp_avg_sq_scales"), self.scales))
+        self.plan = AdamWPlan(self.p, self.m, self.v, self.steps, seed=seed, first=first, **scales)
+
+    def put(self, x, dtype):
+        """On the device, `offset` elements off an allocation's start."""
+
+        wide = torch.zeros(len(x) + self.offset + 3, dtype=dtype, device=self.device)
+        view = wide[self.offset : self.offset + len(x)]
+        view.copy_(torch.from_numpy(np.asarray(x)).to(dtype))
+        return view
+
+    def grads(self, scale=0.1, skip=()):
+        return [None if i in skip else self.put(self.rng.normal(size=n) * scale, self.dtype)
+                for i, n in enumerate(self.sizes)]
+
+    def host(self):
+        wide = lambda x: x.double().cpu().numpy()  # noqa: E731
+        if self.bits == 32:
+            return [(wide(p), wide(m), wide(v)) for p, m, v in zip(self.p, self.m, self.v)]
+        both = lambda c, s: (c.cpu().numpy(), s.cpu().numpy())  # noqa: E731
+        return [(wide(p), both(m, ms), both(v, vs))
+                for p, m, v, ms, vs in zip(self.p, self.m, self.v, *self.scales)]
+
+    def check(self, before, grads, t, max_norm=None, norm=None, **options):
+        o = {**OPTIONS, **options}
+        b1, b2 = o["betas"]
+        clip = 1.0 if max_norm is None else ref.clip_factor(norm, max_norm)
+        for i, ((p, m, v), (x, mm, vv)) in enumerate(zip(before, self.host())):
+            if grads[i] is None or not self.sizes[i]:  # left as it was
+                for a, b in ((p, x), (m, mm), (v, vv)):
+                    for y, z in zip(np.atleast_2d(a) if self.bits == 32 else a, np.atleast_2d(b) if self.bits == 32 else b):
+                        np.testing.assert_array_equal(y, z)
+                continue
+            g = grads[i].double().cpu().numpy() * clip
+            m0, v0 = (m, v) if self.bits == 32 else (ref.decode(*m, True), ref.decode(*v, False))
+            want, m1, v1 = ref.adamw(p, g, m0, v0, t[i], o["lr"], o["betas"], o["eps"], o["weight_decay"])
+            m_size = np.abs(b1 * m0) + np.abs((1 - b1) * g)
+            if self.bits == 32:
+                assert (np.abs(mm - m1) <= 6 * U * m_size).all()
+                assert (np.abs(vv - v1) <= 6 * U * v1 + 1e-44).all()
+            else:
+                _, m8, v8 = ref.adamw8(p, g, m, v, t[i], self.seed, self.first + i, o["lr"], o["betas"], o["eps"],
+                                       o["weight_decay"])
+                for got, expect in ((mm, m8), (vv, v8)):
+                    np.testing.assert_array_equal(got[1], expect[1])
+                    np.testing.assert_array_equal(got[0], expect[0])
+            root = np.sqrt(v1 / (1 - b2 ** t[i])) + o["eps"]
+            update = o["lr"] / (1 - b1 ** t[i]) * m_size / root + o["lr"] * o["weight_decay"] * np.abs(p)
+            step = HALF_STEP[self.dtype] * (np.abs(want) + 16 * U * update)
+            tiny = 2.0**-25 if self.dtype == torch.float16 else 0  # half of its smallest subnormal number
+            assert (np.abs(x - want) <= step + U * np.abs(want) + 16 * U * update + tiny).all(), i
+
+
+SIZES = [1, 2, 3, 5, 255, 256, 257, 1021, 1024, 4095, 4096, 4097, 20001]
+
+
+@pytest.mark.parametrize("offset", [0, 1, 3], ids=["aligned", "off-by-1", "off-by-3"])
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_steps_match_float64(device, dtype, bits, offset):
+    """Three steps over odd sizes, with and without clipping, tensors left out in the second."""
+
+    case = Case(device, SIZES, dtype, bits, seed=bits + offset, offset=offset, first=3)
+    t = [i % 7 for i in range(len(SIZES))]
+    for skip, max_norm in (((), None), ((0, 4, 12), 1.0), ((), 1e9)):
+        before, grads = case.host(), case.grads(skip=skip)
+        norm = case.plan.step(grads, max_norm=max_norm, **OPTIONS)
+        t = [n if i in skip else n + 1 for i, n in enumerate(t)]
+        if max_norm is None:
+            assert norm is None
+        else:
+            exact = np.sqrt(sum((g.double() ** 2).sum().item() for g in grads if g is not None))
+            assert norm.dtype == torch.float64 and abs(norm.item() - exact) <= 1e-13 * exact
+            norm = norm.item()
+        case.check(before, grads, t, max_norm, norm)
+        assert [s.item() for s in case.steps] == t
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_nothing_outside_a_tensor_is_written(device, bits):
+    case = Case(device, [1, 255, 4099], torch.float32, bits, seed=5, offset=1)
+    grads = case.grads()
+    for t in (*case.p, *case.m, *case.v, *(x for s in case.scales or () for x in s)):
+        t._base.fill_(77)
+    for t in (case.m if bits == 8 else ()):
+        t.fill_(3)
+    case.plan.step(grads, max_norm=1.0, **OPTIONS)
+    for t in (*case.p, *case.m, *case.v, *(x for s in case.scales or () for x in s)):
+        assert (t._base[0] == 77).all() and (t._base[1 + t.numel() :] == 77).all()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_many_tensors_take_several_launches(device, bits):
+    """More tensors than any launch's arguments hold, empty ones and gaps among them."""
+
+    rng = np.random.default_rng(9)
+    sizes = [0 if i % 50 == 7 else int(rng.integers(1, 700)) for i in range(700)]
+    case = Case(device, sizes, torch.float32, bits, seed=2)
+    skip = set(range(300, 330)) | {0, 699} | set(range(500, 560, 2))
+    before, grads = case.host(), case.grads(skip=skip)
+    start = [s.item() for s in case.steps]
+    norm = case.plan.step(grads, max_norm=1.0, **OPTIONS)
+    exact = np.sqrt(sum((g.double() ** 2).sum().item() for g in grads if g is not None))
+    assert abs(norm.item() - exact) <= 1e-13 * exact
+    assert abs(grad_norm(grads).item() - exact) <= 1e-13 * exact
+    t = [int(s) + (0 if i in skip or not sizes[i] else 1) for i, s in enumerate(start)]
+    assert [s.item() for s in case.steps] == t
+    case.check(before, grads, t, 1.0, norm.item())
+
+
+@pytest.mark.parametrize("options", [
+    {"betas": (0.0, 0.0)}, {"weight_decay": 0.0, "eps": 1e-3}, {"lr": 0.0}, {"betas": (0.999, 0.9999), "lr": 10.0},
+])
+@pytest.mark.parametrize("bits", [32, 8])
+def test_options(device, bits, options):
+    case = Case(device, [700], torch.float32, bits, seed=7)
+    before, grads = case.host(), case.grads()
+    case.plan.step(grads, **{**OPTIONS, **options})
+    case.check(before, grads, [1], **options)
+
+
+def test_learning_rate_on_the_device(device):
+    numbers = []
+    for lr in (3e-3, torch.tensor(3e-3, device=device)):
+        case = Case(device, SIZES, torch.float32, 32, seed=1)
+        case.plan.step(case.grads(), **{**OPTIONS, "lr": lr})
+        numbers.append([x.clone() for x in case.p])
+    for a, b in zip(*numbers):  # the rate itself is rounded to fp32 in one of the two
+        assert torch.allclose(a, b, rtol=2 * U, atol=4 * U * 3e-2)
+
+
+def test_a_zero_moment_block_and_tiny_gradients(device):
+    """Blocks whose scale is 0, subnormal or among the smallest numbers keep finite, sane values."""
+
+    n = 256 * 6
+    zero = [torch.zeros(n, device=device, dtype=torch.uint8) for _ in range(2)]
+    scales = [torch.zeros(6, device=device) for _ in range(2)]
+    p, step = torch.ones(n, device=device), torch.zeros((), device=device)
+    plan = AdamWPlan([p], zero[:1], zero[1:], [step], exp_avg_scales=scales[:1], exp_avg_sq_scales=scales[1:])
+    g = torch.zeros(n, device=device)
+    for block, size in enumerate((0.0, 1e-30, 1e-19, 1e-10, 1.0, 1e18)):
+        g[256 * block : 256 * (block + 1)] = size
+    plan.step([g], lr=1e-2, weight_decay=0.0)
+    m, v = (moment_values(c, s, signed) for c, s, signed in zip(zero, scales, (True, False)))
+    for block, size in enumerate((0.0, 1e-30, 1e-19, 1e-10, 1.0, 1e18)):
+        at = slice(256 * block, 256 * (block + 1))
+        if size not in (1e-30, 1e-19):  # (v there is below fp32's normal numbers)
+            np.testing.assert_allclose(m[at].cpu().numpy(), 0.1 * size, rtol=1e-6)
+            np.testing.assert_allclose(v[at].cpu().numpy(), 1e-3 * size * size, rtol=1e-6)
+    assert torch.isfinite(p).all() and torch.isfinite(m).all() and torch.isfinite(v).all()
+    # the first step of Adam is lr * sign(g) wherever |g| is far above eps
+    np.testing.assert_allclose(p[256 * 4 :].cpu().numpy(), 0.99, rtol=1e-6)
+    assert (p[:256] == 1).all()
+
+
+@pytest.mark.parametrize("bad", [float("inf"), float("nan")])
+@pytest.mark.parametrize("bits", [32, 8])
+def test_gradients_that_are_not_finite(device, bits, bad):
+    """Without clipping they stay in their element (with 8-bit moments, in the state of their block of
+    256); with clipping an infinite norm scales the others to 0, a NaN one makes everything NaN."""
+
+    case = Case(device, [1000, 600], torch.float32, bits, seed=3)
+    grads = case.grads()
+    grads[0][300] = bad
+    before = [x.clone() for x in case.p]
+    case.plan.step(grads, **OPTIONS)
+    assert torch.isnan(case.p[0][300]) and torch.isnan(case.p[0]).sum() == 1 and torch.isfinite(case.p[1]).all()
+    assert not torch.equal(case.p[0][:300], before[0][:300])
+    m = case.m[0] if bits == 32 else moment_values(case.m[0], case.scales[0][0], True)
+    assert not torch.isfinite(m[300])
+    hurt = torch.zeros(1000, dtype=torch.bool, device=device)
+    hurt[300 if bits == 32 else slice(256, 512)] = True
+    assert torch.isfinite(m[~hurt]).all()
+    if bits == 8:
+        assert not torch.isfinite(m[hurt]).any()
+    case = Case(device, [1000, 600], torch.float32, bits, seed=3)
+    norm = case.plan.step(grads, max_norm=1.0, **OPTIONS)
+    assert not np.isfinite(norm.item())
+    assert torch.isnan(case.p[0][300])
+    assert torch.isfinite(case.p[1]).all() if bad == float("inf") else torch.isnan(case.p[1]).all()
+
+
+def test_norm_of_mixed_types_sizes_and_strides(device):
+    gen = torch.Generator(device=device).manual_seed(0)
+    make = lambda *s: torch.randn(s, generator=gen, device=device)  # noqa: E731
+    grads = [make(3, 5), None, make(100001).bfloat16(), make(777).half(), make(64, 32).t(), make(50)[1:], make(0),
+             make(2_500_000) * 1e-3, make(9) * 1e30, make(9) * 1e-30]
+    total = sum((g.double() ** 2).sum().item() for g in grads if g is not None)
+    assert abs(grad_norm(grads).item() - np.sqrt(total)) <= 1e-12 * np.sqrt(total)
+    small = [g for g in grads if g is not None and g.numel() and g.abs().max() < 1e3]
+    total = sum((g.double() ** 2).sum().item() for g in small)
+    assert abs(grad_norm(small).item() - np.sqrt(total)) <= 1e-12 * np.sqrt(total)
+    assert torch.equal(grad_norm(small), grad_norm(small))  # a fixed order of addition
+    tiny = [torch.full((5,), 1e-30, device=device)]
+    assert abs(grad_norm(tiny).item() / (5**0.5 * float(tiny[0][0].double())) - 1) < 1e-12
+    assert grad_norm([make(0)]).item() == 0
+
+
+def test_a_given_norm_clips(device):
+    case, twin = (Case(device, SIZES, torch.bfloat16, 8, seed=4) for _ in range(2))
+    grads = case.grads()
+    own = case.plan.step(grads, max_norm=0.5, **OPTIONS)
+    given = twin.plan.step(grads, max_norm=0.5, norm=grad_norm(grads), **OPTIONS)
+    assert abs(own.item() - given.item()) <= 1e-14 * own.item()
+    # equal codes: both factors agree to fp64's last bits
+    for a, b in zip(case.host(), twin.host()):
+        np.testing.assert_array_equal(a[0], b[0])
+        np.testing.assert_array_equal(a[1][0], b[1][0])
+        np.testing.assert_array_equal(a[2][0], b[2][0])
+    empty = case.plan.step([None] * len(SIZES), max_norm=0.5, **OPTIONS)
+    assert empty.item() == 0
+
+
+def test_gradients_of_other_strides_are_taken_as_they_read(device):
+    p = [torch.randn(40, 30, device=device) for _ in range(2)]
+    q = [x.clone() for x in p]
+    g = [torch.randn(30, 40, device=device).t(), torch.randn(1, 30, device=device).expand(40, 30)]
+    state = lambda: ([torch.zeros(40, 30, device=device) for _ in range(2)], [torch.zeros(40, 30, device=device)  # noqa: E731
+                     for _ in range(2)], [torch.zeros((), device=device) for _ in range(2)])
+    AdamWPlan(p, *state()).step(g, lr=1e-2)
+    AdamWPlan(q, *state()).step([x.contiguous() for x in g], lr=1e-2)
+    assert torch.equal(p[0], q[0]) and torch.equal(p[1], q[1])
+
+
+def test_moment_values(device):
+    for n in (1, 4, 255, 256, 1023, 5000):
+        codes = torch.randint(0, 256, (n,), dtype=torch.uint8, device=device)
+        scales = torch.rand(moment_blocks(n), device=device)
+        for signed in (True, False):
+            want = ref.decode(codes.cpu().numpy(), scales.cpu().numpy(), signed).astype(np.float32)
+            np.testing.assert_array_equal(moment_values(codes, scales, signed).cpu().numpy(), want)
+            off = torch.zeros(n + 1, dtype=torch.uint8, device=device)[1:].copy_(codes)
+            np.testing.assert_array_equal(moment_values(off, scales, signed).cpu().numpy(), want)
+
+
+def test_elements_past_32_bits(device):
+    """A tensor of over 2^32 elements: its last blocks, and the random words of their indexes."""
+
+    n, keep = 2**32 + 517, 256 * 2 + 5
+    free, _ = torch.cuda.mem_get_info(device)
+    if free < 48 * 2**30:
+        pytest.skip("needs 48 GiB of GPU memory")
+    blocks = moment_blocks(n)
+    rng = np.random.default_rng(1)
+    p = torch.zeros(n, dtype=torch.bfloat16, device=device)
+    g = torch.zeros(n, dtype=torch.bfloat16, device=device)
+    m, v = (torch.zeros(n, dtype=torch.uint8, device=device) for _ in range(2))
+    ms, vs = (torch.zeros(blocks, device=device) for _ in range(2))
+    p[-keep:] = torch.from_numpy(rng.normal(size=keep)).to(p)
+    g[-keep:] = torch.from_numpy(rng.normal(size=keep)).to(g)
+    m[-keep:] = torch.from_numpy(rng.integers(0, 256, keep).astype(np.uint8)).to(device)
+    v[-keep:] = torch.from_numpy(rng.integers(0, 256, keep).astype(np.uint8)).to(device)
+    ms[-3:], vs[-3:] = 0.1, 0.01
+    step = torch.tensor(4.0, device=device)
+    tail = [x[-keep:].double().cpu().numpy() for x in (p, g)]
+    state = [(c[-keep:].cpu().numpy(), s[-3:].cpu().numpy()) for c, s in ((m, ms), (v, vs))]
+    plan = AdamWPlan([p], [m], [v], [step], exp_avg_scales=[ms], exp_avg_sq_scales=[vs], seed=11)
+    norm = plan.step([g], max_norm=1.0, **OPTIONS)
+    exact = np.sqrt((tail[1] ** 2).sum())
+    assert abs(norm.item() - exact) <= 1e-13 * exact
+    elements = np.arange(n - keep, n)
+    want, m8, v8 = ref.adamw8(tail[0], tail[1] * ref.clip_factor(norm.item(), 1.0), *state, 5, 11, 0, *OPTIONS.values(),
+                              elements=elements)
+    for codes, scales, expect in ((m, ms, m8), (v, vs, v8)):
+        np.testing.assert_array_equal(codes[-keep:].cpu().numpy(), expect[0])
+        np.testing.assert_array_equal(scales[-3:].cpu().numpy(), expect[1])
+    got = p[-keep:].double().cpu().numpy()
+    assert (np.abs(got - want) <= 2.0**-8 * np.abs(want) + 1e-6).all()
+    # (2^-8 is bf16's half step; the fp32 update is off by less than 16 u of 3e-3 x 10)
+    assert not p[: n - keep].any() and not m[: n - keep].any() and not v[: n - keep].any()
+
+
+def test_runs_repeat_bit_for_bit_on_any_stream(device):
+    results = []
+    for stream in (torch.cuda.current_stream(), torch.cuda.Stream()):
+        case = Case(device, SIZES, torch.float32, 8, seed=6)
+        grads = [case.grads() for _ in range(3)]
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            for g in grads:
+                case.plan.step(g, max_norm=1.0, **OPTIONS)
+        torch.cuda.synchronize()
+        results.append(case.host())
+    for a, b in zip(*results):
+        for x, y in zip((a[0], *a[1], *a[2]), (b[0], *b[1], *b[2])):
+            np.testing.assert_array_equal(x, y)
+
+
+def test_two_plans_at_once_on_two_streams(device):
+    """Calls that share nothing do not meet: each has a workspace of its own."""
+
+    cases = [Case(device, [50001] * 40, torch.float32, 32, seed=s) for s in (1, 2)]
+    twins = [Case(device, [50001] * 40, torch.float32, 32, seed=s) for s in (1, 2)]
+    grads = [[c.grads() for _ in range(4)] for c in cases]
+    for twin, many in zip(twins, grads):
+        for g in many:
+            twin.plan.step(g, max_norm=1.0, **OPTIONS)
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    for k in range(4):
+        for case, stream, many in zip(cases, streams, grads):
+            with torch.cuda.stream(stream):
+                case.plan.step(many[k], max_norm=1.0, **OPTIONS)
+    torch.cuda.synchronize()
+    for case, twin in zip(cases, twins):
+        assert all(torch.equal(a, b) for a, b in zip(case.p + case.m + case.v, twin.p + twin.m + twin.v))
+
+
+# ---- the optimiser ---------------------------------------------------------------------------------
+
+
+def _model(seed=0, dtype=torch.float64):
+    torch.manual_seed(seed)
+    return torch.nn.Sequential(torch.nn.Linear(13, 300), torch.nn.GELU(), torch.nn.Linear(300, 7)).to(dtype)
+
+
+def test_optimizer_follows_torchs_adamw(device):
+    """Six steps of two groups against float64 torch.optim.AdamW on the CPU with clip_grad_norm_ over both.
+    Each step's update differs by at most 20 u of itself (1e-2) and of what fp32 holds of p: 6 steps."""
+
+    theirs = _model()
+    ours = copy.deepcopy(theirs).float().to(device)
+    groups = lambda model: [{"params": model[0].parameters(), "lr": 1e-2},  # noqa: E731
+                            {"params": model[2].parameters(), "weight_decay": 0.0}]
+    a = torch.optim.AdamW(groups(theirs), lr=3e-3, weight_decay=0.1)
+    b = AdamW(groups(ours), lr=3e-3, weight_decay=0.1, max_norm=2.0)
+    gen = torch.Generator().manual_seed(2)
+    for step in range(6):
+        for x, y in zip(theirs.parameters(), ours.parameters()):
+            x.grad = torch.randn(x.shape, generator=gen).double()
+            y.grad = x.grad.float().to(device)
+        if step == 2:
+            theirs[2].bias.grad = ours[2].bias.grad = None
+        norm = torch.nn.utils.clip_grad_norm_(theirs.parameters(), 2.0)
+        a.step()
+        b.step()
+        assert abs(b.norm.item() - norm.item()) <= 1e-12 * norm.item()
+    for x, y in zip(theirs.parameters(), ours.parameters()):
+        assert (y.double().cpu() - x).abs().max() <= 6 * (20 * U * 1e-2 + U)
+        assert b.state[y]["step"].item() == a.state[x]["step"].item()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_optimizer_state_goes_through_state_dicts_copies_and_pickles(device, bits):
+    model = _model(dtype=torch.float32).to(device)
+    extra = torch.nn.Parameter(torch.randn(50, device=device).bfloat16())
+    optimizer = AdamW([*model.parameters(), extra], lr=1e-2, max_norm=1.0, state_bits=bits, seed=3)
+
+    def steps(params, opt, seed):
+        gen = torch.Generator(device=device).manual_seed(seed)
+        for _ in range(2):
+            for p in params:
+                p.grad = torch.randn(p.shape, generator=gen, device=device).to(p.dtype)
+            opt.step()
+
+    params = [*model.parameters(), extra]
+    steps(params, optimizer, 0)
+    saved = copy.deepcopy(optimizer.state_dict())
+    twin_params, twin = pickle.loads(pickle.dumps((params, optimizer)))
+    other_params = [torch.nn.Parameter(p.detach().clone()) for p in params]
+    other = AdamW(other_params, lr=9.0, max_norm=1.0, state_bits=bits, seed=3)
+    other.load_state_dict(saved)
+    assert other.param_groups[0]["lr"] == 1e-2 and twin.max_norm == 1.0 and twin.state_bits == bits
+    for many, opt in ((params, optimizer), (twin_params, twin), (other_params, other)):
+        steps(many, opt, 1)
+    for many in (twin_params, other_params):
+        assert all(torch.equal(a, b) for a, b in zip(params, many))
+    # loading goes into the state that is there
+    before = optimizer.state[extra]["exp_avg"]
+    optimizer.load_state_dict(saved)
+    assert optimizer.state[extra]["exp_avg"] is before
+    assert torch.equal(before, saved["state"][len(params) - 1]["exp_avg"])
+    assert optimizer.state[extra]["step"].item() == 2
+
+
+def test_optimizer_takes_moved_and_late_parameters(device):
+    model = _model(dtype=torch.float32).to(device)
+    optimizer = AdamW(model.parameters(), lr=1e-2)
+    for p in list(model.parameters())[:2]:
+        p.grad = torch.ones_like(p)
+    optimizer.step()
+    with torch.no_grad():
+        model[0].weight.data = model[0].weight.data.clone()  # (as module.to does)
+    for p in model.parameters():
+        p.grad = torch.ones_like(p)
+    optimizer.add_param_group({"params": [late := torch.nn.Parameter(torch.zeros(5, device=device))]})
+    late.grad = torch.ones(5, device=device)
+    want = [p.detach().clone() for p in model.parameters()]
+    versions = [p._version for p in model.parameters()]
+    optimizer.step()
+    for p, before, version in zip(model.parameters(), want, versions):
+        # weight decay 1e-2 and a step of lr * sign(g)
+        assert torch.allclose(p, before * (1 - 1e-4) - 1e-2, atol=1e-6)
+        assert p._version > version
+    assert torch.allclose(late, torch.full_like(late, -1e-2), atol=1e-7)
+    assert [optimizer.state[p]["step"].item() for p in model.parameters()] == [2, 2, 1, 1]
+
+
+def test_optimizer_closure_and_no_gradients(device):
+    p = torch.nn.Parameter(torch.ones(3, device=device))
+    optimizer = AdamW([p], lr=1e-2, max_norm=1.0)
+    assert optimizer.step() is None and not optimizer.state
+
+    def closure():
+        optimizer.zero_grad()
+        loss = (p**2).sum()
+        loss.backward()
+        return loss
+
+    assert optimizer.step(closure).item() == 3
+    assert abs(optimizer.norm.item() - 12**0.5) < 1e-6
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_captured_step_counts_on(device, bits):
+    """Replays equal eager steps of a twin bit for bit, with a learning rate that changes between them
+    and eager work in between; state made under capture is refused."""
+
+    results = []
+    for captured in (False, True):
+        torch.manual_seed(0)
+        params = [torch.nn.Parameter(torch.randn(n, device=device)) for n in (5, 300, 4097)]
+        lr = torch.tensor(1e-2, device=device)
+        optimizer = AdamW(params, lr=lr, max_norm=1.0, state_bits=bits, seed=1)
+        for p in params:
+            p.grad = torch.zeros_like(p)
+        gen = torch.Generator(device=device).manual_seed(5)
+
+        def new_gradients():
+            for p in params:
+                p.grad.copy_(torch.randn(p.shape, generator=gen, device=device))
+
+        new_gradients()
+        if captured:
+            graph = torch.cuda.CUDAGraph()
+            with pytest.raises(RuntimeError, match="capture"):
+                with torch.cuda.graph(graph):
+                    optimizer.step()
+            torch.cuda.synchronize()
+        optimizer.step()
+        if captured:
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                optimizer.step()
+        for k in range(4):
+            new_gradients()
+            lr.fill_(1e-2 / (k + 1))
+            if captured and k != 2:
+                graph.replay()
+            else:
+                optimizer.step()
+            torch.cuda.synchronize()
+        assert [optimizer.state[p]["step"].item() for p in params] == [5, 5, 5]
+        results.append([x.detach().clone() for p in params for x in (p, *optimizer.state[p].values())])
+    assert all(torch.equal(a, b) for a, b in zip(*results))

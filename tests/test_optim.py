@@ -1,0 +1,236 @@
+"""The optimiser step's host side and oracle, without a GPU: the 8-bit code's properties, the
+oracle against torch.optim.AdamW, and every refusal."""
+
+from __future__ import annotations
+
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+from card_playing_gym_amd import _native as nat
+from card_playing_gym_amd.nn import AdamW, AdamWPlan, grad_norm, moment_values
+from card_playing_gym_amd.nn import optim as O
+from oracle import optim as ref
+
+
+@pytest.fixture
+def anywhere(monkeypatch):
+    """Argument checks on CPU tensors: they come before anything is launched."""
+
+    monkeypatch.setattr(O, "require_device", lambda *tensors: None)
+
+
+def test_oracle_is_torchs_adamw():
+    gen = torch.Generator().manual_seed(0)
+    p = torch.randn(300, generator=gen, dtype=torch.float64).requires_grad_()
+    theirs = torch.optim.AdamW([p], lr=3e-3, betas=(0.8, 0.95), eps=1e-7, weight_decay=0.1)
+    x, m, v = p.detach().numpy().copy(), np.zeros(300), np.zeros(300)
+    for t in range(1, 6):
+        p.grad = torch.randn(300, generator=gen, dtype=torch.float64) * 3
+        g = p.grad.numpy().copy()
+        norm = torch.nn.utils.clip_grad_norm_([p], 10.0)
+        theirs.step()
+        x, m, v = ref.adamw(x, g * ref.clip_factor(float(norm), 10.0), m, v, t, 3e-3, (0.8, 0.95), 1e-7, 0.1)
+        np.testing.assert_allclose(x, p.detach().numpy(), rtol=1e-12, atol=1e-14)
+
+
+@pytest.mark.parametrize("signed, octaves", [(True, 16), (False, 32)])
+def test_codes_cover_their_octaves_in_eighths(signed, octaves):
+    f = ref.code_values(signed)[: 128 if signed else 256]
+    assert f[0] == 0 and f[-1] == 1 and (np.diff(f) > 0).all()
+    assert f[1] == 1.25 * 2.0**-octaves
+    assert (np.diff(f)[1:] / f[1:-1] <= 1 / 8).all()
+
+
+@pytest.mark.parametrize("signed", [True, False])
+def test_rounding_of_codes_is_unbiased_and_keeps_held_values(signed):
+    """Every code's value is kept whatever the random number; between two codes the mean over all 65536
+    random numbers is the value, up to half a random number's step."""
+
+    f = ref.code_values(signed)[: 128 if signed else 256]
+    noise = np.arange(65536)
+    for q in (1, 2, 7, 40, 126):
+        row = np.array([f[q], 1.0])
+        for r in (0, 32768, 65535):
+            codes, scales = ref.encode(row, np.array([r, 0]), signed)
+            assert codes[0] == q and scales[0] == 1
+        x = f[q] + 0.3 * (f[q + 1] - f[q])
+        codes = np.array([ref.encode(np.array([x, 1.0]), np.array([r, 0]), signed)[0][0] for r in noise[::16]])
+        mean = f[codes].mean()
+        assert abs(mean - x) <= (f[q + 1] - f[q]) / 4096
+
+
+def test_random_words_differ_by_step_tensor_and_element():
+    e = np.arange(4096)
+    rows = [ref.words(s, t, i, e) for s, t, i in ((0, 1, 0), (0, 2, 0), (0, 1, 1), (1, 1, 0))]
+    rows.append(ref.words(0, 1, 0, e + 2**32))
+    for a in range(len(rows)):
+        assert len(np.unique(rows[a])) == e.size
+        for b in range(a):
+            assert (rows[a] == rows[b]).mean() < 0.01
+        for part in (rows[a] & np.uint64(0xFFFF), rows[a] >> np.uint64(16)):
+            # mean of 4096 uniform 16-bit numbers: standard error 0.0045 of the range
+            assert abs(part.mean() / 65536 - 0.5) < 0.02
+
+
+# ---- refusals ----------------------------------------------------------------------------------
+
+
+def _lists(bits=32, sizes=(5, 300), dtype=torch.float32):
+    params = [torch.zeros(n, dtype=dtype) for n in sizes]
+    moment = torch.float32 if bits == 32 else torch.uint8
+    state = [[torch.zeros(n, dtype=moment) for n in sizes] for _ in range(2)]
+    steps = [torch.zeros(()) for _ in sizes]
+    scales = {} if bits == 32 else {
+        name: [torch.zeros(-(-n // 256)) for n in sizes] for name in ("exp_avg_scales", "exp_avg_sq_scales")}
+    return params, *state, steps, scales
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_plan_takes_matching_lists(anywhere, bits):
+    params, m, v, steps, scales = _lists(bits)
+    plan = AdamWPlan(params, m, v, steps, **scales)
+    assert plan.state_bits == bits
+
+
+def test_plan_refusals(anywhere):
+    params, m, v, steps, scales = _lists(8)
+    with pytest.raises(ValueError, match="at least one"):
+        AdamWPlan([], [], [], [])
+    with pytest.raises(ValueError, match="both lists"):
+        AdamWPlan(params, m, v, steps, exp_avg_scales=scales["exp_avg_scales"])
+    with pytest.raises(ValueError, match="contiguous torch.float32"):
+        AdamWPlan(params, m, v, steps)  # codes without scales
+    with pytest.raises(ValueError, match=r"\[2\]"):
+        AdamWPlan(params, m, v, steps, exp_avg_scales=scales["exp_avg_scales"],
+                  exp_avg_sq_scales=[torch.zeros(1), torch.zeros(3)])
+    params, m, v, steps, _ = _lists()
+    with pytest.raises(ValueError, match="differ in length"):
+        AdamWPlan(params, m[:1], v, steps)
+    with pytest.raises(ValueError, match="one type"):
+        AdamWPlan([params[0], params[1].bfloat16()], m, v, steps)
+    with pytest.raises(ValueError, match="Unsupported dtype"):
+        AdamWPlan([p.double() for p in params], m, v, steps)
+    with pytest.raises(ValueError, match="contiguous"):
+        AdamWPlan([params[0], torch.zeros(600)[::2]], m, v, steps)
+    with pytest.raises(ValueError, match="exp_avg_sqs"):
+        AdamWPlan(params, m, [v[0], torch.zeros(299)], steps)
+    with pytest.raises(ValueError, match=r"steps\[1\]"):
+        AdamWPlan(params, m, v, [steps[0], torch.zeros((), dtype=torch.int64)])
+    with pytest.raises(ValueError, match="share memory"):
+        AdamWPlan([params[1], params[1]], [m[1], m[0].new_zeros(300)], [v[1], v[1].clone()], steps)
+    with pytest.raises(ValueError, match="share memory"):  # the moments of one tensor inside another's
+        AdamWPlan(params, [m[1][:5], m[1]], v, steps)
+    with pytest.raises(ValueError, match="first"):
+        AdamWPlan(params, m, v, steps, first=-1)
+
+
+def test_step_refusals(anywhere):
+    params, m, v, steps, _ = _lists()
+    plan = AdamWPlan(params, m, v, steps)
+    grads = [torch.ones(5), torch.ones(300)]
+    with pytest.raises(ValueError, match="2 parameters but 1"):
+        plan.step(grads[:1], lr=1e-3)
+    with pytest.raises(ValueError, match="shape"):
+        plan.step([torch.ones(1, 5), grads[1]], lr=1e-3)
+    with pytest.raises(ValueError, match="type or device"):
+        plan.step([grads[0].double(), None], lr=1e-3)
+    with pytest.raises(ValueError, match="sparse"):
+        plan.step([grads[0].to_sparse(), None], lr=1e-3)
+    with pytest.raises(ValueError, match="without max_norm"):
+        plan.step(grads, lr=1e-3, norm=torch.zeros((), dtype=torch.float64))
+    with pytest.raises(ValueError, match="norm must be"):
+        plan.step(grads, lr=1e-3, max_norm=1.0, norm=torch.zeros(()))
+    with pytest.raises(ValueError, match="non-negative"):
+        plan.step(grads, lr=1e-3, max_norm=-1.0)
+    with pytest.raises(ValueError, match="lr must be"):
+        plan.step(grads, lr=torch.zeros((), dtype=torch.float64))
+    params[0].data = torch.zeros(5)
+    with pytest.raises(ValueError, match="moved"):
+        plan.step(grads, lr=1e-3)
+    assert not any(t.any() for t in (*params, *m, *v, *steps))
+
+
+def test_cpu_tensors_are_refused():
+    params, m, v, steps, _ = _lists()
+    with pytest.raises(RuntimeError, match="ROCm"):
+        AdamWPlan(params, m, v, steps)
+    with pytest.raises(RuntimeError, match="ROCm"):
+        grad_norm(params)
+    with pytest.raises(RuntimeError, match="ROCm"):
+        moment_values(torch.zeros(4, dtype=torch.uint8), torch.zeros(1), True)
+
+
+def test_norm_and_values_refusals(anywhere):
+    with pytest.raises(ValueError, match="at least one"):
+        grad_norm([None])
+    with pytest.raises(ValueError, match="Unsupported dtype"):
+        grad_norm([torch.zeros(3, dtype=torch.float64)])
+    with pytest.raises(ValueError, match="uint8"):
+        moment_values(torch.zeros(4), torch.zeros(1), True)
+    with pytest.raises(ValueError, match=r"\[2\]"):
+        moment_values(torch.zeros(257, dtype=torch.uint8), torch.zeros(1), False)
+
+
+def test_native_refusals():
+    """Fake addresses: every check comes before a launch."""
+
+    lib = nat.lib()
+    tensors = (nat.AdamWTensor * 1)(nat.AdamWTensor(16, 16, 16, None, None, 16, 8))
+    grads = (ctypes.c_void_p * 1)(16)
+    need = lib.cg_adamw_workspace_size(1)
+
+    def status(size=need, workspace=16, norm=None, n=1, **options):
+        config = nat.AdamWConfig(1e-3, 0.9, 0.999, 1e-8, 0.0, 1.0, None, 0, 0, nat.CG_F32, 32, nat.CG_CLIP_NONE)
+        for name, value in options.items():
+            setattr(config, name, value)
+        return lib.cg_adamw_step(tensors, grads, n, ctypes.byref(config), norm, workspace, size, None)
+
+    for options in ({"size": need - 1}, {"workspace": None}, {"workspace": 8}, {"n": -1}, {"dtype": 7},
+                    {"state_bits": 16}, {"beta1": 1.0}, {"beta2": -0.1}, {"clip": 3}, {"clip": nat.CG_CLIP_OWN_NORM},
+                    {"clip": nat.CG_CLIP_GIVEN_NORM}, {"state_bits": 8}):
+        assert status(**options) == nat.CG_ERR_INVALID, options
+    tensors[0].step = None
+    assert status() == nat.CG_ERR_INVALID
+    tensors[0].n = -1
+    assert status() == nat.CG_ERR_RANGE
+    assert lib.cg_adamw_step(tensors, grads, 1, None, None, 16, need, None) == nat.CG_ERR_INVALID
+    sizes, dtypes = (ctypes.c_int64 * 1)(4), (ctypes.c_int32 * 1)(9)
+    need = lib.cg_grad_norm_workspace_size(1)
+    assert lib.cg_grad_norm(grads, sizes, dtypes, 1, 16, 16, need, None) == nat.CG_ERR_INVALID
+    dtypes[0] = 0
+    assert lib.cg_grad_norm(grads, sizes, dtypes, 1, None, 16, need, None) == nat.CG_ERR_INVALID
+    assert lib.cg_grad_norm(grads, sizes, dtypes, 1, 16, 16, need - 1, None) == nat.CG_ERR_INVALID
+    assert lib.cg_moment_values(None, None, 1, None, 4, None) == nat.CG_ERR_INVALID
+    assert lib.cg_moment_values(None, None, 1, None, -4, None) == nat.CG_ERR_RANGE
+
+
+def test_optimizer_options():
+    p = torch.nn.Parameter(torch.zeros(3))
+    for options in ({"lr": -1.0}, {"betas": (1.0, 0.9)}, {"eps": -1e-8}, {"weight_decay": -0.1}, {"max_norm": -1.0},
+                    {"state_bits": 16}):
+        with pytest.raises(ValueError):
+            AdamW([p], **options)
+    p.grad = torch.ones(3)
+    with pytest.raises(RuntimeError, match="ROCm"):
+        AdamW([p]).step()
+
+
+def test_state_dict_refusals(anywhere):
+    p = torch.nn.Parameter(torch.zeros(300))
+    theirs = torch.optim.AdamW([p])
+    p.grad = torch.ones(300)
+    theirs.step()
+    eight = AdamW([p], state_bits=8)
+    with pytest.raises(ValueError, match="8-bit"):
+        eight.load_state_dict(theirs.state_dict())
+    wide = AdamW([p])
+    wide.load_state_dict(theirs.state_dict())
+    assert float(wide.state[p]["step"]) == 1 and torch.equal(wide.state[p]["exp_avg"], theirs.state[p]["exp_avg"])
+    with pytest.raises(ValueError, match="32-bit"):
+        wide.load_state_dict({**eight.state_dict(), "state": {0: eight._new_state(p)}})
+    other = AdamW([torch.nn.Parameter(torch.zeros(299))])
+    with pytest.raises(ValueError, match="shape"):
+        other.load_state_dict(theirs.state_dict())
