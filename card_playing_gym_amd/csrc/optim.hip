@@ -11,6 +11,8 @@
 //
 // The update is bound by HBM: 28 bytes an element with fp32 parameters and moments, 16 with moments
 // in 8 bits, 20 and 8 with bf16 parameters.
+#include <cmath>
+
 #include "common.h"
 
 namespace cg {
@@ -56,7 +58,7 @@ struct PrepareArgs {
   const double *sums;
   double *norm;             // written when there are partial sums, else read; NULL: no clipping
   const float *lr_device;   // NULL: lr
-  double lr, beta1, beta2, weight_decay, max_norm;
+  double lr, log_beta1, log_beta2, weight_decay, max_norm;  // logarithms to base 2
   uint32_t seed;
   StepHeader *header;
 };
@@ -104,23 +106,39 @@ __device__ __forceinline__ int tensor_of(const int32_t (&first)[N], int tensors,
 
 // ---- four consecutive elements -----------------------------------------------------------
 
-template <typename T>
-__device__ __forceinline__ f32x4 load4(const T *at) {
-  struct alignas(4 * sizeof(T)) V {
-    T e[4];
-  };
-  const V q = *reinterpret_cast<const V *>(at);
-  return f32x4{to_f32(q.e[0]), to_f32(q.e[1]), to_f32(q.e[2]), to_f32(q.e[3])};
+// STREAM: past the caches' lines that are kept (non-temporal), for data that will not be met there again.
+template <bool STREAM, typename V>
+__device__ __forceinline__ V load_as(const void *at) {
+  if constexpr (STREAM)
+    return __builtin_nontemporal_load(static_cast<const V *>(at));
+  else
+    return *static_cast<const V *>(at);
 }
-template <typename T>
+template <bool STREAM, typename V>
+__device__ __forceinline__ void store_as(void *at, V x) {
+  if constexpr (STREAM)
+    __builtin_nontemporal_store(x, static_cast<V *>(at));
+  else
+    *static_cast<V *>(at) = x;
+}
+template <bool STREAM, typename T>
+__device__ __forceinline__ f32x4 load4(const T *at) {
+  if constexpr (sizeof(T) == 4) {
+    return load_as<STREAM, f32x4>(at);
+  } else {
+    struct V {
+      T e[4];
+    };
+    const V q = __builtin_bit_cast(V, load_as<STREAM, u32x2>(at));
+    return f32x4{to_f32(q.e[0]), to_f32(q.e[1]), to_f32(q.e[2]), to_f32(q.e[3])};
+  }
+}
+template <bool STREAM, typename T>
 __device__ __forceinline__ void store4(T *at, f32x4 x) {
-  struct alignas(4 * sizeof(T)) V {
-    T e[4];
-  };
-  V q;
-#pragma unroll
-  for (int k = 0; k < 4; ++k) q.e[k] = from_f32<T>(x[k]);
-  *reinterpret_cast<V *>(at) = q;
+  if constexpr (sizeof(T) == 4)
+    store_as<STREAM>(at, x);
+  else
+    store_as<STREAM>(at, cvt4<T>(x));
 }
 // The first `count` of four elements; the others are zero, or left alone.
 template <typename T>
@@ -160,7 +178,7 @@ __device__ __forceinline__ double block_sum(double x) {
 
 // Squares of fp32 numbers are exact in fp64 and neither overflow nor vanish there, so the sum needs
 // no scaling and the norm is the same whatever the launch shape up to fp64's rounding.
-template <typename T>
+template <typename T, bool STREAM>
 __global__ __launch_bounds__(THREADS) void square_sums_kernel(const NormArgs a) {
   double sum = 0;
   for (int c = blockIdx.x; c < a.chunks; c += gridDim.x) {
@@ -169,15 +187,14 @@ __global__ __launch_bounds__(THREADS) void square_sums_kernel(const NormArgs a) 
     const int64_t left = a.n[i] - begin;
     const T *g = static_cast<const T *>(a.g[i]) + begin;
     const int n = left < NORM_CHUNK ? int(left) : NORM_CHUNK;
-    if (aligned4(g)) {
-      const int whole = n / 4;
-      for (int k = threadIdx.x; k < whole; k += THREADS) {
-        const f32x4 x = load4(g + 4 * k);
+    if (n == NORM_CHUNK && aligned4(g)) {
+      f32x4 x[NORM_CHUNK / (4 * THREADS)];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sum = fma(double(x[e]), double(x[e]), sum);
-      }
-      const int k = 4 * whole + threadIdx.x;
-      if (k < n) sum = fma(double(to_f32(g[k])), double(to_f32(g[k])), sum);
+      for (int k = 0; k < NORM_CHUNK / (4 * THREADS); ++k) x[k] = load4<STREAM>(g + 4 * (k * THREADS + int(threadIdx.x)));
+#pragma unroll
+      for (int k = 0; k < NORM_CHUNK / (4 * THREADS); ++k)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum = fma(double(x[k][e]), double(x[k][e]), sum);
     } else {
       for (int k = threadIdx.x; k < n; k += THREADS) sum = fma(double(to_f32(g[k])), double(to_f32(g[k])), sum);
     }
@@ -227,8 +244,8 @@ __global__ __launch_bounds__(THREADS) void prepare_kernel(const PrepareArgs a) {
     const float t = *a.step[i] + 1;
     *a.step[i] = t;
     TensorScalars s;
-    s.rate = float(lr / (1 - pow(a.beta1, double(t))));
-    s.second = float(1 / sqrt(1 - pow(a.beta2, double(t))));
+    s.rate = float(lr / (1 - exp2(a.log_beta1 * t)));
+    s.second = float(1 / sqrt(1 - exp2(a.log_beta2 * t)));
     s.key = mix(mix(mix(a.seed) + uint32_t(t)) + uint32_t(a.index[i]));
     s.pad = 0;
     out[i] = s;
@@ -252,7 +269,7 @@ __device__ __forceinline__ void adamw4(f32x4 &p, const f32x4 g, f32x4 &m, f32x4 
   }
 }
 
-template <typename T>
+template <typename T, bool STREAM>
 __global__ __launch_bounds__(THREADS) void adamw_kernel(const UpdateArgs<Tensor32, UPDATE_TENSORS> a) {
   const int i = tensor_of(a.first_chunk, a.tensors, blockIdx.x);
   const Tensor32 t = a.t[i];
@@ -271,10 +288,10 @@ __global__ __launch_bounds__(THREADS) void adamw_kernel(const UpdateArgs<Tensor3
     const int e = 4 * (c * THREADS + int(threadIdx.x));
     if (e >= n) break;
     if (vec && e + 4 <= n) {
-      f32x4 x = load4(p + e), mm = load4(m + e), vv = load4(v + e);
-      const f32x4 gg = load4(g + e);
+      f32x4 x = load4<STREAM>(p + e), mm = load4<STREAM>(m + e), vv = load4<STREAM>(v + e);
+      const f32x4 gg = load4<STREAM>(g + e);
       adamw4(x, gg, mm, vv, r);
-      store4(p + e, x), store4(m + e, mm), store4(v + e, vv);
+      store4<STREAM>(p + e, x), store4<STREAM>(m + e, mm), store4<STREAM>(v + e, vv);
     } else {
       const int some = n - e < 4 ? n - e : 4;
       f32x4 x = load_some(p + e, some), mm = load_some(m + e, some), vv = load_some(v + e, some);
@@ -308,8 +325,8 @@ __global__ __launch_bounds__(THREADS) void adamw_kernel(const UpdateArgs<Tensor3
 constexpr uint32_t ONE = 8184;  // 1.0: a double's exponent and top three mantissa bits
 
 template <int MOST>
-__device__ __forceinline__ double code_value(uint32_t q) {
-  return q ? __hiloint2double(int((q + (ONE - MOST)) << 17), 0) : 0.0;
+__device__ __forceinline__ double code_value(uint32_t q, uint32_t sign = 0) {
+  return __hiloint2double(int(q ? (q + (ONE - MOST)) << 17 | sign : 0u), 0);
 }
 
 __device__ __forceinline__ double moment(double beta, double held, double one, double x) {
@@ -318,92 +335,134 @@ __device__ __forceinline__ double moment(double beta, double held, double one, d
   return kept + added;
 }
 
-template <int MOST>
-__device__ __forceinline__ uint32_t code_of(double size, double inverse, uint32_t noise) {
-  const uint32_t hi = uint32_t(__double2hiint(size * inverse));
-  const int q = int((hi + 2 * noise + 1) >> 17) - int(ONE - MOST);
-  return uint32_t(q < 0 ? 0 : q > MOST ? MOST : q);
+// The code above ONE - MOST: a quotient's upper word and 17 random bits (16, and the middle of their
+// step), cut off behind the third mantissa bit.  least: the lowest to return.
+__device__ __forceinline__ uint32_t code_of(uint32_t hi, uint32_t noise, int least) {
+  const int q = int((hi + noise) >> 17);
+  return uint32_t(min(max(q, least), int(ONE)));
 }
 
 // The largest over the wave; patterns of non-negative floats, of which NaN's is above infinity's.
-__device__ __forceinline__ float wave_largest(uint32_t bits) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    const uint32_t other = uint32_t(__shfl_xor(int(bits), o, 64));
-    bits = bits > other ? bits : other;
-  }
-  return __uint_as_float(bits);
+// Lanes take in their neighbours 1, 2, 4 and 8 below inside rows of 16, then rows the one before and
+// the two before (out of range: 0); lane 63 has seen all.
+template <int CONTROL, int ROWS>
+__device__ __forceinline__ uint32_t larger_of(uint32_t x) {
+  const uint32_t other = uint32_t(__builtin_amdgcn_update_dpp(0, int(x), CONTROL, ROWS, 0xf, ROWS == 0xf));
+  return other > x ? other : x;
+}
+__device__ __forceinline__ float wave_largest(uint32_t x) {
+  x = larger_of<0x111, 0xf>(x);  // row_shr:1, 2, 4, 8
+  x = larger_of<0x112, 0xf>(x);
+  x = larger_of<0x114, 0xf>(x);
+  x = larger_of<0x118, 0xf>(x);
+  x = larger_of<0x142, 0xa>(x);  // row_bcast:15, 31
+  x = larger_of<0x143, 0xc>(x);
+  return __uint_as_float(uint32_t(__builtin_amdgcn_readlane(int(x), 63)));
 }
 
 __device__ __forceinline__ double inverse_of(float scale) {
   return scale < 1.17549435e-38f ? 0.0 : double(1.0f / scale);
 }
 
-template <typename T>
+// Roots within an ulp.  The instruction alone takes subnormal numbers for 0, which beside an eps of
+// 2^-40 or more is far below the sum's last bit.
+__device__ __forceinline__ void roots_of(const float (&v)[4], float (&root)[4], float eps) {
+  if (eps >= 0x1p-40f) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) root[k] = __builtin_amdgcn_sqrtf(v[k]);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const bool small = v[k] < 0x1p-96f;
+      const float r = __builtin_amdgcn_sqrtf(small ? v[k] * 0x1p64f : v[k]);
+      root[k] = small ? r * 0x1p-32f : r;
+    }
+  }
+}
+
+struct Rates8 {
+  double clip, beta1, one1, beta2, one2;
+  float eps, decay, rate, second;
+};
+
+// Four elements of a lane, the block's across the wave: parameters and codes in place, new scales.
+// index, high: the lower and (times an odd constant) the upper 32 bits of the first element's index.
+__device__ __forceinline__ void adamw8(f32x4 &x, const f32x4 g, uint32_t &mq, uint32_t &vq, float &m_scale,
+                                       float &v_scale, uint32_t index, uint32_t key, uint32_t high, const Rates8 &r) {
+  double m[4], v[4];
+  float m32[4], v32[4], root[4];
+  uint32_t m_top = 0, v_top = 0;
+  const double ms = m_scale, vs = v_scale;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const double d = double(g[k]) * r.clip;
+    const uint32_t q = mq >> 8 * k;
+    m[k] = moment(r.beta1, code_value<127>(q & 127, q << 24 & 0x80000000u) * ms, r.one1, d);
+    v[k] = moment(r.beta2, code_value<255>(vq >> 8 * k & 255) * vs, r.one2, d * d);
+    m32[k] = float(m[k]), v32[k] = float(v[k]);
+    m_top = max(m_top, __float_as_uint(m32[k]) & 0x7fffffffu);
+    v_top = max(v_top, __float_as_uint(v32[k]));  // (a sign, of a NaN, puts it on top too)
+  }
+  roots_of(v32, root, r.eps);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const float step = r.rate * m32[k] * __builtin_amdgcn_rcpf(fmaf(root[k], r.second, r.eps));
+    x[k] -= fmaf(r.decay, x[k], step);
+  }
+  m_scale = wave_largest(m_top), v_scale = wave_largest(v_top);
+  const double m_inv = inverse_of(m_scale), v_inv = inverse_of(v_scale);
+  // Each code is formed above 0's, ONE - 127 and ONE - 255; the four offsets come off at once.
+  constexpr uint32_t M0 = ONE - 127, V0 = ONE - 255;
+  mq = -(M0 * 0x01010101u), vq = -(V0 * 0x01010101u);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const uint32_t word = mix(((index + k) ^ key) + high);
+    const uint32_t m_hi = uint32_t(__double2hiint(m[k] * m_inv)), v_hi = uint32_t(__double2hiint(v[k] * v_inv));
+    const uint32_t q = code_of(m_hi & 0x7fffffffu, (word << 1 & 0x1fffeu) | 1, M0);
+    mq += (q + (q != M0 ? m_hi >> 24 & 128 : 0u)) << 8 * k;
+    vq += code_of(v_hi, (word >> 15 & 0x1fffeu) | 1, v_hi ? V0 + 1 : V0) << 8 * k;  // (no quotient is subnormal)
+  }
+}
+
+template <typename T, bool STREAM>
 __global__ __launch_bounds__(THREADS) void adamw8_kernel(const UpdateArgs<Tensor8, UPDATE_TENSORS_8> a) {
   const int i = tensor_of(a.first_chunk, a.tensors, blockIdx.x);
   const Tensor8 t = a.t[i];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const TensorScalars s = reinterpret_cast<const TensorScalars *>(a.header + 1)[a.entry + i];
-  const double clip = a.header->clip;
-  const float decay = a.header->decay;
-  T *p = static_cast<T *>(t.p);
-  const T *g = static_cast<const T *>(t.g);
-  const bool vec = aligned4(p) && aligned4(g) && aligned4(t.m) && aligned4(t.v);
+  const Rates8 r{a.header->clip, a.beta1, 1 - a.beta1, a.beta2, 1 - a.beta2, a.eps, a.header->decay, s.rate, s.second};
+  const bool vec = aligned4(static_cast<T *>(t.p)) && aligned4(static_cast<const T *>(t.g)) && aligned4(t.m) && aligned4(t.v);
   const int64_t blocks = (t.n + MOMENT_BLOCK - 1) / MOMENT_BLOCK;
   const int64_t first = int64_t(int(blockIdx.x) - a.first_chunk[i]) * (CHUNK / MOMENT_BLOCK);
 #pragma unroll
   for (int c = 0; c < CHUNK / MOMENT_BLOCK / (THREADS / 64); ++c) {
     const int64_t b = first + c * (THREADS / 64) + wave;
     if (b >= blocks) break;  // whole wave
-    const int64_t e = b * MOMENT_BLOCK + 4 * lane;
-    const int64_t left = t.n - e;
-    const int some = left >= 4 ? 4 : left > 0 ? int(left) : 0;
+    const int64_t at = b * MOMENT_BLOCK;
+    T *p = static_cast<T *>(t.p) + at;
+    const T *g = static_cast<const T *>(t.g) + at;
+    uint8_t *m = t.m + at, *v = t.v + at;
+    const int e = 4 * lane;
+    const uint32_t index = uint32_t(at) + e, high = uint32_t(uint64_t(at) >> 32) * 0x9E3779B9u;
+    float m_scale = t.m_scale[b], v_scale = t.v_scale[b];
     f32x4 x, grad;
     uint32_t mq = 0, vq = 0;
-    if (vec && some == 4) {
-      x = load4(p + e), grad = load4(g + e);
-      mq = *reinterpret_cast<const uint32_t *>(t.m + e), vq = *reinterpret_cast<const uint32_t *>(t.v + e);
+    if (vec && t.n - at >= MOMENT_BLOCK) {  // whole wave
+      x = load4<STREAM>(p + e), grad = load4<STREAM>(g + e);
+      mq = load_as<STREAM, uint32_t>(m + e), vq = load_as<STREAM, uint32_t>(v + e);
+      adamw8(x, grad, mq, vq, m_scale, v_scale, index, s.key, high, r);
+      store4<STREAM>(p + e, x);
+      store_as<STREAM>(m + e, mq), store_as<STREAM>(v + e, vq);
     } else {
+      const int left = int(t.n - at < MOMENT_BLOCK ? t.n - at : MOMENT_BLOCK) - e;
+      const int some = left > 4 ? 4 : left > 0 ? left : 0;
       x = load_some(p + e, some), grad = load_some(g + e, some);
-      for (int k = 0; k < some; ++k) mq |= uint32_t(t.m[e + k]) << 8 * k, vq |= uint32_t(t.v[e + k]) << 8 * k;
-    }
-    const double m_scale = t.m_scale[b], v_scale = t.v_scale[b];
-    double m[4], v[4];
-    uint32_t m_top = 0, v_top = 0;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const double d = double(grad[k]) * clip;
-      const uint32_t q = mq >> 8 * k & 255;
-      const double held = code_value<127>(q & 127) * m_scale;
-      m[k] = moment(a.beta1, q & 128 ? -held : held, 1 - a.beta1, d);
-      v[k] = moment(a.beta2, code_value<255>(vq >> 8 * k & 255) * v_scale, 1 - a.beta2, d * d);
-      const float m32 = float(m[k]), v32 = float(v[k]);
-      m_top = max(m_top, __float_as_uint(m32) & 0x7fffffffu);
-      v_top = max(v_top, __float_as_uint(v32) & 0x7fffffffu);
-      const float step = s.rate * m32 / fmaf(sqrtf(v32), s.second, a.eps);
-      x[k] -= fmaf(decay, x[k], step);
-    }
-    const float m_new = wave_largest(m_top), v_new = wave_largest(v_top);
-    const double m_inv = inverse_of(m_new), v_inv = inverse_of(v_new);
-    mq = vq = 0;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int64_t j = e + k;
-      const uint32_t word = mix((uint32_t(j) ^ s.key) + uint32_t(uint64_t(j) >> 32) * 0x9E3779B9u);
-      const uint32_t q = code_of<127>(fabs(m[k]), m_inv, word & 0xffff);
-      mq |= (q | (m[k] < 0 && q ? 128u : 0u)) << 8 * k;
-      const uint32_t u = code_of<255>(v[k], v_inv, word >> 16);
-      vq |= (u == 0 && v[k] * v_inv > 0 ? 1u : u) << 8 * k;
-    }
-    if (vec && some == 4) {
-      store4(p + e, x);
-      *reinterpret_cast<uint32_t *>(t.m + e) = mq, *reinterpret_cast<uint32_t *>(t.v + e) = vq;
-    } else {
+      for (int k = 0; k < some; ++k) mq |= uint32_t(m[e + k]) << 8 * k, vq |= uint32_t(v[e + k]) << 8 * k;
+      adamw8(x, grad, mq, vq, m_scale, v_scale, index, s.key, high, r);
       store_some(p + e, x, some);
-      for (int k = 0; k < some; ++k) t.m[e + k] = uint8_t(mq >> 8 * k), t.v[e + k] = uint8_t(vq >> 8 * k);
+      for (int k = 0; k < some; ++k) m[e + k] = uint8_t(mq >> 8 * k), v[e + k] = uint8_t(vq >> 8 * k);
     }
-    if (lane == 0) t.m_scale[b] = m_new, t.v_scale[b] = v_new;
+    if (lane == 0) t.m_scale[b] = m_scale, t.v_scale[b] = v_scale;
   }
 }
 
@@ -426,11 +485,10 @@ __global__ __launch_bounds__(THREADS) void moment_values_kernel(const uint8_t *_
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     const uint32_t c = q >> 8 * k & 255;
-    const double f = code_value<MOST>(c & MOST) * scale;
-    x[k] = float(MOST == 127 && c & 128 ? -f : f);
+    x[k] = float(code_value<MOST>(c & MOST, MOST == 127 ? c << 24 & 0x80000000u : 0u) * scale);
   }
   if (vec)
-    store4(values + e, x);
+    store4<true>(values + e, x);
   else
     store_some(values + e, x, some);
 }
@@ -449,8 +507,8 @@ struct GradList {
 
 // Launches the partial sums of the tensors of type `dtype`; returns how many sums were written.
 template <typename T>
-int launch_square_sums(const GradList &list, const int32_t *dtypes, int32_t dtype, int budget, double *partials,
-                       hipStream_t stream) {
+int launch_square_sums(const GradList &list, const int32_t *dtypes, int32_t dtype, int budget, bool streams,
+                       double *partials, hipStream_t stream) {
   int written = 0, at = 0;
   while (at < list.count) {
     NormArgs a{};
@@ -469,7 +527,7 @@ int launch_square_sums(const GradList &list, const int32_t *dtypes, int32_t dtyp
     a.chunks = int32_t(chunks);
     a.partials = partials + written;
     const int grid = int(chunks < budget ? chunks : budget);
-    square_sums_kernel<T><<<grid, THREADS, 0, stream>>>(a);
+    (streams ? square_sums_kernel<T, true> : square_sums_kernel<T, false>)<<<grid, THREADS, 0, stream>>>(a);
     CG_LAUNCHED();
     written += grid;
   }
@@ -495,19 +553,26 @@ int dtype_index(int32_t dtype) {
   return dtype;
 }
 
-int launch_norm(const GradList &list, const int32_t *dtypes, int32_t dtype, double *partials, hipStream_t stream) {
+// Above this many bytes of parameters, gradients and state together a step goes past the caches
+// (the Infinity Cache has 256 MB): what one launch leaves there is gone before it is met again.
+// fp32 parameters and moments, 174 M elements (2.8 GB): norm 167 -> 105 us, update 912 -> 882; 11.4 M
+// (182 MB): 10.6 -> 9.9, but the update, which meets gradients that the norm has read, 53 -> 67.
+constexpr int64_t STREAM_BYTES = 512 << 20;
+
+int launch_norm(const GradList &list, const int32_t *dtypes, int32_t dtype, bool streams, double *partials,
+                hipStream_t stream) {
   bool seen[3] = {};
   for (int i = 0; i < list.count; ++i) seen[dtype_index(dtypes ? dtypes[i] : dtype)] = true;
   const int budget = norm_budget(list.count, dtypes ? 3 : 1);
   int sums = 0;
-  if (seen[CG_F32]) sums += launch_square_sums<float>(list, dtypes, CG_F32, budget, partials + sums, stream);
-  if (seen[CG_BF16]) sums += launch_square_sums<bf16>(list, dtypes, CG_BF16, budget, partials + sums, stream);
-  if (seen[CG_F16]) sums += launch_square_sums<f16>(list, dtypes, CG_F16, budget, partials + sums, stream);
+  if (seen[CG_F32]) sums += launch_square_sums<float>(list, dtypes, CG_F32, budget, streams, partials + sums, stream);
+  if (seen[CG_BF16]) sums += launch_square_sums<bf16>(list, dtypes, CG_BF16, budget, streams, partials + sums, stream);
+  if (seen[CG_F16]) sums += launch_square_sums<f16>(list, dtypes, CG_F16, budget, streams, partials + sums, stream);
   return sums;
 }
 
-template <typename K, typename T, int N, typename Fill>
-void launch_updates(K kernel, const cg_adamw_tensor *tensors, const void *const *grads, int n,
+template <typename T, int N, typename Fill>
+void launch_updates(void (*kernel)(UpdateArgs<T, N>), const cg_adamw_tensor *tensors, const void *const *grads, int n,
                     const cg_adamw_config &c, StepHeader *header, hipStream_t stream, const Fill &fill) {
   int at = 0, entry = 0;  // entries count the tensors that take part
   while (at < n) {
@@ -552,7 +617,9 @@ int cg_grad_norm(const void *const *grads, const int64_t *sizes, const int32_t *
     CG_REQUIRE(workspace_size >= cg_grad_norm_workspace_size(n), CG_ERR_INVALID, "workspace too small");
     for (int i = 0; i < n; ++i) CG_REQUIRE(sizes[i] >= 0, CG_ERR_INVALID, "sizes must be non-negative");
     double *partials = static_cast<double *>(workspace);
-    const int sums = launch_norm(GradList{grads, sizes, 1, n}, dtypes, 0, partials, as_stream(stream));
+    int64_t bytes = 0;
+    for (int i = 0; i < n; ++i) bytes += grads[i] ? sizes[i] * dtype_size(dtypes[i]) : 0;
+    const int sums = launch_norm(GradList{grads, sizes, 1, n}, dtypes, 0, bytes > STREAM_BYTES, partials, as_stream(stream));
     norm_kernel<<<1, THREADS, 0, as_stream(stream)>>>(partials, sums, norm);
     CG_LAUNCHED();
   });
@@ -590,11 +657,14 @@ int cg_adamw_step(const cg_adamw_tensor *tensors, const void *const *grads, int3
       CG_REQUIRE(c.state_bits == 32 || (t.exp_avg_scale && t.exp_avg_sq_scale), CG_ERR_INVALID,
                  "moments in 8 bits need their scales");
     }
+    int64_t elements = 0;
+    for (int i = 0; i < n; ++i) elements += grads[i] ? tensors[i].n : 0;
+    const bool streams = elements > STREAM_BYTES / (2 * dtype_size(c.dtype) + c.state_bits / 4);
     StepHeader *header = static_cast<StepHeader *>(workspace);
     double *partials = reinterpret_cast<double *>(static_cast<char *>(workspace) + (scalars_bytes(n) + 15) / 16 * 16);
     int sums = 0;
     if (c.clip == CG_CLIP_OWN_NORM)
-      sums = launch_norm(GradList{grads, &tensors[0].n, int64_t(sizeof(cg_adamw_tensor) / 8), n}, nullptr, c.dtype, partials, s);
+      sums = launch_norm(GradList{grads, &tensors[0].n, int64_t(sizeof(cg_adamw_tensor) / 8), n}, nullptr, c.dtype, streams, partials, s);
     if (sums == 0) zero_norm();
     int entry = 0;
     for (int at = 0; at < n;) {
@@ -604,7 +674,7 @@ int cg_adamw_step(const cg_adamw_tensor *tensors, const void *const *grads, int3
       a.sums = partials;
       a.norm = c.clip == CG_CLIP_NONE ? nullptr : norm;
       a.lr_device = c.lr_device;
-      a.lr = c.lr, a.beta1 = c.beta1, a.beta2 = c.beta2, a.weight_decay = c.weight_decay, a.max_norm = c.max_norm;
+      a.lr = c.lr, a.log_beta1 = std::log2(c.beta1), a.log_beta2 = std::log2(c.beta2), a.weight_decay = c.weight_decay, a.max_norm = c.max_norm;
       a.seed = c.seed;
       a.header = header;
       for (; at < n && a.tensors < PREPARE_TENSORS; ++at) {
@@ -624,18 +694,21 @@ int cg_adamw_step(const cg_adamw_tensor *tensors, const void *const *grads, int3
       return Tensor8{t.param, g, static_cast<uint8_t *>(t.exp_avg), static_cast<uint8_t *>(t.exp_avg_sq),
                      t.exp_avg_scale, t.exp_avg_sq_scale, t.n};
     };
-    const auto run = [&](auto kernel32, auto kernel8) {
+    const auto run = [&](auto type) {
+      using T = decltype(type);
       if (c.state_bits == 32)
-        launch_updates<decltype(kernel32), Tensor32, UPDATE_TENSORS>(kernel32, tensors, grads, n, c, header, s, wide);
+        launch_updates<Tensor32, UPDATE_TENSORS>(streams ? adamw_kernel<T, true> : adamw_kernel<T, false>, tensors, grads,
+                                                 n, c, header, s, wide);
       else
-        launch_updates<decltype(kernel8), Tensor8, UPDATE_TENSORS_8>(kernel8, tensors, grads, n, c, header, s, narrow);
+        launch_updates<Tensor8, UPDATE_TENSORS_8>(streams ? adamw8_kernel<T, true> : adamw8_kernel<T, false>, tensors,
+                                                  grads, n, c, header, s, narrow);
     };
     if (c.dtype == CG_F32)
-      run(adamw_kernel<float>, adamw8_kernel<float>);
+      run(float{});
     else if (c.dtype == CG_BF16)
-      run(adamw_kernel<bf16>, adamw8_kernel<bf16>);
+      run(bf16{});
     else
-      run(adamw_kernel<f16>, adamw8_kernel<f16>);
+      run(f16{});
   });
 }
 

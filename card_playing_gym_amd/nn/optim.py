@@ -28,6 +28,7 @@ from __future__ import annotations
 
 import array
 import ctypes
+import operator
 from contextlib import nullcontext
 from typing import Iterable, Sequence
 
@@ -42,6 +43,8 @@ MOMENT_BLOCK = 256  # elements of a tensor that share a scale
 _ptr = torch.Tensor.data_ptr
 _numel = torch.Tensor.numel
 _contiguous = torch.Tensor.is_contiguous
+_dtype = operator.attrgetter("dtype")
+_device_index = torch.Tensor.get_device  # -1 on the CPU
 
 
 def moment_blocks(n: int) -> int:
@@ -184,6 +187,7 @@ class AdamWPlan:
             raise ValueError("first is out of range")
         _check_apart([x for kind in (self.params, *kinds) for x in kind])
         self.seed, self.first = int(seed) & 0xFFFFFFFF, int(first)
+        self._device_index = self.params[0].get_device()
         self._shapes = [p.shape for p in self.params]
         self._addresses = list(map(_ptr, self.params))
         # Storage that the records below name, alive as long as they are (a captured step too).
@@ -200,19 +204,26 @@ class AdamWPlan:
         if len(grads) != len(self.params):
             raise ValueError(f"{len(self.params)} parameters but {len(grads)} gradients")
         shapes, present = self._shapes, grads
-        if any(g is None for g in grads):
+        try:
+            pointers = list(map(_ptr, grads))
+        except (TypeError, RuntimeError):  # some are None, or sparse
             shapes = [shape for shape, g in zip(shapes, grads) if g is not None]
             present = [g for g in grads if g is not None]
+            pointers = None
         if [g.shape for g in present] != shapes:
             raise ValueError("a gradient differs from its parameter in shape")
-        if any(g.dtype != self.dtype or g.device != self.device for g in present):
+        # (sets of types and devices: quicker than comparing them one by one)
+        if not set(map(_dtype, present)) <= {self.dtype} or not set(map(_device_index, present)) <= {self._device_index}:
             raise ValueError("a gradient differs from its parameter in type or device")
-        if any(g.layout != torch.strided for g in present) or not all(map(_contiguous, present)):
-            grads = _dense(grads)
-            present = [g for g in grads if g is not None]
-        if present is grads:
-            return _addresses(map(_ptr, grads)), grads
-        return _addresses([0 if g is None else _ptr(g) for g in grads]), grads
+        try:
+            dense = all(map(_contiguous, present))
+        except RuntimeError:  # sparse layouts have no strides to ask for
+            dense = False
+        if not dense:
+            grads, pointers = _dense(grads), None
+        if pointers is None:
+            pointers = [0 if g is None else _ptr(g) for g in grads]
+        return _addresses(pointers), grads
 
     def step(
         self,
