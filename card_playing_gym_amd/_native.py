@@ -140,6 +140,19 @@ class AdamWConfig(ctypes.Structure):
     ]
 
 
+class Scalar(ctypes.Structure):
+    _fields_ = [("value", c_float), ("device", c_void_p)]
+
+
+class PolicyLoss(ctypes.Structure):
+    _fields_ = [(name, c_void_p) for name in ("logits", "mask", "actions", "old_log_probs", "advantages", "weights",
+                                              "reference_logits", "reference_log_probs")] + [
+        ("ld_logits", c_int64), ("ld_mask", c_int64), ("ld_reference", c_int64), ("rows", c_int32), ("width", c_int32),
+        ("dtype", c_int32), ("clip_low", c_double), ("clip_high", c_double), ("normalizer", Scalar),
+        ("entropy_coef", Scalar), ("kl_coef", Scalar),
+    ]
+
+
 class LayerParams(ctypes.Structure):
     _fields_ = [
         ("ln_attn_w", c_void_p),
@@ -294,6 +307,11 @@ _SIGNATURES = {
          P(TrainGrads), c_void_p, c_void_p, c_void_p, c_void_p],
     ),
     "cg_attn_train_bwd": (c_int32, [P(AttnTrain), c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "cg_policy_loss_workspace_size": (c_size_t, []),
+    "cg_policy_loss_forward": (
+        c_int32, [P(PolicyLoss), c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p],
+    ),
+    "cg_policy_loss_backward": (c_int32, [P(PolicyLoss), c_void_p, c_int32, c_void_p, c_void_p]),
     "cg_grad_norm_workspace_size": (c_size_t, [c_int32]),
     "cg_grad_norm": (
         c_int32, [c_void_p, c_void_p, c_void_p, c_int32, c_void_p, c_void_p, c_size_t, c_void_p],

@@ -19,7 +19,7 @@ ROOT = PACKAGE.parent
 LIBRARY = PACKAGE / "libcardgym_hip.so"
 SOURCES = (
     "kv_ops.hip", "attention.hip", "gemm.hip", "layer.hip", "heads.hip", "sample.hip", "piquet.hip", "train.hip",
-    "trunk.hip", "optim.hip",
+    "trunk.hip", "loss.hip", "optim.hip",
 )
 ARCH = os.environ.get("CARDGYM_HIP_ARCH", "gfx950")
 

@@ -540,6 +540,49 @@ int cg_trunk_train_backward(const cg_train_config *c, const cg_train_block *bloc
                             size_t saved_size, void *scratch, size_t scratch_size, const cg_train_grads *grads,
                             float *dx, float *dple, float *dvalues, void *stream);
 
+/* ---- the policy loss ---------------------------------------------------------------------
+ * The clipped policy loss of an update over rows of logits, beside the masked softmax that the
+ * rollout sampled from (cg_masked_probabilities).  A row's legal entries are those its mask
+ * keeps and whose logit is above -inf; p is the softmax over them.  Per row
+ *   r = exp(log p[action] - old_log_prob)
+ *   l = -min(r A, clamp(r, clip_low, clip_high) A) + kl_coef KL - entropy_coef H
+ * with H = -sum p log p, and KL = sum p (log p - log q) for reference_logits (softmax q over
+ * the same mask) or exp(d) - d - 1, d = reference_log_prob - log p[action]; the value is
+ * sum_i w_i l_i / normalizer.  A row of weight 0 is not read; it and a row without a legal entry
+ * add nothing, have a zero gradient and report zeros.  An action outside [0, width) makes its row
+ * NaN; one that is not legal has log p = -inf (r = 0). */
+typedef struct {
+  float value;
+  const float *device; /* a device scalar in value's place, or NULL */
+} cg_scalar;
+
+typedef struct {
+  const void *logits;           /* [rows, width] of `dtype`, row stride ld_logits (elements) */
+  const uint8_t *mask;          /* [rows, width], 0 = not legal, row stride ld_mask; NULL: all legal */
+  const int64_t *actions;       /* [rows] */
+  const float *old_log_probs;   /* [rows] */
+  const float *advantages;      /* [rows] */
+  const float *weights;         /* [rows] or NULL: ones */
+  const void *reference_logits; /* [rows, width] of `dtype`, row stride ld_reference; or NULL */
+  const float *reference_log_probs; /* [rows] or NULL (at most one of the two references) */
+  int64_t ld_logits, ld_mask, ld_reference;
+  int32_t rows, width;
+  int32_t dtype; /* CG_F32, CG_BF16 or CG_F16 */
+  double clip_low, clip_high;
+  cg_scalar normalizer, entropy_coef, kl_coef;
+} cg_policy_loss;
+
+/* value[0], log_probs / entropy / kl [rows] (kl with a reference, else NULL) and, where grad is
+ * not NULL, the value's gradient [rows, width] dense, of `dtype`.  workspace: 8-byte aligned, of
+ * this call alone until it has run. */
+size_t cg_policy_loss_workspace_size(void);
+int cg_policy_loss_forward(const cg_policy_loss *loss, float *value, float *log_probs, float *entropy, float *kl,
+                           void *grad, void *workspace, size_t workspace_size, void *stream);
+/* grad [rows, width] = upstream[0] times the value's gradient, formed from the inputs and rounded
+ * once.  written != 0: grad holds the forward's, and stays as it is where upstream[0] is 1. */
+int cg_policy_loss_backward(const cg_policy_loss *loss, const float *upstream, int32_t written, void *grad,
+                            void *stream);
+
 /* ---- the optimiser step ------------------------------------------------------------------
  * What follows the training backward in an update: the gradients' global norm and one AdamW
  * step over many tensors (decoupled weight decay, bias-corrected moments), the work of

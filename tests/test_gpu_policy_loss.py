@@ -1,0 +1,489 @@
+"""The policy loss on the GPU (csrc/loss.hip, rl/policy.py) against float64.
+
+Bars, with u = 2^-24 and x = z - max <= 0: an entry's exponential takes the rounding of x, of its product
+with log2(e) (the constant's own rounding among them) and of the instruction, (3 |x| + 4) u of itself; a
+lane adds up to 32 of them in fp32 (32 u), the rest is fp64.  So
+    S is off by s = (3 m1 + 36) u of itself, m1 = sum p |x|, and so log p by s and u of its own rounding;
+    H, from sum e |x|, by (m2 + 40 m1 + 40) u, m2 = 3 sum p x^2, and u of itself;
+    p_j by (3 |x_j| + 4) u + s of itself, a row's coefficients by 16 u + s and the ratio's by its exponent's
+    error, and the gradient takes half a step of its type.
+The exact KL's terms p (log p - log q) are off by the error of p and by that of both normalisers, whose
+first-order effect on the sum of p is the error of the shift between them."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+from card_playing_gym_amd.nn import AdamW, Trunk, TrunkConfig
+from card_playing_gym_amd.rl import masked_probabilities, policy_loss, sample_rows
+from oracle import policy as ref
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0**-24
+HALF_STEP = {torch.float32: U, torch.bfloat16: 2.0**-8, torch.float16: 2.0**-11}
+TINY = {torch.float32: 2.0**-150, torch.bfloat16: 2.0**-134, torch.float16: 2.0**-25}  # half the smallest number
+DTYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+def make(device, rows, width, dtype, seed, masked=True, reference=None, weighted=False, scale=2.0):
+    """Device inputs; log-ratios of spread 0.15, so that about a sixth of the rows is clipped."""
+
+    rng = np.random.default_rng(seed)
+    logits = torch.from_numpy(rng.normal(size=(rows, width)) * scale).to(dtype)
+    mask = rng.random((rows, width)) < 0.5
+    actions = rng.integers(0, width, rows)
+    mask[np.arange(rows), actions] = True
+    z = logits.double().numpy()
+    legal = mask if masked else np.ones_like(mask)
+    logp = ref.log_softmax(z, legal)[np.arange(rows), actions]
+    given = {"logits": logits, "actions": torch.from_numpy(actions),
+             "old": torch.from_numpy(logp + rng.normal(size=rows) * 0.15).float(),
+             "advantages": torch.from_numpy(rng.normal(size=rows)).float()}
+    options = {"entropy_coef": 0.03}
+    if masked:
+        options["mask"] = torch.from_numpy(mask)
+    if weighted:
+        options["weights"] = torch.from_numpy(rng.random(rows) * (rng.random(rows) < 0.7)).float()
+    if reference:
+        options["kl_coef"] = 0.2
+    if reference == "logits":
+        options["reference_logits"] = (logits.float() + torch.from_numpy(rng.normal(size=z.shape) * 0.3).float()).to(dtype)
+    if reference == "sampled":
+        options["reference_log_probs"] = torch.from_numpy(logp + rng.normal(size=rows) * 0.2).float()
+    put = lambda x: x.to(device) if isinstance(x, torch.Tensor) else x  # noqa: E731
+    return {k: put(v) for k, v in given.items()}, {k: put(v) for k, v in options.items()}
+
+
+def run(given, options, upstream=None, leaf=None):
+    leaf = given["logits"].detach().requires_grad_() if leaf is None else leaf
+    out = policy_loss(leaf, given["actions"], given["old"], given["advantages"], **options)
+    loss = out.loss if upstream is None else out.loss * upstream
+    (grad,) = torch.autograd.grad(loss, leaf)
+    return out, grad
+
+
+def host(x):
+    return x.detach().double().cpu().numpy() if x.is_floating_point() else x.cpu().numpy()
+
+
+def expected(given, options):
+    numbers = {k: host(v) if isinstance(v, torch.Tensor) and v.dim() else float(v) for k, v in options.items()}
+    return ref.policy_loss(host(given["logits"]), host(given["actions"]), host(given["old"]), host(given["advantages"]),
+                           **numbers)
+
+
+def check(given, options, out, grad, upstream=1.0):
+    dtype = given["logits"].dtype
+    want = expected(given, options)
+    p, x = want["p"], np.abs(want["x"])
+    m1, m2 = (p * x).sum(1), 3 * (p * x * x).sum(1)
+    s = (3 * m1 + 36) * U
+    log_p = s + U * np.abs(want["log_probs"])
+    assert (np.abs(host(out.log_probs) - want["log_probs"]) <= log_p).all()
+    entropy = (m2 + 40 * m1 + 40) * U + U * want["entropy"]
+    assert (np.abs(host(out.entropy) - want["entropy"]) <= entropy).all()
+    kl = np.zeros_like(s)
+    if "reference_logits" in options:
+        gap = np.abs(want["gap"])
+        y = x + gap + gap.max(1, keepdims=True)  # as far as the reference's own x goes
+        shift = s + ((3 * (p * y).sum(1) + 36) + 4 * (x.max(1) + gap.max(1))) * U  # (its p is within a few times p)
+        kl = 4 * shift + (p * gap * ((3 * x + 4) * U + s[:, None])).sum(1) + 34 * U * (p * gap).sum(1)
+        assert (np.abs(host(out.kl) - want["kl"]) <= kl + U * want["kl"]).all()
+    elif "reference_log_probs" in options:
+        d = np.where(want["log_probs"] != 0, host(options["reference_log_probs"]) - want["log_probs"], 0.0)
+        kl = np.abs(np.expm1(d)) * s + s * s + U * want["kl"] + 1e-15
+        assert (np.abs(host(out.kl) - want["kl"]) <= kl).all()
+    else:
+        assert out.kl is None
+    weights = host(options["weights"]) if "weights" in options else np.ones(len(s))
+    normalizer = float(options.get("normalizer", len(s)))
+    f = weights / normalizer
+    c, beta = float(options["entropy_coef"]), float(options.get("kl_coef", 0.0))
+    loss = (f * (np.abs(want["own"]) * s * 2 + np.abs(host(given["advantages"])) * s + c * entropy + beta * kl)).sum()
+    assert abs(out.loss.item() - want["loss"]) <= loss + U * abs(want["loss"])
+    f = np.abs(f * upstream)[:, None]
+    own = np.abs(want["own"])[:, None]
+    bracket = c * (x + 2 * want["entropy"][:, None] + m1[:, None]) + beta * (np.abs(want["gap"]) + np.abs(want["kl"])[:, None]) + own
+    relative = (3 * x + 40) * U + 3 * s[:, None]
+    off = f * (p * bracket * relative + p * (c * entropy + beta * kl)[:, None])
+    rows = np.arange(len(s))
+    off[rows, host(given["actions"]) % p.shape[1]] += (f * own)[:, 0] * (2 * s + 16 * U)
+    target = want["grad"] * upstream
+    error = np.abs(host(grad) - target)
+    bar = off + HALF_STEP[dtype] * (np.abs(target) + off) + TINY[dtype]
+    assert (error <= bar).all(), (error / bar).max()
+    if "mask" in options:
+        assert (host(grad)[~host(options["mask"])] == 0).all()
+
+
+# Both sides of every width at which the kernel changes, odd widths, widths below one load's.
+WIDTHS = [1, 2, 3, 5, 7, 8, 9, 31, 63, 64, 65, 77, 127, 128, 129, 200, 256, 257, 511, 512, 513, 1000, 1024, 1025]
+
+
+@pytest.mark.parametrize("width", WIDTHS)
+@pytest.mark.parametrize("dtype", DTYPES, ids=["fp32", "bf16", "fp16"])
+def test_rows_of_each_width(device, dtype, width):
+    for k, reference in enumerate((None, "logits", "sampled")):
+        given, options = make(device, 37, width, dtype, seed=width + k, masked=k != 2, reference=reference, weighted=k > 0)
+        check(given, options, *run(given, options))
+
+
+@pytest.mark.parametrize("width", [2047, 2049, 4097, 8191, 8193, 16384, 16391, 32768, 32771, 70001])
+@pytest.mark.parametrize("dtype", DTYPES, ids=["fp32", "bf16", "fp16"])
+def test_wide_rows(device, dtype, width):
+    for k, reference in enumerate((None, "logits", "sampled")):
+        given, options = make(device, 3, width, dtype, seed=width + k, masked=k != 2, reference=reference)
+        check(given, options, *run(given, options))
+
+
+@pytest.mark.parametrize("rows, width", [(1, 40), (8200, 40), (2051, 130), (9001, 513), (2500, 2050)])
+def test_more_rows_than_a_launch_takes_at_a_time(device, rows, width):
+    given, options = make(device, rows, width, torch.bfloat16, seed=rows, reference="logits", weighted=True)
+    check(given, options, *run(given, options))
+
+
+@pytest.mark.parametrize("upstream", [1.0, -2.5, 0.0, 65536.0])
+@pytest.mark.parametrize("width", [40, 600, 40000])
+def test_upstream_gradients_are_rounded_once(device, width, upstream):
+    """Against float64 at the bars of one rounding, in fp16 too, whose small gradients a factor of 65536
+    brings into range."""
+
+    given, options = make(device, 6, width, torch.float16, seed=3, reference="sampled")
+    check(given, options, *run(given, options, upstream), upstream=upstream)
+
+
+def test_no_gradient_wanted(device):
+    given, options = make(device, 50, 40, torch.float32, seed=1)
+    with_grad, _ = run(given, options)
+    out = policy_loss(given["logits"], given["actions"], given["old"], given["advantages"], **options)
+    assert not out.loss.requires_grad and torch.equal(out.loss, with_grad.loss)
+    assert torch.equal(out.entropy, with_grad.entropy) and not with_grad.entropy.requires_grad
+
+
+@pytest.mark.parametrize("width", [40, 600, 3000, 40000])
+def test_rows_that_count_for_nothing(device, width):
+    """Rows without a legal entry (by mask, by -inf logits) and rows of weight 0 that hold NaN, an action far
+    outside and no mask: zeros, and the others as if alone."""
+
+    given, options = make(device, 8, width, torch.float32, seed=2, reference="logits", weighted=False)
+    options["weights"] = torch.ones(8, device=device)
+    alone = {k: v[:4].clone() for k, v in given.items()}
+    alone_options = {k: v[:4].clone() if isinstance(v, torch.Tensor) else v for k, v in options.items()}
+    want, want_grad = run(alone, {**alone_options, "normalizer": 8.0})
+    options["mask"][4] = False
+    given["logits"][5] = -torch.inf
+    given["logits"][6:] = torch.nan
+    given["old"][6:] = torch.nan
+    given["advantages"][7] = torch.inf
+    given["actions"][6], given["actions"][7] = -100, 2**40
+    options["weights"][6:] = 0
+    out, grad = run(given, options)
+    for got, expect in ((out.log_probs, want.log_probs), (out.entropy, want.entropy), (out.kl, want.kl), (grad, want_grad)):
+        assert torch.equal(got[:4], expect) and not got[4:].any()
+    assert torch.equal(out.loss, want.loss)
+    options["mask"][:] = False
+    out, grad = run(given, options)
+    assert out.loss == 0 and not grad.any() and not out.kl.any()
+
+
+@pytest.mark.parametrize("width", [40, 600, 3000, 40000])
+def test_masked_places_hold_anything(device, width):
+    """Infinities, NaN and the type's extremes in masked places change nothing, in either matrix."""
+
+    given, options = make(device, 5, width, torch.bfloat16, seed=6, reference="logits")
+    want, want_grad = run(given, options)
+    off = ~options["mask"]
+    low = torch.finfo(torch.bfloat16)
+    for value in (torch.nan, torch.inf, -torch.inf, low.max, low.min):
+        given["logits"][off] = value
+        options["reference_logits"][off] = value
+        out, grad = run(given, options)
+        assert torch.equal(out.loss, want.loss) and torch.equal(grad, want_grad) and torch.equal(out.kl, want.kl)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("width", [40, 600, 40000])
+def test_masks_by_the_types_lowest_value(device, dtype, width):
+    """Logits of finfo.min beside ordinary ones have p = 0 and no gradient; beside one another they are equal."""
+
+    given, options = make(device, 4, width, dtype, seed=8, masked=False)
+    hidden = torch.rand(4, width, device=device) < 0.5
+    hidden[torch.arange(4), given["actions"]] = False
+    given["logits"][hidden] = torch.finfo(dtype).min
+    given["logits"][3] = torch.finfo(dtype).min
+    given["old"][3] = -np.log(width)
+    out, grad = run(given, options)
+    assert torch.isfinite(out.loss) and torch.isfinite(grad).all() and not grad[:3][hidden[:3]].any()
+    assert abs(out.entropy[3].item() - np.log(width)) <= 4 * U * np.log(width)
+    assert abs(out.log_probs[3].item() + np.log(width)) <= 4 * U * np.log(width)
+    given["logits"][hidden] = -torch.inf
+    given["logits"][3] = 0
+    same, same_grad = run(given, options)
+    assert torch.equal(out.loss, same.loss) and torch.equal(grad, same_grad)
+
+
+@pytest.mark.parametrize("width", [40, 600, 40000])
+def test_values_that_are_not_finite_in_legal_places(device, width):
+    given, options = make(device, 6, width, torch.float32, seed=9, masked=False)
+    given["logits"][1, width // 2] = torch.nan
+    given["logits"][2, width // 3] = torch.inf
+    given["actions"][3] = width
+    given["actions"][4] = -1
+    out, grad = run(given, options)
+    bad = torch.tensor([False, True, True, True, True, False], device=device)
+    assert torch.isnan(out.loss) and torch.equal(torch.isnan(out.log_probs), bad)
+    assert torch.equal(torch.isnan(grad).any(1), bad) and torch.isfinite(grad[~bad]).all()
+
+
+def test_an_action_that_is_not_legal(device):
+    given, options = make(device, 3, 20, torch.float32, seed=10)
+    options["mask"][1, given["actions"][1]] = False
+    given["advantages"][1] = 1.5
+    out, grad = run(given, options)
+    want = expected(given, options)
+    assert out.log_probs[1] == -torch.inf and want["ratio"][1] == 0
+    assert abs(out.loss.item() - want["loss"]) < 1e-6
+    np.testing.assert_allclose(host(grad), want["grad"], atol=1e-7)
+
+
+def test_ends_of_the_clip_range(device):
+    """Ratios at 1 (old = log p exactly), far out on either side, and clip ranges of 0 and infinity."""
+
+    rows = 12
+    given, options = make(device, rows, 33, torch.float32, seed=11)
+    given["old"] += torch.linspace(-30, 30, rows, device=device)
+    for clip, clip_high in ((0.2, None), (0.0, None), (0.1, float("inf")), (1.0, 0.0)):
+        changed = {**options, "clip": clip, "clip_high": clip_high}
+        given["advantages"].neg_()
+        out, grad = run(given, changed)
+        want = expected(given, {**options, "clip": clip, **({} if clip_high is None else {"clip_high": clip_high})})
+        assert abs(out.loss.item() - want["loss"]) <= 1e-5 * abs(want["size"])
+        np.testing.assert_allclose(host(grad), want["grad"], rtol=2e-5, atol=1e-7)
+
+
+def test_gradient_is_the_difference_quotient(device):
+    """Of the device's own loss: the second difference of a smooth loss over h = 2^-7 is below 1e-3 of the
+    slope's scale, rounding of the loss 1e-7 / h."""
+
+    given, options = make(device, 2, 11, torch.float32, seed=12, masked=False, reference="logits")
+    given["advantages"][:] = torch.tensor([1.0, -1.0])
+    given["old"] += 0.0
+    options["clip"] = 10.0
+    _, grad = run(given, options)
+    h = 2.0**-7
+    call = lambda z: policy_loss(z, given["actions"], given["old"], given["advantages"], **options).loss.double()  # noqa: E731
+    for i in range(2):
+        for j in range(11):
+            step = torch.zeros_like(given["logits"])
+            step[i, j] = h
+            slope = (call(given["logits"] + step) - call(given["logits"] - step)) / (2 * h)
+            assert abs(slope.item() - grad[i, j].item()) < 1e-4
+
+
+def test_rows_at_any_stride_and_alignment(device):
+    given, options = make(device, 9, 130, torch.bfloat16, seed=13, reference="logits")
+    want, want_grad = run(given, options)
+    wide = {name: torch.full((9, 151), 3, dtype=t.dtype, device=device)
+            for name, t in (("logits", given["logits"]), ("mask", options["mask"]), ("ref", options["reference_logits"]))}
+    for shift in (0, 1, 7, 16):
+        cut = {name: t[:, shift : shift + 130] for name, t in wide.items()}
+        cut["logits"].copy_(given["logits"])
+        cut["mask"].copy_(options["mask"])
+        cut["ref"].copy_(options["reference_logits"])
+        out, grad = run({**given, "logits": cut["logits"]}, {**options, "mask": cut["mask"], "reference_logits": cut["ref"]})
+        assert torch.equal(out.loss, want.loss) and torch.equal(grad, want_grad)
+    columns = {name: t.t().contiguous().t() for name, t in (("logits", given["logits"]), ("mask", options["mask"]))}
+    every = lambda t: torch.stack([t, t], 1)[:, 0]  # noqa: E731
+    given2 = {name: every(t) for name, t in given.items() if name != "logits"}
+    out, grad = run({**given2, "logits": columns["logits"]}, {**options, "mask": columns["mask"]})
+    assert torch.equal(out.loss, want.loss) and torch.equal(grad, want_grad)
+
+
+def test_broadcast_inputs_and_shared_leaves(device):
+    """One row of logits and of the mask for all rows: its gradient is the sum of the rows'."""
+
+    given, options = make(device, 20, 33, torch.float32, seed=14)
+    leaf = given["logits"][:1].clone().requires_grad_()
+    options["mask"] = options["mask"][:1].expand(20, 33)
+    given["actions"] = given["actions"] * 0 + int(options["mask"][0].nonzero()[0])
+    call = lambda z: policy_loss(z, given["actions"], given["old"], given["advantages"], **options)  # noqa: E731
+    (grad,) = torch.autograd.grad(call(leaf.expand(20, 33)).loss, leaf)
+    out, each = run({**given, "logits": leaf.detach().expand(20, 33).contiguous()}, options)
+    assert torch.equal(call(leaf.expand(20, 33)).loss, out.loss)
+    assert torch.allclose(grad, each.sum(0, keepdim=True), rtol=1e-5, atol=1e-8)
+
+
+def test_scalars_on_the_device(device):
+    given, options = make(device, 30, 50, torch.float32, seed=15, reference="sampled")
+    options["normalizer"] = 64.0
+    want, want_grad = run(given, options)
+    on = {name: torch.tensor(options[name], device=device) for name in ("normalizer", "entropy_coef", "kl_coef")}
+    out, grad = run(given, {**options, **on})
+    assert torch.equal(out.loss, want.loss) and torch.equal(grad, want_grad)
+
+
+def test_backward_twice_and_inputs_that_changed(device):
+    given, options = make(device, 30, 50, torch.float32, seed=16)
+    leaf = given["logits"].clone().requires_grad_()
+    out = policy_loss(leaf, given["actions"], given["old"], given["advantages"], **options)
+    out.loss.backward(retain_graph=True)
+    first = leaf.grad.clone()
+    leaf.grad.mul_(7)  # (the tensor that the forward wrote)
+    (again,) = torch.autograd.grad(out.loss, leaf, retain_graph=True)
+    assert torch.equal(again, first)
+    given["advantages"].add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        torch.autograd.grad(out.loss, leaf)
+
+
+def test_no_rows(device):
+    empty = lambda dtype=torch.float32: torch.zeros(0, device=device, dtype=dtype)  # noqa: E731
+    leaf = torch.zeros((0, 5), device=device, requires_grad=True)
+    out = policy_loss(leaf, empty(torch.int64), empty(), empty())
+    (grad,) = torch.autograd.grad(out.loss, leaf)
+    assert out.loss == 0 and grad.shape == (0, 5) and out.log_probs.shape == (0,)
+
+
+def test_rows_past_32_bit_offsets(device):
+    """A matrix of over 2^31 entries of which a few rows at its end count."""
+
+    rows, width = 70000, 32768
+    free, _ = torch.cuda.mem_get_info(device)
+    if free < 24 * 2**30:
+        pytest.skip("needs 24 GiB of GPU memory")
+    few, options = make(device, 4, width, torch.bfloat16, seed=17, masked=False)
+    want, want_grad = run(few, {**options, "normalizer": float(rows)})
+    logits = torch.zeros((rows, width), dtype=torch.bfloat16, device=device)
+    logits[-4:] = few["logits"]
+    at_end = {name: torch.cat([few[name].new_zeros(rows - 4), few[name]]) for name in ("actions", "old", "advantages")}
+    weights = torch.zeros(rows, device=device)
+    weights[-4:] = 1
+    out, grad = run({"logits": logits, **at_end}, {**options, "weights": weights})
+    assert torch.equal(grad[-4:], want_grad) and not grad[:-4].any()
+    assert torch.allclose(out.loss, want.loss, rtol=2 * U)
+    assert torch.equal(out.log_probs[-4:], want.log_probs)
+
+
+def test_runs_repeat_bit_for_bit_on_any_stream(device):
+    given, options = make(device, 5000, 300, torch.bfloat16, seed=18, reference="logits")
+    want, want_grad = run(given, options)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    results = []
+    for stream in streams:  # three calls at once
+        with torch.cuda.stream(stream):
+            results.append(run(given, options))
+    torch.cuda.synchronize()
+    for out, grad in results:
+        assert torch.equal(out.loss, want.loss) and torch.equal(grad, want_grad) and torch.equal(out.kl, want.kl)
+
+
+@pytest.mark.parametrize("width", [40, 3000])
+def test_a_captured_loss(device, width):
+    """Forward and backward captured together; replays follow inputs, coefficients and the upstream
+    gradient, with eager calls and synchronisation between."""
+
+    given, options = make(device, 300, width, torch.float32, seed=19, reference="logits")
+    entropy_coef, upstream = torch.tensor(0.03, device=device), torch.tensor(1.0, device=device)
+    options["entropy_coef"] = entropy_coef
+    run(given, options, upstream)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    static = {k: v.clone() for k, v in given.items()}
+    leaf = static["logits"].requires_grad_()
+    with torch.cuda.graph(graph):
+        out, grad = run(static, options, upstream, leaf)
+    for k in range(4):
+        other, more = make(device, 300, width, torch.float32, seed=20 + k, reference="logits")
+        entropy_coef.fill_(0.01 * (k + 1))
+        upstream.fill_([1.0, 0.5, 1.0, -3.0][k])
+        with torch.no_grad():
+            for name in given:
+                static[name].copy_(other[name])
+            options["mask"].copy_(more["mask"])
+            options["reference_logits"].copy_(more["reference_logits"])
+        want, want_grad = run(other, {**more, "entropy_coef": entropy_coef}, upstream)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out.loss, want.loss) and torch.equal(grad, want_grad) and torch.equal(out.kl, want.kl)
+
+
+# ---- the update as a program runs it ------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("precision", ["fp32", "bf16"])
+def test_an_update_runs_end_to_end(device, precision, bits):
+    """Sampled actions, trunk forward, policy head, loss, backward, clipped step: three updates equal those
+    through the loss written in torch and, for 32-bit moments, torch.optim.AdamW after clip_grad_norm_, but
+    for rounding; padding rows count for nothing."""
+
+    torch.manual_seed(0)
+    config = TrunkConfig(d_model=64, n_layers=2, n_heads=4, n_kv_heads=2, d_ff=128)
+    trunk, head = Trunk(config).to(device), torch.nn.Linear(64, 50).to(device)
+    params = [*trunk.parameters(), *head.parameters()]
+    batch, length = 6, 20
+    x = torch.randn(batch, length, 64, device=device)
+    mask = torch.rand(batch * length, 50, device=device) < 0.4
+    mask[:, 0] = True
+    weights = (torch.rand(batch * length, device=device) < 0.8).float()
+    mask[weights == 0] = False
+    advantages = torch.randn(batch * length, device=device)
+    autocast = torch.autocast("cuda", dtype=torch.bfloat16, enabled=precision == "bf16")
+
+    def forward():
+        with autocast:
+            return head(trunk(*trunk.condition(x, None, None))).reshape(batch * length, 50)
+
+    with torch.no_grad():
+        probs = masked_probabilities(forward().float(), mask)
+        actions = sample_rows(probs.nan_to_num(0.0), mask, torch.rand(batch * length, device=device, dtype=torch.float64))
+        old = probs.gather(1, actions[:, None])[:, 0].log().nan_to_num(0.0)
+    start = [p.detach().clone() for p in params]
+
+    def ours(optimizer):
+        out = policy_loss(forward(), actions, old, advantages, mask=mask, weights=weights, entropy_coef=0.01,
+                          normalizer=weights.sum())
+        optimizer.zero_grad()
+        out.loss.backward()
+        optimizer.step()
+        return out.loss.item()
+
+    def theirs(optimizer):
+        live = weights != 0
+        z = forward().float()[live].masked_fill(~mask[live], -1e30)
+        logp = torch.log_softmax(z, 1)
+        ratio = (logp.gather(1, actions[live, None])[:, 0] - old[live]).exp()
+        a = advantages[live]
+        entropy = -(logp.exp() * logp.where(mask[live], torch.zeros((), device=device))).sum(1)
+        loss = (-torch.minimum(ratio * a, ratio.clamp(0.8, 1.2) * a) - 0.01 * entropy).mean()
+        optimizer.zero_grad()
+        loss.backward()
+        torch.nn.utils.clip_grad_norm_(params, 0.5)
+        optimizer.step()
+        return loss.item()
+
+    results = []
+    for run_one, make_optimizer in ((ours, lambda: AdamW(params, lr=1e-3, max_norm=0.5, state_bits=bits)),
+                                    (theirs, lambda: torch.optim.AdamW(params, lr=1e-3))):
+        with torch.no_grad():
+            for p, s in zip(params, start):
+                p.copy_(s)
+        optimizer = make_optimizer()
+        losses = [run_one(optimizer) for _ in range(3)]
+        assert all(torch.isfinite(p).all() for p in params)
+        results.append((losses, [p.detach().clone() for p in params]))
+    (a, pa), (b, pb) = results
+    # The first loss comes from equal parameters: fp32 sums of 100 rows, in another order.
+    assert abs(a[0] - b[0]) <= 1e-5
+    # A step moves a parameter by at most lr * 1.1 (Adam's bound at the first steps) and its decay.
+    assert max((x - y).abs().max().item() for x, y in zip(pa, start)) <= 3 * 1.2e-3 * 3
+    if bits == 32 and precision == "fp32":
+        # Entries with a gradient well above rounding take the same steps.
+        assert abs(a[2] - b[2]) <= 1e-4
+        close = torch.cat([((x - y).abs() <= 1e-4).flatten() for x, y in zip(pa, pb)])
+        assert close.float().mean() > 0.99
