@@ -27,7 +27,10 @@ namespace cg {
 namespace {
 
 constexpr int MAX_BLOCKS = 2048;  // and partial sums of the loss
-constexpr float LOG2E = 1.44269504088896340736f;
+// Logits and gradient of more bytes than this go past the caches (256 MB of Infinity Cache): 4096 rows of 32768
+// bf16 entries (537 MB) 135 -> 128 us.  Below, whatever made the logits or takes the gradient may find them there.
+constexpr int64_t STREAM_BYTES = 512 << 20;
+constexpr float LOG2E = 1.44269504088896340736f, LOG2E_REST = float(1.44269504088896340736 - double(LOG2E));
 constexpr float LOWEST = -1e30f;  // in place of the log-probability of an entry with p = 0 where p multiplies it
 
 struct Scalar {
@@ -51,6 +54,7 @@ struct LossArgs {
   float *loss;
   const float *upstream;  // of a backward call
   int32_t written;        // the gradient for an upstream of 1 is in place
+  int32_t streams;        // the logits and their gradient go past the caches (rows of 512 lanes and more)
 };
 
 // ---- a group of G lanes that share a row: reductions that leave the result in every lane ---------------
@@ -77,12 +81,10 @@ template <int G, typename X, typename Op>
 __device__ __forceinline__ X lanes_join(X x, Op op) {
   x = op(x, dpp<0xB1>(x));   // quad_perm [1, 0, 3, 2]
   x = op(x, dpp<0x4E>(x));   // quad_perm [2, 3, 0, 1]
-  x = op(x, dpp<0x141>(x));  // row_half_mirror
+  if constexpr (G > 4) x = op(x, dpp<0x141>(x));  // row_half_mirror
   if constexpr (G > 8) x = op(x, dpp<0x128>(x));  // row_ror:8
-  if constexpr (G > 16) {
-    x = op(x, __shfl_xor(x, 16, 64));
-    x = op(x, __shfl_xor(x, 32, 64));
-  }
+  if constexpr (G > 16) x = op(x, __shfl_xor(x, 16, 64));
+  if constexpr (G > 32) x = op(x, __shfl_xor(x, 32, 64));
   return x;
 }
 
@@ -99,12 +101,7 @@ __device__ __forceinline__ void join(X (&x)[N], X *slot, Op op) {
       for (int i = 0; i < N; ++i) slot[i * W + (threadIdx.x >> 6)] = x[i];
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      X s = slot[i * W];
-#pragma unroll
-      for (int w = 1; w < W; ++w) s = op(s, slot[i * W + w]);
-      x[i] = s;
-    }
+    for (int i = 0; i < N; ++i) x[i] = lanes_join<W>(slot[i * W + threadIdx.x % W], op);
   }
 }
 
@@ -115,68 +112,194 @@ struct Slots {
   double sums[3 * W], gaps[W];
 };
 
+// ---- exponentials and logarithms -------------------------------------------------------------------------
+
+// e^x for x <= 0 (-inf: 0), about an ulp and the rounding of the product.  FINE: what that rounding cuts off
+// comes back as a factor, for sums whose logarithms are then subtracted.
+template <bool FINE = false>
+__device__ __forceinline__ float exp_of(float x) {
+  const float t = x * LOG2E, e = __builtin_amdgcn_exp2f(t);
+  if constexpr (!FINE) return e;
+  const float cut = fmaf(x, LOG2E_REST, fmaf(x, LOG2E, -t));
+  return x > -126.f ? fmaf(e, cut * 0.69314718f, e) : e;  // (below it: inf - inf)
+}
+
+// Reciprocal of a normal number within an ulp or two: the instruction's 2^-26, squared twice.
+__device__ __forceinline__ double reciprocal(double x) {
+  double r = __builtin_amdgcn_rcp(x);
+  r = fma(fma(-x, r, 1.0), r, r);
+  return fma(fma(-x, r, 1.0), r, r);
+}
+
+// A constant formed where it is used, in scalar registers: the compiler keeps those of a loop's body in
+// vector registers around it, 60 of them here, and puts the row into scratch memory for that.
+__device__ __forceinline__ double here(double c) {
+  int lo = __double2loint(c), hi = __double2hiint(c);
+  asm volatile("" : "+s"(lo), "+s"(hi));
+  return __hiloint2double(hi, lo);
+}
+
+// log x = k log 2 + 2 atanh t for x = 2^k f, f in [1/sqrt 2, sqrt 2), t = (f - 1) / (f + 1): t^2 is below 0.0295,
+// so the series to t^15 is off by less than 1e-13.  x: positive and normal, or NaN.
+__device__ __forceinline__ double log_of(double x) {
+  int k = __builtin_amdgcn_frexp_exp(x);
+  double f = __builtin_amdgcn_frexp_mant(x);  // [1/2, 1)
+  const bool low = f < here(0.70710678118654752440);
+  f = low ? 2 * f : f;
+  k -= low;
+  const double t = (f - 1) * reciprocal(f + 1), u = t * t;
+  double p = here(2.0 / 15);
+  p = fma(p, u, here(2.0 / 13));
+  p = fma(p, u, here(2.0 / 11));
+  p = fma(p, u, here(2.0 / 9));
+  p = fma(p, u, here(2.0 / 7));
+  p = fma(p, u, here(2.0 / 5));
+  p = fma(p, u, here(2.0 / 3));
+  p = fma(p, u, 2.0);
+  return fma(double(k), here(0.69314718055994530942), t * p);
+}
+
+// e^x = 2^k e^r, |r| <= log(2) / 2: the series to r^11 is off by less than 1e-14 of it.
+__device__ __forceinline__ double exp_of(double x) {
+  x = x > 800 ? 800 : x < -800 ? -800 : x;  // infinity and 0 from here on; NaN stays
+  const double k = __builtin_rint(x * here(1.44269504088896340736));
+  const double r = fma(k, here(-2.3190468138462996e-17), fma(k, here(-0.69314718055994530942), x));
+  double p = here(1.0 / 39916800);
+  p = fma(p, r, here(1.0 / 3628800));
+  p = fma(p, r, here(1.0 / 362880));
+  p = fma(p, r, here(1.0 / 40320));
+  p = fma(p, r, here(1.0 / 5040));
+  p = fma(p, r, here(1.0 / 720));
+  p = fma(p, r, here(1.0 / 120));
+  p = fma(p, r, here(1.0 / 24));
+  p = fma(p, r, here(1.0 / 6));
+  p = fma(p, r, 0.5);
+  p = fma(p, r, 1.0);
+  p = fma(p, r, 1.0);
+  return __builtin_amdgcn_ldexp(p, int(k));
+}
+
 // ---- entries --------------------------------------------------------------------------------------------
 
 template <typename T>
 constexpr int VEC = 16 / sizeof(T);
 
-// VEC entries of a row from entry i on, -inf for those past its end or (mask) not legal.  Rows may start
-// anywhere: 16 bytes are loaded wherever they begin.  The vector over the row's end is loaded as the
-// row's last VEC entries, of which the vector before has the first.
 template <typename T>
-__device__ __forceinline__ void load_entries(float *z, const T *row, const uint8_t *legal, int i, int width) {
-  constexpr int V = VEC<T>;
-  if (i >= width) {
+constexpr uint32_t NEGATIVE_INFINITY = __is_same(T, float) ? 0xff800000u : __is_same(T, bf16) ? 0xff80ff80u : 0xfc00fc00u;
+
+// E entries as they are stored, four bytes a word.
+template <typename T, int E>
+struct Entries {
+  static constexpr int PER = 4 / sizeof(T), WORDS = E / PER;
+  uint32_t w[WORDS];
+  __device__ __forceinline__ void clear() {
 #pragma unroll
-    for (int k = 0; k < V; ++k) z[k] = -INFINITY;
-    return;
+    for (int j = 0; j < WORDS; ++j) w[j] = NEGATIVE_INFINITY<T>;
   }
-  if (width < V) {
-    for (int k = 0; k < V; ++k) {
-      z[k] = -INFINITY;
-      if (k < width && (!legal || legal[k])) z[k] = to_f32(row[k]);
+  // From here on what was formed of the entries is formed again: a row's exponentials, kept for the next
+  // pass over it, would take twice the registers of its entries.
+  __device__ __forceinline__ void forget() {
+    if constexpr (E > 1) {
+#pragma unroll
+      for (int j = 0; j < WORDS; ++j) asm volatile("" : "+v"(w[j]));
     }
-    return;
   }
-  const int at = i + V <= width ? i : width - V, seen = i - at;
-  T q[V];
-  __builtin_memcpy(q, row + at, sizeof q);
-  uint8_t b[V];
-  if (legal) __builtin_memcpy(b, legal + at, sizeof b);
-  float f[V];
-#pragma unroll
-  for (int k = 0; k < V; ++k) f[k] = !legal || b[k] ? to_f32(q[k]) : -INFINITY;
-  if (seen == 0) {
-#pragma unroll
-    for (int k = 0; k < V; ++k) z[k] = f[k];
+  __device__ __forceinline__ float operator[](int k) const {
+    if constexpr (PER == 1) {
+      return __uint_as_float(w[k]);
+    } else {
+      const uint32_t q = w[k / 2];
+      if constexpr (sizeof(T) == 2 && __is_same(T, bf16)) return __uint_as_float(k % 2 ? q & 0xffff0000u : q << 16);
+      return to_f32(T{uint16_t(k % 2 ? q >> 16 : q)});
+    }
+  }
+};
+
+typedef uint32_t Word4 __attribute__((ext_vector_type(4), aligned(2)));  // wherever a row begins
+
+// Four mask bytes: bit 7 of each byte set where the byte is not 0.
+__device__ __forceinline__ uint32_t nonzero_bytes(uint32_t b) { return ((b & 0x7f7f7f7fu) + 0x7f7f7f7fu) | b; }
+
+// A lane's entries of a row: vectors of V from entry (c G + lane) V on for c < C, -inf for those past the row's
+// end or not legal.  Rows may start anywhere: 16 bytes are loaded wherever they begin.  A vector over the
+// row's end is loaded as its last V entries, of which the first, that a vector before has, count as
+// -inf.  Rows shorter than 16 bytes are loaded entry by entry (V = 1) and kept as fp32.
+template <int G, int C, int V, typename T>
+__device__ __forceinline__ void load_entries(uint32_t *w, const T *row, const uint8_t *legal, int first, int width,
+                                             bool streams = false) {
+  constexpr int PER = 4 / sizeof(T);
+  constexpr uint32_t NONE = NEGATIVE_INFINITY<T>;
+  if constexpr (V == 1) {
+    w[0] = first < width && (!legal || legal[first]) ? __float_as_uint(to_f32(row[first])) : NEGATIVE_INFINITY<float>;
   } else {
-    // entry i + k is f[k + seen]
+    // inside(c): every lane's vector is (the same for the whole launch)
+    const auto inside = [&](int c) { return G > 1 && (c + 1) * G * V <= width; };
+    const auto at = [&](int c) { return inside(c) ? first + c * G * V : min(first + c * G * V, width - V); };
 #pragma unroll
-    for (int k = 0; k < V; ++k) {
-      z[k] = -INFINITY;
+    for (int c = 0; c < C; ++c) {
+      if (streams) {
+        const Word4 q = __builtin_nontemporal_load(reinterpret_cast<const Word4 *>(row + at(c)));
+        __builtin_memcpy(w + 4 * c, &q, 16);
+      } else {
+        __builtin_memcpy(w + 4 * c, row + at(c), 16);
+      }
+    }
+    if (legal) {
+      uint32_t b[C * (V / 4)];
 #pragma unroll
-      for (int s = 1; s < V; ++s)
-        if (k + s < V && seen == s) z[k] = f[k + s];
+      for (int c = 0; c < C; ++c) __builtin_memcpy(b + c * (V / 4), legal + at(c), V);
+#pragma unroll
+      for (int j = 0; j < C * (V / 4); ++j) {
+        if constexpr (PER == 1) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) w[4 * j + k] = b[j] >> 8 * k & 255 ? w[4 * j + k] : NONE;
+        } else {
+          // Sign bits of bytes 0 and 1, then 2 and 3, spread over a half each (v_perm_b32's selectors 8 to 11
+          // repeat the signs of bytes 1, 3, 5 and 7).
+          const uint32_t t = nonzero_bytes(b[j]);
+          const uint32_t lo = __builtin_amdgcn_perm(t << 8, t, 0x08080a0au), hi = __builtin_amdgcn_perm(t << 8, t, 0x09090b0bu);
+          w[2 * j] = (w[2 * j] & lo) | (NONE & ~lo);
+          w[2 * j + 1] = (w[2 * j + 1] & hi) | (NONE & ~hi);
+        }
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      if (inside(c)) continue;
+      const int seen = first + c * G * V - at(c);
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        const uint32_t part = PER == 1 ? ~0u : k % 2 ? 0xffff0000u : 0xffffu;
+        uint32_t &x = w[4 * c + k / PER];
+        x = k < seen ? (x & ~part) | (NONE & part) : x;
+      }
     }
   }
 }
 
-template <typename T>
-__device__ __forceinline__ void store_entries(T *row, const float *g, int i, int width) {
-  constexpr int V = VEC<T>;
-  if (i + V <= width) {
-    T q[V];
+// The gradients of a vector from entry i on.
+template <int V, typename T>
+__device__ __forceinline__ void store_entries(T *row, const float *g, int i, int width, bool inside, bool streams = false) {
+  if constexpr (V == 1) {
+    if (i < width) row[i] = from_f32<T>(g[0]);
+  } else if (inside || i + V <= width) {
+    Word4 q;
+    if constexpr (sizeof(T) == 4) {
+      __builtin_memcpy(&q, g, 16);
+    } else {
+      const u32x2 lo = cvt4<T>(f32x4{g[0], g[1], g[2], g[3]}), hi = cvt4<T>(f32x4{g[4], g[5], g[6], g[7]});
+      q = Word4{lo[0], lo[1], hi[0], hi[1]};
+    }
+    if (streams)
+      __builtin_nontemporal_store(q, reinterpret_cast<Word4 *>(row + i));
+    else
+      __builtin_memcpy(row + i, &q, 16);
+  } else if (i < width) {
 #pragma unroll
-    for (int k = 0; k < V; ++k) q[k] = from_f32<T>(g[k]);
-    __builtin_memcpy(row + i, q, sizeof q);
-  } else {
-#pragma unroll
-    for (int k = 0; k < V; ++k)
-      if (i + k < width) row[i + k] = from_f32<T>(g[k]);
+    for (int k = 1; k < V; ++k)
+      if (width - V + k >= i) row[width - V + k] = from_f32<T>(g[k]);
   }
 }
-
-__device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * LOG2E); }
 
 // ---- a row's scalars ---------------------------------------------------------------------------------------
 
@@ -194,42 +317,57 @@ struct RowScalars {
   bool live;
 };
 
+// What a row is beside its logits.
+struct RowInputs {
+  int64_t action;
+  float weight, old, advantage, ref;
+};
+__device__ __forceinline__ RowInputs row_inputs(const LossArgs &a, int64_t row) {
+  return RowInputs{a.actions[row], a.weights ? a.weights[row] : 1.f, a.old[row], a.advantages[row], a.ref ? a.ref[row] : 0.f};
+}
+struct Coefs {  // of the whole launch
+  double entropy, kl, scale;
+};
+
 // gap(shift): sum of e (z - y - shift), of the whole group (called by all of it).
 template <bool REF, typename Gap>
-__device__ __forceinline__ RowScalars row_scalars(const LossArgs &a, int64_t row, float action_logit, double weight,
-                                                  const RowSums &q, double scale, const Gap &gap) {
+__device__ __forceinline__ RowScalars row_scalars(const LossArgs &a, const RowInputs &in, float action_logit,
+                                                  const RowSums &q, const Coefs &k, const Gap &gap) {
   RowScalars o;
-  o.live = weight != 0 && q.s != 0;
-  const double log_s = log(q.s), c = read(a.entropy_coef), beta = read(a.kl_coef);
+  o.live = in.weight != 0 && q.s != 0;
+  const double log_s = log_of(q.s), inv = reciprocal(q.s), c = k.entropy, beta = k.kl;
+  double base = 0, kl = 0;
+  o.c.shift = 0;
+  if constexpr (REF) {
+    const double shift = (double(q.top) - double(q.ref_top)) + (log_s - log_of(q.ref_s));
+    o.c.shift = float(shift);
+    kl = gap(o.c.shift) * inv;
+  }
   o.log_p = (double(action_logit) - double(q.top)) - log_s;
-  o.entropy = log_s - q.t / q.s;
-  const double adv = a.advantages[row], r = exp(o.log_p - double(a.old[row]));
+  o.entropy = log_s - q.t * inv;
+  base = c * (o.entropy - log_s);
+  const double adv = in.advantage, r = exp_of(o.log_p - double(in.old));
   const double bounded = r < a.lo ? a.lo : r > a.hi ? a.hi : r;  // (NaN stays)
   const double whole = r * adv, part = bounded * adv;
   double value = -(part < whole ? part : whole) - c * o.entropy;
   double own = r == bounded || whole < part ? -whole : 0;
   if (whole != whole) own = value = whole;
-  double shift = 0, base = c * (o.entropy - log_s);
-  o.kl = 0;
   if constexpr (REF) {
-    shift = (double(q.top) - double(q.ref_top)) + (log_s - log(q.ref_s));
-    const double k = gap(float(shift)) / q.s;
-    o.kl = k;
-    value += beta * k;
-    base -= beta * k;
+    value += beta * kl;
+    base -= beta * kl;
   } else if (a.ref) {
-    const double d = double(a.ref[row]) - o.log_p, rise = expm1(d);
-    o.kl = rise == INFINITY ? rise : rise - d;
-    value += beta * o.kl;
+    const double d = double(in.ref) - o.log_p, rise = exp_of(d) - 1;
+    kl = rise == INFINITY ? rise : rise - d;
+    value += beta * kl;
     own -= beta * rise;
   }
-  const double f = weight * scale;
+  o.kl = kl;
+  const double weight = in.weight, f = weight * k.scale;
   o.value = weight * value;
   o.c.own = float(f * own);
-  o.c.base = float(f * (base - own) / q.s);
-  o.c.slope = float(f * c / q.s);
-  o.c.pull = REF ? float(f * beta / q.s) : 0.f;
-  o.c.shift = float(shift);
+  o.c.base = float(f * (base - own) * inv);
+  o.c.slope = float(f * c * inv);
+  o.c.pull = REF ? float(f * beta * inv) : 0.f;
   return o;
 }
 
@@ -237,9 +375,10 @@ __device__ __forceinline__ RowScalars row_scalars(const LossArgs &a, int64_t row
 struct Entry {
   float e, x;
 };
+template <bool FINE = false>
 __device__ __forceinline__ Entry entry_of(float z, float top) {
   const float x = z - top;
-  return Entry{exp_of(x), fmaxf(x, LOWEST)};  // (a NaN is kept by e)
+  return Entry{exp_of<FINE>(x), fmaxf(x, LOWEST)};  // (a NaN is kept by e)
 }
 template <bool REF>
 __device__ __forceinline__ float gap_of(float e, float z, float y, float shift) {
@@ -284,8 +423,8 @@ __global__ __launch_bounds__(256) void loss_kernel(const LossArgs a, int count) 
 // Whether this call has nothing to do: a backward whose gradient is in place already.
 __device__ __forceinline__ bool done(const LossArgs &a) { return a.upstream && a.written && *a.upstream == 1.0f; }
 
-__device__ __forceinline__ double scale_of(const LossArgs &a) {
-  return (a.upstream ? double(*a.upstream) : 1.0) / read(a.normalizer);
+__device__ __forceinline__ Coefs coefs_of(const LossArgs &a) {
+  return Coefs{read(a.entropy_coef), read(a.kl_coef), (a.upstream ? double(*a.upstream) : 1.0) / read(a.normalizer)};
 }
 
 // The action's logit; NaN for an action outside the row, -inf for one that is not legal.
@@ -298,33 +437,45 @@ __device__ __forceinline__ float logit_of(const LossArgs &a, int64_t row, int64_
 
 // ---- rows in registers: E entries a lane, G lanes a row, 256 / G rows a block at a time (one from 256 on) -----
 
-template <typename T, int G, int E, bool REF>
-__global__ __launch_bounds__(G > 256 ? G : 256) void rows_kernel(const LossArgs a) {
-  constexpr int V = VEC<T>, C = E / V, THREADS = G > 256 ? G : 256, ROWS = THREADS / G;
+// The waves of a SIMD that the registers have to leave room for.
+template <typename T, int G, int E, bool REF, int W = Entries<T, E>::WORDS * (REF ? 2 : 1)>
+constexpr int ROOM = G == 1024 ? (W <= 16 ? 8 : 4) : W <= 16 ? 6 : W < 32 ? 5 : 4;
+
+// S: the type in which entries are kept (T, or float where rows are shorter than a load).
+template <typename T, int G, int E, bool REF, typename S = T>
+__global__ __launch_bounds__((G > 256 ? G : 256), (ROOM<S, G, E, REF>)) void rows_kernel(const LossArgs a) {
+  constexpr int V = E == 1 ? 1 : VEC<T>, C = E / V, THREADS = G > 256 ? G : 256, ROWS = THREADS / G;
   if (done(a)) return;
   __shared__ Slots<G> slots;
-  const int lane = threadIdx.x % G;
-  const double scale = scale_of(a);
+  const Coefs coefs = coefs_of(a);
   double value = 0;
+  const int in_block = G == 64 ? __builtin_amdgcn_readfirstlane(threadIdx.x / 64) : int(threadIdx.x / G);
+  const auto row_of = [&](int64_t first) { return min(first + in_block, int64_t(a.rows) - 1); };
+  int64_t first = int64_t(blockIdx.x) * ROWS;
+  RowInputs next = row_inputs(a, row_of(first));
   // every thread of the block takes every turn: lanes of rows past the end have nothing live
-  for (int64_t first = int64_t(blockIdx.x) * ROWS; first < a.rows; first += int64_t(gridDim.x) * ROWS) {
-    const int64_t mine = first + threadIdx.x / G;
-    const bool in = mine < a.rows;
-    const int64_t row = in ? mine : a.rows - 1;
-    const double weight = !in ? 0.0 : a.weights ? double(a.weights[row]) : 1.0;
-    const int width = weight != 0 ? a.width : 0;  // rows without weight are not read
-    const int64_t action = a.actions[row];
+  for (; first < a.rows; first += int64_t(gridDim.x) * ROWS) {
+    int lane = threadIdx.x % G;
+    asm volatile("" : "+v"(lane));  // (what follows from it alone stays here: 60 masks, else, around the loop)
+    const bool in = first + in_block < a.rows;
+    const int64_t row = row_of(first);
+    RowInputs inputs = next;
+    next = row_inputs(a, row_of(first + int64_t(gridDim.x) * ROWS));
+    if (!in) inputs.weight = 0;
     const T *logits = static_cast<const T *>(a.logits) + row * a.ld_logits;
     const T *ref = static_cast<const T *>(a.ref_logits) + (REF ? row * a.ld_ref : 0);
     const uint8_t *legal = a.mask ? a.mask + row * a.ld_mask : nullptr;
-    float z[E], y[REF ? E : 1];
-#pragma unroll
-    for (int c = 0; c < C; ++c) load_entries(z + c * V, logits, legal, (c * G + lane) * V, width);
-    if constexpr (REF) {
-#pragma unroll
-      for (int c = 0; c < C; ++c) load_entries(y + c * V, ref, legal, (c * G + lane) * V, width);
+    Entries<S, E> z;
+    Entries<S, REF ? E : V> y;
+    float action_logit = 0;
+    const bool streams = G >= 512 && a.streams;
+    if (inputs.weight != 0) {  // rows without weight are not read
+      load_entries<G, C, V>(z.w, logits, legal, lane * V, a.width, streams);
+      if constexpr (REF) load_entries<G, C, V>(y.w, ref, legal, lane * V, a.width, streams);
+      action_logit = logit_of<T>(a, row, inputs.action);
+    } else {
+      z.clear(), y.clear();
     }
-    const float action_logit = width ? logit_of<T>(a, row, action) : 0.f;
     RowSums q;
     float tops[REF ? 2 : 1];
     tops[0] = z[0];
@@ -338,20 +489,22 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void rows_kernel(const LossArgs 
     join<G>(tops, slots.tops, Most{});
     q.top = tops[0] > -INFINITY ? tops[0] : 0.f;
     q.ref_top = REF && tops[REF ? 1 : 0] > -INFINITY ? tops[REF ? 1 : 0] : 0.f;
+    z.forget(), y.forget();
     float s = 0, t = 0, rs = 0;
 #pragma unroll
     for (int k = 0; k < E; ++k) {
-      const Entry n = entry_of(z[k], q.top);
+      const Entry n = entry_of<REF>(z[k], q.top);
       s += n.e;
       t = fmaf(n.e, n.x, t);
-      if (REF) rs += exp_of(y[REF ? k : 0] - q.ref_top);
+      if constexpr (REF) rs += exp_of<true>(y[k] - q.ref_top);
     }
     double sums[REF ? 3 : 2];
     sums[0] = s, sums[1] = t;
     if constexpr (REF) sums[2] = rs;
     join<G>(sums, slots.sums, Add{});
     q.s = sums[0], q.t = sums[1], q.ref_s = REF ? sums[REF ? 2 : 0] : 0;
-    const RowScalars o = row_scalars<REF>(a, row, action_logit, weight, q, scale, [&](float shift) {
+    z.forget(), y.forget();
+    const RowScalars o = row_scalars<REF>(a, inputs, action_logit, q, coefs, [&](float shift) {
       float g = 0;
 #pragma unroll
       for (int k = 0; k < E; ++k) {
@@ -362,6 +515,7 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void rows_kernel(const LossArgs 
       join<G>(gaps, slots.gaps, Add{});
       return gaps[0];
     });
+    z.forget(), y.forget();
     if (!in) continue;  // (all lanes of a group; the reductions are behind)
     if (lane == 0 && a.log_probs) {
       if (o.live) value += o.value;
@@ -371,15 +525,14 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void rows_kernel(const LossArgs 
       T *grad = static_cast<T *>(a.grad) + row * int64_t(a.width);
 #pragma unroll
       for (int c = 0; c < C; ++c) {
-        const int i = (c * G + lane) * V;
-        if (i >= a.width) break;
         float g[V];
 #pragma unroll
         for (int k = 0; k < V; ++k)
           g[k] = o.live ? grad_of<REF>(z[c * V + k], y[REF ? c * V + k : 0], q.top, o.c) : 0.f;
-        store_entries(grad, g, i, a.width);
+        store_entries<V>(grad, g, (c * G + lane) * V, a.width, (c + 1) * G * V <= a.width, streams);
       }
       // The action's own term, by the lane that has just written that entry.
+      const int64_t action = inputs.action;
       if (o.live && action >= 0 && action < a.width && action / V % G == lane) {
         const float yr = REF && action_logit > -INFINITY ? to_f32(ref[REF ? action : 0]) : 0.f;
         grad[action] = from_f32<T>(grad_of<REF>(action_logit, yr, q.top, o.c) + o.c.own);
@@ -392,59 +545,59 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void rows_kernel(const LossArgs 
 // ---- rows of any width: a block a row, read again for each pass ----------------------------------------------
 
 template <typename T, bool REF>
-__global__ __launch_bounds__(1024) void long_rows_kernel(const LossArgs a) {
+__global__ __launch_bounds__(1024, 4) void long_rows_kernel(const LossArgs a) {
   constexpr int V = VEC<T>, G = 1024;
   if (done(a)) return;
   __shared__ Slots<G> slots;
-  const double scale = scale_of(a);
+  const Coefs coefs = coefs_of(a);
   double value = 0;
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
-    const double weight = a.weights ? double(a.weights[row]) : 1.0;
-    const int width = weight != 0 ? a.width : 0;
-    const int64_t action = a.actions[row];
+    const RowInputs inputs = row_inputs(a, row);
+    const int width = inputs.weight != 0 ? a.width : 0;
+    const int64_t action = inputs.action;
     const T *logits = static_cast<const T *>(a.logits) + row * a.ld_logits;
     const T *ref = static_cast<const T *>(a.ref_logits) + (REF ? row * a.ld_ref : 0);
     const uint8_t *legal = a.mask ? a.mask + row * a.ld_mask : nullptr;
     const float action_logit = width ? logit_of<T>(a, row, action) : 0.f;
     const auto each = [&](const auto &visit) {  // visit(first entry, logits, reference logits)
       for (int64_t i = int64_t(threadIdx.x) * V; i < width; i += G * V) {
-        float z[V], y[V];
-        load_entries(z, logits, legal, int(i), width);
-        if (REF) load_entries(y, ref, legal, int(i), width);
+        Entries<T, V> z, y;
+        load_entries<1, 1, V>(z.w, logits, legal, int(i), width);
+        if constexpr (REF) load_entries<1, 1, V>(y.w, ref, legal, int(i), width);
         visit(int(i), z, y);
       }
     };
     RowSums q;
     float tops[REF ? 2 : 1];
     tops[0] = tops[REF ? 1 : 0] = -INFINITY;
-    each([&](int, const float *z, const float *y) {
+    each([&](int, const auto &z, const auto &y) {
 #pragma unroll
       for (int k = 0; k < V; ++k) {
         tops[0] = fmaxf(tops[0], z[k]);
-        if (REF) tops[REF ? 1 : 0] = fmaxf(tops[REF ? 1 : 0], y[k]);
+        if constexpr (REF) tops[1] = fmaxf(tops[1], y[k]);
       }
     });
     join<G>(tops, slots.tops, Most{});
     q.top = tops[0] > -INFINITY ? tops[0] : 0.f;
     q.ref_top = REF && tops[REF ? 1 : 0] > -INFINITY ? tops[REF ? 1 : 0] : 0.f;
     double sums[REF ? 3 : 2] = {};
-    each([&](int, const float *z, const float *y) {
+    each([&](int, const auto &z, const auto &y) {
       float s = 0, t = 0, rs = 0;
 #pragma unroll
       for (int k = 0; k < V; ++k) {
-        const Entry n = entry_of(z[k], q.top);
+        const Entry n = entry_of<REF>(z[k], q.top);
         s += n.e;
         t = fmaf(n.e, n.x, t);
-        if (REF) rs += exp_of(y[k] - q.ref_top);
+        if constexpr (REF) rs += exp_of<true>(y[k] - q.ref_top);
       }
       sums[0] += s, sums[1] += t;
-      if (REF) sums[REF ? 2 : 0] += rs;
+      if constexpr (REF) sums[2] += rs;
     });
     join<G>(sums, slots.sums, Add{});
     q.s = sums[0], q.t = sums[1], q.ref_s = REF ? sums[REF ? 2 : 0] : 0;
-    const RowScalars o = row_scalars<REF>(a, row, action_logit, weight, q, scale, [&](float shift) {
+    const RowScalars o = row_scalars<REF>(a, inputs, action_logit, q, coefs, [&](float shift) {
       double gaps[1] = {};
-      each([&](int, const float *z, const float *y) {
+      each([&](int, const auto &z, const auto &y) {
         float g = 0;
 #pragma unroll
         for (int k = 0; k < V; ++k) {
@@ -463,11 +616,11 @@ __global__ __launch_bounds__(1024) void long_rows_kernel(const LossArgs a) {
     if (!a.grad) continue;
     T *grad = static_cast<T *>(a.grad) + row * int64_t(a.width);
     if (o.live) {
-      each([&](int i, const float *z, const float *y) {
+      each([&](int i, const auto &z, const auto &y) {
         float g[V];
 #pragma unroll
-        for (int k = 0; k < V; ++k) g[k] = grad_of<REF>(z[k], y[k], q.top, o.c);
-        store_entries(grad, g, i, a.width);
+        for (int k = 0; k < V; ++k) g[k] = grad_of<REF>(z[k], REF ? y[k] : 0.f, q.top, o.c);
+        store_entries<V>(grad, g, i, a.width, false);
       });
       if (action >= 0 && action < a.width && action / V % G == threadIdx.x) {
         const float yr = REF && action_logit > -INFINITY ? to_f32(ref[REF ? action : 0]) : 0.f;
@@ -475,7 +628,7 @@ __global__ __launch_bounds__(1024) void long_rows_kernel(const LossArgs a) {
       }
     } else {
       const float zero[V] = {};
-      for (int64_t i = int64_t(threadIdx.x) * V; i < a.width; i += G * V) store_entries(grad, zero, int(i), a.width);
+      for (int64_t i = int64_t(threadIdx.x) * V; i < a.width; i += G * V) store_entries<V>(grad, zero, int(i), a.width, false);
     }
   }
   if (a.log_probs) block_loss(a, value);
@@ -488,31 +641,45 @@ struct Launch {
   int rows, threads;  // rows a block takes at a time
 };
 
+template <typename T, int G, int E, bool REF, typename S = T>
+Launch launch_as() {
+  return {rows_kernel<T, G, E, REF, S>, G > 256 ? 1 : 256 / G, G > 256 ? G : 256};
+}
+
 template <typename T, bool REF>
-Launch launch_of(int width) {
-  if (width <= 64) return {rows_kernel<T, 8, 8, REF>, 32, 256};
-  if (width <= 128) return {rows_kernel<T, 16, 8, REF>, 16, 256};
-  if (width <= 256) return {rows_kernel<T, 16, 16, REF>, 16, 256};
-  if (width <= 512) return {rows_kernel<T, 64, 8, REF>, 4, 256};
-  if (width <= 1024) return {rows_kernel<T, 64, 16, REF>, 4, 256};
-  if (width <= 2048) return {rows_kernel<T, 256, 8, REF>, 1, 256};
-  if (width <= 4096) return {rows_kernel<T, 256, 16, REF>, 1, 256};
-  if (width <= 8192) return {rows_kernel<T, 256, 32, REF>, 1, 256};
-  if (width <= 16384) return {rows_kernel<T, 1024, 16, REF>, 1, 1024};
-  if (width <= 32768) return {rows_kernel<T, 1024, 32, REF>, 1, 1024};
+Launch launch_of(int width, int rows) {
+  if (width < VEC<T>) return launch_as<T, 8, 1, REF, float>();
+  if (width <= 32) return launch_as<T, 4, 8, REF>();
+  if (width <= 64) return launch_as<T, 4, 16, REF>();
+  if (width <= 96) return launch_as<T, 4, 24, REF>();
+  if (width <= 128) return launch_as<T, 4, 32, REF>();
+  if (width <= 192) return launch_as<T, 8, 24, REF>();
+  if (width <= 256) return launch_as<T, 8, 32, REF>();
+  if (width <= 512) return rows <= 8192 ? launch_as<T, 32, 16, REF>() : launch_as<T, 16, 32, REF>();
+  if (width <= 1024) return rows <= 8192 ? launch_as<T, 64, 16, REF>() : launch_as<T, 32, 32, REF>();
+  if (width <= 2048) return launch_as<T, 64, 32, REF>();
+  if (width <= 4096) return launch_as<T, 256, 16, REF>();
+  if (width <= 8192) return launch_as<T, 256, 32, REF>();
+  if (width <= 16384) return launch_as<T, 512, 32, REF>();
+  if constexpr (sizeof(T) == 2) {
+    if (width <= 32768) return launch_as<T, 512, 64, REF>();
+    if (width <= 65536) return launch_as<T, 1024, 64, REF>();
+  } else if (width <= 32768) {
+    return launch_as<T, 1024, 32, REF>();
+  }
   return {long_rows_kernel<T, REF>, 1, 1024};
 }
 
 template <typename T>
-Launch launch_of(int width, bool ref) {
-  return ref ? launch_of<T, true>(width) : launch_of<T, false>(width);
+Launch launch_of(const cg_policy_loss &p, bool ref) {
+  return ref ? launch_of<T, true>(p.width, p.rows) : launch_of<T, false>(p.width, p.rows);
 }
 
 Launch launch_of(const cg_policy_loss &p) {
   const bool ref = p.reference_logits != nullptr;
-  return p.dtype == CG_F32    ? launch_of<float>(p.width, ref)
-         : p.dtype == CG_BF16 ? launch_of<bf16>(p.width, ref)
-                              : launch_of<f16>(p.width, ref);
+  return p.dtype == CG_F32    ? launch_of<float>(p, ref)
+         : p.dtype == CG_BF16 ? launch_of<bf16>(p, ref)
+                              : launch_of<f16>(p, ref);
 }
 
 int grid_of(const cg_policy_loss &p, const Launch &l) {
@@ -538,6 +705,7 @@ LossArgs args_of(const cg_policy_loss *loss) {
   a.ld_logits = p.ld_logits, a.ld_ref = p.ld_reference, a.ld_mask = p.ld_mask;
   a.rows = p.rows, a.width = p.width;
   a.lo = p.clip_low, a.hi = p.clip_high;
+  a.streams = int64_t(p.rows) * p.width > STREAM_BYTES / (2 * dtype_size(p.dtype));
   a.normalizer = scalar(p.normalizer), a.entropy_coef = scalar(p.entropy_coef), a.kl_coef = scalar(p.kl_coef);
   return a;
 }

@@ -51,7 +51,8 @@ def require_device(*tensors: torch.Tensor | None) -> None:
 
 
 def stream_handle(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    # The handle of torch.cuda.current_stream(device), without the stream object around it.
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if device.index is None else device.index)
 
 
 def index_tensor(values, device: torch.device) -> torch.Tensor:

@@ -10,7 +10,7 @@ rollout (cardgym/rl/ppo.py:75-94): the same softmax over a row's legal entries, 
 
 from __future__ import annotations
 
-import ctypes
+from functools import lru_cache
 from typing import NamedTuple
 
 import torch
@@ -64,19 +64,23 @@ class _Call:
     def forward(self, grad: torch.Tensor | None) -> torch.Tensor:
         device, rows = self.logits.device, self.logits.shape[0]
         loss = torch.empty((), device=device)
-        stats = torch.empty((3, rows), device=device)
-        self.log_probs, self.entropy, kl = stats.unbind(0)
-        has_kl = self.tensors[5] is not None or self.tensors[6] is not None
-        self.kl = kl if has_kl else None
-        size = nat.lib().cg_policy_loss_workspace_size()
+        self.log_probs = torch.empty(rows, device=device)
+        self.entropy = torch.empty(rows, device=device)
+        self.kl = None if self.tensors[5] is None and self.tensors[6] is None else torch.empty(rows, device=device)
+        size = _workspace_size()
         workspace = torch.empty(size, device=device, dtype=torch.uint8)
         with _on(device):
             nat.call(
-                "cg_policy_loss_forward", ctypes.byref(self.descriptor), loss.data_ptr(), self.log_probs.data_ptr(),
-                self.entropy.data_ptr(), kl.data_ptr() if has_kl else None, None if grad is None else grad.data_ptr(),
-                workspace.data_ptr(), size, stream_handle(device),
+                "cg_policy_loss_forward", self.descriptor, loss.data_ptr(), self.log_probs.data_ptr(),
+                self.entropy.data_ptr(), None if self.kl is None else self.kl.data_ptr(),
+                None if grad is None else grad.data_ptr(), workspace.data_ptr(), size, stream_handle(device),
             )
         return loss
+
+
+@lru_cache(maxsize=1)
+def _workspace_size() -> int:
+    return nat.lib().cg_policy_loss_workspace_size()
 
 
 class PolicyLossFunction(torch.autograd.Function):
@@ -85,14 +89,16 @@ class PolicyLossFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, logits, call):
+        # (call.logits is what the kernel reads: logits, or its copy with the entries side by side)
         ctx.written = torch.empty(logits.shape, device=logits.device, dtype=logits.dtype)
         ctx.save_for_backward(call.logits, *call.tensors)
         ctx.call = call
         return call.forward(ctx.written)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, upstream):
+        if torch.is_grad_enabled():  # (create_graph; once_differentiable costs 13 us of a small loss's 96)
+            raise RuntimeError("policy_loss is differentiable once: its gradient has no graph")
         call = ctx.call
         logits = ctx.saved_tensors[0]  # (an input changed since the forward raises here)
         grad, ctx.written = ctx.written, None  # handed over once: a second backward forms its own
@@ -101,7 +107,7 @@ class PolicyLossFunction(torch.autograd.Function):
             grad = torch.empty(logits.shape, device=logits.device, dtype=logits.dtype)
         upstream = upstream.contiguous()
         with _on(logits.device):
-            nat.call("cg_policy_loss_backward", ctypes.byref(call.descriptor), upstream.data_ptr(), int(written),
+            nat.call("cg_policy_loss_backward", call.descriptor, upstream.data_ptr(), int(written),
                      grad.data_ptr(), stream_handle(logits.device))
         return grad, None
 
@@ -182,7 +188,7 @@ def policy_loss(
             scalars.append(nat.Scalar(x, None))
     tensors = (actions.contiguous(), old_log_probs.contiguous(), advantages.contiguous(),
                None if weights is None else weights.contiguous(), mask, reference_logits, reference_log_probs, *kept)
-    entries = _rows(logits.detach())
+    entries = logits if logits.stride(1) == 1 else logits.detach().contiguous()
     call = _Call(entries, tensors, (1.0 - clip, 1.0 + clip_high, *scalars))
     if torch.is_grad_enabled() and logits.requires_grad:
         loss = PolicyLossFunction.apply(logits, call)

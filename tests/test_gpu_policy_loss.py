@@ -339,6 +339,14 @@ def test_backward_twice_and_inputs_that_changed(device):
         torch.autograd.grad(out.loss, leaf)
 
 
+def test_a_second_derivative_is_refused(device):
+    given, options = make(device, 3, 8, torch.float32, seed=16)
+    leaf = given["logits"].clone().requires_grad_()
+    out = policy_loss(leaf, given["actions"], given["old"], given["advantages"], **options)
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        torch.autograd.grad(out.loss, leaf, create_graph=True)
+
+
 def test_no_rows(device):
     empty = lambda dtype=torch.float32: torch.zeros(0, device=device, dtype=dtype)  # noqa: E731
     leaf = torch.zeros((0, 5), device=device, requires_grad=True)
