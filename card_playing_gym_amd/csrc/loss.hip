@@ -341,7 +341,7 @@ __device__ __forceinline__ RowScalars row_scalars(const LossArgs &a, const RowIn
   if constexpr (REF) {
     const double shift = (double(q.top) - double(q.ref_top)) + (log_s - log_of(q.ref_s));
     o.c.shift = float(shift);
-    kl = gap(o.c.shift) * inv;
+    kl = gap(o.c.shift) * inv - (shift - double(o.c.shift));  // (p sums to 1)
   }
   o.log_p = (double(action_logit) - double(q.top)) - log_s;
   o.entropy = log_s - q.t * inv;
@@ -370,6 +370,19 @@ __device__ __forceinline__ RowScalars row_scalars(const LossArgs &a, const RowIn
   o.c.pull = REF ? float(f * beta * inv) : 0.f;
   return o;
 }
+
+// A lane's sum of exponentials: in fp64 where the logarithms of two rows' sums are subtracted, to a tenth
+// of what either is.
+template <bool REF>
+struct SumType {
+  using type = float;
+};
+template <>
+struct SumType<true> {
+  using type = double;
+};
+template <bool REF>
+using Sum = typename SumType<REF>::type;
 
 // x = z - top and its exponential.  The product of an entry of p = 0 with its x is 0, never 0 * inf.
 struct Entry {
@@ -490,7 +503,8 @@ __global__ __launch_bounds__((G > 256 ? G : 256), (ROOM<S, G, E, REF>)) void row
     q.top = tops[0] > -INFINITY ? tops[0] : 0.f;
     q.ref_top = REF && tops[REF ? 1 : 0] > -INFINITY ? tops[REF ? 1 : 0] : 0.f;
     z.forget(), y.forget();
-    float s = 0, t = 0, rs = 0;
+    Sum<REF> s = 0, rs = 0;
+    float t = 0;
 #pragma unroll
     for (int k = 0; k < E; ++k) {
       const Entry n = entry_of<REF>(z[k], q.top);
@@ -508,7 +522,7 @@ __global__ __launch_bounds__((G > 256 ? G : 256), (ROOM<S, G, E, REF>)) void row
       float g = 0;
 #pragma unroll
       for (int k = 0; k < E; ++k) {
-        const float e = exp_of(z[k] - q.top);
+        const float e = exp_of<true>(z[k] - q.top);
         g = fmaf(e, gap_of<REF>(e, z[k], y[REF ? k : 0], shift), g);
       }
       double gaps[1] = {g};
@@ -582,7 +596,8 @@ __global__ __launch_bounds__(1024, 4) void long_rows_kernel(const LossArgs a) {
     q.ref_top = REF && tops[REF ? 1 : 0] > -INFINITY ? tops[REF ? 1 : 0] : 0.f;
     double sums[REF ? 3 : 2] = {};
     each([&](int, const auto &z, const auto &y) {
-      float s = 0, t = 0, rs = 0;
+      Sum<REF> s = 0, rs = 0;
+      float t = 0;
 #pragma unroll
       for (int k = 0; k < V; ++k) {
         const Entry n = entry_of<REF>(z[k], q.top);
@@ -601,7 +616,7 @@ __global__ __launch_bounds__(1024, 4) void long_rows_kernel(const LossArgs a) {
         float g = 0;
 #pragma unroll
         for (int k = 0; k < V; ++k) {
-          const float e = exp_of(z[k] - q.top);
+          const float e = exp_of<true>(z[k] - q.top);
           g = fmaf(e, gap_of<REF>(e, z[k], y[k], shift), g);
         }
         gaps[0] += g;
