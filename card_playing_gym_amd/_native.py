@@ -307,11 +307,13 @@ _SIGNATURES = {
          P(TrainGrads), c_void_p, c_void_p, c_void_p, c_void_p],
     ),
     "cg_attn_train_bwd": (c_int32, [P(AttnTrain), c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
-    "cg_policy_loss_workspace_size": (c_size_t, []),
+    "cg_policy_loss_workspace_size": (c_size_t, [P(PolicyLoss)]),
     "cg_policy_loss_forward": (
         c_int32, [P(PolicyLoss), c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p],
     ),
-    "cg_policy_loss_backward": (c_int32, [P(PolicyLoss), c_void_p, c_int32, c_void_p, c_void_p]),
+    "cg_policy_loss_backward": (
+        c_int32, [P(PolicyLoss), c_void_p, c_int32, c_void_p, c_void_p, c_size_t, c_void_p],
+    ),
     "cg_grad_norm_workspace_size": (c_size_t, [c_int32]),
     "cg_grad_norm": (
         c_int32, [c_void_p, c_void_p, c_void_p, c_int32, c_void_p, c_void_p, c_size_t, c_void_p],

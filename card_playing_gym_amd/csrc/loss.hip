@@ -54,6 +54,8 @@ struct LossArgs {
   float *loss;
   const float *upstream;  // of a backward call
   int32_t written;        // the gradient for an upstream of 1 is in place
+  double *parts;          // of split rows: SPLIT_PARTS for each segment
+  int32_t splits, segment;  // segments of a row, and entries of one
   int32_t streams;        // the logits and their gradient go past the caches (rows of 512 lanes and more)
 };
 
@@ -329,6 +331,11 @@ struct Coefs {  // of the whole launch
   double entropy, kl, scale;
 };
 
+// log p - log q is z - y less this.
+__device__ __forceinline__ double shift_of(const RowSums &q, double log_s) {
+  return (double(q.top) - double(q.ref_top)) + (log_s - log_of(q.ref_s));
+}
+
 // gap(shift): sum of e (z - y - shift), of the whole group (called by all of it).
 template <bool REF, typename Gap>
 __device__ __forceinline__ RowScalars row_scalars(const LossArgs &a, const RowInputs &in, float action_logit,
@@ -339,7 +346,7 @@ __device__ __forceinline__ RowScalars row_scalars(const LossArgs &a, const RowIn
   double base = 0, kl = 0;
   o.c.shift = 0;
   if constexpr (REF) {
-    const double shift = (double(q.top) - double(q.ref_top)) + (log_s - log_of(q.ref_s));
+    const double shift = shift_of(q, log_s);
     o.c.shift = float(shift);
     kl = gap(o.c.shift) * inv - (shift - double(o.c.shift));  // (p sums to 1)
   }
@@ -556,7 +563,83 @@ __global__ __launch_bounds__((G > 256 ? G : 256), (ROOM<S, G, E, REF>)) void row
   if (a.log_probs) block_loss(a, value);
 }
 
-// ---- rows of any width: a block a row, read again for each pass ----------------------------------------------
+// ---- passes over a row, or a segment of one, that is read again for each --------------------------------------
+//
+// each(visit): calls visit(first entry, logits, reference logits) for this thread's vectors.
+
+template <int G, int V, bool REF, typename Each>
+__device__ __forceinline__ void row_sums(const Each &each, Slots<G> &slots, RowSums &q) {
+  float tops[REF ? 2 : 1];
+  tops[0] = tops[REF ? 1 : 0] = -INFINITY;
+  each([&](int, const auto &z, const auto &y) {
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      tops[0] = fmaxf(tops[0], z[k]);
+      if constexpr (REF) tops[1] = fmaxf(tops[1], y[k]);
+    }
+  });
+  join<G>(tops, slots.tops, Most{});
+  q.top = tops[0] > -INFINITY ? tops[0] : 0.f;
+  q.ref_top = REF && tops[REF ? 1 : 0] > -INFINITY ? tops[REF ? 1 : 0] : 0.f;
+  double sums[REF ? 3 : 2] = {};
+  each([&](int, const auto &z, const auto &y) {
+    Sum<REF> s = 0, rs = 0;
+    float t = 0;
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      const Entry n = entry_of<REF>(z[k], q.top);
+      s += n.e;
+      t = fmaf(n.e, n.x, t);
+      if constexpr (REF) rs += exp_of<true>(y[k] - q.ref_top);
+    }
+    sums[0] += s, sums[1] += t;
+    if constexpr (REF) sums[2] += rs;
+  });
+  join<G>(sums, slots.sums, Add{});
+  q.s = sums[0], q.t = sums[1], q.ref_s = REF ? sums[REF ? 2 : 0] : 0;
+}
+
+template <int G, int V, typename Each>
+__device__ __forceinline__ double gap_sum(const Each &each, Slots<G> &slots, const RowSums &q, float shift) {
+  double gaps[1] = {};
+  each([&](int, const auto &z, const auto &y) {
+    float g = 0;
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      const float e = exp_of<true>(z[k] - q.top);
+      g = fmaf(e, gap_of<true>(e, z[k], y[k], shift), g);
+    }
+    gaps[0] += g;
+  });
+  join<G>(gaps, slots.gaps, Add{});
+  return gaps[0];
+}
+
+// The gradient of entries [begin, end) of a row, by `threads` threads.
+template <typename T, bool REF, typename Each>
+__device__ __forceinline__ void row_grads(const LossArgs &a, T *grad, const T *ref, int64_t action, float action_logit,
+                                          float top, const RowScalars &o, const Each &each, int begin, int end,
+                                          int threads) {
+  constexpr int V = VEC<T>;
+  if (o.live) {
+    each([&](int i, const auto &z, const auto &y) {
+      float g[V];
+#pragma unroll
+      for (int k = 0; k < V; ++k) g[k] = grad_of<REF>(z[k], REF ? y[k] : 0.f, top, o.c);
+      store_entries<V>(grad, g, i, a.width, false);
+    });
+    if (action >= begin && action < end && int(action - begin) / V % threads == int(threadIdx.x)) {
+      const float yr = REF && action_logit > -INFINITY ? to_f32(ref[REF ? action : 0]) : 0.f;
+      grad[action] = from_f32<T>(grad_of<REF>(action_logit, yr, top, o.c) + o.c.own);
+    }
+  } else {
+    const float zero[V] = {};
+    for (int64_t i = begin + int64_t(threadIdx.x) * V; i < end; i += threads * V)
+      store_entries<V>(grad, zero, int(i), a.width, false);
+  }
+}
+
+// ---- rows of any width: a block a row -------------------------------------------------------------------------
 
 template <typename T, bool REF>
 __global__ __launch_bounds__(1024, 4) void long_rows_kernel(const LossArgs a) {
@@ -568,12 +651,11 @@ __global__ __launch_bounds__(1024, 4) void long_rows_kernel(const LossArgs a) {
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const RowInputs inputs = row_inputs(a, row);
     const int width = inputs.weight != 0 ? a.width : 0;
-    const int64_t action = inputs.action;
     const T *logits = static_cast<const T *>(a.logits) + row * a.ld_logits;
     const T *ref = static_cast<const T *>(a.ref_logits) + (REF ? row * a.ld_ref : 0);
     const uint8_t *legal = a.mask ? a.mask + row * a.ld_mask : nullptr;
-    const float action_logit = width ? logit_of<T>(a, row, action) : 0.f;
-    const auto each = [&](const auto &visit) {  // visit(first entry, logits, reference logits)
+    const float action_logit = width ? logit_of<T>(a, row, inputs.action) : 0.f;
+    const auto each = [&](const auto &visit) {
       for (int64_t i = int64_t(threadIdx.x) * V; i < width; i += G * V) {
         Entries<T, V> z, y;
         load_entries<1, 1, V>(z.w, logits, legal, int(i), width);
@@ -582,71 +664,99 @@ __global__ __launch_bounds__(1024, 4) void long_rows_kernel(const LossArgs a) {
       }
     };
     RowSums q;
-    float tops[REF ? 2 : 1];
-    tops[0] = tops[REF ? 1 : 0] = -INFINITY;
-    each([&](int, const auto &z, const auto &y) {
-#pragma unroll
-      for (int k = 0; k < V; ++k) {
-        tops[0] = fmaxf(tops[0], z[k]);
-        if constexpr (REF) tops[1] = fmaxf(tops[1], y[k]);
-      }
-    });
-    join<G>(tops, slots.tops, Most{});
-    q.top = tops[0] > -INFINITY ? tops[0] : 0.f;
-    q.ref_top = REF && tops[REF ? 1 : 0] > -INFINITY ? tops[REF ? 1 : 0] : 0.f;
-    double sums[REF ? 3 : 2] = {};
-    each([&](int, const auto &z, const auto &y) {
-      Sum<REF> s = 0, rs = 0;
-      float t = 0;
-#pragma unroll
-      for (int k = 0; k < V; ++k) {
-        const Entry n = entry_of<REF>(z[k], q.top);
-        s += n.e;
-        t = fmaf(n.e, n.x, t);
-        if constexpr (REF) rs += exp_of<true>(y[k] - q.ref_top);
-      }
-      sums[0] += s, sums[1] += t;
-      if constexpr (REF) sums[2] += rs;
-    });
-    join<G>(sums, slots.sums, Add{});
-    q.s = sums[0], q.t = sums[1], q.ref_s = REF ? sums[REF ? 2 : 0] : 0;
-    const RowScalars o = row_scalars<REF>(a, inputs, action_logit, q, coefs, [&](float shift) {
-      double gaps[1] = {};
-      each([&](int, const auto &z, const auto &y) {
-        float g = 0;
-#pragma unroll
-        for (int k = 0; k < V; ++k) {
-          const float e = exp_of<true>(z[k] - q.top);
-          g = fmaf(e, gap_of<REF>(e, z[k], y[k], shift), g);
-        }
-        gaps[0] += g;
-      });
-      join<G>(gaps, slots.gaps, Add{});
-      return gaps[0];
-    });
+    row_sums<G, V, REF>(each, slots, q);
+    const RowScalars o = row_scalars<REF>(a, inputs, action_logit, q, coefs,
+                                          [&](float shift) { return gap_sum<G, V>(each, slots, q, shift); });
     if (threadIdx.x == 0 && a.log_probs) {
       if (o.live) value += o.value;
       report(a, row, o);
     }
     if (!a.grad) continue;
     T *grad = static_cast<T *>(a.grad) + row * int64_t(a.width);
-    if (o.live) {
-      each([&](int i, const auto &z, const auto &y) {
-        float g[V];
-#pragma unroll
-        for (int k = 0; k < V; ++k) g[k] = grad_of<REF>(z[k], REF ? y[k] : 0.f, q.top, o.c);
-        store_entries<V>(grad, g, i, a.width, false);
-      });
-      if (action >= 0 && action < a.width && action / V % G == threadIdx.x) {
-        const float yr = REF && action_logit > -INFINITY ? to_f32(ref[REF ? action : 0]) : 0.f;
-        grad[action] = from_f32<T>(grad_of<REF>(action_logit, yr, q.top, o.c) + o.c.own);
-      }
-    } else {
-      const float zero[V] = {};
-      for (int64_t i = int64_t(threadIdx.x) * V; i < a.width; i += G * V) store_entries<V>(grad, zero, int(i), a.width, false);
-    }
+    row_grads<T, REF>(a, grad, ref, inputs.action, action_logit, q.top, o, each, 0, a.width, G);
   }
   if (a.log_probs) block_loss(a, value);
+}
+
+// ---- a few long rows: a block a segment of a row, the segments joined by every block of the next launch ---------
+
+constexpr int MOST_SPLITS = 64;  // a lane each
+constexpr int SPLIT_PARTS = 6;   // top, S, T, the reference's top and S, and the sum of the KL's terms
+
+// The whole row's sums from its segments', scaled from their tops to the row's.
+template <bool REF>
+__device__ __forceinline__ RowSums joined_sums(const LossArgs &a, const double *parts) {
+  const int s = threadIdx.x & 63;
+  const bool in = s < a.splits;
+  const double *p = parts + SPLIT_PARTS * (in ? s : 0);
+  RowSums q;
+  const auto part = [&](double top, double sum, float &whole) {  // the segment's factor
+    const float mine = in && sum != 0 ? float(top) : -INFINITY;
+    whole = lanes_join<64>(mine, Most{});
+    whole = whole > -INFINITY ? whole : 0.f;
+    return in && sum != 0 ? exp_of(top - double(whole)) : 0.0;
+  };
+  const double f = part(p[0], p[1], q.top);
+  q.s = lanes_join<64>(f != 0 ? f * p[1] : 0.0, Add{});
+  q.t = lanes_join<64>(f != 0 ? f * (p[2] + (p[0] - double(q.top)) * p[1]) : 0.0, Add{});
+  q.ref_top = 0, q.ref_s = 0;
+  if constexpr (REF) {
+    const double g = part(p[3], p[4], q.ref_top);
+    q.ref_s = lanes_join<64>(g != 0 ? g * p[4] : 0.0, Add{});
+  }
+  return q;
+}
+
+// STEP 0: a segment's sums; 1: its part of the exact KL; 2: its gradient, and the row's numbers.
+template <typename T, bool REF, int STEP>
+__global__ __launch_bounds__(256) void split_rows_kernel(const LossArgs a) {
+  constexpr int V = VEC<T>, G = 256;
+  if (done(a)) return;
+  __shared__ Slots<G> slots;
+  const int row = blockIdx.x / a.splits, segment = blockIdx.x % a.splits;
+  const RowInputs inputs = row_inputs(a, row);
+  const int begin = segment * a.segment, end = min(begin + a.segment, a.width);
+  const T *logits = static_cast<const T *>(a.logits) + row * a.ld_logits;
+  const T *ref = static_cast<const T *>(a.ref_logits) + (REF ? row * a.ld_ref : 0);
+  const uint8_t *legal = a.mask ? a.mask + row * a.ld_mask : nullptr;
+  const bool counts = inputs.weight != 0;
+  double *parts = a.parts + int64_t(row) * a.splits * SPLIT_PARTS, *mine = parts + segment * SPLIT_PARTS;
+  const auto each = [&](const auto &visit) {
+    if (!counts) return;
+    for (int i = begin + int(threadIdx.x) * V; i < end; i += G * V) {
+      Entries<T, V> z, y;
+      load_entries<1, 1, V>(z.w, logits, legal, i, a.width);
+      if constexpr (REF) load_entries<1, 1, V>(y.w, ref, legal, i, a.width);
+      visit(i, z, y);
+    }
+  };
+  if constexpr (STEP == 0) {
+    RowSums q;
+    row_sums<G, V, REF>(each, slots, q);
+    if (threadIdx.x == 0) {
+      mine[0] = q.top, mine[1] = q.s, mine[2] = q.t;
+      if (REF) mine[3] = q.ref_top, mine[4] = q.ref_s;
+    }
+  } else {
+    const RowSums q = joined_sums<REF>(a, parts);
+    if constexpr (STEP == 1) {
+      const double g = gap_sum<G, V>(each, slots, q, float(shift_of(q, log_of(q.s))));
+      if (threadIdx.x == 0) mine[5] = g;
+    } else {
+      const float action_logit = counts ? logit_of<T>(a, row, inputs.action) : 0.f;
+      const RowScalars o = row_scalars<REF>(a, inputs, action_logit, q, coefs_of(a), [&](float) {
+        const int s = threadIdx.x & 63;
+        return lanes_join<64>(s < a.splits ? parts[SPLIT_PARTS * s + 5] : 0.0, Add{});
+      });
+      if (segment == 0 && threadIdx.x == 0 && a.log_probs) {
+        a.partials[row] = o.live ? o.value : 0.0;
+        report(a, row, o);
+      }
+      if (!a.grad) return;
+      T *grad = static_cast<T *>(a.grad) + int64_t(row) * a.width;
+      row_grads<T, REF>(a, grad, ref, inputs.action, action_logit, q.top, o, each, begin, end, G);
+    }
+  }
 }
 
 // ---- host side ---------------------------------------------------------------------------------------------------
@@ -655,6 +765,38 @@ struct Launch {
   void (*kernel)(LossArgs);
   int rows, threads;  // rows a block takes at a time
 };
+
+// Segments of a row: 1 (none) unless rows are long and leave most CUs without one.  A pass over bf16 rows with
+// the backward that has nothing to do, as a block a row and as segments, us: 9 x 50001 beside a reference's
+// 41 and 23, alone 20 and 13.5; 64 x 50001 beside one 43 and 35; but 64 x 30000 13.8 and 15.4, 9 x 9000
+// 10.6 and 14.1, 128 x 50001 22.6 and 25.
+int splits_of(const cg_policy_loss &p) {
+  if (p.rows > 64 || p.rows == 0 || p.width <= 32768) return 1;
+  const int wanted = (512 + p.rows - 1) / p.rows, most = p.width / 2048;
+  const int splits = wanted < most ? wanted : most;
+  return splits < MOST_SPLITS ? splits : MOST_SPLITS;
+}
+
+size_t parts_bytes(const cg_policy_loss &p) {
+  const int splits = splits_of(p);
+  return splits > 1 ? size_t(p.rows) * splits * SPLIT_PARTS * sizeof(double) : 0;
+}
+
+template <typename T, bool REF>
+void launch_splits(LossArgs a, const cg_policy_loss &p, hipStream_t stream) {
+  const int splits = splits_of(p);
+  a.segment = ((p.width + splits - 1) / splits + VEC<T> - 1) / VEC<T> * VEC<T>;
+  a.splits = (p.width + a.segment - 1) / a.segment;
+  const int blocks = p.rows * a.splits;
+  split_rows_kernel<T, REF, 0><<<blocks, 256, 0, stream>>>(a);
+  CG_LAUNCHED();
+  if constexpr (REF) {
+    split_rows_kernel<T, REF, 1><<<blocks, 256, 0, stream>>>(a);
+    CG_LAUNCHED();
+  }
+  split_rows_kernel<T, REF, 2><<<blocks, 256, 0, stream>>>(a);
+  CG_LAUNCHED();
+}
 
 template <typename T, int G, int E, bool REF, typename S = T>
 Launch launch_as() {
@@ -697,9 +839,30 @@ Launch launch_of(const cg_policy_loss &p) {
                               : launch_of<f16>(p, ref);
 }
 
-int grid_of(const cg_policy_loss &p, const Launch &l) {
+// Returns the number of partial sums of the loss that are written (by one block for all rows: the loss itself).
+int launch_rows(const LossArgs &a, const cg_policy_loss &p, hipStream_t stream) {
+  if (splits_of(p) > 1) {
+    const auto of = [&](auto type) {
+      using T = decltype(type);
+      if (p.reference_logits)
+        launch_splits<T, true>(a, p, stream);
+      else
+        launch_splits<T, false>(a, p, stream);
+    };
+    if (p.dtype == CG_F32)
+      of(float{});
+    else if (p.dtype == CG_BF16)
+      of(bf16{});
+    else
+      of(f16{});
+    return p.rows;
+  }
+  const Launch l = launch_of(p);
   const int64_t blocks = (int64_t(p.rows) + l.rows - 1) / l.rows;
-  return int(blocks < MAX_BLOCKS ? blocks : MAX_BLOCKS);
+  const int grid = int(blocks < MAX_BLOCKS ? blocks : MAX_BLOCKS);
+  l.kernel<<<grid, l.threads, 0, stream>>>(a);
+  CG_LAUNCHED();
+  return grid;
 }
 
 Scalar scalar(const cg_scalar &s) { return Scalar{s.value, s.device}; }
@@ -709,6 +872,7 @@ LossArgs args_of(const cg_policy_loss *loss) {
   const cg_policy_loss &p = *loss;
   dtype_size(p.dtype);
   CG_REQUIRE(p.rows >= 0 && p.width > 0, CG_ERR_INVALID, "rows must be non-negative, width positive");
+  CG_REQUIRE(p.width <= 1 << 30, CG_ERR_UNSUPPORTED, "policy loss: rows wider than 2^30");
   CG_REQUIRE(p.rows == 0 || (p.logits && p.actions && p.old_log_probs && p.advantages), CG_ERR_INVALID,
              "logits, actions, old_log_probs and advantages are required");
   CG_REQUIRE(!(p.reference_logits && p.reference_log_probs), CG_ERR_INVALID,
@@ -732,44 +896,44 @@ using namespace cg;
 
 extern "C" {
 
-size_t cg_policy_loss_workspace_size(void) { return MAX_BLOCKS * sizeof(double); }
+size_t cg_policy_loss_workspace_size(const cg_policy_loss *loss) {
+  return loss ? MAX_BLOCKS * sizeof(double) + parts_bytes(*loss) : 0;
+}
 
 int cg_policy_loss_forward(const cg_policy_loss *loss, float *value, float *log_probs, float *entropy, float *kl,
                            void *grad, void *workspace, size_t workspace_size, void *stream) {
   return guarded([&] {
     LossArgs a = args_of(loss);
     CG_REQUIRE(value && workspace, CG_ERR_INVALID, "value and workspace are required");
-    CG_REQUIRE(workspace_size >= cg_policy_loss_workspace_size(), CG_ERR_INVALID, "workspace too small");
+    CG_REQUIRE(workspace_size >= cg_policy_loss_workspace_size(loss), CG_ERR_INVALID, "workspace too small");
     CG_REQUIRE(a.rows == 0 || (log_probs && entropy), CG_ERR_INVALID, "log_probs and entropy are required");
     CG_REQUIRE(a.rows == 0 || !kl == !(a.ref || a.ref_logits), CG_ERR_INVALID, "kl goes with a reference");
     a.partials = static_cast<double *>(workspace);
+    a.parts = a.partials + MAX_BLOCKS;
     a.loss = value;
-    int blocks = 0;
+    int sums = 0;
     if (a.rows > 0) {
       a.log_probs = log_probs, a.entropy = entropy, a.kl = kl, a.grad = grad;
-      const Launch l = launch_of(*loss);
-      blocks = grid_of(*loss, l);
-      l.kernel<<<blocks, l.threads, 0, as_stream(stream)>>>(a);
-      CG_LAUNCHED();
+      sums = launch_rows(a, *loss, as_stream(stream));
     }
-    if (blocks != 1) {
-      loss_kernel<<<1, 256, 0, as_stream(stream)>>>(a, blocks);
+    if (sums != 1 || splits_of(*loss) > 1) {
+      loss_kernel<<<1, 256, 0, as_stream(stream)>>>(a, sums);
       CG_LAUNCHED();
     }
   });
 }
 
 int cg_policy_loss_backward(const cg_policy_loss *loss, const float *upstream, int32_t written, void *grad,
-                            void *stream) {
+                            void *workspace, size_t workspace_size, void *stream) {
   return guarded([&] {
     LossArgs a = args_of(loss);
     CG_REQUIRE(upstream, CG_ERR_INVALID, "upstream is required");
     if (a.rows == 0) return;
     CG_REQUIRE(grad, CG_ERR_INVALID, "grad is required");
+    CG_REQUIRE(workspace && workspace_size >= cg_policy_loss_workspace_size(loss), CG_ERR_INVALID, "workspace too small");
+    a.parts = static_cast<double *>(workspace) + MAX_BLOCKS;
     a.grad = grad, a.upstream = upstream, a.written = written;
-    const Launch l = launch_of(*loss);
-    l.kernel<<<grid_of(*loss, l), l.threads, 0, as_stream(stream)>>>(a);
-    CG_LAUNCHED();
+    launch_rows(a, *loss, as_stream(stream));
   });
 }
 

@@ -10,7 +10,6 @@ rollout (cardgym/rl/ppo.py:75-94): the same softmax over a row's legal entries, 
 
 from __future__ import annotations
 
-from functools import lru_cache
 from typing import NamedTuple
 
 import torch
@@ -45,42 +44,52 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
 
 
 class _Call:
-    """One loss: its inputs, their native descriptor and what the forward writes."""
+    """One loss: its native descriptor, and what the forward writes beside the loss."""
 
-    __slots__ = ("descriptor", "tensors", "kl", "log_probs", "entropy", "logits")
+    __slots__ = ("descriptor", "kl", "log_probs", "entropy")
 
-    def __init__(self, logits, tensors, options) -> None:
-        self.logits = logits
-        self.tensors = tensors  # alive as long as the descriptor's addresses
-        address = [None if t is None else t.data_ptr() for t in tensors]
-        actions, old, advantages, weights, mask, reference_logits, reference_log_probs = address[:7]
-        rows, width = logits.shape
-        self.descriptor = nat.PolicyLoss(
-            logits.data_ptr(), mask, actions, old, advantages, weights, reference_logits, reference_log_probs,
-            logits.stride(0), 0 if mask is None else tensors[4].stride(0),
-            0 if reference_logits is None else tensors[5].stride(0), rows, width, dtype_code(logits.dtype), *options,
-        )
+    def __init__(self, tensors, options) -> None:
+        rows, width = tensors[0].shape
+        self.descriptor = nat.PolicyLoss(*(8 * (None,)), 0, 0, 0, rows, width, dtype_code(tensors[0].dtype), *options)
+        self.bind(tensors)
 
-    def forward(self, grad: torch.Tensor | None) -> torch.Tensor:
-        device, rows = self.logits.device, self.logits.shape[0]
+    def bind(self, tensors) -> None:
+        """Points the descriptor at the inputs: logits, mask, reference logits, then the rows' and scalars."""
+
+        logits, mask, reference_logits, actions, old, advantages, weights, reference_log_probs, *scalars = tensors
+        d = self.descriptor
+        d.logits, d.ld_logits = logits.data_ptr(), logits.stride(0)
+        d.actions, d.old_log_probs, d.advantages = actions.data_ptr(), old.data_ptr(), advantages.data_ptr()
+        if mask is not None:
+            d.mask, d.ld_mask = mask.data_ptr(), mask.stride(0)
+        if reference_logits is not None:
+            d.reference_logits, d.ld_reference = reference_logits.data_ptr(), reference_logits.stride(0)
+        if weights is not None:
+            d.weights = weights.data_ptr()
+        if reference_log_probs is not None:
+            d.reference_log_probs = reference_log_probs.data_ptr()
+        for name, x in zip(("normalizer", "entropy_coef", "kl_coef"), scalars):
+            if x is not None:
+                getattr(d, name).device = x.data_ptr()
+
+    def workspace(self, device: torch.device) -> tuple[torch.Tensor, int]:
+        size = nat.lib().cg_policy_loss_workspace_size(self.descriptor)
+        return torch.empty(size, device=device, dtype=torch.uint8), size
+
+    def forward(self, device: torch.device, grad: torch.Tensor | None) -> torch.Tensor:
+        d = self.descriptor
         loss = torch.empty((), device=device)
-        self.log_probs = torch.empty(rows, device=device)
-        self.entropy = torch.empty(rows, device=device)
-        self.kl = None if self.tensors[5] is None and self.tensors[6] is None else torch.empty(rows, device=device)
-        size = _workspace_size()
-        workspace = torch.empty(size, device=device, dtype=torch.uint8)
+        self.log_probs = torch.empty(d.rows, device=device)
+        self.entropy = torch.empty(d.rows, device=device)
+        self.kl = torch.empty(d.rows, device=device) if d.reference_logits or d.reference_log_probs else None
+        workspace, size = self.workspace(device)
         with _on(device):
             nat.call(
-                "cg_policy_loss_forward", self.descriptor, loss.data_ptr(), self.log_probs.data_ptr(),
-                self.entropy.data_ptr(), None if self.kl is None else self.kl.data_ptr(),
-                None if grad is None else grad.data_ptr(), workspace.data_ptr(), size, stream_handle(device),
+                "cg_policy_loss_forward", d, loss.data_ptr(), self.log_probs.data_ptr(), self.entropy.data_ptr(),
+                None if self.kl is None else self.kl.data_ptr(), None if grad is None else grad.data_ptr(),
+                workspace.data_ptr(), size, stream_handle(device),
             )
         return loss
-
-
-@lru_cache(maxsize=1)
-def _workspace_size() -> int:
-    return nat.lib().cg_policy_loss_workspace_size()
 
 
 class PolicyLossFunction(torch.autograd.Function):
@@ -88,28 +97,30 @@ class PolicyLossFunction(torch.autograd.Function):
     arriving is 1 and forms it again, from the inputs, where it is another."""
 
     @staticmethod
-    def forward(ctx, logits, call):
-        # (call.logits is what the kernel reads: logits, or its copy with the entries side by side)
+    def forward(ctx, logits, call, tensors):
+        # (tensors[0] is what the kernel reads: logits, or its copy with the entries side by side)
         ctx.written = torch.empty(logits.shape, device=logits.device, dtype=logits.dtype)
-        ctx.save_for_backward(call.logits, *call.tensors)
+        ctx.save_for_backward(*tensors)
         ctx.call = call
-        return call.forward(ctx.written)
+        return call.forward(logits.device, ctx.written)
 
     @staticmethod
     def backward(ctx, upstream):
         if torch.is_grad_enabled():  # (create_graph; once_differentiable costs 13 us of a small loss's 96)
             raise RuntimeError("policy_loss is differentiable once: its gradient has no graph")
-        call = ctx.call
-        logits = ctx.saved_tensors[0]  # (an input changed since the forward raises here)
+        tensors = ctx.saved_tensors  # (an input changed since the forward raises here)
+        call, logits, device = ctx.call, tensors[0], upstream.device
+        call.bind(tensors)  # (a saved-tensor hook may have brought them back elsewhere)
         grad, ctx.written = ctx.written, None  # handed over once: a second backward forms its own
         written = grad is not None
         if grad is None:
-            grad = torch.empty(logits.shape, device=logits.device, dtype=logits.dtype)
+            grad = torch.empty(logits.shape, device=device, dtype=logits.dtype)
         upstream = upstream.contiguous()
-        with _on(logits.device):
-            nat.call("cg_policy_loss_backward", call.descriptor, upstream.data_ptr(), int(written),
-                     grad.data_ptr(), stream_handle(logits.device))
-        return grad, None
+        workspace, size = call.workspace(device)
+        with _on(device):
+            nat.call("cg_policy_loss_backward", call.descriptor, upstream.data_ptr(), int(written), grad.data_ptr(),
+                     workspace.data_ptr(), size, stream_handle(device))
+        return grad, None, None
 
 
 @torch.compiler.disable
@@ -179,19 +190,17 @@ def policy_loss(
         normalizer = float(max(rows, 1))
     elif not isinstance(normalizer, torch.Tensor) and not normalizer > 0:
         raise ValueError("normalizer must be positive")
-    scalars, kept = [], []
+    values, scalars = [], []
     for name, x in (("normalizer", normalizer), ("entropy_coef", entropy_coef), ("kl_coef", kl_coef)):
-        if isinstance(x, torch.Tensor):
-            kept.append(_constant(x, name, (), torch.float32, device))
-            scalars.append(nat.Scalar(0.0, x.data_ptr()))
-        else:
-            scalars.append(nat.Scalar(x, None))
-    tensors = (actions.contiguous(), old_log_probs.contiguous(), advantages.contiguous(),
-               None if weights is None else weights.contiguous(), mask, reference_logits, reference_log_probs, *kept)
+        on_device = isinstance(x, torch.Tensor)
+        scalars.append(_constant(x, name, (), torch.float32, device) if on_device else None)
+        values.append(nat.Scalar(0.0 if on_device else x, None))
     entries = logits if logits.stride(1) == 1 else logits.detach().contiguous()
-    call = _Call(entries, tensors, (1.0 - clip, 1.0 + clip_high, *scalars))
+    tensors = (entries, mask, reference_logits, actions.contiguous(), old_log_probs.contiguous(), advantages.contiguous(),
+               None if weights is None else weights.contiguous(), reference_log_probs, *scalars)
+    call = _Call(tensors, (1.0 - clip, 1.0 + clip_high, *values))
     if torch.is_grad_enabled() and logits.requires_grad:
-        loss = PolicyLossFunction.apply(logits, call)
+        loss = PolicyLossFunction.apply(logits, call, tensors)
     else:
-        loss = call.forward(None)
+        loss = call.forward(device, None)
     return PolicyLoss(loss, call.log_probs, call.entropy, call.kl)

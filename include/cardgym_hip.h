@@ -575,13 +575,13 @@ typedef struct {
 /* value[0], log_probs / entropy / kl [rows] (kl with a reference, else NULL) and, where grad is
  * not NULL, the value's gradient [rows, width] dense, of `dtype`.  workspace: 8-byte aligned, of
  * this call alone until it has run. */
-size_t cg_policy_loss_workspace_size(void);
+size_t cg_policy_loss_workspace_size(const cg_policy_loss *loss);
 int cg_policy_loss_forward(const cg_policy_loss *loss, float *value, float *log_probs, float *entropy, float *kl,
                            void *grad, void *workspace, size_t workspace_size, void *stream);
 /* grad [rows, width] = upstream[0] times the value's gradient, formed from the inputs and rounded
  * once.  written != 0: grad holds the forward's, and stays as it is where upstream[0] is 1. */
 int cg_policy_loss_backward(const cg_policy_loss *loss, const float *upstream, int32_t written, void *grad,
-                            void *stream);
+                            void *workspace, size_t workspace_size, void *stream);
 
 /* ---- the optimiser step ------------------------------------------------------------------
  * What follows the training backward in an update: the gradients' global norm and one AdamW

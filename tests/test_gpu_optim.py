@@ -16,6 +16,7 @@ import torch
 
 from card_playing_gym_amd.nn import AdamW, AdamWPlan, grad_norm, moment_values
 from card_playing_gym_amd.nn.optim import moment_blocks
+from card_playing_gym_amd.synthetic import build_model, trunk_config
 from oracle import optim as ref
 
 pytestmark = pytest.mark.gpu
@@ -498,3 +499,32 @@ def test_a_captured_step_counts_on(device, bits):
         assert [optimizer.state[p]["step"].item() for p in params] == [5, 5, 5]
         results.append([x.detach().clone() for p in params for x in (p, *optimizer.state[p].values())])
     assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
+@pytest.mark.parametrize("through", ["optimizer", "plan"])
+def test_a_rollout_after_a_step_uses_the_new_weights(device, through):
+    """The decode path's bf16 weight copies follow the step: bit for bit a model that was loaded with the stepped
+    weights."""
+
+    model = build_model(trunk_config(2), 0, device)
+    tokens = torch.arange(8, device=device)[:, None, None]
+    zeros = torch.zeros(8, dtype=torch.int64, device=device)
+
+    def wave(m):
+        with torch.no_grad(), torch.autocast("cuda", dtype=torch.bfloat16):
+            return m.forward_ragged(tokens, zeros, m.new_cache(8, 16, torch.bfloat16), zeros)
+
+    before = wave(model)
+    params = list(model.parameters())
+    for p in params:
+        p.grad = torch.randn_like(p)
+    if through == "optimizer":
+        AdamW(params, lr=1e-2).step()
+    else:
+        state = [[torch.zeros_like(p) for p in params] for _ in range(2)]
+        steps = [torch.zeros((), device=device) for _ in params]
+        AdamWPlan(params, *state, steps).step([p.grad for p in params], lr=1e-2)
+    after = wave(model)
+    twin = build_model(trunk_config(2), 1, device)
+    twin.load_state_dict(model.state_dict())
+    assert torch.equal(after, wave(twin)) and not torch.equal(after, before)

@@ -108,9 +108,15 @@ def check(given, options, out, grad, upstream=1.0):
     own = np.abs(want["own"])[:, None]
     bracket = c * (x + 2 * want["entropy"][:, None] + m1[:, None]) + beta * (np.abs(want["gap"]) + np.abs(want["kl"])[:, None]) + own
     relative = (3 * x + 40) * U + 3 * s[:, None]
-    off = f * (p * bracket * relative + p * (c * entropy + beta * kl)[:, None])
+    # own = -A r - beta (e^d - 1) with the sampled KL: its derivative by log p is -A r + beta e^d, so where the two
+    # nearly cancel (a clipped row has the second alone, small for d near 0) it is off by more than own's share.
+    slope = np.abs(host(given["advantages"])) * want["ratio"]
+    if "reference_log_probs" in options:
+        slope = slope + beta * np.exp(d)
+    own_off = s * slope + 16 * U * own[:, 0]
+    off = f * (p * bracket * relative + p * (c * entropy + beta * kl + own_off)[:, None])
     rows = np.arange(len(s))
-    off[rows, host(given["actions"]) % p.shape[1]] += (f * own)[:, 0] * (2 * s + 16 * U)
+    off[rows, host(given["actions"]) % p.shape[1]] += f[:, 0] * own_off
     target = want["grad"] * upstream
     error = np.abs(host(grad) - target)
     bar = off + HALF_STEP[dtype] * (np.abs(target) + off) + TINY[dtype]
@@ -137,6 +143,23 @@ def test_wide_rows(device, dtype, width):
     for k, reference in enumerate((None, "logits", "sampled")):
         given, options = make(device, 3, width, dtype, seed=width + k, masked=k != 2, reference=reference)
         check(given, options, *run(given, options))
+
+
+@pytest.mark.parametrize("width", [8193, 16384, 16391, 32768, 32771, 65537, 70001])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+def test_many_wide_rows(device, dtype, width):
+    """Enough of them for a block each (fewer are cut into segments)."""
+
+    for k, reference in enumerate(("logits", "sampled")):
+        given, options = make(device, 130, width, dtype, seed=width + k, masked=k == 0, reference=reference, weighted=True)
+        check(given, options, *run(given, options))
+
+
+@pytest.mark.parametrize("rows, width", [(1, 32769), (2, 300001), (50, 40001), (64, 33000), (65, 33000)])
+@pytest.mark.parametrize("reference", [None, "logits"])
+def test_rows_in_segments(device, rows, width, reference):
+    given, options = make(device, rows, width, torch.bfloat16, seed=rows, reference=reference, weighted=True)
+    check(given, options, *run(given, options))
 
 
 @pytest.mark.parametrize("rows, width", [(1, 40), (8200, 40), (2051, 130), (9001, 513), (2500, 2050)])
@@ -187,6 +210,25 @@ def test_rows_that_count_for_nothing(device, width):
     options["mask"][:] = False
     out, grad = run(given, options)
     assert out.loss == 0 and not grad.any() and not out.kl.any()
+
+
+@pytest.mark.parametrize("width", [3000, 12000, 20000, 40000, 70001])
+def test_rows_that_count_for_nothing_among_many(device, width):
+    """The same where every row has a block of its own."""
+
+    rows = 160
+    given, options = make(device, rows, width, torch.bfloat16, seed=2, reference="logits")
+    kind = torch.arange(rows, device=device) % 8
+    good = kind < 4
+    want, want_grad = run(given, {**options, "weights": good.float()})
+    options["mask"][kind == 4] = False
+    given["logits"][kind == 5] = -torch.inf
+    given["logits"][kind >= 6] = torch.nan
+    given["actions"][kind == 7] = 2**40
+    out, grad = run(given, {**options, "weights": (kind < 6).float()})
+    for got, expect in ((out.log_probs, want.log_probs), (out.entropy, want.entropy), (out.kl, want.kl), (grad, want_grad)):
+        assert torch.equal(got[good], expect[good]) and not got[~good].any()
+    assert torch.equal(out.loss, want.loss)
 
 
 @pytest.mark.parametrize("width", [40, 600, 3000, 40000])
@@ -337,6 +379,33 @@ def test_backward_twice_and_inputs_that_changed(device):
     given["advantages"].add_(1)
     with pytest.raises(RuntimeError, match="modified by an inplace"):
         torch.autograd.grad(out.loss, leaf)
+
+
+def test_saved_inputs_that_come_back_elsewhere(device):
+    """Under a hook that moves saved tensors to the host, the backward reads what it brings back; after a backward the
+    loss keeps no input alive."""
+
+    given, options = make(device, 300, 2100, torch.float32, seed=16, reference="logits")
+    options["entropy_coef"] = torch.tensor(0.03, device=device)
+    _, want = run(given, options, 2.0)
+    leaf = given["logits"].clone().requires_grad_()
+    with torch.autograd.graph.save_on_cpu():
+        out = policy_loss(leaf * 1.0, given["actions"], given["old"], given["advantages"], **options)
+    (grad,) = torch.autograd.grad(out.loss * 2.0, leaf)
+    assert torch.equal(grad, want)
+
+    def alone():
+        z = given["logits"].clone().requires_grad_()
+        loss = policy_loss(z * 1.0, given["actions"], given["old"], given["advantages"], **options).loss
+        loss.backward()
+        return loss
+
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    loss = alone()
+    # The graph keeps the leaf and its gradient; the product and its gradient of the same size are gone.
+    kept = 2 * 300 * 2100 * 4
+    assert torch.cuda.memory_allocated() - before < kept + 2**20 and torch.isfinite(loss)
 
 
 def test_a_second_derivative_is_refused(device):

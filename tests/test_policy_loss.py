@@ -4,6 +4,8 @@ float64 and against differences, and every refusal."""
 from __future__ import annotations
 
 import ctypes
+import shutil
+import subprocess
 
 import numpy as np
 import pytest
@@ -12,6 +14,7 @@ import torch
 from card_playing_gym_amd import _native as nat
 from card_playing_gym_amd.rl import policy, policy_loss
 from oracle import policy as ref
+from tests.conftest import ROOT
 
 
 def _inputs(rows=40, width=9, seed=0):
@@ -135,21 +138,43 @@ def test_native_refusals():
     """Fake addresses: every check comes before a launch."""
 
     lib = nat.lib()
-    size = lib.cg_policy_loss_workspace_size()
     zero = nat.Scalar(0.0, None)
+    size = 1 << 20
 
-    def call(value=16, log_probs=16, entropy=16, kl=None, workspace=16, size=size, upstream=None, **changes):
+    def call(value=16, log_probs=16, entropy=16, kl=None, workspace=16, size=size, upstream=None, grad=16, **changes):
         d = nat.PolicyLoss(16, None, 16, 16, 16, None, None, None, 6, 6, 6, 4, 6, nat.CG_F32, 0.8, 1.2,
                            nat.Scalar(4.0, None), zero, zero)
         for name, x in changes.items():
             setattr(d, name, x)
+        if size < 0:  # short by that much
+            size += lib.cg_policy_loss_workspace_size(ctypes.byref(d))
         if upstream is not None:
-            return lib.cg_policy_loss_backward(ctypes.byref(d), upstream or None, 0, None, None)
+            return lib.cg_policy_loss_backward(ctypes.byref(d), upstream or None, 0, grad, workspace, size, None)
         return lib.cg_policy_loss_forward(ctypes.byref(d), value, log_probs, entropy, kl, None, workspace, size, None)
 
-    for changes in ({"value": None}, {"workspace": None}, {"size": size - 1}, {"log_probs": None}, {"entropy": None},
+    for changes in ({"value": None}, {"workspace": None}, {"size": -1}, {"rows": 3, "width": 20000, "size": -1}, {"log_probs": None}, {"entropy": None},
                     {"kl": 16}, {"rows": -1}, {"width": 0}, {"dtype": 5}, {"logits": None}, {"actions": None},
                     {"old_log_probs": None}, {"advantages": None}, {"ld_logits": -1}, {"reference_logits": 16},
-                    {"reference_logits": 16, "reference_log_probs": 16, "kl": 16}, {"upstream": 0}, {"upstream": 16}):
+                    {"reference_logits": 16, "reference_log_probs": 16, "kl": 16}, {"upstream": 0}, {"upstream": 16, "grad": None}, {"upstream": 16, "workspace": None},
+                    {"upstream": 16, "size": -1}):
         assert call(**changes) == nat.CG_ERR_INVALID, changes
     assert lib.cg_policy_loss_forward(None, 16, 16, 16, None, None, 16, size, None) == nat.CG_ERR_INVALID
+    assert call(width=(1 << 30) + 1) == nat.CG_ERR_UNSUPPORTED
+
+
+@pytest.mark.skipif(shutil.which("gcc") is None, reason="needs gcc")
+def test_struct_layouts_of_the_update_match_the_header(tmp_path):
+    structs = {"cg_scalar": nat.Scalar, "cg_policy_loss": nat.PolicyLoss, "cg_adamw_tensor": nat.AdamWTensor,
+               "cg_adamw_config": nat.AdamWConfig}
+    lines = []
+    for cname, py in structs.items():
+        lines.append(f'printf("{cname} size %zu\\n", sizeof({cname}));')
+        lines += [f'printf("{cname} {field} %zu\\n", offsetof({cname}, {field}));' for field, _ in py._fields_]
+    source, exe = tmp_path / "layout.c", tmp_path / "layout"
+    source.write_text("#include <stdio.h>\n#include <stddef.h>\n#include \"cardgym_hip.h\"\nint main(void){\n"
+                      + "\n".join(lines) + "\nreturn 0;}\n")
+    subprocess.run(["gcc", "-I", str(ROOT / "include"), str(source), "-o", str(exe)], check=True)
+    for line in subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout.splitlines():
+        cname, field, value = line.split()
+        py = structs[cname]
+        assert int(value) == (ctypes.sizeof(py) if field == "size" else getattr(py, field).offset), line
