@@ -19,7 +19,10 @@ namespace cg {
 namespace {
 
 constexpr int THREADS = 256;
-constexpr int CHUNK = 4096;       // elements of one tensor that a block updates
+// Elements of one tensor that a block updates.  With moments in 32 bits 1024 (against 4096 us: 11.4 M elements
+// 63 -> 58, 174 M 889 -> 868); in 8 bits, where a block's start weighs against more arithmetic, 1024 below
+// STREAM_BYTES (11.4 M 52 -> 43) and 4096 above (174 M bf16 376, 404 with 1024).
+constexpr int CHUNK = 1024, LONG_CHUNK = 4096;
 constexpr int NORM_CHUNK = 8192;  // elements whose squares a block sums at a time
 constexpr int NORM_BLOCKS = 2048; // most blocks (and partial sums) of a step's norm, over all its launches
 constexpr int MOMENT_BLOCK = 256; // elements that share a scale: four a lane
@@ -432,10 +435,11 @@ __global__ __launch_bounds__(THREADS) void adamw8_kernel(const UpdateArgs<Tensor
   const TensorScalars s = reinterpret_cast<const TensorScalars *>(a.header + 1)[a.entry + i];
   const Rates8 r{a.header->clip, a.beta1, 1 - a.beta1, a.beta2, 1 - a.beta2, a.eps, a.header->decay, s.rate, s.second};
   const bool vec = aligned4(static_cast<T *>(t.p)) && aligned4(static_cast<const T *>(t.g)) && aligned4(t.m) && aligned4(t.v);
+  constexpr int BLOCKS = (STREAM ? LONG_CHUNK : CHUNK) / MOMENT_BLOCK;
   const int64_t blocks = (t.n + MOMENT_BLOCK - 1) / MOMENT_BLOCK;
-  const int64_t first = int64_t(int(blockIdx.x) - a.first_chunk[i]) * (CHUNK / MOMENT_BLOCK);
+  const int64_t first = int64_t(int(blockIdx.x) - a.first_chunk[i]) * BLOCKS;
 #pragma unroll
-  for (int c = 0; c < CHUNK / MOMENT_BLOCK / (THREADS / 64); ++c) {
+  for (int c = 0; c < BLOCKS / (THREADS / 64); ++c) {
     const int64_t b = first + c * (THREADS / 64) + wave;
     if (b >= blocks) break;  // whole wave
     const int64_t at = b * MOMENT_BLOCK;
@@ -555,8 +559,8 @@ int dtype_index(int32_t dtype) {
 
 // Above this many bytes of parameters, gradients and state together a step goes past the caches
 // (the Infinity Cache has 256 MB): what one launch leaves there is gone before it is met again.
-// fp32 parameters and moments, 174 M elements (2.8 GB): norm 167 -> 105 us, update 912 -> 882; 11.4 M
-// (182 MB): 10.6 -> 9.9, but the update, which meets gradients that the norm has read, 53 -> 67.
+// fp32 parameters and moments, in blocks of 4096, us: 174 M elements (2.8 GB) norm 167 -> 105, update 912 -> 884;
+// but 11.4 M (182 MB) norm 16 -> 10.5 and the update, which meets gradients that the norm has read, 53 -> 67.
 constexpr int64_t STREAM_BYTES = 512 << 20;
 
 int launch_norm(const GradList &list, const int32_t *dtypes, int32_t dtype, bool streams, double *partials,
@@ -572,7 +576,7 @@ int launch_norm(const GradList &list, const int32_t *dtypes, int32_t dtype, bool
 }
 
 template <typename T, int N, typename Fill>
-void launch_updates(void (*kernel)(UpdateArgs<T, N>), const cg_adamw_tensor *tensors, const void *const *grads, int n,
+void launch_updates(void (*kernel)(UpdateArgs<T, N>), int chunk, const cg_adamw_tensor *tensors, const void *const *grads, int n,
                     const cg_adamw_config &c, StepHeader *header, hipStream_t stream, const Fill &fill) {
   int at = 0, entry = 0;  // entries count the tensors that take part
   while (at < n) {
@@ -581,7 +585,7 @@ void launch_updates(void (*kernel)(UpdateArgs<T, N>), const cg_adamw_tensor *ten
     int64_t chunks = 0;
     for (; at < n && a.tensors < N; ++at) {
       if (grads[at] == nullptr || tensors[at].n == 0) continue;
-      const int64_t more = chunks_of(tensors[at].n, CHUNK);
+      const int64_t more = chunks_of(tensors[at].n, chunk);
       if (chunks + more >= (int64_t(1) << 30)) break;
       a.t[a.tensors] = fill(tensors[at], grads[at]);
       a.first_chunk[a.tensors++] = int32_t(chunks);
@@ -651,7 +655,7 @@ int cg_adamw_step(const cg_adamw_tensor *tensors, const void *const *grads, int3
     CG_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, CG_ERR_INVALID, "workspace must be 16-byte aligned");
     for (int i = 0; i < n; ++i) {
       const cg_adamw_tensor &t = tensors[i];
-      CG_REQUIRE(t.n >= 0 && t.n < int64_t(1) << 42, CG_ERR_RANGE, "a tensor's size is out of range");
+      CG_REQUIRE(t.n >= 0 && t.n < int64_t(1) << 39, CG_ERR_RANGE, "a tensor's size is out of range");
       if (t.n == 0 || grads[i] == nullptr) continue;
       CG_REQUIRE(t.param && t.exp_avg && t.exp_avg_sq && t.step, CG_ERR_INVALID, "a tensor's state is NULL");
       CG_REQUIRE(c.state_bits == 32 || (t.exp_avg_scale && t.exp_avg_sq_scale), CG_ERR_INVALID,
@@ -697,11 +701,11 @@ int cg_adamw_step(const cg_adamw_tensor *tensors, const void *const *grads, int3
     const auto run = [&](auto type) {
       using T = decltype(type);
       if (c.state_bits == 32)
-        launch_updates<Tensor32, UPDATE_TENSORS>(streams ? adamw_kernel<T, true> : adamw_kernel<T, false>, tensors, grads,
-                                                 n, c, header, s, wide);
+        launch_updates<Tensor32, UPDATE_TENSORS>(streams ? adamw_kernel<T, true> : adamw_kernel<T, false>, CHUNK,
+                                                 tensors, grads, n, c, header, s, wide);
       else
-        launch_updates<Tensor8, UPDATE_TENSORS_8>(streams ? adamw8_kernel<T, true> : adamw8_kernel<T, false>, tensors,
-                                                  grads, n, c, header, s, narrow);
+        launch_updates<Tensor8, UPDATE_TENSORS_8>(streams ? adamw8_kernel<T, true> : adamw8_kernel<T, false>,
+                                                  streams ? LONG_CHUNK : CHUNK, tensors, grads, n, c, header, s, narrow);
     };
     if (c.dtype == CG_F32)
       run(float{});
