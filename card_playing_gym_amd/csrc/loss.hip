@@ -279,6 +279,15 @@ __device__ __forceinline__ void load_entries(uint32_t *w, const T *row, const ui
   }
 }
 
+// Four gradients rounded to nearest even; a NaN stays one, whichever.
+template <typename T>
+__device__ __forceinline__ u32x2 packed(f32x4 g) {
+  if constexpr (__is_same(T, bf16))
+    return __builtin_bit_cast(u32x2, __builtin_convertvector(g, bf16x4));
+  else
+    return cvt4<T>(g);
+}
+
 // The gradients of a vector from entry i on.
 template <int V, typename T>
 __device__ __forceinline__ void store_entries(T *row, const float *g, int i, int width, bool inside, bool streams = false) {
@@ -289,7 +298,7 @@ __device__ __forceinline__ void store_entries(T *row, const float *g, int i, int
     if constexpr (sizeof(T) == 4) {
       __builtin_memcpy(&q, g, 16);
     } else {
-      const u32x2 lo = cvt4<T>(f32x4{g[0], g[1], g[2], g[3]}), hi = cvt4<T>(f32x4{g[4], g[5], g[6], g[7]});
+      const u32x2 lo = packed<T>(f32x4{g[0], g[1], g[2], g[3]}), hi = packed<T>(f32x4{g[4], g[5], g[6], g[7]});
       q = Word4{lo[0], lo[1], hi[0], hi[1]};
     }
     if (streams)
@@ -371,10 +380,12 @@ __device__ __forceinline__ RowScalars row_scalars(const LossArgs &a, const RowIn
   o.kl = kl;
   const double weight = in.weight, f = weight * k.scale;
   o.value = weight * value;
+  // The entries of a row that does not count have e = 0: with these the gradient is 0 without asking.
   o.c.own = float(f * own);
-  o.c.base = float(f * (base - own) * inv);
-  o.c.slope = float(f * c * inv);
-  o.c.pull = REF ? float(f * beta * inv) : 0.f;
+  o.c.base = o.live ? float(f * (base - own) * inv) : 0.f;
+  o.c.slope = o.live ? float(f * c * inv) : 0.f;
+  o.c.pull = REF && o.live ? float(f * beta * inv) : 0.f;
+  o.c.shift = o.live ? o.c.shift : 0.f;
   return o;
 }
 
@@ -548,8 +559,7 @@ __global__ __launch_bounds__((G > 256 ? G : 256), (ROOM<S, G, E, REF>)) void row
       for (int c = 0; c < C; ++c) {
         float g[V];
 #pragma unroll
-        for (int k = 0; k < V; ++k)
-          g[k] = o.live ? grad_of<REF>(z[c * V + k], y[REF ? c * V + k : 0], q.top, o.c) : 0.f;
+        for (int k = 0; k < V; ++k) g[k] = grad_of<REF>(z[c * V + k], y[REF ? c * V + k : 0], q.top, o.c);
         store_entries<V>(grad, g, (c * G + lane) * V, a.width, (c + 1) * G * V <= a.width, streams);
       }
       // The action's own term, by the lane that has just written that entry.
