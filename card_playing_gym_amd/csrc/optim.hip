@@ -499,6 +499,10 @@ __global__ __launch_bounds__(THREADS) void moment_values_kernel(const uint8_t *_
 
 // ---- host side ----------------------------------------------------------------------------------
 
+// A launch counts its threads in 32 bits.
+constexpr int64_t MOST_ELEMENTS = int64_t(1) << 33, MOST_BLOCKS = (int64_t(1) << 24) - 1;
+static_assert(MOST_ELEMENTS / CHUNK <= MOST_BLOCKS && MOST_BLOCKS * THREADS < (int64_t(1) << 32), "grid");
+
 int64_t chunks_of(int64_t n, int chunk) { return (n + chunk - 1) / chunk; }
 
 struct GradList {
@@ -520,8 +524,7 @@ int launch_square_sums(const GradList &list, const int32_t *dtypes, int32_t dtyp
     for (; at < list.count && a.tensors < NORM_TENSORS; ++at) {
       if (list.g[at] == nullptr || list.size(at) == 0 || (dtypes && dtypes[at] != dtype)) continue;
       const int64_t more = chunks_of(list.size(at), NORM_CHUNK);
-      CG_REQUIRE(more < (int64_t(1) << 30), CG_ERR_RANGE, "a gradient of over 2^43 elements");
-      if (chunks + more >= (int64_t(1) << 30)) break;
+      if (chunks + more > INT32_MAX) break;
       a.g[a.tensors] = list.g[at];
       a.n[a.tensors] = list.size(at);
       a.first_chunk[a.tensors++] = int32_t(chunks);
@@ -586,7 +589,7 @@ void launch_updates(void (*kernel)(UpdateArgs<T, N>), int chunk, const cg_adamw_
     for (; at < n && a.tensors < N; ++at) {
       if (grads[at] == nullptr || tensors[at].n == 0) continue;
       const int64_t more = chunks_of(tensors[at].n, chunk);
-      if (chunks + more >= (int64_t(1) << 30)) break;
+      if (chunks + more > MOST_BLOCKS) break;
       a.t[a.tensors] = fill(tensors[at], grads[at]);
       a.first_chunk[a.tensors++] = int32_t(chunks);
       chunks += more;
@@ -619,7 +622,8 @@ int cg_grad_norm(const void *const *grads, const int64_t *sizes, const int32_t *
     CG_REQUIRE(n == 0 || (grads && sizes && dtypes), CG_ERR_INVALID, "grads, sizes and dtypes are required");
     CG_REQUIRE(n == 0 || workspace, CG_ERR_INVALID, "workspace is NULL");
     CG_REQUIRE(workspace_size >= cg_grad_norm_workspace_size(n), CG_ERR_INVALID, "workspace too small");
-    for (int i = 0; i < n; ++i) CG_REQUIRE(sizes[i] >= 0, CG_ERR_INVALID, "sizes must be non-negative");
+    for (int i = 0; i < n; ++i)
+      CG_REQUIRE(sizes[i] >= 0 && sizes[i] <= MOST_ELEMENTS, CG_ERR_RANGE, "a gradient's size is out of range");
     double *partials = static_cast<double *>(workspace);
     int64_t bytes = 0;
     for (int i = 0; i < n; ++i) bytes += grads[i] ? sizes[i] * dtype_size(dtypes[i]) : 0;
@@ -655,7 +659,7 @@ int cg_adamw_step(const cg_adamw_tensor *tensors, const void *const *grads, int3
     CG_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, CG_ERR_INVALID, "workspace must be 16-byte aligned");
     for (int i = 0; i < n; ++i) {
       const cg_adamw_tensor &t = tensors[i];
-      CG_REQUIRE(t.n >= 0 && t.n < int64_t(1) << 39, CG_ERR_RANGE, "a tensor's size is out of range");
+      CG_REQUIRE(t.n >= 0 && t.n <= MOST_ELEMENTS, CG_ERR_RANGE, "a tensor's size is out of range");
       if (t.n == 0 || grads[i] == nullptr) continue;
       CG_REQUIRE(t.param && t.exp_avg && t.exp_avg_sq && t.step, CG_ERR_INVALID, "a tensor's state is NULL");
       CG_REQUIRE(c.state_bits == 32 || (t.exp_avg_scale && t.exp_avg_sq_scale), CG_ERR_INVALID,
@@ -719,7 +723,7 @@ int cg_adamw_step(const cg_adamw_tensor *tensors, const void *const *grads, int3
 int cg_moment_values(const uint8_t *codes, const float *scales, int32_t is_signed, float *values, int64_t n,
                      void *stream) {
   return guarded([&] {
-    CG_REQUIRE(n >= 0 && n < int64_t(1) << 40, CG_ERR_RANGE, "n is out of range");
+    CG_REQUIRE(n >= 0 && n <= MOST_ELEMENTS, CG_ERR_RANGE, "n is out of range");
     if (n == 0) return;
     CG_REQUIRE(codes && scales && values, CG_ERR_INVALID, "codes, scales and values are required");
     const unsigned grid = unsigned(chunks_of(n, 4 * THREADS));

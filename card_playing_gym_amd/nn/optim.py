@@ -1,9 +1,9 @@
 """The optimiser step of an update on the HIP path: the gradients' global norm and AdamW over
 a model's tensors at once (csrc/optim.hip), moments in 32 bits or in 8-bit blocks.
 
-After ``loss.backward()`` through the trunk (nn/train.py), the trainer clips the gradients by
-their global norm and steps a fused ``torch.optim.AdamW`` (cardgym/rl/trainer.py:392-395).
-``AdamW`` does both in one call with a handful of launches, whatever the number of tensors::
+After ``loss.backward()`` through the trunk (nn/train.py) an update clips the gradients by their
+global norm and steps its optimiser (a fused Adam in cardgym/rl/trainer.py:392-395, which this is
+with ``weight_decay=0``).  ``AdamW`` does both in one call with a handful of launches::
 
     optimizer = AdamW(model.parameters(), lr=3e-4, max_norm=1.0)
     loss.backward()

@@ -585,8 +585,9 @@ int cg_policy_loss_backward(const cg_policy_loss *loss, const float *upstream, i
 
 /* ---- the optimiser step ------------------------------------------------------------------
  * What follows the training backward in an update: the gradients' global norm and one AdamW
- * step over many tensors (decoupled weight decay, bias-corrected moments), the work of
- * torch.nn.utils.clip_grad_norm_ and a fused torch.optim.AdamW.  Per element, with t the
+ * step over many tensors (decoupled weight decay, bias-corrected moments): the work of
+ * torch.nn.utils.clip_grad_norm_ and a fused torch.optim.AdamW (the reference's update steps a
+ * fused Adam, cardgym/rl/trainer.py:392-395: this one without weight decay).  Per element, with t the
  * tensor's step count after this step and c the clipping factor,
  *   g = c * grad;  m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2;
  *   p -= lr wd p + lr / (1 - beta1^t) * m / (sqrt(v / (1 - beta2^t)) + eps)

@@ -316,6 +316,46 @@ def test_elements_past_32_bits(device):
     assert not p[: n - keep].any() and not m[: n - keep].any() and not v[: n - keep].any()
 
 
+@pytest.mark.parametrize("offset", [0, 1], ids=["aligned", "off-by-1"])
+@pytest.mark.parametrize("dtype, bits", [(torch.float32, 32), (torch.float32, 8), (torch.bfloat16, 32)])
+def test_a_step_past_the_caches_is_the_same(device, dtype, bits, offset):
+    """Above 512 MB in all; the first and (32 bits) last elements against a small step over copies of them."""
+
+    n, few = 60_000_001, 40_000
+    gen = torch.Generator(device=device).manual_seed(3)
+    cut = lambda t: torch.cat([t.new_zeros(offset), t])[offset:]  # noqa: E731
+    p, g = (cut(torch.randn(n, generator=gen, device=device).to(dtype)) for _ in range(2))
+    if bits == 32:
+        state = [cut(torch.rand(n, generator=gen, device=device)) for _ in range(2)]
+    else:
+        state = [cut(torch.randint(0, 256, (n,), generator=gen, device=device, dtype=torch.uint8)) for _ in range(2)]
+    scales = [torch.rand(moment_blocks(n), generator=gen, device=device) for _ in range(2 if bits == 8 else 0)]
+
+    def plan(first, last):
+        part = lambda t: t[first:last].clone()  # noqa: E731
+        whole = first == 0 and last == n
+        p2, m2, v2 = (t if whole else part(t) for t in (p, *state))
+        s2 = [s if whole else s[first // 256 : first // 256 + moment_blocks(last - first)].clone() for s in scales]
+        names = dict(zip(("exp_avg_scales", "exp_avg_sq_scales"), ([s] for s in s2)))
+        return AdamWPlan([p2], [m2], [v2], [torch.tensor(3.0, device=device)], seed=5, **names), (p2, m2, v2, *s2)
+
+    norm = grad_norm([g])
+    exact = g.double().square().sum().sqrt().item()
+    assert abs(norm.item() - exact) <= 1e-12 * exact
+    parts = [(0, few - few % 256)] + ([(n - few, n)] if bits == 32 else [])
+    twins = [plan(a, b) for a, b in parts]
+    big, held = plan(0, n)
+    assert abs(big.step([g], max_norm=1.0, **OPTIONS).item() - exact) <= 1e-12 * exact
+    for (a, b), (small, expect) in zip(parts, twins):
+        small.step([g[a:b].clone()], max_norm=1.0, norm=norm, **OPTIONS)
+        for got, want in zip(held, expect):
+            got = got[a // 256 : a // 256 + want.numel()] if got.numel() != n else got[a:b]
+            if got.dtype == torch.uint8 or bits == 8:
+                assert torch.equal(got, want)
+            else:  # the two norms differ in fp64's last bits
+                assert torch.allclose(got.float(), want.float(), rtol=2 * HALF_STEP[got.dtype], atol=1e-12)
+
+
 def test_runs_repeat_bit_for_bit_on_any_stream(device):
     results = []
     for stream in (torch.cuda.current_stream(), torch.cuda.Stream()):

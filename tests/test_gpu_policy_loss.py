@@ -444,6 +444,23 @@ def test_rows_past_32_bit_offsets(device):
     assert torch.equal(out.log_probs[-4:], want.log_probs)
 
 
+@pytest.mark.parametrize("rows, width, dtype", [(9000, 32763, torch.bfloat16), (9000, 16387, torch.float32)])
+def test_a_loss_past_the_caches_is_the_same(device, rows, width, dtype):
+    """Above 512 MB of logits and gradient, rows at odd starts: as a call of a few hundred of them."""
+
+    gen = torch.Generator(device=device).manual_seed(1)
+    logits = torch.randn((rows, width), generator=gen, device=device, dtype=dtype)
+    inputs = [torch.randint(0, width, (rows,), generator=gen, device=device),
+              torch.full((rows,), -float(np.log(width)), device=device), torch.randn(rows, generator=gen, device=device)]
+    call = lambda a, b: run({"logits": logits[a:b], **dict(zip(("actions", "old", "advantages"), (t[a:b] for t in inputs)))},  # noqa: E731
+                            {"entropy_coef": 0.03, "normalizer": float(rows)})
+    out, grad = call(0, rows)
+    for a in (0, 4311, rows - 200):
+        few, few_grad = call(a, a + 200)
+        assert torch.equal(grad[a : a + 200], few_grad) and torch.equal(out.entropy[a : a + 200], few.entropy)
+        assert torch.equal(out.log_probs[a : a + 200], few.log_probs)
+
+
 def test_runs_repeat_bit_for_bit_on_any_stream(device):
     given, options = make(device, 5000, 300, torch.bfloat16, seed=18, reference="logits")
     want, want_grad = run(given, options)

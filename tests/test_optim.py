@@ -194,8 +194,9 @@ def test_native_refusals():
         assert status(**options) == nat.CG_ERR_INVALID, options
     tensors[0].step = None
     assert status() == nat.CG_ERR_INVALID
-    tensors[0].n = -1
-    assert status() == nat.CG_ERR_RANGE
+    for n in (-1, 2**33 + 1):
+        tensors[0].n = n
+        assert status() == nat.CG_ERR_RANGE
     assert lib.cg_adamw_step(tensors, grads, 1, None, None, 16, need, None) == nat.CG_ERR_INVALID
     sizes, dtypes = (ctypes.c_int64 * 1)(4), (ctypes.c_int32 * 1)(9)
     need = lib.cg_grad_norm_workspace_size(1)
@@ -203,6 +204,8 @@ def test_native_refusals():
     dtypes[0] = 0
     assert lib.cg_grad_norm(grads, sizes, dtypes, 1, None, 16, need, None) == nat.CG_ERR_INVALID
     assert lib.cg_grad_norm(grads, sizes, dtypes, 1, 16, 16, need - 1, None) == nat.CG_ERR_INVALID
+    sizes[0] = 2**33 + 1
+    assert lib.cg_grad_norm(grads, sizes, dtypes, 1, 16, 16, need, None) == nat.CG_ERR_RANGE
     assert lib.cg_moment_values(None, None, 1, None, 4, None) == nat.CG_ERR_INVALID
     assert lib.cg_moment_values(None, None, 1, None, -4, None) == nat.CG_ERR_RANGE
 
