@@ -308,6 +308,7 @@ _SIGNATURES = {
     ),
     "cg_attn_train_bwd": (c_int32, [P(AttnTrain), c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
     "cg_policy_loss_workspace_size": (c_size_t, [P(PolicyLoss)]),
+    "cg_policy_loss_backward_workspace_size": (c_size_t, [P(PolicyLoss)]),
     "cg_policy_loss_forward": (
         c_int32, [P(PolicyLoss), c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p],
     ),

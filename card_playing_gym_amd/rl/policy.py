@@ -72,17 +72,14 @@ class _Call:
             if x is not None:
                 getattr(d, name).device = x.data_ptr()
 
-    def workspace(self, device: torch.device) -> tuple[torch.Tensor, int]:
-        size = nat.lib().cg_policy_loss_workspace_size(self.descriptor)
-        return torch.empty(size, device=device, dtype=torch.uint8), size
-
     def forward(self, device: torch.device, grad: torch.Tensor | None) -> torch.Tensor:
         d = self.descriptor
         loss = torch.empty((), device=device)
         self.log_probs = torch.empty(d.rows, device=device)
         self.entropy = torch.empty(d.rows, device=device)
         self.kl = torch.empty(d.rows, device=device) if d.reference_logits or d.reference_log_probs else None
-        workspace, size = self.workspace(device)
+        size = nat.lib().cg_policy_loss_workspace_size(d)
+        workspace = torch.empty(size, device=device, dtype=torch.uint8)
         with _on(device):
             nat.call(
                 "cg_policy_loss_forward", d, loss.data_ptr(), self.log_probs.data_ptr(), self.entropy.data_ptr(),
@@ -116,10 +113,11 @@ class PolicyLossFunction(torch.autograd.Function):
         if grad is None:
             grad = torch.empty(logits.shape, device=device, dtype=logits.dtype)
         upstream = upstream.contiguous()
-        workspace, size = call.workspace(device)
+        size = nat.lib().cg_policy_loss_backward_workspace_size(call.descriptor)
+        workspace = torch.empty(size, device=device, dtype=torch.uint8) if size else None
         with _on(device):
             nat.call("cg_policy_loss_backward", call.descriptor, upstream.data_ptr(), int(written), grad.data_ptr(),
-                     workspace.data_ptr(), size, stream_handle(device))
+                     workspace.data_ptr() if size else None, size, stream_handle(device))
         return grad, None, None
 
 

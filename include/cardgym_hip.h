@@ -579,7 +579,9 @@ size_t cg_policy_loss_workspace_size(const cg_policy_loss *loss);
 int cg_policy_loss_forward(const cg_policy_loss *loss, float *value, float *log_probs, float *entropy, float *kl,
                            void *grad, void *workspace, size_t workspace_size, void *stream);
 /* grad [rows, width] = upstream[0] times the value's gradient, formed from the inputs and rounded
- * once.  written != 0: grad holds the forward's, and stays as it is where upstream[0] is 1. */
+ * once.  written != 0: grad holds the forward's, and stays as it is where upstream[0] is 1.
+ * workspace: of its own size, 0 (then NULL) for most shapes. */
+size_t cg_policy_loss_backward_workspace_size(const cg_policy_loss *loss);
 int cg_policy_loss_backward(const cg_policy_loss *loss, const float *upstream, int32_t written, void *grad,
                             void *workspace, size_t workspace_size, void *stream);
 

@@ -147,7 +147,8 @@ def test_native_refusals():
         for name, x in changes.items():
             setattr(d, name, x)
         if size < 0:  # short by that much
-            size += lib.cg_policy_loss_workspace_size(ctypes.byref(d))
+            size += (lib.cg_policy_loss_workspace_size if upstream is None else lib.cg_policy_loss_backward_workspace_size)(
+                ctypes.byref(d))
         if upstream is not None:
             return lib.cg_policy_loss_backward(ctypes.byref(d), upstream or None, 0, grad, workspace, size, None)
         return lib.cg_policy_loss_forward(ctypes.byref(d), value, log_probs, entropy, kl, None, workspace, size, None)
@@ -155,8 +156,8 @@ def test_native_refusals():
     for changes in ({"value": None}, {"workspace": None}, {"size": -1}, {"rows": 3, "width": 20000, "size": -1}, {"log_probs": None}, {"entropy": None},
                     {"kl": 16}, {"rows": -1}, {"width": 0}, {"dtype": 5}, {"logits": None}, {"actions": None},
                     {"old_log_probs": None}, {"advantages": None}, {"ld_logits": -1}, {"reference_logits": 16},
-                    {"reference_logits": 16, "reference_log_probs": 16, "kl": 16}, {"upstream": 0}, {"upstream": 16, "grad": None}, {"upstream": 16, "workspace": None},
-                    {"upstream": 16, "size": -1}):
+                    {"reference_logits": 16, "reference_log_probs": 16, "kl": 16}, {"upstream": 0}, {"upstream": 16, "grad": None},
+                    {"upstream": 16, "width": 40000, "workspace": None}, {"upstream": 16, "width": 40000, "size": -1}):
         assert call(**changes) == nat.CG_ERR_INVALID, changes
     assert lib.cg_policy_loss_forward(None, 16, 16, 16, None, None, 16, size, None) == nat.CG_ERR_INVALID
     assert call(width=(1 << 30) + 1) == nat.CG_ERR_UNSUPPORTED
