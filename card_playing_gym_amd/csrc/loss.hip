@@ -368,14 +368,16 @@ __device__ __forceinline__ RowScalars row_scalars(const LossArgs &a, const RowIn
   double value = -(part < whole ? part : whole) - c * o.entropy;
   double own = r == bounded || whole < part ? -whole : 0;
   if (whole != whole) own = value = whole;
-  if constexpr (REF) {
-    value += beta * kl;
-    base -= beta * kl;
-  } else if (a.ref) {
-    const double d = double(in.ref) - o.log_p, rise = exp_of(d) - 1;
+  double rise = 0;
+  if (!REF && a.ref) {
+    const double d = double(in.ref) - o.log_p;
+    rise = exp_of(d) - 1;
     kl = rise == INFINITY ? rise : rise - d;
+  }
+  if (beta != 0) {  // (with a coefficient of 0 a reference is reported only, whatever it holds)
     value += beta * kl;
     own -= beta * rise;
+    if (REF) base -= beta * kl;
   }
   o.kl = kl;
   const double weight = in.weight, f = weight * k.scale;
@@ -419,7 +421,8 @@ template <bool REF>
 __device__ __forceinline__ float grad_of(float z, float y, float top, const RowCoefs &c) {
   const Entry n = entry_of(z, top);
   float u = fmaf(c.slope, n.x, c.base);
-  if (REF) u = fmaf(c.pull, gap_of<REF>(n.e, z, y, c.shift), u);
+  // (finite: a reference's 0 where p is not, or its NaN, is the KL's to tell, and none of a pull of 0)
+  if (REF) u = fmaf(c.pull, fminf(gap_of<REF>(n.e, z, y, c.shift), 3e38f), u);
   return n.e * u;
 }
 
@@ -505,7 +508,8 @@ __global__ __launch_bounds__((G > 256 ? G : 256), (ROOM<S, G, E, REF>)) void row
       if constexpr (REF) load_entries<G, C, V>(y.w, ref, legal, lane * V, a.width, streams);
       action_logit = logit_of<T>(a, row, inputs.action);
     } else {
-      z.clear(), y.clear();
+      z.clear();
+      if constexpr (REF) y.clear();
     }
     RowSums q;
     float tops[REF ? 2 : 1];
@@ -520,7 +524,8 @@ __global__ __launch_bounds__((G > 256 ? G : 256), (ROOM<S, G, E, REF>)) void row
     join<G>(tops, slots.tops, Most{});
     q.top = tops[0] > -INFINITY ? tops[0] : 0.f;
     q.ref_top = REF && tops[REF ? 1 : 0] > -INFINITY ? tops[REF ? 1 : 0] : 0.f;
-    z.forget(), y.forget();
+    z.forget();
+    if constexpr (REF) y.forget();
     Sum<REF> s = 0, rs = 0;
     float t = 0;
 #pragma unroll
@@ -535,7 +540,8 @@ __global__ __launch_bounds__((G > 256 ? G : 256), (ROOM<S, G, E, REF>)) void row
     if constexpr (REF) sums[2] = rs;
     join<G>(sums, slots.sums, Add{});
     q.s = sums[0], q.t = sums[1], q.ref_s = REF ? sums[REF ? 2 : 0] : 0;
-    z.forget(), y.forget();
+    z.forget();
+    if constexpr (REF) y.forget();
     const RowScalars o = row_scalars<REF>(a, inputs, action_logit, q, coefs, [&](float shift) {
       float g = 0;
 #pragma unroll
@@ -547,7 +553,8 @@ __global__ __launch_bounds__((G > 256 ? G : 256), (ROOM<S, G, E, REF>)) void row
       join<G>(gaps, slots.gaps, Add{});
       return gaps[0];
     });
-    z.forget(), y.forget();
+    z.forget();
+    if constexpr (REF) y.forget();
     if (!in) continue;  // (all lanes of a group; the reductions are behind)
     if (lane == 0 && a.log_probs) {
       if (o.live) value += o.value;

@@ -156,7 +156,7 @@ def policy_loss(
 
     A row of weight 0 (padding) is not read: like a row without a legal entry it adds nothing, has a
     zero gradient and reports zeros.  An action outside the row makes its row, and the loss, NaN; one that
-    is not legal has log p = -inf."""
+    is not legal has log p = -inf.  With a ``kl_coef`` of 0 a reference is reported only, whatever it holds."""
 
     if logits.dim() != 2 or logits.shape[1] == 0:
         raise ValueError("logits must be [rows, width] with at least one entry a row")

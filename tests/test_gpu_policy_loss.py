@@ -280,6 +280,32 @@ def test_values_that_are_not_finite_in_legal_places(device, width):
     assert torch.equal(torch.isnan(grad).any(1), bad) and torch.isfinite(grad[~bad]).all()
 
 
+@pytest.mark.parametrize("width", [40, 600, 40000])
+def test_a_reference_that_is_only_reported(device, width):
+    """With a coefficient of 0 the loss and its gradient are those without a reference (to the roundings of
+    the other sums), though the reference excludes legal entries or holds NaN; with another its infinite KL shows."""
+
+    given, options = make(device, 6, width, torch.float32, seed=21, reference="logits")
+    plain = {k: v for k, v in options.items() if k not in ("reference_logits", "kl_coef")}
+    want, want_grad = run(given, plain)
+    options["reference_logits"][1] = -torch.inf
+    options["reference_logits"][2, given["actions"][2]] = -torch.inf
+    options["reference_logits"][3] = torch.nan
+    for zero in (0.0, torch.zeros((), device=device)):
+        out, grad = run(given, {**options, "kl_coef": zero})
+        assert abs(out.loss.item() - want.loss.item()) <= 1e-6
+        assert (grad - want_grad).abs().max() <= 1e-5 * want_grad.abs().max()
+        assert torch.isinf(out.kl[1:3]).all() and torch.isnan(out.kl[3]) and torch.isfinite(out.kl[4:]).all()
+    out, _ = run(given, {**options, "weights": torch.tensor([1, 1, 1, 0, 1, 1.0], device=device)})
+    assert out.loss == torch.inf
+    sampled = {**plain, "reference_log_probs": given["old"].clone()}
+    sampled["mask"] = sampled["mask"].clone()
+    sampled["mask"][2, given["actions"][2]] = False
+    out, grad = run(given, sampled)
+    assert torch.isfinite(out.loss) and torch.isfinite(grad).all() and out.kl[2] == torch.inf
+    assert run(given, {**sampled, "kl_coef": 0.1})[0].loss == torch.inf
+
+
 def test_an_action_that_is_not_legal(device):
     given, options = make(device, 3, 20, torch.float32, seed=10)
     options["mask"][1, given["actions"][1]] = False
