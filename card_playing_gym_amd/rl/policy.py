@@ -99,6 +99,7 @@ class PolicyLossFunction(torch.autograd.Function):
         ctx.written = torch.empty(logits.shape, device=logits.device, dtype=logits.dtype)
         ctx.save_for_backward(*tensors)
         ctx.call = call
+        ctx.capturing = torch.cuda.is_current_stream_capturing()
         return call.forward(logits.device, ctx.written)
 
     @staticmethod
@@ -109,6 +110,8 @@ class PolicyLossFunction(torch.autograd.Function):
         call, logits, device = ctx.call, tensors[0], upstream.device
         call.bind(tensors)  # (a saved-tensor hook may have brought them back elsewhere)
         grad, ctx.written = ctx.written, None  # handed over once: a second backward forms its own
+        if torch.cuda.is_current_stream_capturing() != ctx.capturing:
+            grad = None  # a replay of one alone would find, or leave, what the other's buffer holds by then
         written = grad is not None
         if grad is None:
             grad = torch.empty(logits.shape, device=device, dtype=logits.dtype)
@@ -152,7 +155,7 @@ def policy_loss(
     ``reference_log_probs``: float32 [rows].  ``normalizer``: the number of rows; pass the whole
     minibatch's count where a microbatch's gradients are accumulated.  ``clip_high``: ``clip``.
     ``normalizer`` and the coefficients may be float32 device scalars, which a captured loss reads at
-    every replay.
+    every replay.  A backward captured in a graph of its own follows one replay of its forward's each time.
 
     A row of weight 0 (padding) is not read: like a row without a legal entry it adds nothing, has a
     zero gradient and reports zeros.  An action outside the row makes its row, and the loss, NaN; one that

@@ -532,6 +532,47 @@ def test_a_captured_loss(device, width):
         assert torch.equal(out.loss, want.loss) and torch.equal(grad, want_grad) and torch.equal(out.kl, want.kl)
 
 
+def test_one_direction_captured(device):
+    """An eager forward's backward in a graph forms its gradient at every replay, whatever became of the last;
+    a captured forward's eager gradient is no buffer of the graph's."""
+
+    given, options = make(device, 40, 50, torch.float32, seed=31)
+    static = {k: v.clone() for k, v in given.items()}
+    leaf = static["logits"].requires_grad_()
+    _, want = run(given, options)
+    stream = torch.cuda.Stream()
+
+    def loss():
+        return policy_loss(leaf, static["actions"], static["old"], static["advantages"], **options).loss
+
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        eager = loss()
+        torch.autograd.grad(loss(), leaf)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        grad, = torch.autograd.grad(eager, leaf, retain_graph=True)
+    for _ in range(3):
+        grad.fill_(7)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(grad, want)
+    forward = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(forward, stream=stream):
+        captured = loss()
+    forward.replay()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        mine, = torch.autograd.grad(captured, leaf, retain_graph=True)
+        mine.fill_(5)
+        again, = torch.autograd.grad(captured, leaf)
+    forward.replay()
+    torch.cuda.synchronize()
+    assert (mine == 5).all() and torch.equal(again, want)
+
+
 # ---- the update as a program runs it ------------------------------------------------------------------
 
 
