@@ -136,7 +136,8 @@ class AdamWPlan:
     ``params``: contiguous tensors of one type (float32, bfloat16 or float16) on one GPU.
     ``exp_avgs`` / ``exp_avg_sqs``: float32 of the parameters' sizes; or, with moments in 8 bits,
     uint8 codes of those sizes beside ``exp_avg_scales`` / ``exp_avg_sq_scales``, float32
-    [ceil(size / 256)] each.  All zeros before the first step.  ``steps``: a float32 scalar each, the
+    [ceil(size / 256)] each.  All zeros before the first step.  A gradient that is not finite spoils its
+    element; with moments in 8 bits, its block.  ``steps``: a float32 scalar each, the
     number of steps taken.  ``seed`` and ``first`` (the place of the first tensor) choose the 8-bit
     moments' random numbers.
 
@@ -288,8 +289,9 @@ class AdamW(torch.optim.Optimizer):
     reads at every replay; its other options are captured as they are.
 
     ``state_dict`` has ``torch.optim.AdamW``'s layout, and with ``state_bits=32`` its state dicts
-    load; 8-bit state holds codes (uint8) and ``exp_avg_scale`` / ``exp_avg_sq_scale``.  Loading
-    copies into state that is already there, so a captured step goes on with what was loaded.
+    load (not with options that this step lacks); 8-bit state holds codes (uint8) and
+    ``exp_avg_scale`` / ``exp_avg_sq_scale``.  Loading copies into state, and a learning rate on the
+    device, that is already there, so a captured step goes on with what was loaded.
     ``state`` itself is read, not replaced: to start over, build a new optimiser."""
 
     def __init__(
@@ -318,7 +320,7 @@ class AdamW(torch.optim.Optimizer):
     def _forget(self) -> None:
         self.norm: torch.Tensor | None = None
         self._plans: list[tuple[int, AdamWPlan]] | None = None  # (group, plan); None: to be built
-        self._captured: list[AdamWPlan] = []  # a graph's replays use what these hold
+        self._captured: list[tuple] = []  # plans and learning rates: a graph's replays use what these hold
         self._planned: tuple[int, int] | None = None
         self._stateless: list[torch.Tensor] = []
 
@@ -362,6 +364,10 @@ class AdamW(torch.optim.Optimizer):
         ours = [p for group in self.param_groups for p in group["params"]]
         theirs = [i for group in state_dict["param_groups"] for i in group["params"]]
         names = _STATE[self.state_bits]
+        for group in state_dict["param_groups"]:
+            if group.get("amsgrad") or group.get("maximize") or (
+                    group["weight_decay"] and not group.get("decoupled_weight_decay", True)):
+                raise ValueError("the state dict's options (amsgrad, maximize, a coupled decay) are not this step's")
         loaded = {}
         for p, i in zip(ours, theirs):
             given = state_dict["state"].get(i)
@@ -379,7 +385,12 @@ class AdamW(torch.optim.Optimizer):
                     raise ValueError(f"{name} must hold uint8 codes")
             loaded[p] = given
         before = {p: self.state[p] for p in ours if p in self.state}
+        rates = [group["lr"] for group in self.param_groups]
         super().load_state_dict(state_dict)  # groups; its copies of the state are of the parameters' types
+        for group, lr in zip(self.param_groups, rates):
+            if isinstance(lr, torch.Tensor):
+                lr.copy_(torch.as_tensor(group["lr"]).reshape(lr.shape))
+                group["lr"] = lr
         for p, given in loaded.items():
             state = before.get(p) or self._new_state(p)
             for name in names:
@@ -441,6 +452,6 @@ class AdamW(torch.optim.Optimizer):
             group = self.param_groups[index]
             self.norm = plan.step(many, lr=group["lr"], betas=group["betas"], eps=group["eps"],
                                   weight_decay=group["weight_decay"], max_norm=self.max_norm, norm=norm)
-            if capturing and plan not in self._captured:
-                self._captured.append(plan)
+            if capturing and not any(plan is p and group["lr"] is lr for p, lr in self._captured):
+                self._captured.append((plan, group["lr"]))
         return loss

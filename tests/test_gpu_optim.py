@@ -541,6 +541,33 @@ def test_a_captured_step_counts_on(device, bits):
     assert all(torch.equal(a, b) for a, b in zip(*results))
 
 
+def test_a_captured_step_follows_a_loaded_state(device):
+    """State and learning rate are loaded into what a captured step reads."""
+
+    p = torch.nn.Parameter(torch.randn(300, device=device))
+    optimizer = AdamW([p], lr=torch.tensor(1e-2, device=device))
+    p.grad = torch.ones_like(p)
+    optimizer.step()
+    saved = copy.deepcopy(optimizer.state_dict())
+    saved["param_groups"][0]["lr"] = torch.tensor(1e-3)  # (a file's, on the host)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        optimizer.step()
+    graph.replay()
+    optimizer.load_state_dict(saved)
+    twin = torch.nn.Parameter(p.detach().clone())
+    other = AdamW([twin], lr=1.0)
+    other.load_state_dict(saved)
+    other.param_groups[0]["lr"] = torch.tensor(1e-3, device=device)
+    for _ in range(3):
+        twin.grad = p.grad.clone()
+        other.step()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(p, twin) and optimizer.state[p]["step"] == other.state[twin]["step"]
+
+
 @pytest.mark.parametrize("through", ["optimizer", "plan"])
 def test_a_rollout_after_a_step_uses_the_new_weights(device, through):
     """The decode path's bf16 weight copies follow the step: bit for bit a model that was loaded with the stepped

@@ -237,3 +237,30 @@ def test_state_dict_refusals(anywhere):
     other = AdamW([torch.nn.Parameter(torch.zeros(299))])
     with pytest.raises(ValueError, match="shape"):
         other.load_state_dict(theirs.state_dict())
+
+
+def test_state_dicts_of_other_steps_are_refused(anywhere):
+    """Options that change the step, which it would leave out without a word."""
+
+    p = torch.nn.Parameter(torch.zeros(300))
+    p.grad = torch.ones(300)
+    for theirs in (torch.optim.AdamW([p], amsgrad=True), torch.optim.AdamW([p], maximize=True),
+                   torch.optim.Adam([p], weight_decay=0.1)):
+        theirs.step()
+        with pytest.raises(ValueError, match="options"):
+            AdamW([p]).load_state_dict(theirs.state_dict())
+    theirs = torch.optim.Adam([p])
+    theirs.step()
+    ours = AdamW([p])
+    ours.load_state_dict(theirs.state_dict())
+    assert ours.param_groups[0]["weight_decay"] == 0 and float(ours.state[p]["step"]) == 1
+
+
+def test_a_loaded_learning_rate_goes_into_the_one_that_is_there(anywhere):
+    """A captured step reads it there; a state dict's may lie on another device."""
+
+    p, lr = torch.nn.Parameter(torch.zeros(3)), torch.tensor(0.5)
+    ours = AdamW([p], lr=lr)
+    for given in (0.25, torch.tensor(0.125), torch.tensor([0.0625])):
+        ours.load_state_dict(AdamW([torch.nn.Parameter(torch.zeros(3))], lr=given).state_dict())
+        assert ours.param_groups[0]["lr"] is lr and lr == given
