@@ -166,6 +166,8 @@ def policy_loss(
     require_device(logits)
     dtype_code(logits.dtype)
     rows, width = logits.shape
+    if rows >= 2**31 or width > 2**30:  # (the descriptor's 32 bits would keep their lower ones)
+        raise ValueError("logits may have up to 2^31 - 1 rows of up to 2^30 entries")
     device = logits.device
     vector = (rows,)
     _constant(actions, "actions", vector, torch.int64, device)

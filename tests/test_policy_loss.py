@@ -129,6 +129,16 @@ def test_refusals(anywhere, changes, message):
         _call(**changes)
 
 
+@pytest.mark.parametrize("rows, width", [(2**32 + 4, 6), (2**31, 1), (4, 2**32 + 6), (4, 2**30 + 1)])
+def test_sizes_past_the_descriptors_are_refused(anywhere, rows, width):
+    """2^32 + 4 rows must not become 4."""
+
+    vector = lambda dtype=torch.float32: torch.zeros((), dtype=dtype).expand(rows)  # noqa: E731
+    with pytest.raises(ValueError, match="up to"):
+        _call(logits=torch.zeros(()).expand(rows, width), actions=vector(torch.int64), old_log_probs=vector(),
+              advantages=vector())
+
+
 def test_cpu_tensors_are_refused():
     with pytest.raises(RuntimeError, match="ROCm"):
         _call()
