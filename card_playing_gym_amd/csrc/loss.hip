@@ -31,7 +31,9 @@ constexpr int MAX_BLOCKS = 2048;  // and partial sums of the loss
 // bf16 entries (537 MB) 135 -> 128 us.  Below, whatever made the logits or takes the gradient may find them there.
 constexpr int64_t STREAM_BYTES = 512 << 20;
 constexpr float LOG2E = 1.44269504088896340736f, LOG2E_REST = float(1.44269504088896340736 - double(LOG2E));
-constexpr float LOWEST = -1e30f;  // in place of the log-probability of an entry with p = 0 where p multiplies it
+// The least x = z - top that p = e^x is multiplied by: e^x is 0 from -104 on.  No lower, so that the coefficient
+// of x may be as large as 2^120 before the product is infinite, which times p = 0 is NaN.
+constexpr float LOWEST = -128.f;
 
 struct Scalar {
   float value;

@@ -573,6 +573,21 @@ def test_one_direction_captured(device):
     assert (mine == 5).all() and torch.equal(again, want)
 
 
+@pytest.mark.parametrize("upstream", [2.0**32, 2.0**110])
+@pytest.mark.parametrize("rows, width", [(6, 3), (6, 40), (6, 600), (6, 3000), (6, 40000), (70, 70001)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+def test_large_coefficients_leave_masked_places_zero(device, dtype, rows, width, upstream):
+    """The gradient of an entry of p = 0 is 0 by whatever factor the row's coefficients are large (a loss scale, or a
+    small normalizer); the others stay at the bars of one rounding."""
+
+    given, options = make(device, rows, width, dtype, seed=23, reference="logits" if width % 2 else None)
+    options |= {"entropy_coef": 0.5, "normalizer": 1.0}
+    given["logits"][1, (given["actions"][1] + 1) % width] = -torch.inf  # (not legal by its logit)
+    out, grad = run(given, options, upstream)
+    assert torch.isfinite(grad).all() and (grad[~options["mask"]] == 0).all()
+    check(given, options, out, grad, upstream=upstream)
+
+
 # ---- the update as a program runs it ------------------------------------------------------------------
 
 
