@@ -361,6 +361,25 @@ class AdamW(torch.optim.Optimizer):
         return state
 
     def load_state_dict(self, state_dict) -> None:
+        # Between the caller's hooks: the dict is checked as the last pre-hook leaves it, before anything is loaded, and
+        # the state is in place for the first post-hook.
+        held = {p: self.state[p] for group in self.param_groups for p in group["params"] if p in self.state}
+        rates = [group["lr"] for group in self.param_groups]
+        loaded: dict[torch.Tensor, dict] = {}
+        hooks = [
+            self.register_load_state_dict_pre_hook(lambda _, given: loaded.update(self._checked(given))),
+            self.register_load_state_dict_post_hook(lambda _: self._place(loaded, held, rates), prepend=True),
+        ]
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            for hook in hooks:
+                hook.remove()
+        self._plans = None
+
+    def _checked(self, state_dict) -> dict[torch.Tensor, dict]:
+        """The parameters' entries of a state dict, if its options and its state are this step's."""
+
         ours = [p for group in self.param_groups for p in group["params"]]
         theirs = [i for group in state_dict["param_groups"] for i in group["params"]]
         names = _STATE[self.state_bits]
@@ -384,19 +403,20 @@ class AdamW(torch.optim.Optimizer):
                 if self.state_bits == 8 and name in ("exp_avg", "exp_avg_sq") and x.dtype != torch.uint8:
                     raise ValueError(f"{name} must hold uint8 codes")
             loaded[p] = given
-        before = {p: self.state[p] for p in ours if p in self.state}
-        rates = [group["lr"] for group in self.param_groups]
-        super().load_state_dict(state_dict)  # groups; its copies of the state are of the parameters' types
+        return loaded
+
+    def _place(self, loaded: dict[torch.Tensor, dict], held: dict[torch.Tensor, dict], rates: list) -> None:
+        """What was loaded, in the types of this state, into the state and the learning rates that were there."""
+
         for group, lr in zip(self.param_groups, rates):
             if isinstance(lr, torch.Tensor):
                 lr.copy_(torch.as_tensor(group["lr"]).reshape(lr.shape))
                 group["lr"] = lr
         for p, given in loaded.items():
-            state = before.get(p) or self._new_state(p)
-            for name in names:
+            state = held.get(p) or self._new_state(p)
+            for name in _STATE[self.state_bits]:
                 state[name].copy_(torch.as_tensor(given[name]).reshape(state[name].shape))
             self.state[p] = state
-        self._plans = None
 
     # -- the step --------------------------------------------------------------------------
 

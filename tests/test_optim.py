@@ -3,6 +3,7 @@ oracle against torch.optim.AdamW, and every refusal."""
 
 from __future__ import annotations
 
+import copy
 import ctypes
 
 import numpy as np
@@ -264,3 +265,90 @@ def test_a_loaded_learning_rate_goes_into_the_one_that_is_there(anywhere):
     for given in (0.25, torch.tensor(0.125), torch.tensor([0.0625])):
         ours.load_state_dict(AdamW([torch.nn.Parameter(torch.zeros(3))], lr=given).state_dict())
         assert ours.param_groups[0]["lr"] is lr and lr == given
+
+
+def _stepped(optimizer):
+    """A parameter of ones with one step of torch's, and its optimiser's state dict."""
+
+    p = torch.nn.Parameter(torch.zeros(300))
+    p.grad = torch.ones(300)
+    theirs = optimizer([p])
+    theirs.step()
+    return p, theirs.state_dict()
+
+
+@pytest.mark.parametrize("in_place", [False, True])
+def test_load_hooks_are_obeyed(anywhere, in_place):
+    """What a pre-hook makes of the dict is what is checked and loaded, state and options; a post-hook finds the state
+    loaded and what it sets stays.  As torch.optim.AdamW does it."""
+
+    p, saved = _stepped(torch.optim.AdamW)
+    seen = []
+
+    def before(optimizer, given):
+        entry = {**given["state"][0], "exp_avg": torch.full((300,), 7.0)}
+        groups = [{**group, "lr": 0.5} for group in given["param_groups"]]
+        if in_place:
+            given["state"], given["param_groups"] = {0: entry}, groups
+            return None
+        return {"state": {0: entry}, "param_groups": groups}
+
+    def after(optimizer):
+        state = optimizer.state[p]
+        seen.append((float(state["exp_avg"][0]), float(state["step"]), optimizer.param_groups[0]["lr"]))
+        state["exp_avg_sq"].fill_(3)
+        optimizer.param_groups[0]["eps"] = 0.25
+
+    for kind in (torch.optim.AdamW, AdamW):
+        optimizer = kind([p])
+        optimizer.register_load_state_dict_pre_hook(before)
+        optimizer.register_load_state_dict_post_hook(after)
+        for _ in range(2):  # (the second into state that is there)
+            given = copy.deepcopy(saved)
+            optimizer.load_state_dict(given)
+            state = optimizer.state[p]
+            assert (state["exp_avg"] == 7).all() and (state["exp_avg_sq"] == 3).all() and float(state["step"]) == 1
+            assert optimizer.param_groups[0]["lr"] == 0.5 and optimizer.param_groups[0]["eps"] == 0.25
+    assert seen == [(7.0, 1.0, 0.5)] * 4
+    assert torch.equal(given["state"][0]["exp_avg_sq"], saved["state"][0]["exp_avg_sq"])  # (the caller's, not ours)
+
+
+def test_hooks_see_moments_as_they_are_saved(anywhere):
+    """Not by way of the parameter's type: 1 + 2^-20 has no bf16, code 200 of uint8 stays a code."""
+
+    p = torch.nn.Parameter(torch.zeros(300, dtype=torch.bfloat16))
+    seen = []
+    for bits, value in ((32, 1 + 2.0**-20), (8, 200)):
+        optimizer = AdamW([p], state_bits=bits)
+        optimizer.register_load_state_dict_post_hook(lambda o: seen.append(o.state[p]["exp_avg"].clone()))
+        state = {name: x + (value if name == "exp_avg" else 0) for name, x in optimizer._new_state(p).items()}
+        optimizer.load_state_dict({**optimizer.state_dict(), "state": {0: state}})
+        assert seen[-1].dtype == state["exp_avg"].dtype and (seen[-1] == value).all()
+
+
+def test_dicts_that_hooks_make_are_checked(anywhere):
+    """Before anything is loaded: a hook may repair a dict, and one that breaks it changes nothing."""
+
+    p, saved = _stepped(lambda params: torch.optim.AdamW(params, amsgrad=True))
+    repaired = AdamW([p])
+    repaired.register_load_state_dict_pre_hook(
+        lambda o, given: {**given, "param_groups": [{**g, "amsgrad": False} for g in given["param_groups"]]})
+    repaired.load_state_dict(saved)
+    assert float(repaired.state[p]["step"]) == 1
+    lr = torch.tensor(0.5)
+    ours = AdamW([p], lr=lr)
+    ours.load_state_dict({**repaired.state_dict(), "param_groups": ours.state_dict()["param_groups"]})
+    held = ours.state[p]
+    kept = {name: x.clone() for name, x in held.items()}
+    handle = ours.register_load_state_dict_pre_hook(
+        lambda o, given: {**given, "state": {0: {**given["state"][0], "exp_avg": torch.zeros(299)}}})
+    groups = ours.param_groups
+    given = repaired.state_dict()
+    for _ in range(2):
+        with pytest.raises(ValueError, match="shape"):
+            ours.load_state_dict(given)
+        assert ours.state[p] is held and all(torch.equal(held[name], x) for name, x in kept.items())
+        assert ours.param_groups is groups and groups[0]["lr"] is lr and lr == 0.5
+    handle.remove()
+    ours.load_state_dict(given)
+    assert lr == 1e-3
