@@ -13,6 +13,7 @@ from __future__ import annotations
 from typing import NamedTuple
 
 import torch
+from torch.autograd import forward_ad
 
 from .. import _native as nat
 from ..nn.kv_cache import dtype_code, require_device, stream_handle
@@ -35,6 +36,15 @@ def _constant(t: torch.Tensor, name: str, shape: tuple[int, ...], dtype: torch.d
     if t.requires_grad:
         raise ValueError(f"{name} is a constant of the loss: detach it")
     return t
+
+
+def _no_tangents(*tensors) -> None:
+    """Refuses forward-mode derivatives, which nothing behind this would carry on.  (Outside a level no tensor has
+    one: asking each would be 6 us of a small loss's 96.)"""
+
+    if getattr(forward_ad, "_current_level", 0) >= 0:
+        if any(isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+            raise RuntimeError("policy_loss has no forward-mode derivative: pass the inputs without tangents")
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
@@ -142,7 +152,7 @@ def policy_loss(
     reference_log_probs: torch.Tensor | None = None,
 ) -> PolicyLoss:
     """sum_i weights_i l_i / normalizer over the rows of ``logits`` [rows, width] (float32, bfloat16
-    or float16), differentiable in the logits, with
+    or float16), differentiable in the logits (once, backwards; forward-mode tangents are refused), with
 
         r = exp(log p[action] - old_log_prob)
         l = -min(r A, clamp(r, 1 - clip, 1 + clip_high) A) + kl_coef KL - entropy_coef H
@@ -165,6 +175,8 @@ def policy_loss(
         raise ValueError("logits must be [rows, width] with at least one entry a row")
     require_device(logits)
     dtype_code(logits.dtype)
+    _no_tangents(logits, old_log_probs, advantages, weights, normalizer, entropy_coef, kl_coef, reference_logits,
+                 reference_log_probs)
     rows, width = logits.shape
     if rows >= 2**31 or width > 2**30:  # (the descriptor's 32 bits would keep their lower ones)
         raise ValueError("logits may have up to 2^31 - 1 rows of up to 2^30 entries")

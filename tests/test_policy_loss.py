@@ -189,3 +189,20 @@ def test_struct_layouts_of_the_update_match_the_header(tmp_path):
         cname, field, value = line.split()
         py = structs[cname]
         assert int(value) == (ctypes.sizeof(py) if field == "size" else getattr(py, field).offset), line
+
+
+@pytest.mark.parametrize("name", ["logits", "old_log_probs", "advantages", "weights", "reference_logits",
+                                  "reference_log_probs", "normalizer", "entropy_coef", "kl_coef"])
+@pytest.mark.parametrize("wanted", [False, True])
+def test_forward_derivatives_are_refused(anywhere, name, wanted):
+    """The loss would come back without the derivative that was asked for; with its own gradient wanted or not."""
+
+    from torch.autograd import forward_ad
+
+    shape = {"logits": (4, 6), "reference_logits": (4, 6), "normalizer": (), "entropy_coef": (), "kl_coef": ()}.get(name, (4,))
+    changes = {"logits": torch.zeros(4, 6, requires_grad=wanted and name != "logits")}
+    if name == "kl_coef":
+        changes["reference_log_probs"] = torch.zeros(4)
+    with forward_ad.dual_level():
+        with pytest.raises(RuntimeError, match="forward"):
+            _call(**(changes | {name: forward_ad.make_dual(torch.ones(shape), torch.ones(shape))}))
