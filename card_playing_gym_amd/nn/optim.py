@@ -85,6 +85,12 @@ def grad_norm(grads: Iterable[torch.Tensor | None]) -> torch.Tensor:
     device: the norm that ``torch.nn.utils.clip_grad_norm_`` clips by.  The squares are added in
     float64, so neither large nor tiny gradients lose it."""
 
+    return _grad_norm(grads, None)
+
+
+def _grad_norm(grads: Iterable[torch.Tensor | None], out: torch.Tensor | None) -> torch.Tensor:
+    """``grad_norm``, into ``out`` where it is given."""
+
     grads = _dense([g for g in grads if g is not None])
     if not grads:
         raise ValueError("grad_norm needs at least one gradient")
@@ -95,7 +101,7 @@ def grad_norm(grads: Iterable[torch.Tensor | None]) -> torch.Tensor:
     n = len(grads)
     dtypes = array.array("i", [dtype_code(g.dtype) for g in grads])
     pointers, sizes = _addresses([_ptr(g) for g in grads]), array.array("q", [_numel(g) for g in grads])
-    norm = torch.empty((), device=device, dtype=torch.float64)
+    norm = torch.empty((), device=device, dtype=torch.float64) if out is None else out
     size = nat.lib().cg_grad_norm_workspace_size(n)
     workspace = torch.empty(size, device=device, dtype=torch.uint8)
     with _on(device):
@@ -243,6 +249,11 @@ class AdamWPlan:
         scaled by min(1, max_norm / (norm + 1e-6)): by ``norm`` (a float64 scalar, ``grad_norm``'s)
         where it is given, else by the norm of these gradients.  Returns the norm it clipped by."""
 
+        return self._step(grads, lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, max_norm=max_norm, norm=norm)
+
+    def _step(self, grads, *, lr, betas, eps, weight_decay, max_norm, norm, out=None) -> torch.Tensor | None:
+        """``step``, its own norm written into ``out`` where that is given."""
+
         if list(map(_ptr, self.params)) != self._addresses:
             raise ValueError("a parameter's data moved since the plan was built: build a new plan")
         pointers, kept = self._gradient_addresses(list(grads))
@@ -254,7 +265,7 @@ class AdamWPlan:
         if max_norm is not None:
             clip = nat.CG_CLIP_OWN_NORM if norm is None else nat.CG_CLIP_GIVEN_NORM
             if norm is None:
-                norm = torch.empty((), device=self.device, dtype=torch.float64)
+                norm = torch.empty((), device=self.device, dtype=torch.float64) if out is None else out
             else:
                 _scalar(norm, "norm", torch.float64, self.device)
         config = nat.AdamWConfig(
@@ -284,7 +295,8 @@ class AdamW(torch.optim.Optimizer):
 
     ``max_norm``: the norm of all groups' gradients together is clipped to it, as
     ``clip_grad_norm_`` before the step would; ``norm`` then holds the last step's norm (a float64
-    device scalar).  ``state_bits``: 32, or 8 for moments in blocks of 256 (see
+    device scalar; 0 of no gradients): a new one each step until a step is captured, from then on one that
+    every step and replay writes.  ``state_bits``: 32, or 8 for moments in blocks of 256 (see
     :class:`AdamWPlan`).  A group's ``lr`` may be a float32 device scalar, which a captured step
     reads at every replay; its other options are captured as they are.
 
@@ -319,6 +331,7 @@ class AdamW(torch.optim.Optimizer):
 
     def _forget(self) -> None:
         self.norm: torch.Tensor | None = None
+        self._norm_held: torch.Tensor | None = None  # what captured steps write, and those after them
         self._plans: list[tuple[int, AdamWPlan]] | None = None  # (group, plan); None: to be built
         self._captured: list[tuple] = []  # plans and learning rates: a graph's replays use what these hold
         self._planned: tuple[int, int] | None = None
@@ -439,6 +452,26 @@ class AdamW(torch.optim.Optimizer):
         self._planned = (id(self.state), len(self.state))
         self._stateless = [p for group in self.param_groups for p in group["params"] if p not in self.state]
 
+    def _norms(self, grads: list[list], capturing: bool) -> tuple[torch.Tensor | None, torch.Tensor | None]:
+        """For a step that clips: the norm of several plans' gradients, and the scalar that its norm goes to (None: a
+        new one)."""
+
+        gradient = next((g for many in grads for g in many if g is not None), None)
+        tensors = (p for group in self.param_groups for p in group["params"]) if gradient is None else [gradient]
+        device = next((t.device for t in tensors), None)
+        if device is None:
+            return None, None
+        if capturing and self._norm_held is None:
+            self._norm_held = torch.empty((), device=device, dtype=torch.float64)
+        out = self._norm_held
+        if out is not None and out.device != device:
+            out = None
+        if gradient is None:
+            self.norm = (torch.empty((), device=device, dtype=torch.float64) if out is None else out).zero_()
+        elif len(grads) > 1:
+            return _grad_norm([g for many in grads for g in many], out), out
+        return None, out
+
     @torch.no_grad()
     def step(self, closure=None):
         """One step over every parameter with a gradient; the closure's value, if there is one."""
@@ -462,16 +495,13 @@ class AdamW(torch.optim.Optimizer):
         if fresh or stale:
             self._build_plans()
         grads = [[p.grad for p in plan.params] for _, plan in self._plans]
-        norm = None
-        if self.max_norm is not None and len(grads) > 1:
-            given = [g for many in grads for g in many if g is not None]
-            norm = grad_norm(given) if given else None
+        norm, out = (None, None) if self.max_norm is None else self._norms(grads, capturing)
         for (index, plan), many in zip(self._plans, grads):
             if all(g is None for g in many):
                 continue
             group = self.param_groups[index]
-            self.norm = plan.step(many, lr=group["lr"], betas=group["betas"], eps=group["eps"],
-                                  weight_decay=group["weight_decay"], max_norm=self.max_norm, norm=norm)
+            self.norm = plan._step(many, lr=group["lr"], betas=group["betas"], eps=group["eps"],
+                                   weight_decay=group["weight_decay"], max_norm=self.max_norm, norm=norm, out=out)
             if capturing and not any(plan is p and group["lr"] is lr for p, lr in self._captured):
                 self._captured.append((plan, group["lr"]))
         return loss

@@ -595,3 +595,55 @@ def test_a_rollout_after_a_step_uses_the_new_weights(device, through):
     twin = build_model(trunk_config(2), 1, device)
     twin.load_state_dict(model.state_dict())
     assert torch.equal(after, wave(twin)) and not torch.equal(after, before)
+
+
+@pytest.mark.parametrize("types", [1, 2], ids=["one-plan", "two-plans"])
+def test_the_norm_follows_steps_and_replays(device, types):
+    """`norm` is the last step's, eager or replayed, whichever came before; of no gradient it is 0.  Eager steps'
+    norms of a program that captures none stay as they were."""
+
+    params = [torch.nn.Parameter(torch.randn(n, device=device)) for n in (5, 300)]
+    if types == 2:
+        params.append(torch.nn.Parameter(torch.randn(70, device=device).bfloat16()))
+    optimizer = AdamW(params, lr=1e-3, max_norm=1.0)
+    optimizer.step()
+    assert optimizer.norm == 0
+    gen = torch.Generator(device=device).manual_seed(1)
+
+    def new_gradients():
+        for p in params:
+            p.grad = torch.zeros_like(p) if p.grad is None else p.grad
+            p.grad.copy_(torch.randn(p.shape, generator=gen, device=device) * (1 + 10 * torch.rand((), device=device)))
+        return sum(p.grad.double().square().sum() for p in params).sqrt().item()
+
+    kept = []
+    for _ in range(3):
+        want = new_gradients()
+        optimizer.step()
+        kept.append((optimizer.norm, want))
+    assert all(abs(norm.item() - want) <= 1e-12 * want for norm, want in kept)  # (read after the last step)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        optimizer.step()
+    captured = optimizer.norm
+    for k in range(6):
+        want = new_gradients()
+        if k % 2:
+            optimizer.step()
+        else:
+            graph.replay()
+        torch.cuda.synchronize()
+        assert abs(optimizer.norm.item() - want) <= 1e-12 * want
+        assert abs(captured.item() - want) <= 1e-12 * want
+    assert all(abs(norm.item() - want) <= 1e-12 * want for norm, want in kept)
+    grads = [p.grad for p in params]
+    for p in params:
+        p.grad = None
+    optimizer.step()
+    assert optimizer.norm == 0
+    for p, g in zip(params, grads):
+        p.grad = g
+    graph.replay()
+    torch.cuda.synchronize()
+    assert abs(optimizer.norm.item() - want) <= 1e-12 * want
