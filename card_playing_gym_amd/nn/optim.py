@@ -80,6 +80,10 @@ def _scalar(value: torch.Tensor, name: str, dtype: torch.dtype, device: torch.de
     return value
 
 
+def _on_host(lr) -> bool:
+    return isinstance(lr, torch.Tensor) and lr.device.type == "cpu"
+
+
 def grad_norm(grads: Iterable[torch.Tensor | None]) -> torch.Tensor:
     """The Euclidean norm of the gradients together (None: skipped), a float64 scalar on their
     device: the norm that ``torch.nn.utils.clip_grad_norm_`` clips by.  The squares are added in
@@ -298,7 +302,8 @@ class AdamW(torch.optim.Optimizer):
     device scalar; 0 of no gradients): a new one each step until a step is captured, from then on one that
     every step and replay writes.  ``state_bits``: 32, or 8 for moments in blocks of 256 (see
     :class:`AdamWPlan`).  A group's ``lr`` may be a float32 device scalar, which a captured step
-    reads at every replay; its other options are captured as they are.
+    reads at every replay (its other options are captured as they are), or a scalar on the host, which is read
+    at each step and not captured.
 
     ``state_dict`` has ``torch.optim.AdamW``'s layout, and with ``state_bits=32`` its state dicts
     load (not with options that this step lacks); 8-bit state holds codes (uint8) and
@@ -482,10 +487,12 @@ class AdamW(torch.optim.Optimizer):
                 loss = closure()
         stale = self._plans is None or self._planned != (id(self.state), len(self.state)) or any(
             list(map(_ptr, plan.params)) != plan._addresses for _, plan in self._plans)
+        capturing = torch.cuda.is_current_stream_capturing()
+        if capturing and any(_on_host(group["lr"]) for group in self.param_groups):
+            raise RuntimeError("a learning rate on the host would stay as captured: give a device scalar, or a number")
         if stale:
             self._stateless = [p for group in self.param_groups for p in group["params"] if p not in self.state]
         fresh = [p for p in self._stateless if p.grad is not None]
-        capturing = torch.cuda.is_current_stream_capturing()
         if fresh:
             require_device(*fresh)
             if capturing:
@@ -500,8 +507,9 @@ class AdamW(torch.optim.Optimizer):
             if all(g is None for g in many):
                 continue
             group = self.param_groups[index]
-            self.norm = plan._step(many, lr=group["lr"], betas=group["betas"], eps=group["eps"],
+            lr = float(group["lr"]) if _on_host(group["lr"]) else group["lr"]
+            self.norm = plan._step(many, lr=lr, betas=group["betas"], eps=group["eps"],
                                    weight_decay=group["weight_decay"], max_norm=self.max_norm, norm=norm, out=out)
-            if capturing and not any(plan is p and group["lr"] is lr for p, lr in self._captured):
-                self._captured.append((plan, group["lr"]))
+            if capturing and not any(plan is p and lr is rate for p, rate in self._captured):
+                self._captured.append((plan, lr))
         return loss

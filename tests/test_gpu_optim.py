@@ -647,3 +647,31 @@ def test_the_norm_follows_steps_and_replays(device, types):
     graph.replay()
     torch.cuda.synchronize()
     assert abs(optimizer.norm.item() - want) <= 1e-12 * want
+
+
+def test_a_learning_rate_on_the_host(device):
+    """As a tensor there (a state dict's from a file, say) it is read at every step; a capture would keep one value, so
+    it is refused."""
+
+    params = [torch.nn.Parameter(torch.ones(300, device=device)) for _ in range(2)]
+    lr = torch.tensor(1e-2)
+    optimizers = [AdamW(params[:1], lr=lr), AdamW(params[1:], lr=1e-2)]
+    for k in range(3):
+        lr.fill_(1e-2 / (k + 1))
+        optimizers[1].param_groups[0]["lr"] = lr.item()
+        for p, optimizer in zip(params, optimizers):
+            p.grad = torch.full_like(p, 0.1 * (k + 1))
+            optimizer.step()
+        assert torch.equal(*params)
+    saved = copy.deepcopy(optimizers[0].state_dict())
+    optimizers[1].load_state_dict(saved)
+    for p, optimizer in zip(params, optimizers):
+        optimizer.step()
+    assert torch.equal(*params)
+    before = params[0].detach().clone()
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="host"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            optimizers[0].step()
+    torch.cuda.synchronize()
+    assert torch.equal(params[0], before) and optimizers[0].state[params[0]]["step"] == 4

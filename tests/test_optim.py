@@ -352,3 +352,19 @@ def test_dicts_that_hooks_make_are_checked(anywhere):
     handle.remove()
     ours.load_state_dict(given)
     assert lr == 1e-3
+
+
+def test_a_learning_rate_on_the_host_is_a_number(anywhere, monkeypatch):
+    """The step's launch gets its value as it is by then."""
+
+    given = []
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    monkeypatch.setattr(AdamWPlan, "_step", lambda self, grads, *, lr, **_: given.append(lr), raising=False)
+    monkeypatch.setattr(AdamWPlan, "step", lambda self, grads, *, lr, **_: given.append(lr))
+    p, lr = torch.nn.Parameter(torch.zeros(3)), torch.tensor(0.5, dtype=torch.float64)
+    p.grad = torch.ones(3)
+    optimizer = AdamW([p], lr=lr)
+    for value in (0.5, 0.25):
+        lr.fill_(value)
+        optimizer.step()
+    assert given == [0.5, 0.25] and all(isinstance(x, float) for x in given)
