@@ -27,8 +27,9 @@ namespace cg {
 namespace {
 
 constexpr int MAX_BLOCKS = 2048;  // and partial sums of the loss
-// Logits and gradient of more bytes than this go past the caches (256 MB of Infinity Cache): 4096 rows of 32768
-// bf16 entries (537 MB) 135 -> 128 us.  Below, whatever made the logits or takes the gradient may find them there.
+// Logits and gradient of this many bytes go past the caches (256 MB of Infinity Cache); below, whatever made the
+// logits or takes the gradient may find them there.  us kept and past them: fp32 4096 x 16384 (512 MB) 102 and 98,
+// 8192 x 16384 205 and 201; bf16, whose time is arithmetic, 4096 x 32768 128-133 and 127-129.
 constexpr int64_t STREAM_BYTES = 512 << 20;
 constexpr float LOG2E = 1.44269504088896340736f, LOG2E_REST = float(1.44269504088896340736 - double(LOG2E));
 // The least x = z - top that p = e^x is multiplied by: e^x is 0 from -104 on.  No lower, so that the coefficient
@@ -906,7 +907,7 @@ LossArgs args_of(const cg_policy_loss *loss) {
   a.ld_logits = p.ld_logits, a.ld_ref = p.ld_reference, a.ld_mask = p.ld_mask;
   a.rows = p.rows, a.width = p.width;
   a.lo = p.clip_low, a.hi = p.clip_high;
-  a.streams = int64_t(p.rows) * p.width > STREAM_BYTES / (2 * dtype_size(p.dtype));
+  a.streams = int64_t(p.rows) * p.width >= STREAM_BYTES / (2 * dtype_size(p.dtype));
   a.normalizer = scalar(p.normalizer), a.entropy_coef = scalar(p.entropy_coef), a.kl_coef = scalar(p.kl_coef);
   return a;
 }

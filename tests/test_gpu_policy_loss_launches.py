@@ -141,3 +141,10 @@ def check_wide(given, options, out, grad):
 def test_wide_rows_of_several_turns(device, dtype, rows, width):
     compare(device, rows, width, dtype, None, masked=rows % 2 == 0, count=8, check=check_wide)
     compare(device, rows, width, dtype, "logits", masked=rows % 2 == 1, count=8)
+
+
+@pytest.mark.parametrize("rows, width, dtype", [(4096, 32768, torch.bfloat16), (4096, 16384, torch.float32)])
+def test_a_loss_of_as_many_bytes_as_go_past_the_caches(device, rows, width, dtype):
+    """512 MB of logits and gradient to the byte."""
+
+    compare(device, rows, width, dtype, None, masked=False, count=8, check=check_wide)
