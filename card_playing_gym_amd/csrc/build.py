@@ -29,7 +29,7 @@ FLAGS = [
     "-O3",
     "-std=c++17",
     "-fPIC",
-    # Packed fp32 VALU forms are kept out of every kernel (see the build notes in DESIGN).
+    # Packed fp32 VALU forms are kept out of every kernel: some have given wrong results.
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
     "-Wall",
     "-Wno-unused-function",

@@ -14,7 +14,9 @@
 // inputs, so it is rounded once whatever the upstream scale.
 //
 // Bound by HBM: every logit (mask byte, reference logit) is read once and every gradient written once.
-// A row stays in registers between the passes over it: its maximum, its sums, its gradient.
+// A row stays in registers between the passes over it: its maximum, its sums, its gradient.  (Not all of it where
+// a lane has 64 entries beside a reference's 64: 16-bit rows of over 16384 entries with reference logits keep up to
+// 32 registers of a lane in scratch memory, bf16 4096 x 32768 320 us beside 169 for its bytes at a copy's rate.)
 //
 // The row's scalars are formed in fp64: the ends of the clip range are borders where the gradient jumps,
 // and a ratio off by fp32's 1e-6 would cross one in a few of a million rows.  A lane's partial sums over
@@ -823,6 +825,14 @@ Launch launch_as() {
   return {rows_kernel<T, G, E, REF, S>, G > 256 ? 1 : 256 / G, G > 256 ? G : 256};
 }
 
+// Lanes and entries a lane by width: few lanes a row keep the row's scalars, which each of them forms, few; up to
+// 32 entries (64 of 16 bits where rows are wide) leave room for the waves that hide the loads.  us of a pass:
+//   257 to 1024 entries, half as many lanes from 8193 rows on: 16384 x 512 fp32 15.0 and 16.4, bf16 13.8 and 15.2,
+//   32768 x 1024 bf16 34.5 and 42.6, but 1024 x 512 bf16 6.4 and 5.8, with a reference 10.0 and 7.9.  Between 4096
+//   and 8192 rows 512 entries are even, 1024 would gain up to 2 of 16.
+//   A wave a row up to 2048, a block a row beyond: 4096 x 2048 bf16 14.8 and 20.1, fp32 16.5 and 20.8; 4096 x 4096
+//   fp32 36 and 29, with a reference 174 and 51, but bf16 20.9 and 25.5, with a reference 47.0 and 49.5; 256 x 4096
+//   bf16 8.3 and 6.3.
 template <typename T, bool REF>
 Launch launch_of(int width, int rows) {
   if (width < VEC<T>) return launch_as<T, 8, 1, REF, float>();

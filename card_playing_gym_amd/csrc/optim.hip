@@ -10,7 +10,7 @@
 // them; the step counts are read and advanced on the device, so its replays count on.
 //
 // The update is bound by HBM: 28 bytes an element with fp32 parameters and moments, 16 with moments
-// in 8 bits, 20 and 8 with bf16 parameters.
+// in 8 bits, 22 and 10 with 16-bit parameters.
 #include <cmath>
 
 #include "common.h"

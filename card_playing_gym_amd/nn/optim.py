@@ -87,7 +87,7 @@ def _on_host(lr) -> bool:
 def grad_norm(grads: Iterable[torch.Tensor | None]) -> torch.Tensor:
     """The Euclidean norm of the gradients together (None: skipped), a float64 scalar on their
     device: the norm that ``torch.nn.utils.clip_grad_norm_`` clips by.  The squares are added in
-    float64, so neither large nor tiny gradients lose it."""
+    float64, so neither large nor tiny gradients lose it.  A constant: no derivative goes through it."""
 
     return _grad_norm(grads, None)
 
@@ -305,8 +305,12 @@ class AdamW(torch.optim.Optimizer):
     reads at every replay (its other options are captured as they are), or a scalar on the host, which is read
     at each step and not captured.
 
+    Parameters must be contiguous and those of one group and type on one device, all of them with clipping.  No
+    step is skipped for gradients that are not finite: with clipping a NaN among them makes every parameter NaN.
+
     ``state_dict`` has ``torch.optim.AdamW``'s layout, and with ``state_bits=32`` its state dicts
-    load (not with options that this step lacks); 8-bit state holds codes (uint8) and
+    load (not with options that this step lacks, as far as the dict tells: a coupled decay of ``torch.optim.Adam``
+    shows only in dicts with ``decoupled_weight_decay``); 8-bit state holds codes (uint8) and
     ``exp_avg_scale`` / ``exp_avg_sq_scale``.  Loading copies into state, and a learning rate on the
     device, that is already there, so a captured step goes on with what was loaded.
     ``state`` itself is read, not replaced: to start over, build a new optimiser."""

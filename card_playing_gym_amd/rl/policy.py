@@ -158,12 +158,12 @@ def policy_loss(
         l = -min(r A, clamp(r, 1 - clip, 1 + clip_high) A) + kl_coef KL - entropy_coef H
 
     p is the softmax over the row's legal entries: those that ``mask`` (bool [rows, width]) keeps
-    and whose logit is above -inf.  KL is sum p (log p - log q) with ``reference_logits`` (q over the same
-    mask), or exp(d) - d - 1 with d = ``reference_log_probs`` - log p[action].
+    and whose logit is above -inf.  KL is sum p (log p - log q) with ``reference_logits`` (of the logits'
+    type; q over the same mask), or exp(d) - d - 1 with d = ``reference_log_probs`` - log p[action].
 
     ``actions``: int64 [rows].  ``old_log_probs``, ``advantages``, ``weights`` (ones) and
-    ``reference_log_probs``: float32 [rows].  ``normalizer``: the number of rows; pass the whole
-    minibatch's count where a microbatch's gradients are accumulated.  ``clip_high``: ``clip``.
+    ``reference_log_probs``: float32 [rows].  ``normalizer``: the number of rows, padding among them; pass the
+    count of those with weight for their mean, the whole minibatch's where a microbatch's gradients are accumulated.  ``clip_high``: ``clip``.
     ``normalizer`` and the coefficients may be float32 device scalars, which a captured loss reads at
     every replay.  A backward captured in a graph of its own follows one replay of its forward's each time.
 
