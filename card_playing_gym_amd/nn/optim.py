@@ -385,7 +385,7 @@ class AdamW(torch.optim.Optimizer):
     def load_state_dict(self, state_dict) -> None:
         # Between the caller's hooks: the dict is checked as the last pre-hook leaves it, before anything is loaded, and
         # the state is in place for the first post-hook.
-        held = {p: self.state[p] for group in self.param_groups for p in group["params"] if p in self.state}
+        held = {p: self.state[p] for group in self.param_groups for p in group["params"] if self.state.get(p)}
         rates = [group["lr"] for group in self.param_groups]
         loaded: dict[torch.Tensor, dict] = {}
         hooks = [
@@ -449,7 +449,7 @@ class AdamW(torch.optim.Optimizer):
         for index, group in enumerate(self.param_groups):
             by_type: dict[torch.dtype, list[torch.Tensor]] = {}
             for p in group["params"]:
-                if p in self.state:
+                if self.state.get(p):
                     by_type.setdefault(p.dtype, []).append(p)
             for params in by_type.values():
                 held = [[self.state[p][name] for p in params] for name in _STATE[self.state_bits]]
@@ -459,7 +459,7 @@ class AdamW(torch.optim.Optimizer):
                 first += len(params)
         self._plans = plans
         self._planned = (id(self.state), len(self.state))
-        self._stateless = [p for group in self.param_groups for p in group["params"] if p not in self.state]
+        self._stateless = [p for group in self.param_groups for p in group["params"] if not self.state.get(p)]
 
     def _norms(self, grads: list[list], capturing: bool) -> tuple[torch.Tensor | None, torch.Tensor | None]:
         """For a step that clips: the norm of several plans' gradients, and the scalar that its norm goes to (None: a
@@ -495,7 +495,7 @@ class AdamW(torch.optim.Optimizer):
         if capturing and any(_on_host(group["lr"]) for group in self.param_groups):
             raise RuntimeError("a learning rate on the host would stay as captured: give a device scalar, or a number")
         if stale:
-            self._stateless = [p for group in self.param_groups for p in group["params"] if p not in self.state]
+            self._stateless = [p for group in self.param_groups for p in group["params"] if not self.state.get(p)]
         fresh = [p for p in self._stateless if p.grad is not None]
         if fresh:
             require_device(*fresh)

@@ -368,3 +368,37 @@ def test_a_learning_rate_on_the_host_is_a_number(anywhere, monkeypatch):
         lr.fill_(value)
         optimizer.step()
     assert given == [0.5, 0.25] and all(isinstance(x, float) for x in given)
+
+
+@pytest.fixture
+def recorded(anywhere, monkeypatch):
+    """Steps on CPU tensors up to their launch: the parameters, rates and gradients of each launch."""
+
+    launches = []
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    monkeypatch.setattr(AdamWPlan, "_step", lambda self, grads, *, lr, **_: launches.append((self, list(grads), lr)))
+    return launches
+
+
+def test_a_look_at_state_makes_none(recorded):
+    """An entry that reading `state` left there, empty, is no state."""
+
+    params = [torch.nn.Parameter(torch.ones(n)) for n in (3, 5)]
+    optimizer = AdamW(params, lr=1e-2)
+    assert not optimizer.state[params[0]] and not optimizer.state[params[1]].get("exp_avg")
+    params[0].grad = torch.ones(3)
+    optimizer.step()
+    params[1].grad = torch.ones(5)
+    optimizer.step()
+    assert [[p.numel() for p in plan.params] for plan, _, _ in recorded] == [[3], [3, 5]]
+    assert optimizer.state[params[1]]["exp_avg"].shape == (5,)
+    twin = AdamW([torch.nn.Parameter(torch.ones(n)) for n in (3, 5)], lr=1e-2)
+    for p in twin.param_groups[0]["params"]:
+        assert not twin.state[p]
+    saved = optimizer.state_dict()
+    saved["state"][1] = {}
+    twin.load_state_dict(saved)
+    for p in twin.param_groups[0]["params"]:
+        p.grad = torch.ones_like(p)
+    twin.step()
+    assert [p.numel() for p in recorded[-1][0].params] == [3, 5]
