@@ -253,13 +253,13 @@ class AdamWPlan:
         scaled by min(1, max_norm / (norm + 1e-6)): by ``norm`` (a float64 scalar, ``grad_norm``'s)
         where it is given, else by the norm of these gradients.  Returns the norm it clipped by."""
 
+        if list(map(_ptr, self.params)) != self._addresses:
+            raise ValueError("a parameter's data moved since the plan was built: build a new plan")
         return self._step(grads, lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, max_norm=max_norm, norm=norm)
 
     def _step(self, grads, *, lr, betas, eps, weight_decay, max_norm, norm, out=None) -> torch.Tensor | None:
-        """``step``, its own norm written into ``out`` where that is given."""
+        """``step`` with parameters that are where they were, its own norm written into ``out`` where that is given."""
 
-        if list(map(_ptr, self.params)) != self._addresses:
-            raise ValueError("a parameter's data moved since the plan was built: build a new plan")
         pointers, kept = self._gradient_addresses(list(grads))
         if norm is not None and max_norm is None:
             raise ValueError("norm is given without max_norm")
@@ -313,7 +313,8 @@ class AdamW(torch.optim.Optimizer):
     shows only in dicts with ``decoupled_weight_decay``); 8-bit state holds codes (uint8) and
     ``exp_avg_scale`` / ``exp_avg_sq_scale``.  Loading copies into state, and a learning rate on the
     device, that is already there, so a captured step goes on with what was loaded.
-    ``state`` itself is read, not replaced: to start over, build a new optimiser."""
+    ``state``'s tensors are taken when a parameter joins: change them in place, or exchange them together with their
+    parameter in its group."""
 
     def __init__(
         self,
@@ -343,7 +344,7 @@ class AdamW(torch.optim.Optimizer):
         self._norm_held: torch.Tensor | None = None  # what captured steps write, and those after them
         self._plans: list[tuple[int, AdamWPlan]] | None = None  # (group, plan); None: to be built
         self._captured: list[tuple] = []  # plans and learning rates: a graph's replays use what these hold
-        self._planned: tuple[int, int] | None = None
+        self._planned: tuple | None = None  # what the plans were built over (_members)
         self._stateless: list[torch.Tensor] = []
 
     def __getstate__(self):
@@ -442,6 +443,12 @@ class AdamW(torch.optim.Optimizer):
 
     # -- the step --------------------------------------------------------------------------
 
+    def _members(self) -> tuple:
+        """The groups' parameters and how many have state, to tell a change by.  (All of them are kept alive by the
+        plans or _stateless: no other takes an identity over.)"""
+
+        return id(self.state), len(self.state), [list(map(id, group["params"])) for group in self.param_groups]
+
     def _build_plans(self) -> None:
         """A plan over the parameters with state, for each group and type."""
 
@@ -458,7 +465,7 @@ class AdamW(torch.optim.Optimizer):
                                                seed=self._options["seed"], first=first)))
                 first += len(params)
         self._plans = plans
-        self._planned = (id(self.state), len(self.state))
+        self._planned = self._members()
         self._stateless = [p for group in self.param_groups for p in group["params"] if not self.state.get(p)]
 
     def _norms(self, grads: list[list], capturing: bool) -> tuple[torch.Tensor | None, torch.Tensor | None]:
@@ -489,7 +496,7 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        stale = self._plans is None or self._planned != (id(self.state), len(self.state)) or any(
+        stale = self._plans is None or self._planned != self._members() or any(
             list(map(_ptr, plan.params)) != plan._addresses for _, plan in self._plans)
         capturing = torch.cuda.is_current_stream_capturing()
         if capturing and any(_on_host(group["lr"]) for group in self.param_groups):

@@ -402,3 +402,29 @@ def test_a_look_at_state_makes_none(recorded):
         p.grad = torch.ones_like(p)
     twin.step()
     assert [p.numel() for p in recorded[-1][0].params] == [3, 5]
+
+
+def test_parameters_exchanged_in_their_group(recorded):
+    """Groups edited in place, as programs that grow or prune tensors do: the step follows them."""
+
+    a, b, c, d = (torch.nn.Parameter(torch.ones(n)) for n in (3, 5, 7, 9))
+    optimizer = AdamW([{"params": [a, b], "lr": 0.5}, {"params": [c], "lr": 0.25}])
+    for p in (a, b, c, d):
+        p.grad = torch.ones_like(p)
+    optimizer.step()
+    # b's place goes to d, with b's state cut to its size
+    held = optimizer.state.pop(b)
+    optimizer.state[d] = {name: x if name == "step" else torch.zeros(9) for name, x in held.items()}
+    optimizer.param_groups[0]["params"][1] = d
+    optimizer.step()
+    # c to the other group, in the same order
+    optimizer.param_groups[0]["params"].append(optimizer.param_groups[1]["params"].pop())
+    optimizer.step()
+    # a parameter more without add_param_group, one less
+    optimizer.param_groups[1]["params"].append(b)
+    optimizer.param_groups[0]["params"].remove(a)
+    optimizer.step()
+    sizes = [([p.numel() for p in plan.params], [g.numel() for g in grads], lr) for plan, grads, lr in recorded]
+    assert sizes == [([3, 5], [3, 5], 0.5), ([7], [7], 0.25), ([3, 9], [3, 9], 0.5), ([7], [7], 0.25),
+                     ([3, 9, 7], [3, 9, 7], 0.5), ([9, 7], [9, 7], 0.5), ([5], [5], 0.25)]
+    assert recorded[3][0].params[0] is c and recorded[-1][0].params[0] is b and b in optimizer.state
