@@ -317,7 +317,8 @@ __global__ __launch_bounds__(THREADS) void adamw_kernel(const UpdateArgs<Tensor3
 // to nearest, v would stay where the first steps left it, a fraction of the mean of g^2.  So codes are
 // rounded up with the probability of the fraction cut off (16 random bits hashed from seed, step, tensor
 // and element), which keeps the running means unbiased.  A v above 0 never becomes 0, or a kept m would
-// be divided by eps alone.
+// be divided by eps alone, except where a whole block's v is below fp32's normal numbers (gradients below
+// 3e-18): its codes are 0, and sqrt(v) was far below any eps of 1e-16 or more.
 //
 // New moments are formed in fp64 and their codes cut from its bits: a code is a border for the
 // rounding, so equal inputs give equal codes whatever forms the same products elsewhere.  (fp64 adds

@@ -147,7 +147,8 @@ class AdamWPlan:
     ``exp_avgs`` / ``exp_avg_sqs``: float32 of the parameters' sizes; or, with moments in 8 bits,
     uint8 codes of those sizes beside ``exp_avg_scales`` / ``exp_avg_sq_scales``, float32
     [ceil(size / 256)] each.  All zeros before the first step.  A gradient that is not finite spoils its
-    element; with moments in 8 bits, its block.  ``steps``: a float32 scalar each, the
+    element; with moments in 8 bits, its block.  (Blocks of gradients below 3e-18 lose their second moment in 8 bits:
+    keep ``eps`` at 1e-16 or more.)  ``steps``: a float32 scalar each, the
     number of steps taken.  ``seed`` and ``first`` (the place of the first tensor) choose the 8-bit
     moments' random numbers.
 

@@ -608,7 +608,9 @@ int cg_grad_norm(const void *const *grads, const int64_t *sizes, const int32_t *
  * with u = 889 + q for exp_avg (q up to 127, bit 7 the sign) and u = 761 + q for exp_avg_sq (q
  * up to 255), so 1 is the largest code's.  New codes are rounded up with the probability of
  * what is cut off, by 16-bit random numbers hashed from (seed, t, first + the tensor's index,
- * the element's index).  A gradient that is not finite makes its block of 256 not finite. */
+ * the element's index).  A block whose scale is below fp32's normal numbers has codes of 0 (for v:
+ * gradients below 3e-18, nothing beside an eps of 1e-16 or more).  A gradient that is not finite
+ * makes its block of 256 not finite. */
 typedef struct {
   void *param;
   void *exp_avg, *exp_avg_sq;
