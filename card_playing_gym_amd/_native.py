@@ -140,6 +140,16 @@ class AdamWConfig(ctypes.Structure):
     ]
 
 
+class PolicyRows(ctypes.Structure):
+    _fields_ = [("logits", c_void_p), ("mask", c_void_p), ("ld_logits", c_int64), ("ld_mask", c_int64),
+                ("rows", c_int32), ("width", c_int32), ("dtype", c_int32)]
+
+
+class SampleControls(ctypes.Structure):
+    _fields_ = [(name, c_double) for name in ("temperature", "top_p", "min_p")] + [("top_k", c_int64)] + [
+        (name, c_void_p) for name in ("temperatures", "top_ps", "min_ps", "top_ks")]
+
+
 class Scalar(ctypes.Structure):
     _fields_ = [("value", c_float), ("device", c_void_p)]
 
@@ -151,6 +161,11 @@ class PolicyLoss(ctypes.Structure):
         ("dtype", c_int32), ("clip_low", c_double), ("clip_high", c_double), ("normalizer", Scalar),
         ("entropy_coef", Scalar), ("kl_coef", Scalar),
     ]
+
+
+class DistillLoss(ctypes.Structure):
+    _fields_ = [("rows", PolicyRows)] + [(name, c_void_p) for name in ("indices", "log_probs", "log_rest", "weights")] + [
+        ("k", c_int32), ("temperature", c_double), ("normalizer", Scalar)]
 
 
 class LayerParams(ctypes.Structure):
@@ -307,6 +322,8 @@ _SIGNATURES = {
          P(TrainGrads), c_void_p, c_void_p, c_void_p, c_void_p],
     ),
     "cg_attn_train_bwd": (c_int32, [P(AttnTrain), c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "cg_sample_logits": (c_int32, [P(PolicyRows), c_void_p, P(SampleControls), c_void_p, c_void_p, c_void_p]),
+    "cg_top_logits": (c_int32, [P(PolicyRows), c_int32, c_double, c_void_p, c_void_p, c_void_p, c_void_p]),
     "cg_policy_loss_workspace_size": (c_size_t, [P(PolicyLoss)]),
     "cg_policy_loss_backward_workspace_size": (c_size_t, [P(PolicyLoss)]),
     "cg_policy_loss_forward": (
@@ -315,6 +332,11 @@ _SIGNATURES = {
     "cg_policy_loss_backward": (
         c_int32, [P(PolicyLoss), c_void_p, c_int32, c_void_p, c_void_p, c_size_t, c_void_p],
     ),
+    "cg_distill_loss_workspace_size": (c_size_t, []),
+    "cg_distill_loss_forward": (
+        c_int32, [P(DistillLoss), c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p],
+    ),
+    "cg_distill_loss_backward": (c_int32, [P(DistillLoss), c_void_p, c_int32, c_void_p, c_void_p]),
     "cg_grad_norm_workspace_size": (c_size_t, [c_int32]),
     "cg_grad_norm": (
         c_int32, [c_void_p, c_void_p, c_void_p, c_int32, c_void_p, c_void_p, c_size_t, c_void_p],

@@ -18,8 +18,8 @@ PACKAGE = CSRC.parent
 ROOT = PACKAGE.parent
 LIBRARY = PACKAGE / "libcardgym_hip.so"
 SOURCES = (
-    "kv_ops.hip", "attention.hip", "gemm.hip", "layer.hip", "heads.hip", "sample.hip", "piquet.hip", "train.hip",
-    "trunk.hip", "loss.hip", "optim.hip",
+    "kv_ops.hip", "attention.hip", "gemm.hip", "layer.hip", "heads.hip", "sample.hip", "choose.hip", "piquet.hip", "train.hip",
+    "trunk.hip", "loss.hip", "distill.hip", "optim.hip",
 )
 ARCH = os.environ.get("CARDGYM_HIP_ARCH", "gfx950")
 

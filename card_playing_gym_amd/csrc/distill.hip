@@ -1,0 +1,431 @@
+// The distillation loss towards a record of another policy's top entries (gfx950): forward and gradient over rows
+// of logits in one pass.
+//
+// A row's legal entries are those its mask keeps and whose logit is above -inf; p = softmax(z / T) over them.  The
+// record R holds entries k with the logs of the teacher's q_k, and may hold the log of q_r, what the teacher has
+// outside.  With p_r p's mass outside R and Q the sum of q:
+//   KL = sum_R q_k (log q_k - log p_k) + q_r (log q_r - log p_r),
+//   dKL/dz_j = (Q p_j - q_j) / T in R,  p_j (Q - q_r / p_r) / T outside;
+// without q_r, q is made to sum to 1 over R and the second term is not there.  The loss is the sum of w KL over `normalizer`.
+//
+// Entries in R are set aside: a bit each in LDS, by which the lanes that hold the row leave them out, and a lane
+// each for their terms, in fp64.  So p_r is a sum of its own, measured from its own largest entry, and not 1 minus what
+// R has; and the gradient outside R is e^((z - m_r) / T) times one number a row, whose two terms nearly cancel where the policies
+// agree and are therefore subtracted in fp64.
+//
+// Bound by HBM: every logit (mask byte) is read once and every gradient written once; a row stays in registers between
+// its maximum, its sum and its gradient.  The forward writes the gradient for an upstream of 1; a backward with another
+// one forms it again from the inputs, so it is rounded once whatever the scale.
+#include "rows.h"
+
+namespace cg {
+namespace {
+
+constexpr int MAX_WIDTH = 1 << 18;
+constexpr int MAX_TOP = 256;
+
+struct DistillArgs {
+  const void *logits;
+  const uint8_t *mask;
+  const int64_t *indices;  // [rows, k]
+  const float *top, *rest;  // [rows, k], and [rows] or NULL
+  const float *weights;
+  int64_t ld_logits, ld_mask;
+  int32_t rows, width, k;
+  double inverse;     // 1 / T
+  float fast, slow;   // log2(e) / T, and what that leaves out
+  Scalar normalizer;
+  float *kl;   // NULL in a backward call
+  void *grad;  // NULL: none
+  double *partials;
+  float *loss;
+  const float *upstream;  // of a backward call
+  int32_t written;        // the gradient for an upstream of 1 is in place
+};
+
+// e^((z - from) / T) for z <= from (-inf: 0), with what the rounding of the product cuts off.
+__device__ __forceinline__ float exp_from(const DistillArgs &a, float z, float from) {
+  const float d = z - from, t = d * a.fast, e = __builtin_amdgcn_exp2f(t);
+  const float cut = fmaf(d, a.slow, fmaf(d, a.fast, -t));
+  return t > -126.f ? fmaf(e, cut * 0.69314718f, e) : e;  // (below it: inf - inf)
+}
+
+// ---- the record's entries in a row -------------------------------------------------------------------------
+
+// Bit i % 32 of word i / 32 is set for entries in R.  A word more than the row has, so that two side by side can be read.
+template <int CAPACITY>
+struct Bits {
+  static constexpr int WORDS = (CAPACITY + 31) / 32 + 1;
+  uint32_t w[WORDS];
+  // Bits i to i + 31, i a multiple of nothing.
+  __device__ __forceinline__ uint32_t from(int i) const {
+    return __builtin_amdgcn_alignbit(w[(i >> 5) + 1], w[i >> 5], i & 31);
+  }
+};
+
+template <int G>
+__device__ __forceinline__ void group_sync() {
+  if constexpr (G > 64) {
+    __syncthreads();
+  } else {  // the wave's LDS writes to its own reads
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  }
+}
+
+// The entry's logit, -inf where it is not legal.
+template <typename T>
+__device__ __forceinline__ float logit_at(const T *row, const uint8_t *legal, int i) {
+  return !legal || legal[i] ? to_f32(row[i]) : -INFINITY;
+}
+
+// visit(index, log q) for this lane's entries of R that are there.
+template <int G, typename Visit>
+__device__ __forceinline__ void each_top(const DistillArgs &a, int64_t r, int lane, const Visit &visit) {
+  for (int k = lane; k < a.k; k += G) {
+    const int64_t i = a.indices[r * a.k + k];
+    if (i != -1) visit(i, a.top[r * a.k + k]);
+  }
+}
+
+// Marks R.  Returns whether its indices are in the row, and each there once.
+template <int G, typename B>
+__device__ __forceinline__ bool mark(const DistillArgs &a, int64_t r, int lane, B &bits) {
+  const int words = min((a.width >> 5) + 2, B::WORDS);  // (of vectors that begin before the row's end, and one more)
+  for (int i = lane; i < words; i += G) bits.w[i] = 0;
+  group_sync<G>();
+  bool good = true;
+  each_top<G>(a, r, lane, [&](int64_t i, float) {
+    if (i < 0 || i >= a.width) {
+      good = false;
+    } else {
+      const uint32_t bit = 1u << (i & 31);
+      if (atomicOr(&bits.w[i >> 5], bit) & bit) good = false;
+    }
+  });
+  group_sync<G>();
+  return good;
+}
+
+// ---- a row's scalars -----------------------------------------------------------------------------------------
+
+// Sums over R: e^((z - m) / T), q, q log q and q (z - m) / T.  Without q_r, q is measured from its largest.
+struct TopSums {
+  double s, q, own, cross;
+};
+
+struct RowScalars {
+  double kl, value;
+  float outer;         // the gradient's factor of e outside R
+  double inner, pull;  // in R: inner e^((z - m) / T) - pull q
+  bool live;
+};
+
+// top, rest_top: the row's largest entry, and the largest outside R; rest: the sum outside, from rest_top.
+__device__ __forceinline__ RowScalars row_scalars(const DistillArgs &a, int64_t r, float weight, float top, float rest_top,
+                                                  double rest, const TopSums &t, bool good, double scale) {
+  RowScalars o;
+  const double gap = rest > 0 ? (double(rest_top) - double(top)) * a.inverse : 0.0;
+  const double lower = rest > 0 ? exp_of(gap) : 0.0;
+  double s = t.s + (rest > 0 ? rest * lower : rest);  // (rest: NaN stays)
+  if (!good) s = NAN;
+  o.live = weight != 0 && s != 0;
+  const double log_s = log_of(s);
+  double mass = t.q, outer = 0;
+  if (a.rest) {
+    const double log_q = a.rest[r], q = exp_of(log_q);
+    mass += q;
+    o.kl = t.own - t.cross + t.q * log_s;
+    if (!(q <= 0)) {
+      const double log_p = rest > 0 ? gap + log_of(rest) - log_s : -INFINITY;
+      o.kl += q * (log_q - log_p);
+      if (rest > 0) outer = q * reciprocal(rest);
+    }
+    o.pull = 1;
+  } else {
+    const double inv = t.q > 0 ? reciprocal(t.q) : 0;
+    o.kl = t.q > 0 ? (t.own - t.cross) * inv - log_of(t.q) + log_s : t.q;
+    mass = t.q > 0 ? 1 : t.q;
+    o.pull = inv;
+  }
+  const double f = double(weight) * scale * a.inverse;
+  o.inner = f * mass * reciprocal(s);
+  o.pull *= f;
+  o.outer = o.live ? float(o.inner * lower - f * outer) : 0.f;
+  o.value = double(weight) * o.kl;
+  return o;
+}
+
+__device__ __forceinline__ double scale_of(const DistillArgs &a) {
+  return (a.upstream ? double(*a.upstream) : 1.0) / read(a.normalizer);
+}
+
+template <int G>
+struct Slots {
+  static constexpr int W = G > 64 ? G / 64 : 1;
+  float tops[3 * W];
+  double sums[6 * W];
+};
+
+// From a row's entries outside R to its numbers and its gradient: what every kernel does with a row.
+// each(visit): visit(first entry, entries, inside) for this lane's vectors, those in R as -inf.
+template <int G, int V, typename T, typename Each>
+__device__ __forceinline__ void distill_row(const DistillArgs &a, int64_t r, int lane, float weight, bool good,
+                                            const T *logits, const uint8_t *legal, Slots<G> &slots, double scale,
+                                            bool in, const Each &each, double &value) {
+  float tops[3] = {-INFINITY, -INFINITY, -INFINITY};  // of z outside R, in it, and of log q
+  if (weight != 0) {
+    each([&](int, const auto &z, bool) {
+#pragma unroll
+      for (int k = 0; k < V; ++k) tops[0] = fmaxf(tops[0], z(k));
+    });
+    each_top<G>(a, r, lane, [&](int64_t i, float log_q) {
+      if (i >= 0 && i < a.width) tops[1] = fmaxf(tops[1], logit_at(logits, legal, int(i)));
+      tops[2] = fmaxf(tops[2], log_q);
+    });
+  }
+  join<G>(tops, slots.tops, Most{});
+  const float rest_top = tops[0] > -INFINITY ? tops[0] : 0.f;
+  const float most = fmaxf(tops[0], tops[1]), top = most > -INFINITY ? most : 0.f;
+  // Without q_r, only the differences of the log q count.
+  const float base = !a.rest && tops[2] > -INFINITY ? tops[2] : 0.f;
+  double sums[6] = {};  // the rest, then TopSums, then whether the record is in order
+  if (weight != 0) {
+    each([&](int, const auto &z, bool) {
+      float s = 0;
+#pragma unroll
+      for (int k = 0; k < V; ++k) s += exp_from(a, z(k), rest_top);
+      sums[0] += s;
+    });
+    each_top<G>(a, r, lane, [&](int64_t i, float log_q) {
+      if (i < 0 || i >= a.width) return;
+      const float z = logit_at(logits, legal, int(i));
+      const double x = (double(z) - double(top)) * a.inverse, l = double(log_q) - double(base), q = exp_of(l);
+      sums[1] += exp_of(x);
+      sums[2] += q;
+      if (!(q <= 0)) sums[3] += q * l, sums[4] += q * x;
+    });
+  }
+  sums[5] = good ? 0 : 1;
+  join<G>(sums, slots.sums, Add{});
+  const RowScalars o = row_scalars(a, r, weight, top, rest_top, sums[0], TopSums{sums[1], sums[2], sums[3], sums[4]},
+                                   sums[5] == 0, scale);
+  if (in && lane == 0 && a.kl) {
+    if (o.live) value += o.value;
+    a.kl[r] = o.live ? float(o.kl) : 0.f;
+  }
+  if (!a.grad) return;
+  T *grad = static_cast<T *>(a.grad) + r * int64_t(a.width);
+  if (in) {
+    each([&](int i, const auto &z, bool inside) {
+      float g[V];
+#pragma unroll
+      for (int k = 0; k < V; ++k) g[k] = o.outer * exp_from(a, z(k), rest_top);
+      store_entries<V>(grad, g, i, a.width, inside);
+    });
+  }
+  if constexpr (G > 64) __syncthreads();  // (the zeros just written at R's entries come first)
+  if (in && o.live) {
+    each_top<G>(a, r, lane, [&](int64_t i, float log_q) {
+      if (i < 0 || i >= a.width) return;
+      const float z = logit_at(logits, legal, int(i));
+      if (z == -INFINITY) return;
+      const double x = (double(z) - double(top)) * a.inverse;
+      grad[i] = from_f32<T>(float(o.inner * exp_of(x) - o.pull * exp_of(double(log_q) - double(base))));
+    });
+  }
+}
+
+// ---- rows in registers: E entries a lane, G lanes a row, 256 / G rows a block at a time (one from 256 on) -----
+
+// S: the type in which entries are kept (T, or float where rows are shorter than a load).
+template <typename T, int G, int E, typename S = T>
+__global__ __launch_bounds__((G > 256 ? G : 256)) void rows_kernel(const DistillArgs a) {
+  constexpr int V = E == 1 ? 1 : VEC<T>, C = E / V, THREADS = G > 256 ? G : 256, ROWS = THREADS / G;
+  if (done(a)) return;
+  __shared__ Slots<G> slots;
+  __shared__ Bits<G * E> bits[ROWS];
+  const double scale = scale_of(a);
+  double value = 0;
+  const int in_block = threadIdx.x / G, lane = threadIdx.x % G;
+  // every thread of the block takes every turn: lanes of rows past the end have nothing live
+  for (int64_t first = int64_t(blockIdx.x) * ROWS; first < a.rows; first += int64_t(gridDim.x) * ROWS) {
+    const bool in = first + in_block < a.rows;
+    const int64_t r = min(first + in_block, int64_t(a.rows) - 1);
+    const float weight = in ? a.weights ? a.weights[r] : 1.f : 0.f;
+    const T *logits = static_cast<const T *>(a.logits) + r * a.ld_logits;
+    const uint8_t *legal = a.mask ? a.mask + r * a.ld_mask : nullptr;
+    Entries<S, E> z;
+    bool good = true;
+    if (weight != 0) {  // rows without weight are not read
+      load_entries<G, C, V>(z.w, logits, legal, lane * V, a.width);
+    } else {
+      z.clear();
+    }
+    // (groups of a wave go through their barriers together, weight or not)
+    if (weight != 0 || G <= 64) good = mark<G>(a, r, lane, bits[in_block]) || weight == 0;
+    if (weight != 0) {
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        const int at = V == 1 ? lane : min((c * G + lane) * V, a.width - V);
+        const uint32_t set = at < a.width ? bits[in_block].from(at) & ((1u << V) - 1) : 0;
+        if (set == 0) continue;
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+          const uint32_t part = Entries<S, E>::PER == 1 ? ~0u : k % 2 ? 0xffff0000u : 0xffffu;
+          uint32_t &w = z.w[(c * V + k) / Entries<S, E>::PER];
+          if (set >> k & 1) w = (w & ~part) | (NEGATIVE_INFINITY<S> & part);
+        }
+      }
+    }
+    const auto each = [&](const auto &visit) {
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+        visit((c * G + lane) * V, [&](int k) { return z[c * V + k]; }, (c + 1) * G * V <= a.width);
+    };
+    distill_row<G, V>(a, r, lane, weight, good, logits, legal, slots, scale, in, each, value);
+    group_sync<G>();  // (the bits and slots are written again)
+  }
+  if (a.kl) block_loss(a, value);
+}
+
+// ---- rows of any width, read again for each pass: a block a row ---------------------------------------------------
+
+template <typename T>
+__global__ __launch_bounds__(1024) void long_rows_kernel(const DistillArgs a) {
+  constexpr int V = VEC<T>, G = 1024;
+  if (done(a)) return;
+  __shared__ Slots<G> slots;
+  __shared__ Bits<MAX_WIDTH> bits;
+  const double scale = scale_of(a);
+  double value = 0;
+  const int lane = threadIdx.x;
+  for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
+    const float weight = a.weights ? a.weights[r] : 1.f;
+    const T *logits = static_cast<const T *>(a.logits) + r * a.ld_logits;
+    const uint8_t *legal = a.mask ? a.mask + r * a.ld_mask : nullptr;
+    const bool good = weight != 0 ? mark<G>(a, r, lane, bits) : true;
+    const auto each = [&](const auto &visit) {
+      for (int i = lane * V; i < a.width; i += G * V) {
+        Entries<T, V> z;
+        z.clear();
+        uint32_t set = 0;
+        if (weight != 0) {
+          load_entries<1, 1, V>(z.w, logits, legal, i, a.width);
+          set = bits.from(min(i, a.width - V));
+        }
+        visit(i, [&](int k) { return set >> k & 1 ? -INFINITY : z[k]; }, false);
+      }
+    };
+    distill_row<G, V>(a, r, lane, weight, good, logits, legal, slots, scale, true, each, value);
+    __syncthreads();
+  }
+  if (a.kl) block_loss(a, value);
+}
+
+// ---- host side ---------------------------------------------------------------------------------------------------
+
+struct Launch {
+  void (*kernel)(DistillArgs);
+  int rows, threads;  // rows a block takes at a time
+};
+
+template <typename T, int G, int E, typename S = T>
+Launch launch_as() {
+  return {rows_kernel<T, G, E, S>, G > 256 ? 1 : 256 / G, G > 256 ? G : 256};
+}
+
+template <typename T>
+Launch launch_of(int width) {
+  if (width < VEC<T>) return launch_as<T, 8, 1, float>();
+  if (width <= 32) return launch_as<T, 4, 8>();
+  if (width <= 128) return launch_as<T, 16, 8>();
+  if (width <= 512) return launch_as<T, 32, 16>();
+  if (width <= 2048) return launch_as<T, 64, 32>();
+  if (width <= 8192) return launch_as<T, 256, 32>();
+  if (width <= 16384) return launch_as<T, 512, 32>();
+  if constexpr (sizeof(T) == 2) {
+    if (width <= 32768) return launch_as<T, 512, 64>();
+    if (width <= 65536) return launch_as<T, 1024, 64>();
+  } else if (width <= 32768) {
+    return launch_as<T, 1024, 32>();
+  }
+  return {long_rows_kernel<T>, 1, 1024};
+}
+
+// Returns the number of partial sums of the loss that are written (by one block for all rows: the loss itself).
+int launch_rows(const DistillArgs &a, int dtype, hipStream_t stream) {
+  const Launch l = dtype == CG_F32 ? launch_of<float>(a.width) : dtype == CG_BF16 ? launch_of<bf16>(a.width) : launch_of<f16>(a.width);
+  const int64_t blocks = (int64_t(a.rows) + l.rows - 1) / l.rows;
+  const int most = l.threads >= 512 ? 512 : MAX_BLOCKS;
+  const int grid = int(blocks < most ? blocks : most);
+  l.kernel<<<grid, l.threads, 0, stream>>>(a);
+  CG_LAUNCHED();
+  return grid;
+}
+
+DistillArgs args_of(const cg_distill_loss *loss) {
+  CG_REQUIRE(loss != nullptr, CG_ERR_INVALID, "loss is NULL");
+  const cg_distill_loss &p = *loss;
+  const cg_policy_rows &q = p.rows;
+  dtype_size(q.dtype);
+  CG_REQUIRE(q.rows >= 0 && q.width > 0, CG_ERR_INVALID, "rows must be non-negative, width positive");
+  CG_REQUIRE(q.width <= MAX_WIDTH, CG_ERR_UNSUPPORTED, "distill_loss: rows wider than 2^18");
+  CG_REQUIRE(p.k > 0 && p.k <= MAX_TOP, CG_ERR_INVALID, "k must be from 1 to 256");
+  CG_REQUIRE(p.temperature >= 1e-30 && p.temperature <= 1e30, CG_ERR_INVALID, "temperature must be from 1e-30 to 1e30");
+  CG_REQUIRE(q.rows == 0 || (q.logits && p.indices && p.log_probs), CG_ERR_INVALID,
+             "logits, indices and log_probs are required");
+  CG_REQUIRE(q.ld_logits >= 0 && q.ld_mask >= 0, CG_ERR_INVALID, "row strides must be non-negative");
+  DistillArgs a{};
+  a.logits = q.logits, a.mask = q.mask, a.indices = p.indices, a.top = p.log_probs, a.rest = p.log_rest;
+  a.weights = p.weights;
+  a.ld_logits = q.ld_logits, a.ld_mask = q.ld_mask;
+  a.rows = q.rows, a.width = q.width, a.k = p.k;
+  a.inverse = 1 / p.temperature;
+  const double c = 1.44269504088896340736 / p.temperature;
+  a.fast = float(c), a.slow = float(c - double(a.fast));
+  a.normalizer = scalar(p.normalizer);
+  return a;
+}
+
+}  // namespace
+}  // namespace cg
+
+using namespace cg;
+
+extern "C" {
+
+size_t cg_distill_loss_workspace_size(void) { return MAX_BLOCKS * sizeof(double); }
+
+int cg_distill_loss_forward(const cg_distill_loss *loss, float *value, float *kl, void *grad, void *workspace,
+                            size_t workspace_size, void *stream) {
+  return guarded([&] {
+    DistillArgs a = args_of(loss);
+    CG_REQUIRE(value && workspace, CG_ERR_INVALID, "value and workspace are required");
+    CG_REQUIRE(workspace_size >= cg_distill_loss_workspace_size(), CG_ERR_INVALID, "workspace too small");
+    CG_REQUIRE(a.rows == 0 || kl, CG_ERR_INVALID, "kl is required");
+    a.partials = static_cast<double *>(workspace);
+    a.loss = value, a.kl = kl, a.grad = grad;
+    int sums = 0;
+    if (a.rows > 0) sums = launch_rows(a, loss->rows.dtype, as_stream(stream));
+    if (sums != 1) {
+      loss_kernel<DistillArgs><<<1, 256, 0, as_stream(stream)>>>(a, sums);
+      CG_LAUNCHED();
+    }
+  });
+}
+
+int cg_distill_loss_backward(const cg_distill_loss *loss, const float *upstream, int32_t written, void *grad,
+                             void *stream) {
+  return guarded([&] {
+    DistillArgs a = args_of(loss);
+    CG_REQUIRE(upstream, CG_ERR_INVALID, "upstream is required");
+    if (a.rows == 0) return;
+    CG_REQUIRE(grad, CG_ERR_INVALID, "grad is required");
+    a.grad = grad, a.upstream = upstream, a.written = written;
+    launch_rows(a, loss->rows.dtype, as_stream(stream));
+  });
+}
+
+}  // extern "C"

@@ -26,7 +26,6 @@
 namespace cg {
 namespace {
 
-constexpr int MAX_BLOCKS = 2048;  // and partial sums of the loss
 // Logits and gradient of this many bytes go past the caches (256 MB of Infinity Cache); below, whatever made the
 // logits or takes the gradient may find them there.  us kept and past them: fp32 4096 x 16384 (512 MB) 102 and 98,
 // 8192 x 16384 205 and 201; bf16, whose time is arithmetic, 4096 x 32768 128-133 and 127-129.
@@ -34,12 +33,6 @@ constexpr int64_t STREAM_BYTES = 512 << 20;
 // The least x = z - top that p = e^x is multiplied by: e^x is 0 from -104 on.  No lower, so that the coefficient
 // of x may be as large as 2^120 before the product is infinite, which times p = 0 is NaN.
 constexpr float LOWEST = -128.f;
-
-struct Scalar {
-  float value;
-  const float *at;  // NULL: value
-};
-__device__ __forceinline__ double read(const Scalar &s) { return double(s.at ? *s.at : s.value); }
 
 struct LossArgs {
   const void *logits, *ref_logits;
@@ -187,31 +180,6 @@ __device__ __forceinline__ void report(const LossArgs &a, int64_t row, const Row
   a.entropy[row] = o.live ? float(o.entropy) : 0.f;
   if (a.kl) a.kl[row] = o.live ? float(o.kl) : 0.f;
 }
-
-// The block's sum of `value` over its threads, to its partial sum, or the loss where it is the only one.
-__device__ __forceinline__ void block_loss(const LossArgs &a, double value) {
-  __shared__ double sums[16];
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) value += __shfl_xor(value, o, 64);
-  if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = value;
-  __syncthreads();
-  if (threadIdx.x != 0) return;
-  double s = 0;
-  for (int w = 0; w < int(blockDim.x >> 6); ++w) s += sums[w];
-  if (gridDim.x == 1)
-    *a.loss = float(s / read(a.normalizer));
-  else
-    a.partials[blockIdx.x] = s;
-}
-
-__global__ __launch_bounds__(256) void loss_kernel(const LossArgs a, int count) {
-  double s = 0;
-  for (int k = threadIdx.x; k < count; k += 256) s += a.partials[k];
-  block_loss(a, s);  // (of one block)
-}
-
-// Whether this call has nothing to do: a backward whose gradient is in place already.
-__device__ __forceinline__ bool done(const LossArgs &a) { return a.upstream && a.written && *a.upstream == 1.0f; }
 
 __device__ __forceinline__ Coefs coefs_of(const LossArgs &a) {
   return Coefs{read(a.entropy_coef), read(a.kl_coef), (a.upstream ? double(*a.upstream) : 1.0) / read(a.normalizer)};
@@ -649,8 +617,6 @@ int launch_rows(const LossArgs &a, const cg_policy_loss &p, hipStream_t stream) 
   return grid;
 }
 
-Scalar scalar(const cg_scalar &s) { return Scalar{s.value, s.device}; }
-
 LossArgs args_of(const cg_policy_loss *loss) {
   CG_REQUIRE(loss != nullptr, CG_ERR_INVALID, "loss is NULL");
   const cg_policy_loss &p = *loss;
@@ -701,7 +667,7 @@ int cg_policy_loss_forward(const cg_policy_loss *loss, float *value, float *log_
       sums = launch_rows(a, *loss, as_stream(stream));
     }
     if (sums != 1 || splits_of(*loss) > 1) {
-      loss_kernel<<<1, 256, 0, as_stream(stream)>>>(a, sums);
+      loss_kernel<LossArgs><<<1, 256, 0, as_stream(stream)>>>(a, sums);
       CG_LAUNCHED();
     }
   });

@@ -21,6 +21,20 @@ __device__ __forceinline__ double dpp(double x) {
   return __hiloint2double(__builtin_amdgcn_update_dpp(0, __double2hiint(x), CONTROL, 0xf, 0xf, false),
                           __builtin_amdgcn_update_dpp(0, __double2loint(x), CONTROL, 0xf, 0xf, false));
 }
+template <int CONTROL>
+__device__ __forceinline__ uint64_t dpp(uint64_t x) {
+  return __builtin_bit_cast(uint64_t, dpp<CONTROL>(__builtin_bit_cast(double, x)));
+}
+template <int CONTROL>
+__device__ __forceinline__ int dpp(int x) {
+  return __builtin_amdgcn_update_dpp(0, x, CONTROL, 0xf, 0xf, false);
+}
+struct Plus {
+  template <typename X>
+  __device__ __forceinline__ X operator()(X a, X b) const {
+    return a + b;
+  }
+};
 struct Add {
   __device__ __forceinline__ double operator()(double a, double b) const { return a + b; }
 };
@@ -255,6 +269,45 @@ __device__ __forceinline__ void store_entries(T *row, const float *g, int i, int
       if (width - V + k >= i) row[width - V + k] = from_f32<T>(g[k]);
   }
 }
+
+// ---- a loss over rows: its scalars, its partial sums ------------------------------------------------------
+
+constexpr int MAX_BLOCKS = 2048;  // and partial sums of the loss
+
+struct Scalar {
+  float value;
+  const float *at;  // NULL: value
+};
+__device__ __forceinline__ double read(const Scalar &s) { return double(s.at ? *s.at : s.value); }
+Scalar scalar(const cg_scalar &s) { return Scalar{s.value, s.device}; }
+
+// The block's sum of `value` over its threads, to its partial sum, or the loss where it is the only one.
+template <typename Args>
+__device__ __forceinline__ void block_loss(const Args &a, double value) {
+  __shared__ double sums[16];
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) value += __shfl_xor(value, o, 64);
+  if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = value;
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+  double s = 0;
+  for (int w = 0; w < int(blockDim.x >> 6); ++w) s += sums[w];
+  if (gridDim.x == 1)
+    *a.loss = float(s / read(a.normalizer));
+  else
+    a.partials[blockIdx.x] = s;
+}
+
+template <typename Args>
+__global__ __launch_bounds__(256) void loss_kernel(const Args a, int count) {
+  double s = 0;
+  for (int k = threadIdx.x; k < count; k += 256) s += a.partials[k];
+  block_loss(a, s);  // (of one block)
+}
+
+// Whether this call has nothing to do: a backward whose gradient is in place already.
+template <typename Args>
+__device__ __forceinline__ bool done(const Args &a) { return a.upstream && a.written && *a.upstream == 1.0f; }
 
 }  // namespace
 }  // namespace cg

@@ -38,13 +38,13 @@ def _constant(t: torch.Tensor, name: str, shape: tuple[int, ...], dtype: torch.d
     return t
 
 
-def _no_tangents(*tensors) -> None:
+def _no_tangents(*tensors, name: str = "policy_loss") -> None:
     """Refuses forward-mode derivatives, which nothing behind this would carry on.  (Outside a level no tensor has
     one: asking each would be 6 us of a small loss's 96.)"""
 
     if getattr(forward_ad, "_current_level", 0) >= 0:
         if any(isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
-            raise RuntimeError("policy_loss has no forward-mode derivative: pass the inputs without tangents")
+            raise RuntimeError(f"{name} has no forward-mode derivative: pass the inputs without tangents")
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:

@@ -540,6 +540,43 @@ int cg_trunk_train_backward(const cg_train_config *c, const cg_train_block *bloc
                             size_t saved_size, void *scratch, size_t scratch_size, const cg_train_grads *grads,
                             float *dx, float *dple, float *dvalues, void *stream);
 
+/* ---- answers of a policy from its logits --------------------------------------------------
+ * Beside the reference's sampling of given probabilities (cg_sample_rows): actions straight
+ * from logits under sampling controls, and the record of a row's top entries.  A row's legal entries
+ * are those its mask keeps and whose logit is above -inf; with m the largest, d = (z - m) / T and
+ * w = e^d.  Their order: larger logits first, of equal ones the lower index.  Where the largest is
+ * +inf, the entries at +inf share everything. */
+typedef struct {
+  const void *logits;  /* [rows, width] of `dtype`, row stride ld_logits (elements) */
+  const uint8_t *mask; /* [rows, width], 0 = not legal, row stride ld_mask; NULL: all legal */
+  int64_t ld_logits, ld_mask;
+  int32_t rows, width; /* width up to 2^18 */
+  int32_t dtype;       /* CG_F32, CG_BF16 or CG_F16 */
+} cg_policy_rows;
+
+/* One value for all rows, or (not NULL) a device array [rows] in its place. */
+typedef struct {
+  double temperature, top_p, min_p;
+  int64_t top_k;
+  const float *temperatures, *top_ps, *min_ps;
+  const int64_t *top_ks;
+} cg_sample_controls;
+
+/* Kept are the first top_k of the order (all: 0 or less); of these, S being their sum, those before
+ * which weights of less than top_p S are summed up (all: 1 or more); of these, those of w >= min_p
+ * (all: 0 or less); the first entry always.  actions[row] is the first of the order whose running sum over the
+ * kept, S' in all, exceeds uniforms[row] S' (the last kept for a uniform of 1 or more, or NaN), and
+ * log_probs[row] = d - log S'.  Temperature 0: the first of the order, with 0.  A row without a legal entry
+ * has action -1 and 0; one with a NaN among them, or a temperature that is negative or NaN, -1 and NaN. */
+int cg_sample_logits(const cg_policy_rows *rows, const double *uniforms, const cg_sample_controls *controls,
+                     int64_t *actions, float *log_probs, void *stream);
+
+/* indices / log_probs [rows, k]: the first k of the order and d - log S, S the sum over the whole row;
+ * log_rest [rows]: the log of the other entries' share, -inf where there are none.  Places without a legal
+ * entry hold -1 and -inf; a row with a NaN among its legal entries -1 and NaN.  k: 1 to 256. */
+int cg_top_logits(const cg_policy_rows *rows, int32_t k, double temperature, float *log_probs, int64_t *indices,
+                  float *log_rest, void *stream);
+
 /* ---- the policy loss ---------------------------------------------------------------------
  * The clipped policy loss of an update over rows of logits, beside the masked softmax that the
  * rollout sampled from (cg_masked_probabilities).  A row's legal entries are those its mask
@@ -584,6 +621,37 @@ int cg_policy_loss_forward(const cg_policy_loss *loss, float *value, float *log_
 size_t cg_policy_loss_backward_workspace_size(const cg_policy_loss *loss);
 int cg_policy_loss_backward(const cg_policy_loss *loss, const float *upstream, int32_t written, void *grad,
                             void *workspace, size_t workspace_size, void *stream);
+
+/* ---- the distillation loss -----------------------------------------------------------------
+ * Towards a record of another policy's top entries, as cg_top_logits writes it.  With p the softmax of
+ * logits / temperature over a row's legal entries, q_k = exp(log_probs) over the record R and q_r =
+ * exp(log_rest), p_r being p's mass outside R,
+ *   KL = sum_R q_k (log q_k - log p_k) + q_r (log q_r - log p_r);
+ * without log_rest, q is made to sum to 1 over R (logits / temperature will do for log_probs) and the second term is not
+ * there.  The value is
+ * sum_i w_i KL_i / normalizer.  Index -1: no entry.  An index outside the row, or twice in it, makes the row NaN; an entry that
+ * is not legal but has a q above 0 makes its KL infinite.  A row of weight 0 is not read; it and a row without a
+ * legal entry add nothing, have a zero gradient and report 0, as does, without log_rest, one whose record is empty. */
+typedef struct {
+  cg_policy_rows rows;
+  const int64_t *indices;  /* [rows, k] dense */
+  const float *log_probs;  /* [rows, k] dense */
+  const float *log_rest;   /* [rows] or NULL */
+  const float *weights;    /* [rows] or NULL: ones */
+  int32_t k;               /* 1 to 256 */
+  double temperature;      /* 1e-30 to 1e30 */
+  cg_scalar normalizer;
+} cg_distill_loss;
+
+/* value[0], kl [rows] and, where grad is not NULL, the value's gradient [rows, width] dense, of the
+ * logits' type.  workspace: 8-byte aligned, of this call alone until it has run. */
+size_t cg_distill_loss_workspace_size(void);
+int cg_distill_loss_forward(const cg_distill_loss *loss, float *value, float *kl, void *grad, void *workspace,
+                            size_t workspace_size, void *stream);
+/* grad = upstream[0] times the value's gradient, formed from the inputs and rounded once.  written != 0: grad
+ * holds the forward's, and stays as it is where upstream[0] is 1. */
+int cg_distill_loss_backward(const cg_distill_loss *loss, const float *upstream, int32_t written, void *grad,
+                             void *stream);
 
 /* ---- the optimiser step ------------------------------------------------------------------
  * What follows the training backward in an update: the gradients' global norm and one AdamW

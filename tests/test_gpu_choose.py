@@ -1,0 +1,254 @@
+"""Sampling under controls and the record of top entries on the GPU (csrc/choose.hip, rl/choose.py) against float64.
+
+Actions and indices are whole numbers and have to be equal; the inputs' uniforms are further from every border
+between two actions than the weights' error, 2^-44 and half a unit of 2^-(62 - log2 width) each.
+log_probs of a sample: float64 to a few units of 2^-44, rounded once: half a step of float32.
+The record's: the sum of the others' exponentials is float32's, off by (3 |x| + 4) 2^-24 of an entry with
+x = (z - m) / T (rounding of the difference, of the product and of the instruction), so log_probs by that of the
+entries' mean |x|, and half a step; the log of the rest by twice as much."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+from card_playing_gym_amd.rl import masked_probabilities, sample_logits, sample_rows, top_logits
+from oracle import choose as ref
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0**-24
+DTYPES = [torch.float32, torch.bfloat16, torch.float16]
+# Both sides of every change of launch, a row's last vector over the one before, and rows read again for each pass.
+WIDTHS = [1, 2, 3, 5, 8, 9, 31, 64, 127, 511, 512, 513, 1000, 1024, 1025, 4096, 4097, 8193, 16385, 32769, 65537, 70001]
+
+
+def make(device, rows, width, dtype, seed, masked=True, sharp=2.0):
+    rng = np.random.default_rng(seed)
+    logits = torch.from_numpy(rng.normal(size=(rows, width)) * sharp * np.exp(rng.normal(size=(rows, 1)) * 0.5)).to(dtype)
+    mask = rng.random((rows, width)) < 0.4
+    mask[np.arange(rows), rng.integers(0, width, rows)] = True
+    return logits.to(device), (torch.from_numpy(mask).to(device) if masked else None), torch.from_numpy(rng.random(rows)).to(device)
+
+
+def numpy_of(t):
+    return None if t is None else (t.double() if t.is_floating_point() else t).cpu().numpy()
+
+
+def check_sample(logits, uniforms, mask, **controls):
+    out = sample_logits(logits, uniforms, mask=mask, **controls)
+    given = {n: numpy_of(x) if isinstance(x, torch.Tensor) else x for n, x in controls.items() if x is not None}
+    actions, log_probs, margin = ref.sample(numpy_of(logits), numpy_of(uniforms), numpy_of(mask), **given)
+    assert out.actions.dtype == torch.int64 and out.log_probs.dtype == torch.float32
+    assert (margin > 1e-9).all()  # (of the inputs, not of the kernel)
+    np.testing.assert_array_equal(out.actions.cpu().numpy(), actions)
+    bar = np.abs(log_probs) * U + 1e-9
+    assert (np.abs(numpy_of(out.log_probs) - log_probs) <= bar).all()
+    return out
+
+
+CONTROLS = [{}, {"temperature": 0.6}, {"top_k": 5}, {"top_p": 0.8}, {"min_p": 0.07}, {"temperature": 0.0},
+            {"temperature": 1.7, "top_k": 40, "top_p": 0.9, "min_p": 0.02}]
+
+
+@pytest.mark.parametrize("width", WIDTHS)
+def test_sample_is_the_definition(device, width):
+    for i, controls in enumerate(CONTROLS):
+        rows = 37 if width <= 1024 else 3
+        logits, mask, u = make(device, rows, width, DTYPES[i % 3], width + i, masked=i % 2 == 0)
+        check_sample(logits, u, mask, **controls)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("width", [6, 300, 5000, 66000])
+def test_every_row_has_its_own_controls(device, width, dtype):
+    rows = 24
+    logits, mask, u = make(device, rows, width, dtype, width)
+    rng = np.random.default_rng(width)
+    of = lambda options, dtype=torch.float32: torch.tensor(rng.choice(options, rows), dtype=dtype, device=device)  # noqa: E731
+    controls = {"temperature": of([0, 0.3, 1, 2]), "top_k": of([-3, 0, 1, 2, 100, 10**12], torch.int64),
+                "top_p": of([1, 0.5, 0.95, 0, 7]), "min_p": of([0, -1, 0.05, 0.5, 1])}
+    check_sample(logits, u, mask, **controls)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("width", [1, 4, 50, 512, 3000, 40000, 70000])
+def test_equal_entries_go_by_their_index(device, width, dtype):
+    """n equal entries: the action of u is number floor(u n) of the kept."""
+
+    n = 65
+    u = torch.from_numpy(np.concatenate([(np.arange(n - 1) + 0.5) / (n - 1), [1 - 2.0**-53]])).to(device)
+    for value in (0.0, -0.0, torch.finfo(dtype).min, torch.finfo(dtype).max, float("inf")):
+        logits = torch.full((n, width), value, dtype=dtype, device=device)
+        if value == 0:  # (-0 and 0 are equal)
+            logits[:, ::2] *= -1
+        for kept, controls in ((width, {}), (min(width, 7), {"top_k": 7}), (-(-width // 4), {"top_p": 0.25}),
+                               (width, {"min_p": 1.0}), (1, {"top_p": 0.0}), (1, {"top_k": 1})):
+            out = sample_logits(logits, u, **controls)
+            want = torch.clamp((u * kept).long(), max=kept - 1)
+            assert torch.equal(out.actions, want), (value, controls)
+            torch.testing.assert_close(out.log_probs, torch.full_like(out.log_probs, -np.log(kept)), rtol=U, atol=1e-9)
+        top = top_logits(logits, 5)
+        assert torch.equal(top.indices, torch.arange(5, device=device).where(torch.arange(5, device=device) < width, -1).expand(n, 5))
+
+
+def test_uniforms_at_their_ends(device):
+    logits = torch.tensor([[0.0, 1.0, -float("inf"), 0.5, -1e9]], device=device).expand(6, 5)
+    u = torch.tensor([0.0, 1 - 2.0**-53, 1.0, 2.0, -1.0, float("nan")], dtype=torch.float64, device=device)
+    assert sample_logits(logits, u).actions.tolist() == [1, 0, 0, 0, 1, 0]  # (-1e9 weighs nothing)
+    assert sample_logits(logits, u, top_k=2).actions.tolist() == [1, 3, 3, 3, 1, 3]
+
+
+@pytest.mark.parametrize("width", [4, 40, 600, 20000, 70000])
+def test_rows_with_nothing_to_choose(device, width):
+    rows = 6
+    logits = torch.randn(rows, width, device=device)
+    mask = torch.ones(rows, width, dtype=torch.bool, device=device)
+    mask[0] = False
+    logits[1] = -float("inf")
+    logits[2, width // 2] = float("nan")
+    logits[3, width // 2], mask[3, width // 2] = float("nan"), False  # not legal: not read as one
+    logits[4, :3] = float("inf")
+    temperature = torch.ones(rows, device=device)
+    temperature[5] = float("nan")
+    out = sample_logits(logits, torch.full((rows,), 0.5, dtype=torch.float64, device=device), mask=mask, temperature=temperature)
+    assert out.actions[:3].tolist() == [-1, -1, -1] and out.actions[4] == 1 and out.actions[5] == -1
+    assert out.actions[3] >= 0 and out.actions[3] != width // 2
+    assert out.log_probs[:2].tolist() == [0, 0] and out.log_probs[[2, 5]].isnan().all()
+    assert abs(out.log_probs[4] + np.log(3)) < 1e-6
+    top = top_logits(logits, 4, mask=mask)
+    assert (top.indices[:3] == -1).all() and (top.log_probs[:2] == -float("inf")).all() and top.log_probs[2].isnan().all()
+    assert (top.log_rest[:2] == -float("inf")).all() and top.log_rest[2].isnan() and not top.log_probs[3].isnan().any()
+    assert top.indices[4].tolist()[:3] == [0, 1, 2] and top.log_rest[4] == -float("inf")
+    np.testing.assert_allclose(top.log_probs[4, :3].cpu(), -np.log(3), rtol=1e-6)
+
+
+def check_top(logits, k, mask, temperature=1.0):
+    out = top_logits(logits, k, mask=mask, temperature=temperature)
+    log_probs, indices, log_rest = ref.top(numpy_of(logits), k, numpy_of(mask), temperature)
+    np.testing.assert_array_equal(out.indices.cpu().numpy(), indices)
+    z = numpy_of(logits)
+    z = z if mask is None else np.where(numpy_of(mask), z, -np.inf)
+    with np.errstate(invalid="ignore"):
+        x = (z.max(1, keepdims=True) - z) / temperature
+    x = np.where(np.isfinite(x), x, 0.0)
+    mean = np.maximum((np.exp(-x) * x).sum(1) / np.exp(-x).sum(1), 0)
+    bar = (3 * mean + 4) * U
+    got, rest = numpy_of(out.log_probs), numpy_of(out.log_rest)
+    there = np.isfinite(log_probs)
+    assert (got[~there] == -np.inf).all()
+    wide = np.broadcast_to(bar[:, None], got.shape)[there]
+    assert (np.abs(got[there] - log_probs[there]) <= wide + np.abs(log_probs[there]) * U).all()
+    some = np.isfinite(log_rest)
+    assert (rest[~some] == -np.inf).all()
+    # (of the rest, entries are measured from their own largest: theirs is at most the row's span)
+    assert (np.abs(rest[some] - log_rest[some]) <= (2 * bar + (3 * mean + 12) * U)[some] + np.abs(log_rest[some]) * U).all()
+    return out
+
+
+@pytest.mark.parametrize("width", WIDTHS)
+def test_top_is_the_definition(device, width):
+    for i, (k, temperature) in enumerate(((1, 1.0), (8, 0.5), (64, 2.0), (256, 1.0))):
+        rows = 37 if width <= 1024 else 3
+        logits, mask, _ = make(device, rows, width, DTYPES[i % 3], width + i, masked=i % 2 == 0)
+        check_top(logits, k, mask, temperature)
+
+
+@pytest.mark.parametrize("width", [300, 3000, 33000, 70000])
+@pytest.mark.parametrize("how", ["few_values", "falling", "rising", "one_vector"])
+def test_top_of_rows_that_crowd(device, width, how):
+    """Many ties at the border, and top entries that all lie side by side."""
+
+    z = torch.linspace(4, -4, width, dtype=torch.float32)
+    if how == "few_values":
+        z = torch.round(torch.randn(width, generator=torch.Generator().manual_seed(3)))
+    elif how == "rising":
+        z = z.flip(0)
+    elif how == "one_vector":
+        z = torch.randn(width, generator=torch.Generator().manual_seed(4)) * 0.1
+        z[100:300] += 5
+    for dtype in DTYPES:
+        logits = z.to(dtype).to(device)[None].repeat(3, 1)
+        for k in (1, 70, 256):
+            check_top(logits, k, None)
+        for controls in ({"top_k": 100}, {"top_p": 0.6}, {"top_k": 30, "temperature": 0.5, "min_p": 0.3}):
+            check_sample(logits, torch.tensor([0.111, 0.5234, 0.901], dtype=torch.float64, device=device), None, **controls)
+
+
+def test_a_rest_far_below_one_keeps_its_digits(device):
+    logits = torch.tensor([[0.0, -80.0, -81.0, 0.5]], device=device)
+    out = top_logits(logits, 2, temperature=0.25)
+    want = ref.top(numpy_of(logits), 2, None, 0.25)[2]
+    assert abs(out.log_rest.item() - want[0]) <= 2e-5 and want[0] < -320
+
+
+@pytest.mark.parametrize("width", [7, 300, 5000, 70000])
+def test_strides(device, width):
+    rows = 9
+    logits, mask, u = make(device, rows, width, torch.bfloat16, 5)
+    wide = torch.zeros(rows, width + 11, dtype=torch.bfloat16, device=device)
+    wide[:, 3 : 3 + width] = logits
+    legal = torch.zeros(rows, width + 5, dtype=torch.bool, device=device)
+    legal[:, 1 : 1 + width] = mask
+    want, top = sample_logits(logits, u, mask=mask, top_p=0.9), top_logits(logits, 20, mask=mask)
+    views = [(wide[:, 3 : 3 + width], legal[:, 1 : 1 + width]),
+             (logits.t().contiguous().t(), mask.t().contiguous().t())]
+    for z, m in views:
+        got = sample_logits(z, u, mask=m, top_p=0.9)
+        assert torch.equal(got.actions, want.actions) and torch.equal(got.log_probs, want.log_probs)
+        for a, b in zip(top_logits(z, 20, mask=m), top):
+            assert torch.equal(a, b)
+    one = logits[:1].expand(rows, width)
+    got = sample_logits(one, u.repeat_interleave(2)[::2], mask=mask[:1].expand(rows, width))
+    for r in range(rows):
+        single = sample_logits(logits[:1], u[r : r + 1], mask=mask[:1])
+        assert torch.equal(got.actions[r : r + 1], single.actions) and torch.equal(got.log_probs[r : r + 1], single.log_probs)
+
+
+def test_no_rows(device):
+    none = torch.empty(0, 5, device=device)
+    assert sample_logits(none, torch.empty(0, dtype=torch.float64, device=device)).actions.shape == (0,)
+    assert top_logits(none, 3).indices.shape == (0, 3)
+
+
+def test_two_streams_and_a_graph(device):
+    logits, mask, u = make(device, 50, 700, torch.bfloat16, 8)
+    want, top = sample_logits(logits, u, mask=mask, top_p=0.7), top_logits(logits, 10, mask=mask)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(device) for _ in range(2)]
+    outs = []
+    for s in streams:
+        with torch.cuda.stream(s):
+            outs.append((sample_logits(logits, u, mask=mask, top_p=0.7), top_logits(logits, 10, mask=mask)))
+    torch.cuda.synchronize()
+    for sampled, record in outs:
+        assert all(torch.equal(a, b) for a, b in zip(sampled, want)) and all(torch.equal(a, b) for a, b in zip(record, top))
+    temperature = torch.ones(50, device=device)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        sampled, record = sample_logits(logits, u, mask=mask, temperature=temperature), top_logits(logits, 10, mask=mask)
+    for turn in range(3):
+        logits.copy_(torch.randn(50, 700, device=device))
+        temperature.fill_(0.5 + turn)
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip((*sampled, *record), (*sample_logits(logits, u, mask=mask, temperature=temperature),
+                                              *top_logits(logits, 10, mask=mask))):
+            assert torch.equal(a, b)
+
+
+def test_sampled_shares_are_the_policys(device):
+    """Uniforms evenly over [0, 1) pick every entry as often as its probability says, as sample_rows does."""
+
+    n = 1 << 14
+    row = torch.randn(1, 40, device=device) * 1.5
+    mask = torch.rand(1, 40, device=device) < 0.7
+    mask[0, 0] = True
+    u = (torch.arange(n, device=device, dtype=torch.float64) + 0.5) / n
+    p = masked_probabilities(row, mask)
+    share = lambda actions: torch.bincount(actions, minlength=40).double() / n  # noqa: E731
+    got = share(sample_logits(row.expand(n, 40), u, mask=mask.expand(n, 40)).actions)
+    also = share(sample_rows(p.repeat(n, 1), mask.repeat(n, 1), u))
+    # an entry's share of n evenly spread uniforms is off by one of them at most
+    assert ((got - p[0].double()).abs() <= 1.0 / n + 40 * U).all() and ((also - p[0].double()).abs() <= 1.0 / n + 40 * U).all()
