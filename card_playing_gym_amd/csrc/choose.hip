@@ -14,8 +14,13 @@
 // keeps a beginning of the order, so S' is the least of their sums, and sampling comes down to
 // finding the entry at a given place in the order's running sum.
 //
-// F(v) = sum of the weights of entries above v falls as v rises, and changes at entries only: the entry at place P is
-// among those of the least v with F(v) <= P, found by halving the range of v, its ties by halving their index.
+// Finding that entry, or the k-th: a histogram of the row's weights (or of ones) in LDS, over bins of equal width in z, says
+// which bin the place falls into and what is summed up before it.  The entries of that bin, a few dozen, go into a
+// list, where each one adds up what stands before it.  A bin of more entries than the list has room for is cut into
+// bins again, between its least and its largest entry; one of equal entries is decided by halving the range of their indices.
+// The first k of a row with k up to the lanes of its group need no histogram: at least k entries are as large as the k-th
+// largest of the lanes' own maxima, and not many more, so these are the list.
+//
 #include "rows.h"
 
 namespace cg {
@@ -52,10 +57,53 @@ struct ChooseArgs {
 
 // ---- a row's group of lanes: a wave, or a block ----------------------------------------------------------------
 
+struct Least {
+  template <typename X>
+  __device__ __forceinline__ X operator()(X a, X b) const {
+    return a < b ? a : b;
+  }
+};
+struct Largest {
+  template <typename X>
+  __device__ __forceinline__ X operator()(X a, X b) const {
+    return a > b ? a : b;
+  }
+};
+
+// The sum over a wave's lanes up to and with this one: within rows of 16 lanes, then rows 0 and 2 into the next, then the
+// lower half into the upper.
+template <int CONTROL, int ROWS = 0xf>
+__device__ __forceinline__ uint64_t from_lower(uint64_t x) {
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, int(uint32_t(x)), CONTROL, ROWS, 0xf, false);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0, int(uint32_t(x >> 32)), CONTROL, ROWS, 0xf, false);
+  return uint64_t(hi) << 32 | lo;
+}
+__device__ __forceinline__ uint64_t wave_running_sum(uint64_t x) {
+  x += from_lower<0x111>(x);       // row_shr:1
+  x += from_lower<0x112>(x);       // row_shr:2
+  x += from_lower<0x114>(x);       // row_shr:4
+  x += from_lower<0x118>(x);       // row_shr:8
+  x += from_lower<0x142, 0xa>(x);  // row_bcast:15
+  x += from_lower<0x143, 0xc>(x);  // row_bcast:31
+  return x;
+}
+
+// An entry in a list: its place in the order as a number (larger ones first), and its weight.
+struct Item {
+  uint64_t key, weight;
+};
+
 template <int G>
 struct Shared {
   static constexpr int W = G > 64 ? G / 64 : 1;
+  static constexpr int BINS = G > 64 ? 1024 : 256, LIST = G > 64 ? 512 : 256;
   uint64_t slots[2][W];
+  union {  // (the bins are in registers when a list is made)
+    uint64_t bins[BINS];
+    Item list[LIST];
+  };
+  uint64_t found[2];
+  int count;
 };
 
 template <int G>
@@ -89,47 +137,101 @@ struct Group {
     }
     return x;
   }
+  // The sum over the lanes before this one, and over all.
+  __device__ __forceinline__ uint64_t sum_before(uint64_t x, uint64_t &all) {
+    const uint64_t upto = wave_running_sum(x);
+    uint64_t before = upto - x;
+    all = __shfl(upto, 63, 64);
+    if constexpr (G > 64) {
+      constexpr int W = G / 64;
+      uint64_t *slot = shared.slots[turn];
+      turn ^= 1;
+      if ((threadIdx.x & 63) == 63) slot[threadIdx.x >> 6] = upto;
+      __syncthreads();
+      all = 0;
+      const int wave = threadIdx.x >> 6;
+#pragma unroll
+      for (int w = 0; w < W; ++w) {
+        before += w < wave ? slot[w] : 0;
+        all += slot[w];
+      }
+    }
+    return before;
+  }
 };
 
-// ---- a row's entries: in registers, or read again for every pass ---------------------------------------------
+// ---- a row's entries: in LDS, or read again for every pass ----------------------------------------------------
 //
-// each(visit): visit(index of entry 0, z) for this lane's vectors, z(k) the k-th logit, -inf where it is not legal.
+// A row is looked through several times, each time with little to do for most entries: from LDS that costs a fifth of
+// what the entries' weights cost, while kept in registers they take most of what a lane has, and code of their number.
+// each(visit): visit(index of entry 0, z) for this lane's vectors, z(k) the k-th logit, -inf where it is not legal.  A
+// lane reads what it has written: no barrier stands between.
 
-// S: the type in which entries are kept (T, or float where rows are shorter than a load).
-template <typename T, int G, int E, typename S = T>
-struct Held {
-  static constexpr int V = E == 1 ? 1 : VEC<T>, C = E / V;
-  Entries<S, E> z;
-  int width;
-  __device__ __forceinline__ Held(const T *row, const uint8_t *legal, int width) : width(width) {
-    load_entries<G, C, V>(z.w, row, legal, int(threadIdx.x % G) * V, width);
+template <typename T, int G, int BYTES>
+struct InLds {
+  static constexpr int V = VEC<T>, VECTORS = BYTES / 16, BATCH = VECTORS / G < 8 ? VECTORS / G : 8;
+  struct alignas(16) Vector {
+    uint32_t w[4];
+  };
+  Vector *held;
+  int width, vectors;
+  __device__ __forceinline__ InLds(Vector *held, const T *row, const uint8_t *legal, int width)
+      : held(held), width(width), vectors((width + V - 1) / V) {
+    const int lane = threadIdx.x % G;
+    if (width < V) {
+      if (lane > 0) return;
+      Vector q;
+      for (int k = 0; k < 4; ++k) q.w[k] = NEGATIVE_INFINITY<T>;
+      for (int k = 0; k < V; ++k) {
+        if (k >= width || (legal && !legal[k])) continue;
+        if constexpr (sizeof(T) == 4) {
+          q.w[k] = __float_as_uint(row[k]);
+        } else {
+          const int shift = 16 * (k % 2);
+          q.w[k / 2] = (q.w[k / 2] & ~(0xffffu << shift)) | uint32_t(row[k].bits) << shift;
+        }
+      }
+      held[0] = q;
+      return;
+    }
+    for (int first = lane; first < vectors; first += G * BATCH) {
+      uint32_t w[BATCH][4];
+#pragma unroll
+      for (int c = 0; c < BATCH; ++c) load_entries<1, 1, V>(w[c], row, legal, min(first + c * G, vectors - 1) * V, width);
+#pragma unroll
+      for (int c = 0; c < BATCH; ++c)
+        if (first + c * G < vectors) __builtin_memcpy(&held[first + c * G], w[c], 16);
+    }
   }
+  __device__ __forceinline__ int at(int j) const { return max(min(j * V, width - V), 0); }
   template <typename Visit>
   __device__ __forceinline__ void each(const Visit &visit) const {
-    const int first = int(threadIdx.x % G) * V;
-#pragma unroll
-    for (int c = 0; c < C; ++c) {
-      const int at = V == 1 ? first : min(first + c * G * V, width - V);
-      visit(at, [&](int k) { return z[c * V + k]; });
+#pragma unroll 2
+    for (int j = threadIdx.x % G; j < vectors; j += G) {
+      Entries<T, V> q;
+      __builtin_memcpy(q.w, &held[j], 16);
+      visit(at(j), [&](int k) { return q[k]; });
     }
   }
   // A row whose largest entry is +inf: these share everything.
   __device__ __forceinline__ void unbounded() {
-    constexpr int PER = Entries<S, E>::PER;
-    constexpr uint32_t NONE = NEGATIVE_INFINITY<S>;
+    for (int j = threadIdx.x % G; j < vectors; j += G) {
+      Entries<T, V> q;
+      __builtin_memcpy(q.w, &held[j], 16);
 #pragma unroll
-    for (int k = 0; k < E; ++k) {
-      const uint32_t part = PER == 1 ? ~0u : k % 2 ? 0xffff0000u : 0xffffu;
-      const bool is = z[k] == INFINITY;
-      uint32_t &w = z.w[k / PER];
-      w = (w & ~part) | (is ? 0u : NONE & part);
+      for (int k = 0; k < V; ++k) {
+        const uint32_t part = sizeof(T) == 4 ? ~0u : k % 2 ? 0xffff0000u : 0xffffu;
+        uint32_t &w = q.w[k / Entries<T, V>::PER];
+        w = (w & ~part) | (q[k] == INFINITY ? 0u : NEGATIVE_INFINITY<T> & part);
+      }
+      __builtin_memcpy(&held[j], q.w, 16);
     }
   }
 };
 
 template <typename T, int G>
 struct Read {
-  static constexpr int V = VEC<T>;
+  static constexpr int V = VEC<T>, BATCH = 4;
   const T *row;
   const uint8_t *legal;
   int width;
@@ -137,10 +239,16 @@ struct Read {
   __device__ __forceinline__ Read(const T *row, const uint8_t *legal, int width) : row(row), legal(legal), width(width) {}
   template <typename Visit>
   __device__ __forceinline__ void each(const Visit &visit) const {
-    for (int i = int(threadIdx.x % G) * V; i < width; i += G * V) {
-      Entries<T, V> q;
-      load_entries<1, 1, V>(q.w, row, legal, i, width);
-      visit(min(i, width - V), [&](int k) { return infinite ? (q[k] == INFINITY ? 0.f : -INFINITY) : q[k]; });
+    const int vectors = (width + V - 1) / V;
+    for (int first = threadIdx.x % G; first < vectors; first += G * BATCH) {
+      Entries<T, V> q[BATCH];
+#pragma unroll
+      for (int c = 0; c < BATCH; ++c) load_entries<1, 1, V>(q[c].w, row, legal, min(first + c * G, vectors - 1) * V, width);
+#pragma unroll
+      for (int c = 0; c < BATCH; ++c)
+        if (first + c * G < vectors)
+          visit(min((first + c * G) * V, width - V),
+                [&](int k) { return infinite ? (q[c][k] == INFINITY ? 0.f : -INFINITY) : q[c][k]; });
     }
   }
   __device__ __forceinline__ void unbounded() { infinite = true; }
@@ -165,7 +273,8 @@ struct Weights {
   // off by 2^-44.6 of it at most, and 1 at 0.
   __device__ __forceinline__ uint64_t operator()(float z) const {
     const double t = fmax((double(z) - top) * c, -64.0);  // (a NaN of -inf and c = 0 too: a weight of 0 from -63 on)
-    const double k = __builtin_rint(t), f = t - k;
+    // (adding 1.5 * 2^52 rounds to whole numbers, k's low bits the sum's)
+    const double whole = t + 6755399441055744.0, f = t - (whole - 6755399441055744.0);
     double p = 1.0202923985536321e-07;
     p = fma(p, f, 1.3255228630225242e-06);
     p = fma(p, f, 1.5252687853419455e-05);
@@ -176,47 +285,54 @@ struct Weights {
     p = fma(p, f, 0.24022650695813);
     p = fma(p, f, 0.6931471805599454);
     p = fma(p, f, 1.0);
-    const double sum = __builtin_amdgcn_ldexp(p, int(k)) + magic;
+    const double sum = __hiloint2double(__double2hiint(p) + (__double2loint(whole) << 20), __double2loint(p)) + magic;
     return __builtin_bit_cast(uint64_t, sum) - __builtin_bit_cast(uint64_t, magic);
   }
 };
 
-// The sum of the weights above v; their count.
+// An entry's place in the order as a number: larger ones come first.
+__device__ __forceinline__ uint64_t place_of(float z, int index) { return uint64_t(key_of(z)) << 32 | uint32_t(~index); }
+__device__ __forceinline__ float value_at(uint64_t place) { return of_key(uint32_t(place >> 32)); }
+__device__ __forceinline__ int index_at(uint64_t place) { return int(~uint32_t(place)); }
+
+// A row's largest entry, -inf where none is legal and NaN where one of them is; of this lane's entries: `mine`.
 template <typename Row, int G>
-__device__ __forceinline__ uint64_t mass_above(const Row &row, Group<G> &group, const Weights &weight, float v) {
-  uint64_t s = 0;
-  row.each([&](int, const auto &z) {
+__device__ __forceinline__ float row_top(Row &row, Group<G> &group, float &mine) {
+  const auto pass = [&] {
+    mine = -INFINITY;
+    bool nan = false;
+    row.each([&](int, const auto &z) {
 #pragma unroll
-    for (int k = 0; k < Row::V; ++k)
-      if (z(k) > v) s += weight(z(k));
-  });
-  return group.join(s, Plus{});
-}
-template <typename Row, int G>
-__device__ __forceinline__ int count_above(const Row &row, Group<G> &group, float v) {
-  int n = 0;
-  row.each([&](int, const auto &z) {
-#pragma unroll
-    for (int k = 0; k < Row::V; ++k) n += z(k) > v;
-  });
-  return group.join(n, Plus{});
+      for (int k = 0; k < Row::V; ++k) {
+        mine = fmaxf(mine, z(k));
+        nan |= z(k) != z(k);
+      }
+    });
+    // (the larger of two, NaN where one is)
+    return group.join(nan ? NAN : mine, [](float a, float b) { return a > b || a != a ? a : b; });
+  };
+  float top = pass();
+  if (top == INFINITY) {
+    row.unbounded();
+    top = pass();
+  }
+  return top;
 }
 
-// The least v up to `top` at which of(v) < limit; of(v) falls as v rises, of(-inf) >= limit, of(top) = 0.
-// value: of(v) there.
-template <typename X, typename Of>
-__device__ __forceinline__ float least_value(float top, X limit, const Of &of, X &value) {
-  uint32_t lo = key_of(-INFINITY), hi = key_of(top);
-  value = 0;
-  while (hi - lo > 1) {
-    const uint32_t mid = lo + (hi - lo) / 2;
-    const X x = of(of_key(mid));
-    if (x < limit)
-      hi = mid, value = x;
-    else
-      lo = mid;
-  }
-  return of_key(hi);
+// The least and the largest of the entries for which in(z, index) holds, inf and -inf where none does.
+template <typename Row, int G, typename In>
+__device__ __forceinline__ void range_of(const Row &row, Group<G> &group, const In &in, float &least, float &most) {
+  least = INFINITY, most = -INFINITY;
+  row.each([&](int at, const auto &z) {
+#pragma unroll
+    for (int k = 0; k < Row::V; ++k) {
+      const bool is = in(z(k), at + k);
+      least = fminf(least, is ? z(k) : INFINITY);
+      most = fmaxf(most, is ? z(k) : -INFINITY);
+    }
+  });
+  least = group.join(least, Least{});
+  most = group.join(most, Largest{});
 }
 
 // The index of entry number r (from 0) of those equal to v.
@@ -238,192 +354,478 @@ __device__ __forceinline__ int tie(const Row &row, Group<G> &group, float v, int
   return hi;
 }
 
-// The row's largest entry, -inf where none is legal; nan: one of them is.
 template <typename Row, int G>
-__device__ __forceinline__ float row_top(Row &row, Group<G> &group, bool &nan) {
-  float top = -INFINITY;
-  int bad = 0;
-  row.each([&](int, const auto &z) {
+__device__ __forceinline__ int first_index(const Row &row, Group<G> &group, float v) {
+  int first = row.width;
+  row.each([&](int at, const auto &z) {
+#pragma unroll
+    for (int k = 0; k < Row::V; ++k) first = min(first, z(k) == v ? at + k : row.width);
+  });
+  return group.join(first, Least{});
+}
+
+// A value that at least n <= G of the row's entries are as large as, and not many more: near the n-th largest of
+// the lanes' maxima.  -inf where fewer lanes have an entry.
+template <int G>
+__device__ __forceinline__ float bound_of_top(Group<G> &group, float top, float mine, int n) {
+  constexpr int W = G / 64;
+  float tops[W];
+  if constexpr (G > 64) {
+    float *all = reinterpret_cast<float *>(group.shared.bins);
+    all[threadIdx.x] = mine;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < W; ++w) tops[w] = all[w * 64 + (threadIdx.x & 63)];
+    __syncthreads();  // (the bins are used next)
+  } else {
+    tops[0] = mine;
+  }
+  const auto count = [&](float v) {
+    int c = 0;
+#pragma unroll
+    for (int w = 0; w < W; ++w) c += __popcll(__ballot(tops[w] >= v));
+    return c;
+  };
+  float lo = INFINITY;
+#pragma unroll
+  for (int w = 0; w < W; ++w) lo = fminf(lo, tops[w] == -INFINITY ? INFINITY : tops[w]);
+  lo = lanes_join<64>(lo, Least{});
+  if (lo == INFINITY || count(lo) < n) return -INFINITY;
+  float hi = top;
+  for (int turn = 0; turn < 40; ++turn) {  // (lo: at least n are as large)
+    const float mid = 0.5f * lo + 0.5f * hi;
+    if (!(mid > lo && mid < hi)) break;
+    const int c = count(mid);
+    if (c >= n) {
+      lo = mid;
+      if (c <= n + n / 8) break;
+    } else {
+      hi = mid;
+    }
+  }
+  return lo;
+}
+
+// The entries for which in(z, index) holds, with weight(z), into the list.  Returns how many there are, of which
+// those past the list's room are not in it.
+template <typename Row, int G, typename In, typename Weight>
+__device__ __forceinline__ int gather(const Row &row, Group<G> &group, const In &in, const Weight &weight) {
+  Shared<G> &s = group.shared;
+  if (group.lane() == 0) s.count = 0;
+  group.sync();
+  row.each([&](int at, const auto &z) {
+    bool any = false;
+#pragma unroll
+    for (int k = 0; k < Row::V; ++k) any |= in(z(k), at + k);
+    if (!any) return;
 #pragma unroll
     for (int k = 0; k < Row::V; ++k) {
-      top = fmaxf(top, z(k));
-      bad |= z(k) != z(k);
+      if (!in(z(k), at + k)) continue;
+      const int slot = atomicAdd(&s.count, 1);
+      if (slot < Shared<G>::LIST) s.list[slot] = Item{place_of(z(k), at + k), weight(z(k))};
     }
   });
-  if (bad) top = NAN;
-  // (the larger of two, NaN where one is)
-  top = group.join(top, [](float a, float b) { return a > b || a != a ? a : b; });
-  nan = top != top;
-  if (top == INFINITY) {
-    row.unbounded();
-    top = 0;
-  }
-  return top;
+  group.sync();
+  return s.count;
 }
+
+// This lane's items of a list, with what stands before each.
+template <int G>
+struct Mine {
+  static constexpr int N = Shared<G>::LIST / G > 0 ? Shared<G>::LIST / G : 1;
+  Item item[N];
+  uint64_t before[N];
+  int rank[N];
+  bool in[N];
+  __device__ __forceinline__ Mine(const Shared<G> &s, int n) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int at = Group<G>::lane() + i * G;
+      in[i] = at < n;
+      item[i] = in[i] ? s.list[at] : Item{0, 0};
+      before[i] = 0;
+      rank[i] = 0;
+    }
+    if (int(threadIdx.x % G) / 64 * 64 >= n) return;  // (waves without items)
+    for (int j = 0; j < n; ++j) {
+      const Item other = s.list[j];
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const bool ahead = other.key > item[i].key;
+        before[i] += ahead ? other.weight : 0;
+        rank[i] += ahead;
+      }
+    }
+  }
+};
+
+// ---- the entry at a place of the running sum over the order ------------------------------------------------------
+
+// Bins of equal width from `from` downwards, the last one for all below.  A z further away than float32 can say is
+// in the last one; a range that it cannot divide is one bin.
+struct Bins {
+  float from, scale, last;
+  __device__ __forceinline__ Bins(float from, float low, int n) : from(from), last(float(n - 1)) {
+    const float span = from - low;
+    scale = last / span;
+    if (!(span > 0 && scale < INFINITY)) scale = 0;
+  }
+  __device__ __forceinline__ float at(float z) const { return fminf((from - z) * scale, last); }
+  __device__ __forceinline__ bool in(int b, float z) const {
+    const float x = at(z);
+    return x >= float(b) && x < float(b + 1);
+  }
+};
+
+struct Entry {
+  uint64_t place;  // in the order, as place_of
+  uint64_t upto;   // the running sum with it
+};
+
+// The histogram of weight(z) over the entries for which in(z, index) holds and whose weight is at least `bound` (1 or more).
+template <typename Row, int G>
+struct Histogram {
+  static constexpr int PER = Shared<G>::BINS / G;
+  Bins bins;
+  uint64_t value[PER], before, total;  // of this lane's bins
+  uint64_t less;                       // this lane's weights below `bound`
+
+  template <typename Weight, typename In>
+  __device__ __forceinline__ Histogram(const Row &row, Group<G> &group, const Weight &weight, float from, float low,
+                                       uint64_t bound, const In &in)
+      : bins(from, low, Shared<G>::BINS), less(0) {
+    Shared<G> &s = group.shared;
+    const int lane = group.lane();
+    for (int b = lane; b < Shared<G>::BINS; b += G) s.bins[b] = 0;
+    group.sync();
+    row.each([&](int at, const auto &z) {
+#pragma unroll
+      for (int k = 0; k < Row::V; ++k) {
+        if (!in(z(k), at + k)) continue;
+        const uint64_t w = weight(z(k));
+        if (w >= bound)
+          atomicAdd(reinterpret_cast<unsigned long long *>(&s.bins[int(bins.at(z(k)))]), w);
+        else
+          less += w;
+      }
+    });
+    group.sync();
+    uint64_t mine = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      value[i] = s.bins[lane * PER + i];
+      mine += value[i];
+    }
+    before = group.sum_before(mine, total);
+  }
+  // The bin where the running sum reaches `sum` (1 to total), and what is summed up before it.
+  __device__ __forceinline__ int locate(Group<G> &group, uint64_t sum, uint64_t &ahead) const {
+    Shared<G> &s = group.shared;
+    uint64_t b = before;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      if (b < sum && sum <= b + value[i]) {
+        s.found[0] = group.lane() * PER + i;
+        s.found[1] = b;
+      }
+      b += value[i];
+    }
+    group.sync();
+    ahead = s.found[1];
+    return int(s.found[0]);
+  }
+  // The entry at which the running sum reaches `sum`.
+  template <typename Weight, typename In>
+  __device__ __forceinline__ Entry entry(const Row &row, Group<G> &group, const Weight &weight, uint64_t sum,
+                                         const In &in) const;
+};
+
+template <typename Row, int G>
+template <typename Weight, typename In>
+__device__ __forceinline__ Entry Histogram<Row, G>::entry(const Row &row, Group<G> &group, const Weight &weight,
+                                                          uint64_t sum, const In &in) const {
+  Shared<G> &s = group.shared;
+  uint64_t ahead;
+  const int bin = locate(group, sum, ahead);
+  const auto here = [&](float z, int i) { return bins.in(bin, z) && in(z, i); };
+  const int n = gather(row, group, here, weight);
+  if (n <= Shared<G>::LIST) {
+    const Mine<G> mine(s, n);
+#pragma unroll
+    for (int i = 0; i < Mine<G>::N; ++i) {
+      const uint64_t b = ahead + mine.before[i];
+      if (mine.in[i] && b < sum && sum <= b + mine.item[i].weight) {
+        s.found[0] = mine.item[i].key;
+        s.found[1] = b + mine.item[i].weight;
+      }
+    }
+    group.sync();
+    const Entry e{s.found[0], s.found[1]};
+    group.sync();
+    return e;
+  }
+  // Too many for the list: the least value above which less than `sum` is, by halving the range of the bin's values.
+  float least, most;
+  range_of(row, group, here, least, most);
+  uint32_t lo = key_of(least), hi = key_of(most);
+  uint64_t above = ahead;  // above hi, ahead of the bin included
+  while (lo < hi) {
+    const uint32_t mid = lo + (hi - lo) / 2;
+    const float v = of_key(mid);
+    uint64_t x = 0;
+    row.each([&](int at, const auto &z) {
+#pragma unroll
+      for (int k = 0; k < Row::V; ++k)
+        if (z(k) > v && here(z(k), at + k)) x += weight(z(k));
+    });
+    x = ahead + group.join(x, Plus{});
+    if (x < sum)
+      hi = mid, above = x;
+    else
+      lo = mid + 1;
+  }
+  const float v = of_key(hi);
+  const uint64_t w = weight(v);
+  const uint64_t r = (sum - 1 - above) / w;  // of those equal to v
+  return Entry{place_of(v, tie(row, group, v, int(r))), above + (r + 1) * w};
+}
+
+struct One {
+  __device__ __forceinline__ uint64_t operator()(float) const { return 1; }
+};
 
 // ---- sampling ----------------------------------------------------------------------------------------------------
 
+// The largest k for which the lanes' maxima say where a row's first k end, and the list holds them.
+template <int G>
+constexpr int SHORT = G < Shared<G>::LIST / 2 ? G : Shared<G>::LIST / 2;
+
 template <typename Row, int G>
 __device__ __forceinline__ void sample_row(const ChooseArgs &a, int64_t r, Row &row, Group<G> &group) {
+  Shared<G> &s = group.shared;
   const double temperature = a.temperature.of(r), p = a.top_p.of(r), least = a.min_p.of(r), u = a.uniforms[r];
   const int64_t most = a.top_k.of(r);
-  bool nan;
-  const float top = row_top(row, group, nan);
-  int64_t action = -1;
-  float log_prob = 0;
-  if (nan || !(temperature >= 0)) {
-    log_prob = NAN;
-  } else if (top > -INFINITY) {
-    if (temperature == 0) {
-      action = tie(row, group, top, 0);
-    } else {
-      const Weights weight(top, temperature, a.scale);
-      const uint64_t one = uint64_t(1) << a.scale;
-      uint64_t total = mass_above(row, group, weight, -INFINITY);
-      if (most > 0 && most < a.width && most < count_above(row, group, -INFINITY)) {
-        int above;
-        const float v = least_value(top, int(most), [&](float x) { return count_above(row, group, x); }, above);
-        total = mass_above(row, group, weight, v) + (most - above) * weight(v);
-      }
-      const auto mass = [&](float x) { return mass_above(row, group, weight, x); };
-      uint64_t kept = total;
-      if (p < 1) {
-        const uint64_t limit = p > 0 ? uint64_t(ceil(p * double(total))) : 1;
-        uint64_t above;
-        const float v = least_value(top, limit > 0 ? limit : 1, mass, above);
-        const uint64_t w = weight(v);
-        kept = min(kept, above + (limit - above + w - 1) / w * w);
-      }
-      if (least > 0) {
-        const double x = ceil(least * double(one));
-        const uint64_t bound = x < double(one) ? uint64_t(x) : one;
-        uint64_t s = 0;
-        row.each([&](int, const auto &z) {
+  float mine;
+  const float top = row_top(row, group, mine);
+  const auto answer = [&](int64_t action, float log_prob) { a.actions[r] = action, a.log_probs[r] = log_prob; };
+  if (top != top || !(temperature >= 0)) {
+    if (group.lane() == 0) answer(-1, NAN);
+    return;
+  }
+  if (top == -INFINITY) {
+    if (group.lane() == 0) answer(-1, 0);
+    return;
+  }
+  if (temperature == 0) {
+    const int first = first_index(row, group, top);
+    if (group.lane() == 0) answer(first, 0);
+    return;
+  }
+  const Weights weight(top, temperature, a.scale);
+  const uint64_t one = uint64_t(1) << a.scale;
+  // min_p as the least weight that is kept (the first entry's at most)
+  uint64_t bound = 1;
+  if (least > 0) {
+    const double x = ceil(least * double(one));
+    bound = x < double(one) ? uint64_t(x) : one;
+  }
+  const auto limit_of = [&](uint64_t total) {  // top_p as a sum: entries before which less than this is summed up are kept
+    const double x = ceil(p * double(total));
+    return x > 1 ? uint64_t(x) : 1;
+  };
+  // The running sum that the answer's is the first to reach: u of what is kept, and a unit more.
+  const auto target = [&](uint64_t kept) {
+    const double x = u * double(kept);
+    const uint64_t place = x > 0 ? x < double(kept) ? uint64_t(x) : kept - 1 : u != u ? kept - 1 : 0;
+    return (place < kept ? place : kept - 1) + 1;
+  };
+  const auto log_share = [&](uint64_t place, uint64_t kept) {
+    return float((double(value_at(place)) - double(top)) / temperature -
+                 (log_of(double(kept)) - a.scale * 0.69314718055994530942));
+  };
+  const bool limited = most > 0 && most < a.width;
+  if (limited ? most <= SHORT<G> : a.width <= 64) {
+    const float from = limited ? bound_of_top(group, top, mine, int(most)) : -INFINITY;
+    const int n = gather(row, group, [&](float z, int) { return z >= from && z > -INFINITY; }, weight);
+    if (n <= Shared<G>::LIST) {
+      const Mine<G> list(s, n);
+      const int last = limited && most < n ? int(most) - 1 : n - 1;
+      const auto each = [&](const auto &visit) {
 #pragma unroll
-          for (int k = 0; k < Row::V; ++k) {
-            const uint64_t w = weight(z(k));
-            s += w >= bound ? w : 0;
-          }
+        for (int i = 0; i < Mine<G>::N; ++i)
+          if (list.in[i]) visit(list.item[i], list.before[i], list.rank[i]);
+      };
+      each([&](const Item &item, uint64_t before, int rank) {
+        if (rank == last) s.found[0] = before + item.weight;
+      });
+      group.sync();
+      uint64_t kept = s.found[0];
+      if (p < 1) {
+        const uint64_t limit = limit_of(kept);
+        each([&](const Item &item, uint64_t before, int) {
+          if (before < limit && limit <= before + item.weight) s.found[1] = before + item.weight;
         });
-        s = group.join(s, Plus{});
-        kept = min(kept, least > 1 ? one : s);
+        group.sync();
+        kept = s.found[1];
       }
-      // The entry at place u S' (as integers: the first running sum above it); the last one for a u of 1 or NaN.
-      const double at = u * double(kept);
-      uint64_t place = at > 0 ? at < double(kept) ? uint64_t(at) : kept - 1 : u != u ? kept - 1 : 0;
-      place = min(place, kept - 1);
-      uint64_t above;
-      const float v = least_value(top, place + 1, mass, above);
-      const uint64_t w = weight(v);
-      action = tie(row, group, v, int((place - above) / w));
-      log_prob = float((double(v) - double(top)) / temperature - (log_of(double(kept)) - a.scale * 0.69314718055994530942));
+      if (bound > 1) {
+        uint64_t upto = 0;
+        each([&](const Item &item, uint64_t before, int) {
+          if (item.weight >= bound) upto = Largest{}(upto, before + item.weight);
+        });
+        kept = min(kept, least > 1 ? one : group.join(upto, Largest{}));
+      }
+      const uint64_t sum = target(kept);
+      each([&](const Item &item, uint64_t before, int) {
+        if (before < sum && sum <= before + item.weight) answer(index_at(item.key), log_share(item.key, kept));
+      });
+      return;
     }
   }
-  if (group.lane() == 0) {
-    a.actions[r] = action;
-    a.log_probs[r] = log_prob;
+  const auto legal = [](float z, int) { return z > -INFINITY; };
+  float low, high;
+  range_of(row, group, legal, low, high);
+  float from = -INFINITY;  // the last of the first k, and its index
+  int index = -1;
+  if (limited) {
+    const One one;
+    const Histogram<Row, G> h(row, group, one, top, low, 1, legal);
+    if (uint64_t(most) < h.total) {
+      const uint64_t place = h.entry(row, group, one, uint64_t(most), legal).place;
+      from = value_at(place), index = index_at(place);
+    }
   }
+  // (weights end scale + 1 octaves down; in float32, and a little further)
+  const float end = float(double(top) - (a.scale + 2) / weight.c);
+  const auto in = [&](float z, int i) { return z > from || (z == from && i <= index); };
+  const Histogram<Row, G> h(row, group, weight, top, fmaxf(fmaxf(low, from), end), bound, in);
+  uint64_t kept = h.total;
+  if (p < 1) {
+    const uint64_t limit = limit_of(bound > 1 ? kept + group.join(h.less, Plus{}) : kept);
+    if (limit < kept) kept = h.entry(row, group, weight, limit, in).upto;
+  }
+  if (least > 1) kept = one;
+  const uint64_t place = h.entry(row, group, weight, target(kept), in).place;
+  if (group.lane() == 0) answer(index_at(place), log_share(place, kept));
 }
 
 // ---- the record --------------------------------------------------------------------------------------------------
 
-struct Top {
-  float z;
-  int index;
-  // Whether this stands before o in the order.
-  __device__ __forceinline__ bool before(const Top &o) const { return z > o.z || (z == o.z && index < o.index); }
-};
-
 template <typename Row, int G>
-__device__ __forceinline__ void top_row(const ChooseArgs &a, int64_t r, Row &row, Group<G> &group, Top *list, int *count) {
-  const double temperature = a.temperature.of(r);
+__device__ __forceinline__ void top_row(const ChooseArgs &a, int64_t r, Row &row, Group<G> &group) {
+  Shared<G> &s = group.shared;
+  const double inverse = 1 / a.temperature.value;
   const int lane = group.lane();
   float *log_probs = a.log_probs + r * a.k;
   int64_t *indices = a.indices + r * a.k;
-  bool nan;
-  const float top = row_top(row, group, nan);
-  int held = 0;
-  double log_total = 0;
-  float log_rest = nan ? NAN : -INFINITY;
-  if (!nan && top > -INFINITY) {
-    const int legal = count_above(row, group, -INFINITY);
-    held = min(a.k, legal);
-    // Entries above v, and those equal to it up to index `last`.
-    float v = -INFINITY;
-    int last = -1;
-    if (held < legal) {
-      int above;
-      v = least_value(top, held, [&](float x) { return count_above(row, group, x); }, above);
-      last = tie(row, group, v, held - above - 1);
-    }
-    if (lane == 0) *count = 0;
-    group.sync();
-    const auto in = [&](float z, int i) { return z > v || (z == v && i <= last); };
-    float next = -INFINITY;  // the largest of the others
-    row.each([&](int at, const auto &z) {
-#pragma unroll
-      for (int k = 0; k < Row::V; ++k) {
-        if (z(k) == -INFINITY) continue;
-        if (in(z(k), at + k))
-          list[atomicAdd(count, 1)] = Top{z(k), at + k};
-        else
-          next = fmaxf(next, z(k));
-      }
-    });
-    next = group.join(next, Most{});
-    const float from = next > -INFINITY ? next : 0.f;
-    const double c = 1.44269504088896340736 / temperature;
-    const float fast = float(c), rest = float(c - double(fast));
-    // e^((z - from) / T), with what the rounding of the product cuts off
-    double s = 0;
-    row.each([&](int at, const auto &z) {
-#pragma unroll
-      for (int k = 0; k < Row::V; ++k) {
-        if (z(k) == -INFINITY || in(z(k), at + k)) continue;
-        const float d = z(k) - from, t = d * fast;
-        s += __builtin_amdgcn_exp2f(t) * (1 + fmaf(d, rest, fmaf(d, fast, -t)) * 0.69314718f);
-      }
-    });
-    s = group.join(s, Add{});
-    group.sync();
-    double in_list = 0;
-    for (int i = lane; i < held; i += G) in_list += exp_of((double(list[i].z) - double(top)) / temperature);
-    in_list = group.join(in_list, Add{});
-    const double gap = (double(from) - double(top)) / temperature;
-    log_total = log_of(in_list + (s > 0 ? s * exp_of(gap) : 0.0));
-    if (s > 0) log_rest = float(gap + log_of(s) - log_total);
-    for (int i = lane; i < held; i += G) {
-      const Top mine = list[i];
-      int rank = 0;
-      for (int j = 0; j < held; ++j) rank += list[j].before(mine);
-      log_probs[rank] = float((double(mine.z) - double(top)) / temperature - log_total);
-      indices[rank] = mine.index;
-    }
+  float mine;
+  const float top = row_top(row, group, mine);
+  if (top != top || top == -INFINITY) {
+    for (int i = lane; i < a.k; i += G) log_probs[i] = top, indices[i] = -1;
+    if (lane == 0) a.log_rest[r] = top;
+    return;
   }
-  for (int i = held + lane; i < a.k; i += G) {
-    log_probs[i] = nan ? NAN : -INFINITY;
-    indices[i] = -1;
+  // The list: entries above `from`, and those equal to it up to `index`.
+  const One one;
+  float from = -INFINITY;
+  int index = -1, n = Shared<G>::LIST + 1;
+  const auto in = [&](float z, int i) { return z > from || (z == from && i <= index); };
+  if (a.k >= a.width) {
+    n = gather(row, group, in, one);
+  } else if (a.k <= SHORT<G>) {
+    from = bound_of_top(group, top, mine, a.k);
+    index = from > -INFINITY ? a.width : -1;
+    n = gather(row, group, in, one);
   }
-  if (lane == 0) a.log_rest[r] = log_rest;
+  if (n > Shared<G>::LIST) {
+    const auto legal = [](float z, int) { return z > -INFINITY; };
+    float low, high;
+    range_of(row, group, legal, low, high);
+    from = -INFINITY, index = -1;
+    const Histogram<Row, G> h(row, group, one, top, low, 1, legal);
+    if (uint64_t(a.k) < h.total) {
+      const uint64_t place = h.entry(row, group, one, uint64_t(a.k), legal).place;
+      from = value_at(place), index = index_at(place);
+    }
+    n = gather(row, group, in, one);
+  }
+  const Mine<G> list(s, n);
+  const int held = min(n, a.k);
+  // The others: those behind in the list, and those not in it; `next` is their largest.
+  float next;
+  if (n > a.k) {
+#pragma unroll
+    for (int i = 0; i < Mine<G>::N; ++i)
+      if (list.in[i] && list.rank[i] == a.k) s.found[0] = list.item[i].key;
+    group.sync();
+    next = value_at(s.found[0]);
+  } else {
+    float least;
+    range_of(row, group, [&](float z, int i) { return !in(z, i); }, least, next);
+  }
+  const float base = next > -INFINITY ? next : 0.f;
+  const double c = 1.44269504088896340736 * inverse;
+  const float fast = float(c), slow = float(c - double(fast));
+  const auto weigh = [&](float z) {
+    const float d = z - base;
+    return __builtin_amdgcn_exp2f(fmaf(d, fast, d * slow));
+  };
+  double sums[2] = {0, 0};  // of the others, and of the record
+  row.each([&](int at, const auto &z) {
+    float sum = 0;
+#pragma unroll
+    for (int k = 0; k < Row::V; ++k) sum += in(z(k), at + k) || z(k) == -INFINITY ? 0.f : weigh(z(k));
+    sums[0] += sum;
+  });
+#pragma unroll
+  for (int i = 0; i < Mine<G>::N; ++i) {
+    if (!list.in[i]) continue;
+    const float z = value_at(list.item[i].key);
+    if (list.rank[i] < a.k)
+      sums[1] += exp_of((double(z) - double(top)) * inverse);
+    else
+      sums[0] += weigh(z);
+  }
+  const double rest = group.join(sums[0], Add{}), held_sum = group.join(sums[1], Add{});
+  const double gap = (double(base) - double(top)) * inverse;
+  const double log_total = log_of(held_sum + (rest > 0 ? rest * exp_of(gap) : 0.0));
+#pragma unroll
+  for (int i = 0; i < Mine<G>::N; ++i) {
+    if (!list.in[i] || list.rank[i] >= a.k) continue;
+    const float z = value_at(list.item[i].key);
+    log_probs[list.rank[i]] = float((double(z) - double(top)) * inverse - log_total);
+    indices[list.rank[i]] = index_at(list.item[i].key);
+  }
+  for (int i = held + lane; i < a.k; i += G) log_probs[i] = -INFINITY, indices[i] = -1;
+  if (lane == 0) a.log_rest[r] = rest > 0 ? float(gap + log_of(rest) - log_total) : -INFINITY;
 }
 
 // ---- kernels -------------------------------------------------------------------------------------------------------
 
-template <typename T, int G, typename Row, bool RECORD>
+// BYTES: of LDS for a row; 0: it is read again for each pass.
+template <typename T, int G, int BYTES, bool RECORD>
 __global__ __launch_bounds__((G > 256 ? G : 256)) void choose_kernel(const ChooseArgs a) {
   constexpr int ROWS = G > 256 ? 1 : 256 / G;
   __shared__ Shared<G> shared[ROWS];
-  __shared__ Top list[RECORD ? ROWS : 1][RECORD ? MAX_TOP : 1];
-  __shared__ int count[ROWS];
   const int in_block = G < 256 ? __builtin_amdgcn_readfirstlane(threadIdx.x / G) : 0;
   const int64_t r = int64_t(blockIdx.x) * ROWS + in_block;
   if (r >= a.rows) return;  // (whole groups; a group's barriers are its own wave's, or its own block's)
   Group<G> group(shared[in_block]);
-  Row row(static_cast<const T *>(a.logits) + r * a.ld_logits, a.mask ? a.mask + r * a.ld_mask : nullptr, a.width);
-  if constexpr (RECORD)
-    top_row(a, r, row, group, list[in_block], &count[in_block]);
-  else
-    sample_row(a, r, row, group);
+  const T *logits = static_cast<const T *>(a.logits) + r * a.ld_logits;
+  const uint8_t *legal = a.mask ? a.mask + r * a.ld_mask : nullptr;
+  const auto run = [&](auto row) {
+    if constexpr (RECORD)
+      top_row(a, r, row, group);
+    else
+      sample_row(a, r, row, group);
+  };
+  if constexpr (BYTES > 0) {
+    using Row = InLds<T, G, BYTES>;
+    __shared__ typename Row::Vector held[ROWS][Row::VECTORS];
+    run(Row(held[in_block], logits, legal, a.width));
+  } else {
+    run(Read<T, G>(logits, legal, a.width));
+  }
 }
 
 struct Launch {
@@ -431,26 +833,19 @@ struct Launch {
   int rows, threads;  // rows a block takes
 };
 
-template <typename T, int G, int E, bool RECORD, typename S = T>
+template <typename T, int G, int BYTES, bool RECORD>
 Launch launch_as() {
-  return {choose_kernel<T, G, Held<T, G, E, S>, RECORD>, G > 256 ? 1 : 256 / G, G > 256 ? G : 256};
+  return {choose_kernel<T, G, BYTES, RECORD>, G > 256 ? 1 : 256 / G, G > 256 ? G : 256};
 }
 
 template <typename T, bool RECORD>
 Launch launch_of(int width) {
-  if (width < VEC<T>) return launch_as<T, 64, 1, RECORD, float>();
-  if (width <= 512) return launch_as<T, 64, 8, RECORD>();
-  if (width <= 1024) return launch_as<T, 64, 16, RECORD>();
-  if (width <= 4096) return launch_as<T, 256, 16, RECORD>();
-  if (width <= 8192) return launch_as<T, 256, 32, RECORD>();
-  if (width <= 16384) return launch_as<T, 512, 32, RECORD>();
-  if constexpr (sizeof(T) == 2) {
-    if (width <= 32768) return launch_as<T, 512, 64, RECORD>();
-    if (width <= 65536) return launch_as<T, 1024, 64, RECORD>();
-  } else if (width <= 32768) {
-    return launch_as<T, 1024, 32, RECORD>();
-  }
-  return {choose_kernel<T, 1024, Read<T, 1024>, RECORD>, 1, 1024};
+  const int bytes = width * int(sizeof(T));
+  if (bytes <= 2048) return launch_as<T, 64, 2048, RECORD>();
+  if (bytes <= 16384) return launch_as<T, 256, 16384, RECORD>();
+  if (bytes <= 65536) return launch_as<T, 512, 65536, RECORD>();
+  if (bytes <= 147456) return launch_as<T, 1024, 147456, RECORD>();
+  return launch_as<T, 1024, 0, RECORD>();
 }
 
 template <bool RECORD>
