@@ -206,15 +206,16 @@ struct InLds {
   __device__ __forceinline__ int at(int j) const { return max(min(j * V, width - V), 0); }
   template <typename Visit>
   __device__ __forceinline__ void each(const Visit &visit) const {
-#pragma unroll 2
+#pragma unroll 1
     for (int j = threadIdx.x % G; j < vectors; j += G) {
       Entries<T, V> q;
       __builtin_memcpy(q.w, &held[j], 16);
       visit(at(j), [&](int k) { return q[k]; });
     }
   }
-  // A row whose largest entry is +inf: these share everything.
-  __device__ __forceinline__ void unbounded() {
+  // Every entry becomes what to(z, index) says: 0 or -inf in place of it, or (NaN) itself.
+  template <typename To>
+  __device__ __forceinline__ void change(const To &to) {
     for (int j = threadIdx.x % G; j < vectors; j += G) {
       Entries<T, V> q;
       __builtin_memcpy(q.w, &held[j], 16);
@@ -222,10 +223,19 @@ struct InLds {
       for (int k = 0; k < V; ++k) {
         const uint32_t part = sizeof(T) == 4 ? ~0u : k % 2 ? 0xffff0000u : 0xffffu;
         uint32_t &w = q.w[k / Entries<T, V>::PER];
-        w = (w & ~part) | (q[k] == INFINITY ? 0u : NEGATIVE_INFINITY<T> & part);
+        const float x = to(q[k], at(j) + k);
+        if (x == x) w = (w & ~part) | (x == 0 ? 0u : NEGATIVE_INFINITY<T> & part);
       }
       __builtin_memcpy(&held[j], q.w, 16);
     }
+  }
+  // A row whose largest entry is +inf: these share everything.
+  __device__ __forceinline__ void unbounded() {
+    change([](float z, int) { return z == INFINITY ? 0.f : -INFINITY; });
+  }
+  // Drops what comes after the entry of value v and index i.
+  __device__ __forceinline__ void cut(float v, int i) {
+    change([&](float z, int k) { return z > v || (z == v && k <= i) ? NAN : -INFINITY; });
   }
 };
 
@@ -236,6 +246,8 @@ struct Read {
   const uint8_t *legal;
   int width;
   bool infinite = false;
+  float end = -INFINITY;  // cut()'s, for any entry before
+  int index = 1 << 30;
   __device__ __forceinline__ Read(const T *row, const uint8_t *legal, int width) : row(row), legal(legal), width(width) {}
   template <typename Visit>
   __device__ __forceinline__ void each(const Visit &visit) const {
@@ -246,12 +258,17 @@ struct Read {
       for (int c = 0; c < BATCH; ++c) load_entries<1, 1, V>(q[c].w, row, legal, min(first + c * G, vectors - 1) * V, width);
 #pragma unroll
       for (int c = 0; c < BATCH; ++c)
-        if (first + c * G < vectors)
-          visit(min((first + c * G) * V, width - V),
-                [&](int k) { return infinite ? (q[c][k] == INFINITY ? 0.f : -INFINITY) : q[c][k]; });
+        if (first + c * G < vectors) {
+          const int at = min((first + c * G) * V, width - V);
+          visit(at, [&](int k) {
+            const float z = infinite ? (q[c][k] == INFINITY ? 0.f : -INFINITY) : q[c][k];
+            return z > end || (z == end && at + k <= index) || z != z ? z : -INFINITY;
+          });
+        }
     }
   }
   __device__ __forceinline__ void unbounded() { infinite = true; }
+  __device__ __forceinline__ void cut(float v, int i) { end = v, index = i; }
 };
 
 // ---- order, weights --------------------------------------------------------------------------------------------
@@ -319,14 +336,14 @@ __device__ __forceinline__ float row_top(Row &row, Group<G> &group, float &mine)
   return top;
 }
 
-// The least and the largest of the entries for which in(z, index) holds, inf and -inf where none does.
+// The least and the largest of the entries for which in(z) holds, inf and -inf where none does.
 template <typename Row, int G, typename In>
 __device__ __forceinline__ void range_of(const Row &row, Group<G> &group, const In &in, float &least, float &most) {
   least = INFINITY, most = -INFINITY;
-  row.each([&](int at, const auto &z) {
+  row.each([&](int, const auto &z) {
 #pragma unroll
     for (int k = 0; k < Row::V; ++k) {
-      const bool is = in(z(k), at + k);
+      const bool is = in(z(k));
       least = fminf(least, is ? z(k) : INFINITY);
       most = fmaxf(most, is ? z(k) : -INFINITY);
     }
@@ -406,30 +423,26 @@ __device__ __forceinline__ float bound_of_top(Group<G> &group, float top, float 
   return lo;
 }
 
-// The entries for which in(z, index) holds, with weight(z), into the list.  Returns how many there are, of which
-// those past the list's room are not in it.
-template <typename Row, int G, typename In, typename Weight>
-__device__ __forceinline__ int gather(const Row &row, Group<G> &group, const In &in, const Weight &weight) {
+// The entries for which in(z, index) holds into the list.  Returns how many there are, of which those past the list's
+// room are not in it.
+template <typename Row, int G, typename In>
+__device__ __forceinline__ int gather(const Row &row, Group<G> &group, const In &in) {
   Shared<G> &s = group.shared;
   if (group.lane() == 0) s.count = 0;
   group.sync();
   row.each([&](int at, const auto &z) {
-    bool any = false;
-#pragma unroll
-    for (int k = 0; k < Row::V; ++k) any |= in(z(k), at + k);
-    if (!any) return;
 #pragma unroll
     for (int k = 0; k < Row::V; ++k) {
       if (!in(z(k), at + k)) continue;
       const int slot = atomicAdd(&s.count, 1);
-      if (slot < Shared<G>::LIST) s.list[slot] = Item{place_of(z(k), at + k), weight(z(k))};
+      if (slot < Shared<G>::LIST) s.list[slot].key = place_of(z(k), at + k);
     }
   });
   group.sync();
   return s.count;
 }
 
-// This lane's items of a list, with what stands before each.
+// This lane's items of a list, their weights (weight(z)), and what stands before each.
 template <int G>
 struct Mine {
   static constexpr int N = Shared<G>::LIST / G > 0 ? Shared<G>::LIST / G : 1;
@@ -437,15 +450,22 @@ struct Mine {
   uint64_t before[N];
   int rank[N];
   bool in[N];
-  __device__ __forceinline__ Mine(const Shared<G> &s, int n) {
+  template <typename Weight>
+  __device__ __forceinline__ Mine(Group<G> &group, int n, const Weight &weight) {
+    Shared<G> &s = group.shared;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int at = Group<G>::lane() + i * G;
+      const int at = group.lane() + i * G;
       in[i] = at < n;
-      item[i] = in[i] ? s.list[at] : Item{0, 0};
+      item[i] = Item{0, 0};
       before[i] = 0;
       rank[i] = 0;
+      if (in[i]) {
+        item[i].key = s.list[at].key;
+        s.list[at].weight = item[i].weight = weight(value_at(item[i].key));
+      }
     }
+    group.sync();
     if (int(threadIdx.x % G) / 64 * 64 >= n) return;  // (waves without items)
     for (int j = 0; j < n; ++j) {
       const Item other = s.list[j];
@@ -475,6 +495,15 @@ struct Bins {
     const float x = at(z);
     return x >= float(b) && x < float(b + 1);
   }
+  // A little more than the range of a bin's values: the roundings of at() and of these lines are 5 of 2^-24 together.
+  __device__ __forceinline__ void range(int b, float &low, float &high) const {
+    low = -0x1.fffffep127f, high = INFINITY;
+    if (scale == 0) return;
+    const float near = float(b) / scale, far = float(b + 1) / scale;
+    const float slack = 8 * 0x1p-24f * (fabsf(from) + far);
+    high = from - near + slack;
+    if (float(b) < last) low = from - far - slack;
+  }
 };
 
 struct Entry {
@@ -482,31 +511,27 @@ struct Entry {
   uint64_t upto;   // the running sum with it
 };
 
-// The histogram of weight(z) over the entries for which in(z, index) holds and whose weight is at least `bound` (1 or more).
+// The histogram of weight(z) over the entries whose weight is at least `bound` (1 or more).
 template <typename Row, int G>
 struct Histogram {
   static constexpr int PER = Shared<G>::BINS / G;
   Bins bins;
+  uint64_t bound;
   uint64_t value[PER], before, total;  // of this lane's bins
-  uint64_t less;                       // this lane's weights below `bound`
 
-  template <typename Weight, typename In>
+  template <typename Weight>
   __device__ __forceinline__ Histogram(const Row &row, Group<G> &group, const Weight &weight, float from, float low,
-                                       uint64_t bound, const In &in)
-      : bins(from, low, Shared<G>::BINS), less(0) {
+                                       uint64_t bound)
+      : bins(from, low, Shared<G>::BINS), bound(bound) {
     Shared<G> &s = group.shared;
     const int lane = group.lane();
     for (int b = lane; b < Shared<G>::BINS; b += G) s.bins[b] = 0;
     group.sync();
-    row.each([&](int at, const auto &z) {
+    row.each([&](int, const auto &z) {
 #pragma unroll
       for (int k = 0; k < Row::V; ++k) {
-        if (!in(z(k), at + k)) continue;
         const uint64_t w = weight(z(k));
-        if (w >= bound)
-          atomicAdd(reinterpret_cast<unsigned long long *>(&s.bins[int(bins.at(z(k)))]), w);
-        else
-          less += w;
+        if (w >= bound) atomicAdd(reinterpret_cast<unsigned long long *>(&s.bins[int(bins.at(z(k)))]), w);
       }
     });
     group.sync();
@@ -535,22 +560,25 @@ struct Histogram {
     return int(s.found[0]);
   }
   // The entry at which the running sum reaches `sum`.
-  template <typename Weight, typename In>
-  __device__ __forceinline__ Entry entry(const Row &row, Group<G> &group, const Weight &weight, uint64_t sum,
-                                         const In &in) const;
+  template <typename Weight>
+  __device__ __forceinline__ Entry entry(const Row &row, Group<G> &group, const Weight &weight, uint64_t sum) const;
 };
 
 template <typename Row, int G>
-template <typename Weight, typename In>
+template <typename Weight>
 __device__ __forceinline__ Entry Histogram<Row, G>::entry(const Row &row, Group<G> &group, const Weight &weight,
-                                                          uint64_t sum, const In &in) const {
+                                                          uint64_t sum) const {
   Shared<G> &s = group.shared;
   uint64_t ahead;
   const int bin = locate(group, sum, ahead);
-  const auto here = [&](float z, int i) { return bins.in(bin, z) && in(z, i); };
-  const int n = gather(row, group, here, weight);
+  float low, high;
+  bins.range(bin, low, high);
+  const int n = gather(row, group, [&](float z, int) { return z >= low && z <= high; });
   if (n <= Shared<G>::LIST) {
-    const Mine<G> mine(s, n);
+    const Mine<G> mine(group, n, [&](float z) {  // (entries that are not counted here weigh nothing)
+      const uint64_t w = weight(z);
+      return bins.in(bin, z) && w >= bound ? w : 0;
+    });
 #pragma unroll
     for (int i = 0; i < Mine<G>::N; ++i) {
       const uint64_t b = ahead + mine.before[i];
@@ -565,6 +593,7 @@ __device__ __forceinline__ Entry Histogram<Row, G>::entry(const Row &row, Group<
     return e;
   }
   // Too many for the list: the least value above which less than `sum` is, by halving the range of the bin's values.
+  const auto here = [&](float z) { return z >= low && z <= high && bins.in(bin, z) && weight(z) >= bound; };
   float least, most;
   range_of(row, group, here, least, most);
   uint32_t lo = key_of(least), hi = key_of(most);
@@ -573,10 +602,10 @@ __device__ __forceinline__ Entry Histogram<Row, G>::entry(const Row &row, Group<
     const uint32_t mid = lo + (hi - lo) / 2;
     const float v = of_key(mid);
     uint64_t x = 0;
-    row.each([&](int at, const auto &z) {
+    row.each([&](int, const auto &z) {
 #pragma unroll
       for (int k = 0; k < Row::V; ++k)
-        if (z(k) > v && here(z(k), at + k)) x += weight(z(k));
+        if (z(k) > v && here(z(k))) x += weight(z(k));
     });
     x = ahead + group.join(x, Plus{});
     if (x < sum)
@@ -590,9 +619,24 @@ __device__ __forceinline__ Entry Histogram<Row, G>::entry(const Row &row, Group<
   return Entry{place_of(v, tie(row, group, v, int(r))), above + (r + 1) * w};
 }
 
+// Counts legal entries.
 struct One {
-  __device__ __forceinline__ uint64_t operator()(float) const { return 1; }
+  __device__ __forceinline__ uint64_t operator()(float z) const { return z > -INFINITY; }
 };
+
+// Where a histogram may end: as far below the least of the lanes' maxima as the row's largest is above it.  A lane's maximum
+// is the largest of what it has, so little is below; what is goes into the last bin.
+template <int G>
+__device__ __forceinline__ float low_end(Group<G> &group, float top, float mine) {
+  const float least = group.join(mine == -INFINITY ? INFINITY : mine, Least{});
+  return least - (top - least);
+}
+
+// The next number below z (below 0, not -0, which equals it).
+__device__ __forceinline__ float below(float z) {
+  const uint32_t k = key_of(z);
+  return z == -INFINITY ? z : of_key(k == 0x80000000u ? k - 2 : k - 1);
+}
 
 // ---- sampling ----------------------------------------------------------------------------------------------------
 
@@ -646,9 +690,10 @@ __device__ __forceinline__ void sample_row(const ChooseArgs &a, int64_t r, Row &
   const bool limited = most > 0 && most < a.width;
   if (limited ? most <= SHORT<G> : a.width <= 64) {
     const float from = limited ? bound_of_top(group, top, mine, int(most)) : -INFINITY;
-    const int n = gather(row, group, [&](float z, int) { return z >= from && z > -INFINITY; }, weight);
+    const float under = below(from);
+    const int n = gather(row, group, [&](float z, int) { return z > under; });
     if (n <= Shared<G>::LIST) {
-      const Mine<G> list(s, n);
+      const Mine<G> list(group, n, weight);
       const int last = limited && most < n ? int(most) - 1 : n - 1;
       const auto each = [&](const auto &visit) {
 #pragma unroll
@@ -682,30 +727,36 @@ __device__ __forceinline__ void sample_row(const ChooseArgs &a, int64_t r, Row &
       return;
     }
   }
-  const auto legal = [](float z, int) { return z > -INFINITY; };
-  float low, high;
-  range_of(row, group, legal, low, high);
-  float from = -INFINITY;  // the last of the first k, and its index
-  int index = -1;
+  const float low = low_end(group, top, mine);
   if (limited) {
     const One one;
-    const Histogram<Row, G> h(row, group, one, top, low, 1, legal);
+    const Histogram<Row, G> h(row, group, one, top, low, 1);
     if (uint64_t(most) < h.total) {
-      const uint64_t place = h.entry(row, group, one, uint64_t(most), legal).place;
-      from = value_at(place), index = index_at(place);
+      const uint64_t place = h.entry(row, group, one, uint64_t(most)).place;
+      row.cut(value_at(place), index_at(place));
     }
   }
   // (weights end scale + 1 octaves down; in float32, and a little further)
   const float end = float(double(top) - (a.scale + 2) / weight.c);
-  const auto in = [&](float z, int i) { return z > from || (z == from && i <= index); };
-  const Histogram<Row, G> h(row, group, weight, top, fmaxf(fmaxf(low, from), end), bound, in);
+  const Histogram<Row, G> h(row, group, weight, top, fmaxf(low, end), p < 1 ? 1 : bound);
   uint64_t kept = h.total;
   if (p < 1) {
-    const uint64_t limit = limit_of(bound > 1 ? kept + group.join(h.less, Plus{}) : kept);
-    if (limit < kept) kept = h.entry(row, group, weight, limit, in).upto;
+    const uint64_t limit = limit_of(kept);
+    if (limit < kept) kept = h.entry(row, group, weight, limit).upto;
+    if (bound > 1) {
+      uint64_t x = 0;
+      row.each([&](int, const auto &z) {
+#pragma unroll
+        for (int k = 0; k < Row::V; ++k) {
+          const uint64_t w = weight(z(k));
+          x += w >= bound ? w : 0;
+        }
+      });
+      kept = min(kept, group.join(x, Plus{}));
+    }
   }
   if (least > 1) kept = one;
-  const uint64_t place = h.entry(row, group, weight, target(kept), in).place;
+  const uint64_t place = h.entry(row, group, weight, target(kept)).place;
   if (group.lane() == 0) answer(index_at(place), log_share(place, kept));
 }
 
@@ -725,33 +776,33 @@ __device__ __forceinline__ void top_row(const ChooseArgs &a, int64_t r, Row &row
     if (lane == 0) a.log_rest[r] = top;
     return;
   }
-  // The list: entries above `from`, and those equal to it up to `index`.
+  // The list: entries above `under`, or (too many) those up to the k-th, at `under` up to `index`.
   const One one;
-  float from = -INFINITY;
+  float under = -INFINITY;
   int index = -1, n = Shared<G>::LIST + 1;
-  const auto in = [&](float z, int i) { return z > from || (z == from && i <= index); };
-  if (a.k >= a.width) {
-    n = gather(row, group, in, one);
-  } else if (a.k <= SHORT<G>) {
-    from = bound_of_top(group, top, mine, a.k);
-    index = from > -INFINITY ? a.width : -1;
-    n = gather(row, group, in, one);
+  if (a.k >= a.width || a.k <= SHORT<G>) {
+    if (a.k < a.width) under = below(bound_of_top(group, top, mine, a.k));
+    n = gather(row, group, [&](float z, int) { return z > under; });
   }
+  int ties = 0;  // of the others, those equal to the k-th
   if (n > Shared<G>::LIST) {
-    const auto legal = [](float z, int) { return z > -INFINITY; };
-    float low, high;
-    range_of(row, group, legal, low, high);
-    from = -INFINITY, index = -1;
-    const Histogram<Row, G> h(row, group, one, top, low, 1, legal);
+    const Histogram<Row, G> h(row, group, one, top, low_end(group, top, mine), 1);
+    under = -INFINITY;
     if (uint64_t(a.k) < h.total) {
-      const uint64_t place = h.entry(row, group, one, uint64_t(a.k), legal).place;
-      from = value_at(place), index = index_at(place);
+      const uint64_t place = h.entry(row, group, one, uint64_t(a.k)).place;
+      under = value_at(place), index = index_at(place);
+      row.each([&](int at, const auto &z) {
+#pragma unroll
+        for (int k = 0; k < Row::V; ++k) ties += z(k) == under && at + k > index;
+      });
+      ties = group.join(ties, Plus{});
     }
-    n = gather(row, group, in, one);
+    n = gather(row, group, [&](float z, int i) { return z > under || (z == under && i <= index); });
+    if (index >= 0) under = below(under);
   }
-  const Mine<G> list(s, n);
+  const Mine<G> list(group, n, one);
   const int held = min(n, a.k);
-  // The others: those behind in the list, and those not in it; `next` is their largest.
+  // The others: those behind in the list, those not in it, and ties; `next` is their largest.
   float next;
   if (n > a.k) {
 #pragma unroll
@@ -759,9 +810,11 @@ __device__ __forceinline__ void top_row(const ChooseArgs &a, int64_t r, Row &row
       if (list.in[i] && list.rank[i] == a.k) s.found[0] = list.item[i].key;
     group.sync();
     next = value_at(s.found[0]);
+  } else if (ties > 0) {
+    next = of_key(key_of(under) + 1);
   } else {
     float least;
-    range_of(row, group, [&](float z, int i) { return !in(z, i); }, least, next);
+    range_of(row, group, [&](float z) { return z <= under; }, least, next);
   }
   const float base = next > -INFINITY ? next : 0.f;
   const double c = 1.44269504088896340736 * inverse;
@@ -771,12 +824,13 @@ __device__ __forceinline__ void top_row(const ChooseArgs &a, int64_t r, Row &row
     return __builtin_amdgcn_exp2f(fmaf(d, fast, d * slow));
   };
   double sums[2] = {0, 0};  // of the others, and of the record
-  row.each([&](int at, const auto &z) {
+  row.each([&](int, const auto &z) {
     float sum = 0;
 #pragma unroll
-    for (int k = 0; k < Row::V; ++k) sum += in(z(k), at + k) || z(k) == -INFINITY ? 0.f : weigh(z(k));
+    for (int k = 0; k < Row::V; ++k) sum += z(k) <= under ? weigh(z(k)) : 0.f;
     sums[0] += sum;
   });
+  if (lane == 0) sums[0] += ties;  // (the largest of the others, where there are any)
 #pragma unroll
   for (int i = 0; i < Mine<G>::N; ++i) {
     if (!list.in[i]) continue;
