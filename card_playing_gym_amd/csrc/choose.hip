@@ -167,6 +167,23 @@ struct Group {
 // each(visit): visit(index of entry 0, z) for this lane's vectors, z(k) the k-th logit, -inf where it is not legal.  A
 // lane reads what it has written: no barrier stands between.
 
+// The vector from entry i on, -inf for those that are not legal; a row's last one is its last V entries, of which those
+// that the one before has count as -inf.
+template <typename T, int V = VEC<T>>
+__device__ __forceinline__ void load_vector(uint32_t (&w)[4], const T *row, const uint8_t *legal, int i, int width) {
+  if (i + V <= width) {
+    __builtin_memcpy(w, row + i, 16);
+    if (legal) {
+      uint32_t b[V / 4];
+      __builtin_memcpy(b, legal + i, V);
+#pragma unroll
+      for (int j = 0; j < V / 4; ++j) bar<T>(w + (sizeof(T) == 4 ? 4 : 2) * j, b[j]);
+    }
+  } else {
+    load_entries<1, 1, V>(w, row, legal, i, width);
+  }
+}
+
 template <typename T, int G, int BYTES>
 struct InLds {
   static constexpr int V = VEC<T>, VECTORS = BYTES / 16, BATCH = VECTORS / G < 8 ? VECTORS / G : 8;
@@ -197,7 +214,7 @@ struct InLds {
     for (int first = lane; first < vectors; first += G * BATCH) {
       uint32_t w[BATCH][4];
 #pragma unroll
-      for (int c = 0; c < BATCH; ++c) load_entries<1, 1, V>(w[c], row, legal, min(first + c * G, vectors - 1) * V, width);
+      for (int c = 0; c < BATCH; ++c) load_vector(w[c], row, legal, min(first + c * G, vectors - 1) * V, width);
 #pragma unroll
       for (int c = 0; c < BATCH; ++c)
         if (first + c * G < vectors) __builtin_memcpy(&held[first + c * G], w[c], 16);
@@ -213,9 +230,8 @@ struct InLds {
       visit(at(j), [&](int k) { return q[k]; });
     }
   }
-  // Every entry becomes what to(z, index) says: 0 or -inf in place of it, or (NaN) itself.
-  template <typename To>
-  __device__ __forceinline__ void change(const To &to) {
+  // A row whose largest entry is +inf: these share everything.
+  __device__ __forceinline__ void unbounded() {
     for (int j = threadIdx.x % G; j < vectors; j += G) {
       Entries<T, V> q;
       __builtin_memcpy(q.w, &held[j], 16);
@@ -223,19 +239,10 @@ struct InLds {
       for (int k = 0; k < V; ++k) {
         const uint32_t part = sizeof(T) == 4 ? ~0u : k % 2 ? 0xffff0000u : 0xffffu;
         uint32_t &w = q.w[k / Entries<T, V>::PER];
-        const float x = to(q[k], at(j) + k);
-        if (x == x) w = (w & ~part) | (x == 0 ? 0u : NEGATIVE_INFINITY<T> & part);
+        w = (w & ~part) | (q[k] == INFINITY ? 0u : NEGATIVE_INFINITY<T> & part);
       }
       __builtin_memcpy(&held[j], q.w, 16);
     }
-  }
-  // A row whose largest entry is +inf: these share everything.
-  __device__ __forceinline__ void unbounded() {
-    change([](float z, int) { return z == INFINITY ? 0.f : -INFINITY; });
-  }
-  // Drops what comes after the entry of value v and index i.
-  __device__ __forceinline__ void cut(float v, int i) {
-    change([&](float z, int k) { return z > v || (z == v && k <= i) ? NAN : -INFINITY; });
   }
 };
 
@@ -246,8 +253,6 @@ struct Read {
   const uint8_t *legal;
   int width;
   bool infinite = false;
-  float end = -INFINITY;  // cut()'s, for any entry before
-  int index = 1 << 30;
   __device__ __forceinline__ Read(const T *row, const uint8_t *legal, int width) : row(row), legal(legal), width(width) {}
   template <typename Visit>
   __device__ __forceinline__ void each(const Visit &visit) const {
@@ -255,20 +260,16 @@ struct Read {
     for (int first = threadIdx.x % G; first < vectors; first += G * BATCH) {
       Entries<T, V> q[BATCH];
 #pragma unroll
-      for (int c = 0; c < BATCH; ++c) load_entries<1, 1, V>(q[c].w, row, legal, min(first + c * G, vectors - 1) * V, width);
+      for (int c = 0; c < BATCH; ++c) load_vector(q[c].w, row, legal, min(first + c * G, vectors - 1) * V, width);
 #pragma unroll
       for (int c = 0; c < BATCH; ++c)
         if (first + c * G < vectors) {
           const int at = min((first + c * G) * V, width - V);
-          visit(at, [&](int k) {
-            const float z = infinite ? (q[c][k] == INFINITY ? 0.f : -INFINITY) : q[c][k];
-            return z > end || (z == end && at + k <= index) || z != z ? z : -INFINITY;
-          });
+          visit(at, [&](int k) { return infinite ? (q[c][k] == INFINITY ? 0.f : -INFINITY) : q[c][k]; });
         }
     }
   }
   __device__ __forceinline__ void unbounded() { infinite = true; }
-  __device__ __forceinline__ void cut(float v, int i) { end = v, index = i; }
 };
 
 // ---- order, weights --------------------------------------------------------------------------------------------
@@ -280,30 +281,53 @@ __device__ __forceinline__ uint32_t key_of(float z) {
 }
 __device__ __forceinline__ float of_key(uint32_t k) { return __uint_as_float(k >> 31 ? k & 0x7fffffffu : ~k); }
 
+// A constant in scalar registers: from vector registers the compiler copies it for each use.
+__device__ __forceinline__ double scalar_of(double c) {
+  int lo = __double2loint(c), hi = __double2hiint(c);
+  asm("" : "+s"(lo), "+s"(hi));
+  return __hiloint2double(hi, lo);
+}
+
 // Integer weights: 2^scale e^((z - top) / T).
 struct Weights {
   double top, c;  // c = log2(e) / T, finite: the top weighs 1
   double magic;   // 1.5 * 2^(52 - scale): a sum with it has the weight in its low bits, to the nearest
-  __device__ __forceinline__ Weights(float top, double temperature, int scale)
-      : top(top), c(fmin(1.44269504088896340736 / temperature, 1e300)), magic(__builtin_amdgcn_ldexp(1.5, 52 - scale)) {}
+  double g[9];
   // 2^t = 2^k 2^f, |f| <= 1/2: 2^f = 1 + f g(f), g interpolated at the nodes of Chebyshev's polynomial of degree 9;
   // off by 2^-44.6 of it at most, and 1 at 0.
-  __device__ __forceinline__ uint64_t operator()(float z) const {
-    const double t = fmax((double(z) - top) * c, -64.0);  // (a NaN of -inf and c = 0 too: a weight of 0 from -63 on)
+  __device__ __forceinline__ Weights(float top, double temperature, int scale)
+      : top(top), c(fmin(1.44269504088896340736 / temperature, 1e300)), magic(__builtin_amdgcn_ldexp(1.5, 52 - scale)),
+        g{scalar_of(0.6931471805599454), scalar_of(0.24022650695813), scalar_of(0.055504108664767154),
+          scalar_of(0.009618129159415947), scalar_of(0.0013333558177508053), scalar_of(0.00015403455837972657),
+          scalar_of(1.5252687853419455e-05), scalar_of(1.3255228630225242e-06), 1.0202923985536321e-07} {
+    asm("" : "+v"(g[8]));  // (one operand of an instruction may be scalar)
+  }
+  // Of any z; 0 below 2^-64.
+  __device__ __forceinline__ uint64_t operator()(float z) const { return z >= least() ? near(z) : 0; }
+  // Of z >= least().
+  __device__ __forceinline__ uint64_t near(float z) const {
+    const double d = double(z) - top;
     // (adding 1.5 * 2^52 rounds to whole numbers, k's low bits the sum's)
-    const double whole = t + 6755399441055744.0, f = t - (whole - 6755399441055744.0);
-    double p = 1.0202923985536321e-07;
-    p = fma(p, f, 1.3255228630225242e-06);
-    p = fma(p, f, 1.5252687853419455e-05);
-    p = fma(p, f, 0.00015403455837972657);
-    p = fma(p, f, 0.0013333558177508053);
-    p = fma(p, f, 0.009618129159415947);
-    p = fma(p, f, 0.055504108664767154);
-    p = fma(p, f, 0.24022650695813);
-    p = fma(p, f, 0.6931471805599454);
+    const double whole = fma(d, c, 6755399441055744.0), f = fma(d, c, 6755399441055744.0 - whole);
+    double p = fma(g[8], f, g[7]);
+    p = fma(p, f, g[6]);
+    p = fma(p, f, g[5]);
+    p = fma(p, f, g[4]);
+    p = fma(p, f, g[3]);
+    p = fma(p, f, g[2]);
+    p = fma(p, f, g[1]);
+    p = fma(p, f, g[0]);
     p = fma(p, f, 1.0);
     const double sum = __hiloint2double(__double2hiint(p) + (__double2loint(whole) << 20), __double2loint(p)) + magic;
-    return __builtin_bit_cast(uint64_t, sum) - __builtin_bit_cast(uint64_t, magic);
+    int high = __double2hiint(sum) - __double2hiint(magic);  // (magic's low word is 0)
+    asm("" : "+v"(high));  // (or the compiler makes a subtraction of both words of it)
+    return uint64_t(uint32_t(high)) << 32 | uint32_t(__double2loint(sum));
+  }
+  // All that weigh anything are as large (2^scale e^d is below 1/2 from t = -52 on), and t >= -64.
+  __device__ __forceinline__ float least() const {
+    const double z = top - 60.0 / c;
+    float x = z > -0x1.fffffep127 ? float(z) : -0x1.fffffep127f;
+    return (double(x) - top) * c < -64.0 ? of_key(key_of(x) + 1) : x;  // (one step, where z was rounded down)
   }
 };
 
@@ -316,17 +340,13 @@ __device__ __forceinline__ int index_at(uint64_t place) { return int(~uint32_t(p
 template <typename Row, int G>
 __device__ __forceinline__ float row_top(Row &row, Group<G> &group, float &mine) {
   const auto pass = [&] {
+    const auto larger = [](float a, float b) { return __builtin_elementwise_maximum(a, b); };  // (NaN where one is)
     mine = -INFINITY;
-    bool nan = false;
     row.each([&](int, const auto &z) {
 #pragma unroll
-      for (int k = 0; k < Row::V; ++k) {
-        mine = fmaxf(mine, z(k));
-        nan |= z(k) != z(k);
-      }
+      for (int k = 0; k < Row::V; ++k) mine = larger(mine, z(k));
     });
-    // (the larger of two, NaN where one is)
-    return group.join(nan ? NAN : mine, [](float a, float b) { return a > b || a != a ? a : b; });
+    return group.join(mine, larger);
   };
   float top = pass();
   if (top == INFINITY) {
@@ -334,22 +354,6 @@ __device__ __forceinline__ float row_top(Row &row, Group<G> &group, float &mine)
     top = pass();
   }
   return top;
-}
-
-// The least and the largest of the entries for which in(z) holds, inf and -inf where none does.
-template <typename Row, int G, typename In>
-__device__ __forceinline__ void range_of(const Row &row, Group<G> &group, const In &in, float &least, float &most) {
-  least = INFINITY, most = -INFINITY;
-  row.each([&](int, const auto &z) {
-#pragma unroll
-    for (int k = 0; k < Row::V; ++k) {
-      const bool is = in(z(k));
-      least = fminf(least, is ? z(k) : INFINITY);
-      most = fmaxf(most, is ? z(k) : -INFINITY);
-    }
-  });
-  least = group.join(least, Least{});
-  most = group.join(most, Largest{});
 }
 
 // The index of entry number r (from 0) of those equal to v.
@@ -466,11 +470,19 @@ struct Mine {
       }
     }
     group.sync();
+    if (n <= G)
+      add_up<1>(s, n);
+    else
+      add_up<N>(s, n);
+  }
+  template <int USED>
+  __device__ __forceinline__ void add_up(const Shared<G> &s, int n) {
     if (int(threadIdx.x % G) / 64 * 64 >= n) return;  // (waves without items)
+#pragma unroll 4
     for (int j = 0; j < n; ++j) {
       const Item other = s.list[j];
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
+      for (int i = 0; i < USED; ++i) {
         const bool ahead = other.key > item[i].key;
         before[i] += ahead ? other.weight : 0;
         rank[i] += ahead;
@@ -481,23 +493,23 @@ struct Mine {
 
 // ---- the entry at a place of the running sum over the order ------------------------------------------------------
 
-// Bins of equal width from `from` downwards, the last one for all below.  A z further away than float32 can say is
-// in the last one; a range that it cannot divide is one bin.
+// Bins of equal width from `from` downwards, the last one for all below (and what float32 cannot tell from there).  A
+// range of one value is one bin; of any other, its ends are in different ones.
 struct Bins {
   float from, scale, last;
-  __device__ __forceinline__ Bins(float from, float low, int n) : from(from), last(float(n - 1)) {
-    const float span = from - low;
-    scale = last / span;
-    if (!(span > 0 && scale < INFINITY)) scale = 0;
+  Bins() = default;
+  __device__ __forceinline__ Bins(float from, float end, int n) : from(from), last(float(n - 1)) {
+    const float half = 0.5f * from - 0.5f * end;  // (the whole may be above float32's largest)
+    scale = half > 0 ? fminf(0.5f * last / half, 1e38f) : 0;
   }
   __device__ __forceinline__ float at(float z) const { return fminf((from - z) * scale, last); }
   __device__ __forceinline__ bool in(int b, float z) const {
     const float x = at(z);
     return x >= float(b) && x < float(b + 1);
   }
-  // A little more than the range of a bin's values: the roundings of at() and of these lines are 5 of 2^-24 together.
+  // A little more than the range of a bin's values: the roundings of at() and of these lines are 6 of 2^-24 together.
   __device__ __forceinline__ void range(int b, float &low, float &high) const {
-    low = -0x1.fffffep127f, high = INFINITY;
+    low = -INFINITY, high = INFINITY;
     if (scale == 0) return;
     const float near = float(b) / scale, far = float(b + 1) / scale;
     const float slack = 8 * 0x1p-24f * (fabsf(from) + far);
@@ -511,28 +523,28 @@ struct Entry {
   uint64_t upto;   // the running sum with it
 };
 
-// The histogram of weight(z) over the entries whose weight is at least `bound` (1 or more).
+// The histogram of weight.near(z) over the entries of `low` to `high`; WITHIN: some are above `high`.
 template <typename Row, int G>
 struct Histogram {
   static constexpr int PER = Shared<G>::BINS / G;
   Bins bins;
-  uint64_t bound;
+  float low, high;
   uint64_t value[PER], before, total;  // of this lane's bins
 
-  template <typename Weight>
-  __device__ __forceinline__ Histogram(const Row &row, Group<G> &group, const Weight &weight, float from, float low,
-                                       uint64_t bound)
-      : bins(from, low, Shared<G>::BINS), bound(bound) {
+  // The bins end at `end`, or lower.
+  template <bool WITHIN = false, typename Weight>
+  __device__ __forceinline__ void make(const Row &row, Group<G> &group, const Weight &weight, float from, float end, float least) {
+    bins = Bins(from, end, Shared<G>::BINS);
+    low = least, high = from;
     Shared<G> &s = group.shared;
     const int lane = group.lane();
     for (int b = lane; b < Shared<G>::BINS; b += G) s.bins[b] = 0;
     group.sync();
     row.each([&](int, const auto &z) {
 #pragma unroll
-      for (int k = 0; k < Row::V; ++k) {
-        const uint64_t w = weight(z(k));
-        if (w >= bound) atomicAdd(reinterpret_cast<unsigned long long *>(&s.bins[int(bins.at(z(k)))]), w);
-      }
+      for (int k = 0; k < Row::V; ++k)
+        if (z(k) >= low && !(WITHIN && z(k) > high))
+          atomicAdd(reinterpret_cast<unsigned long long *>(&s.bins[int(bins.at(z(k)))]), weight.near(z(k)));
     });
     group.sync();
     uint64_t mine = 0;
@@ -561,75 +573,67 @@ struct Histogram {
   }
   // The entry at which the running sum reaches `sum`.
   template <typename Weight>
-  __device__ __forceinline__ Entry entry(const Row &row, Group<G> &group, const Weight &weight, uint64_t sum) const;
-};
-
-template <typename Row, int G>
-template <typename Weight>
-__device__ __forceinline__ Entry Histogram<Row, G>::entry(const Row &row, Group<G> &group, const Weight &weight,
-                                                          uint64_t sum) const {
-  Shared<G> &s = group.shared;
-  uint64_t ahead;
-  const int bin = locate(group, sum, ahead);
-  float low, high;
-  bins.range(bin, low, high);
-  const int n = gather(row, group, [&](float z, int) { return z >= low && z <= high; });
-  if (n <= Shared<G>::LIST) {
-    const Mine<G> mine(group, n, [&](float z) {  // (entries that are not counted here weigh nothing)
-      const uint64_t w = weight(z);
-      return bins.in(bin, z) && w >= bound ? w : 0;
-    });
+  __device__ __forceinline__ Entry entry(const Row &row, Group<G> &group, const Weight &weight, uint64_t sum) const {
+    Shared<G> &s = group.shared;
+    Histogram h = *this;
+    for (uint64_t ahead = 0;;) {
+      uint64_t more;
+      const int bin = h.locate(group, sum - ahead, more);
+      ahead += more;
+      float least, most;
+      h.bins.range(bin, least, most);
+      least = fmaxf(least, h.low), most = fminf(most, h.high);
+      const Bins bins = h.bins;
+      const int n = gather(row, group, [&](float z, int) { return z >= least && z <= most; });
+      if (n <= Shared<G>::LIST) {
+        // (those of the bins beside it weigh nothing here)
+        const Mine<G> mine(group, n, [&](float z) { return bins.in(bin, z) ? weight.near(z) : 0; });
 #pragma unroll
-    for (int i = 0; i < Mine<G>::N; ++i) {
-      const uint64_t b = ahead + mine.before[i];
-      if (mine.in[i] && b < sum && sum <= b + mine.item[i].weight) {
-        s.found[0] = mine.item[i].key;
-        s.found[1] = b + mine.item[i].weight;
+        for (int i = 0; i < Mine<G>::N; ++i) {
+          const uint64_t b = ahead + mine.before[i];
+          if (mine.in[i] && b < sum && sum <= b + mine.item[i].weight) {
+            s.found[0] = mine.item[i].key;
+            s.found[1] = b + mine.item[i].weight;
+          }
+        }
+        group.sync();
+        const Entry e{s.found[0], s.found[1]};
+        group.sync();
+        return e;
       }
-    }
-    group.sync();
-    const Entry e{s.found[0], s.found[1]};
-    group.sync();
-    return e;
-  }
-  // Too many for the list: the least value above which less than `sum` is, by halving the range of the bin's values.
-  const auto here = [&](float z) { return z >= low && z <= high && bins.in(bin, z) && weight(z) >= bound; };
-  float least, most;
-  range_of(row, group, here, least, most);
-  uint32_t lo = key_of(least), hi = key_of(most);
-  uint64_t above = ahead;  // above hi, ahead of the bin included
-  while (lo < hi) {
-    const uint32_t mid = lo + (hi - lo) / 2;
-    const float v = of_key(mid);
-    uint64_t x = 0;
-    row.each([&](int, const auto &z) {
+      // Too many: bins within the bin, from its largest entry to its least.
+      float lowest = INFINITY, largest = -INFINITY;
+      row.each([&](int, const auto &z) {
 #pragma unroll
-      for (int k = 0; k < Row::V; ++k)
-        if (z(k) > v && here(z(k))) x += weight(z(k));
-    });
-    x = ahead + group.join(x, Plus{});
-    if (x < sum)
-      hi = mid, above = x;
-    else
-      lo = mid + 1;
+        for (int k = 0; k < Row::V; ++k) {
+          const bool is = z(k) >= least && z(k) <= most && bins.in(bin, z(k));
+          lowest = fminf(lowest, is ? z(k) : INFINITY);
+          largest = fmaxf(largest, is ? z(k) : -INFINITY);
+        }
+      });
+      lowest = group.join(lowest, Least{});
+      largest = group.join(largest, Largest{});
+      if (lowest == largest) {  // equal entries
+        const uint64_t w = weight.near(lowest), r = (sum - 1 - ahead) / w;
+        return Entry{place_of(lowest, tie(row, group, lowest, int(r))), ahead + (r + 1) * w};
+      }
+      h.template make<true>(row, group, weight, largest, lowest, lowest);
+    }
   }
-  const float v = of_key(hi);
-  const uint64_t w = weight(v);
-  const uint64_t r = (sum - 1 - above) / w;  // of those equal to v
-  return Entry{place_of(v, tie(row, group, v, int(r))), above + (r + 1) * w};
-}
-
-// Counts legal entries.
-struct One {
-  __device__ __forceinline__ uint64_t operator()(float z) const { return z > -INFINITY; }
 };
 
-// Where a histogram may end: as far below the least of the lanes' maxima as the row's largest is above it.  A lane's maximum
-// is the largest of what it has, so little is below; what is goes into the last bin.
+// Counts.
+struct One {
+  __device__ __forceinline__ uint64_t operator()(float) const { return 1; }
+  __device__ __forceinline__ uint64_t near(float) const { return 1; }
+};
+
+// Where a histogram may end: half as far again below the least of the lanes' maxima as the row's largest is above
+// it.  A lane's maximum is the largest of what it has, so little is below; what is goes into the last bin.
 template <int G>
 __device__ __forceinline__ float low_end(Group<G> &group, float top, float mine) {
   const float least = group.join(mine == -INFINITY ? INFINITY : mine, Least{});
-  return least - (top - least);
+  return fmaxf(least - 1.5f * (top - least), -0x1.fffffep127f);
 }
 
 // The next number below z (below 0, not -0, which equals it).
@@ -685,7 +689,7 @@ __device__ __forceinline__ void sample_row(const ChooseArgs &a, int64_t r, Row &
   };
   const auto log_share = [&](uint64_t place, uint64_t kept) {
     return float((double(value_at(place)) - double(top)) / temperature -
-                 (log_of(double(kept)) - a.scale * 0.69314718055994530942));
+                 log_of(__builtin_amdgcn_ldexp(double(kept), -a.scale)));  // (0 for the whole of it)
   };
   const bool limited = most > 0 && most < a.width;
   if (limited ? most <= SHORT<G> : a.width <= 64) {
@@ -727,32 +731,51 @@ __device__ __forceinline__ void sample_row(const ChooseArgs &a, int64_t r, Row &
       return;
     }
   }
-  const float low = low_end(group, top, mine);
+  const float end = low_end(group, top, mine);
+  Histogram<Row, G> h;
+  float after = INFINITY;  // the first k: entries above the k-th's value, and this many of those equal to it
+  int ties = 0;
   if (limited) {
-    const One one;
-    const Histogram<Row, G> h(row, group, one, top, low, 1);
+    h.make(row, group, One{}, top, end, -0x1.fffffep127f);
     if (uint64_t(most) < h.total) {
-      const uint64_t place = h.entry(row, group, one, uint64_t(most)).place;
-      row.cut(value_at(place), index_at(place));
+      after = value_at(h.entry(row, group, One{}, uint64_t(most)).place);
+      int above = 0;
+      row.each([&](int, const auto &z) {
+#pragma unroll
+        for (int k = 0; k < Row::V; ++k) above += z(k) > after;
+      });
+      ties = int(most) - group.join(above, Plus{});
     }
   }
-  // (weights end scale + 1 octaves down; in float32, and a little further)
-  const float end = float(double(top) - (a.scale + 2) / weight.c);
-  const Histogram<Row, G> h(row, group, weight, top, fmaxf(low, end), p < 1 ? 1 : bound);
+  const float lowest = weight.least();
+  const auto sum_above = [&](float v) {  // of the entries above v
+    uint64_t x = 0;
+    row.each([&](int, const auto &z) {
+#pragma unroll
+      for (int k = 0; k < Row::V; ++k)
+        if (z(k) > v && z(k) >= lowest) x += weight.near(z(k));
+    });
+    return group.join(x, Plus{});
+  };
+  h.make(row, group, weight, top, fmaxf(end, lowest), lowest);
   uint64_t kept = h.total;
+  if (after < INFINITY) kept = sum_above(after) + ties * weight(after);
   if (p < 1) {
     const uint64_t limit = limit_of(kept);
     if (limit < kept) kept = h.entry(row, group, weight, limit).upto;
-    if (bound > 1) {
-      uint64_t x = 0;
-      row.each([&](int, const auto &z) {
-#pragma unroll
-        for (int k = 0; k < Row::V; ++k) {
-          const uint64_t w = weight(z(k));
-          x += w >= bound ? w : 0;
-        }
-      });
-      kept = min(kept, group.join(x, Plus{}));
+  }
+  if (bound > 1) {
+    // The least value whose weight is kept, by halving.
+    uint32_t lo = key_of(lowest), hi = key_of(top);
+    if (weight(lowest) < bound) {
+      while (hi - lo > 1) {
+        const uint32_t mid = lo + (hi - lo) / 2;
+        if (weight(of_key(mid)) < bound)
+          lo = mid;
+        else
+          hi = mid;
+      }
+      kept = min(kept, sum_above(of_key(lo)));
     }
   }
   if (least > 1) kept = one;
@@ -781,12 +804,14 @@ __device__ __forceinline__ void top_row(const ChooseArgs &a, int64_t r, Row &row
   float under = -INFINITY;
   int index = -1, n = Shared<G>::LIST + 1;
   if (a.k >= a.width || a.k <= SHORT<G>) {
-    if (a.k < a.width) under = below(bound_of_top(group, top, mine, a.k));
+    // (one more, where the lanes suffice: the largest of the others)
+    if (a.k < a.width) under = below(bound_of_top(group, top, mine, min(a.k + 1, G)));
     n = gather(row, group, [&](float z, int) { return z > under; });
   }
   int ties = 0;  // of the others, those equal to the k-th
   if (n > Shared<G>::LIST) {
-    const Histogram<Row, G> h(row, group, one, top, low_end(group, top, mine), 1);
+    Histogram<Row, G> h;
+    h.make(row, group, one, top, low_end(group, top, mine), -0x1.fffffep127f);
     under = -INFINITY;
     if (uint64_t(a.k) < h.total) {
       const uint64_t place = h.entry(row, group, one, uint64_t(a.k)).place;
@@ -813,16 +838,17 @@ __device__ __forceinline__ void top_row(const ChooseArgs &a, int64_t r, Row &row
   } else if (ties > 0) {
     next = of_key(key_of(under) + 1);
   } else {
-    float least;
-    range_of(row, group, [&](float z) { return z <= under; }, least, next);
+    next = -INFINITY;
+    row.each([&](int, const auto &z) {
+#pragma unroll
+      for (int k = 0; k < Row::V; ++k) next = fmaxf(next, z(k) <= under ? z(k) : -INFINITY);
+    });
+    next = group.join(next, Most{});
   }
   const float base = next > -INFINITY ? next : 0.f;
   const double c = 1.44269504088896340736 * inverse;
-  const float fast = float(c), slow = float(c - double(fast));
-  const auto weigh = [&](float z) {
-    const float d = z - base;
-    return __builtin_amdgcn_exp2f(fmaf(d, fast, d * slow));
-  };
+  const float scale = float(c);
+  const auto weigh = [&](float z) { return __builtin_amdgcn_exp2f((z - base) * scale); };
   double sums[2] = {0, 0};  // of the others, and of the record
   row.each([&](int, const auto &z) {
     float sum = 0;

@@ -180,6 +180,23 @@ typedef uint32_t Word4 __attribute__((ext_vector_type(4), aligned(2)));  // wher
 // Four mask bytes: bit 7 of each byte set where the byte is not 0.
 __device__ __forceinline__ uint32_t nonzero_bytes(uint32_t b) { return ((b & 0x7f7f7f7fu) + 0x7f7f7f7fu) | b; }
 
+// Four entries, -inf for those whose byte of `legal` is 0.
+template <typename T>
+__device__ __forceinline__ void bar(uint32_t *w, uint32_t legal) {
+  constexpr uint32_t NONE = NEGATIVE_INFINITY<T>;
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) w[k] = legal >> 8 * k & 255 ? w[k] : NONE;
+  } else {
+    // Sign bits of bytes 0 and 1, then 2 and 3, spread over a half each (v_perm_b32's selectors 8 to 11
+    // repeat the signs of bytes 1, 3, 5 and 7).
+    const uint32_t t = nonzero_bytes(legal);
+    const uint32_t lo = __builtin_amdgcn_perm(t << 8, t, 0x08080a0au), hi = __builtin_amdgcn_perm(t << 8, t, 0x09090b0bu);
+    w[0] = (w[0] & lo) | (NONE & ~lo);
+    w[1] = (w[1] & hi) | (NONE & ~hi);
+  }
+}
+
 // A lane's entries of a row: vectors of V from entry (c G + lane) V on for c < C, -inf for those past the row's
 // end or not legal.  Rows may start anywhere: 16 bytes are loaded wherever they begin.  A vector over the
 // row's end is loaded as its last V entries, of which the first, that a vector before has, count as
@@ -209,19 +226,7 @@ __device__ __forceinline__ void load_entries(uint32_t *w, const T *row, const ui
 #pragma unroll
       for (int c = 0; c < C; ++c) __builtin_memcpy(b + c * (V / 4), legal + at(c), V);
 #pragma unroll
-      for (int j = 0; j < C * (V / 4); ++j) {
-        if constexpr (PER == 1) {
-#pragma unroll
-          for (int k = 0; k < 4; ++k) w[4 * j + k] = b[j] >> 8 * k & 255 ? w[4 * j + k] : NONE;
-        } else {
-          // Sign bits of bytes 0 and 1, then 2 and 3, spread over a half each (v_perm_b32's selectors 8 to 11
-          // repeat the signs of bytes 1, 3, 5 and 7).
-          const uint32_t t = nonzero_bytes(b[j]);
-          const uint32_t lo = __builtin_amdgcn_perm(t << 8, t, 0x08080a0au), hi = __builtin_amdgcn_perm(t << 8, t, 0x09090b0bu);
-          w[2 * j] = (w[2 * j] & lo) | (NONE & ~lo);
-          w[2 * j + 1] = (w[2 * j + 1] & hi) | (NONE & ~hi);
-        }
-      }
+      for (int j = 0; j < C * (V / 4); ++j) bar<T>(w + 4 / PER * j, b[j]);
     }
 #pragma unroll
     for (int c = 0; c < C; ++c) {

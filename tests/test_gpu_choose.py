@@ -93,6 +93,19 @@ def test_equal_entries_go_by_their_index(device, width, dtype):
         assert torch.equal(top.indices, torch.arange(5, device=device).where(torch.arange(5, device=device) < width, -1).expand(n, 5))
 
 
+@pytest.mark.parametrize("width", [5, 600, 20000, 70000])
+def test_the_whole_of_a_row_has_log_probability_zero(device, width):
+    logits = torch.randn(4, width, device=device)
+    u = torch.tensor([0.1, 0.4, 0.7, 0.9], dtype=torch.float64, device=device)
+    for controls in ({"top_k": 1}, {"top_p": 0.0}, {"min_p": 1.0}, {"temperature": 0.0}, {"temperature": 1e-6}):
+        out = sample_logits(logits, u, **controls)
+        assert torch.equal(out.actions, logits.argmax(1)) and out.log_probs.tolist() == [0, 0, 0, 0], controls
+    mask = torch.zeros(4, width, dtype=torch.bool, device=device)
+    mask[:, 3] = True
+    assert sample_logits(logits, u, mask=mask).log_probs.tolist() == [0, 0, 0, 0]
+    assert top_logits(logits, 1, mask=mask).log_probs.tolist() == [[0], [0], [0], [0]]
+
+
 def test_uniforms_at_their_ends(device):
     logits = torch.tensor([[0.0, 1.0, -float("inf"), 0.5, -1e9]], device=device).expand(6, 5)
     u = torch.tensor([0.0, 1 - 2.0**-53, 1.0, 2.0, -1.0, float("nan")], dtype=torch.float64, device=device)
