@@ -292,11 +292,13 @@ __device__ __forceinline__ double scalar_of(double c) {
 struct Weights {
   double top, c;  // c = log2(e) / T, finite: the top weighs 1
   double magic;   // 1.5 * 2^(52 - scale): a sum with it has the weight in its low bits, to the nearest
+  double reach;   // 60 octaves
   double g[9];
   // 2^t = 2^k 2^f, |f| <= 1/2: 2^f = 1 + f g(f), g interpolated at the nodes of Chebyshev's polynomial of degree 9;
   // off by 2^-44.6 of it at most, and 1 at 0.
   __device__ __forceinline__ Weights(float top, double temperature, int scale)
       : top(top), c(fmin(1.44269504088896340736 / temperature, 1e300)), magic(__builtin_amdgcn_ldexp(1.5, 52 - scale)),
+        reach(60 * 0.69314718055994530942 * temperature),
         g{scalar_of(0.6931471805599454), scalar_of(0.24022650695813), scalar_of(0.055504108664767154),
           scalar_of(0.009618129159415947), scalar_of(0.0013333558177508053), scalar_of(0.00015403455837972657),
           scalar_of(1.5252687853419455e-05), scalar_of(1.3255228630225242e-06), 1.0202923985536321e-07} {
@@ -325,7 +327,7 @@ struct Weights {
   }
   // All that weigh anything are as large (2^scale e^d is below 1/2 from t = -52 on), and t >= -64.
   __device__ __forceinline__ float least() const {
-    const double z = top - 60.0 / c;
+    const double z = top - reach;
     float x = z > -0x1.fffffep127 ? float(z) : -0x1.fffffep127f;
     return (double(x) - top) * c < -64.0 ? of_key(key_of(x) + 1) : x;  // (one step, where z was rounded down)
   }
@@ -472,6 +474,8 @@ struct Mine {
     group.sync();
     if (n <= G)
       add_up<1>(s, n);
+    else if (n <= 2 * G)
+      add_up<(N < 2 ? N : 2)>(s, n);
     else
       add_up<N>(s, n);
   }
@@ -496,23 +500,24 @@ struct Mine {
 // Bins of equal width from `from` downwards, the last one for all below (and what float32 cannot tell from there).  A
 // range of one value is one bin; of any other, its ends are in different ones.
 struct Bins {
-  float from, scale, last;
+  float from, scale, last, width;
   Bins() = default;
   __device__ __forceinline__ Bins(float from, float end, int n) : from(from), last(float(n - 1)) {
     const float half = 0.5f * from - 0.5f * end;  // (the whole may be above float32's largest)
     scale = half > 0 ? fminf(0.5f * last / half, 1e38f) : 0;
+    width = 1 / scale;
   }
   __device__ __forceinline__ float at(float z) const { return fminf((from - z) * scale, last); }
   __device__ __forceinline__ bool in(int b, float z) const {
     const float x = at(z);
     return x >= float(b) && x < float(b + 1);
   }
-  // A little more than the range of a bin's values: the roundings of at() and of these lines are 6 of 2^-24 together.
+  // A little more than the range of a bin's values: the roundings of at() and of these lines are 7 of 2^-24 together.
   __device__ __forceinline__ void range(int b, float &low, float &high) const {
     low = -INFINITY, high = INFINITY;
     if (scale == 0) return;
-    const float near = float(b) / scale, far = float(b + 1) / scale;
-    const float slack = 8 * 0x1p-24f * (fabsf(from) + far);
+    const float near = float(b) * width, far = float(b + 1) * width;
+    const float slack = 9 * 0x1p-24f * (fabsf(from) + far);
     high = from - near + slack;
     if (float(b) < last) low = from - far - slack;
   }
@@ -570,6 +575,37 @@ struct Histogram {
     group.sync();
     ahead = s.found[1];
     return int(s.found[0]);
+  }
+  // The sum of the entries above v, v from `low` to `high`.
+  template <typename Weight>
+  __device__ __forceinline__ uint64_t above(const Row &row, Group<G> &group, const Weight &weight, float v) const {
+    Shared<G> &s = group.shared;
+    const int bin = int(bins.at(v));
+    uint64_t b = before;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      if (group.lane() * PER + i == bin) s.found[0] = b;
+      b += value[i];
+    }
+    float least, most;
+    bins.range(bin, least, most);
+    most = fminf(most, high);
+    const int n = gather(row, group, [&](float z, int) { return z > v && z <= most; });
+    const uint64_t ahead = s.found[0];
+    uint64_t x = 0;
+    if (n <= Shared<G>::LIST) {
+      for (int i = group.lane(); i < n; i += G) {
+        const float z = value_at(s.list[i].key);
+        x += bins.in(bin, z) ? weight.near(z) : 0;
+      }
+    } else {
+      row.each([&](int, const auto &z) {
+#pragma unroll
+        for (int k = 0; k < Row::V; ++k)
+          if (z(k) > v && z(k) <= most && bins.in(bin, z(k))) x += weight.near(z(k));
+      });
+    }
+    return ahead + group.join(x, Plus{});
   }
   // The entry at which the running sum reaches `sum`.
   template <typename Weight>
@@ -644,9 +680,10 @@ __device__ __forceinline__ float below(float z) {
 
 // ---- sampling ----------------------------------------------------------------------------------------------------
 
-// The largest k for which the lanes' maxima say where a row's first k end, and the list holds them.
+// The largest k for which the lanes' maxima say where a row's first k end, and the list holds them.  Of a wave's 64
+// lanes half: beyond, the list has more entries than the wave lanes (4096 x 512 fp32, k 50: 30 us, with the histogram 16).
 template <int G>
-constexpr int SHORT = G < Shared<G>::LIST / 2 ? G : Shared<G>::LIST / 2;
+constexpr int SHORT = G == 64 ? 32 : Shared<G>::LIST / 2;
 
 template <typename Row, int G>
 __device__ __forceinline__ void sample_row(const ChooseArgs &a, int64_t r, Row &row, Group<G> &group) {
@@ -748,34 +785,28 @@ __device__ __forceinline__ void sample_row(const ChooseArgs &a, int64_t r, Row &
     }
   }
   const float lowest = weight.least();
-  const auto sum_above = [&](float v) {  // of the entries above v
-    uint64_t x = 0;
-    row.each([&](int, const auto &z) {
-#pragma unroll
-      for (int k = 0; k < Row::V; ++k)
-        if (z(k) > v && z(k) >= lowest) x += weight.near(z(k));
-    });
-    return group.join(x, Plus{});
-  };
   h.make(row, group, weight, top, fmaxf(end, lowest), lowest);
   uint64_t kept = h.total;
-  if (after < INFINITY) kept = sum_above(after) + ties * weight(after);
+  if (after >= lowest && after < INFINITY) kept = h.above(row, group, weight, after) + ties * weight.near(after);
   if (p < 1) {
     const uint64_t limit = limit_of(kept);
     if (limit < kept) kept = h.entry(row, group, weight, limit).upto;
   }
   if (bound > 1) {
-    // The least value whose weight is kept, by halving.
+    // The largest value whose weight is not kept, by halving, near where the logarithm says it is.
+    const uint32_t near = key_of(float(double(top) + log_of(least) * temperature));
     uint32_t lo = key_of(lowest), hi = key_of(top);
-    if (weight(lowest) < bound) {
+    if (weight.near(lowest) < bound) {
+      if (near - 4 > lo && near < hi && weight.near(of_key(near - 4)) < bound) lo = near - 4;
+      if (near > lo && near + 4 < hi && weight.near(of_key(near + 4)) >= bound) hi = near + 4;
       while (hi - lo > 1) {
         const uint32_t mid = lo + (hi - lo) / 2;
-        if (weight(of_key(mid)) < bound)
+        if (weight.near(of_key(mid)) < bound)
           lo = mid;
         else
           hi = mid;
       }
-      kept = min(kept, sum_above(of_key(lo)));
+      kept = min(kept, h.above(row, group, weight, of_key(lo)));
     }
   }
   if (least > 1) kept = one;
@@ -884,7 +915,7 @@ __device__ __forceinline__ void top_row(const ChooseArgs &a, int64_t r, Row &row
 
 // BYTES: of LDS for a row; 0: it is read again for each pass.
 template <typename T, int G, int BYTES, bool RECORD>
-__global__ __launch_bounds__((G > 256 ? G : 256)) void choose_kernel(const ChooseArgs a) {
+__global__ __launch_bounds__((G > 256 ? G : 256), 4) void choose_kernel(const ChooseArgs a) {
   constexpr int ROWS = G > 256 ? 1 : 256 / G;
   __shared__ Shared<G> shared[ROWS];
   const int in_block = G < 256 ? __builtin_amdgcn_readfirstlane(threadIdx.x / G) : 0;
