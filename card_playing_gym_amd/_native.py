@@ -332,7 +332,7 @@ _SIGNATURES = {
     "cg_policy_loss_backward": (
         c_int32, [P(PolicyLoss), c_void_p, c_int32, c_void_p, c_void_p, c_size_t, c_void_p],
     ),
-    "cg_distill_loss_workspace_size": (c_size_t, []),
+    "cg_distill_loss_workspace_size": (c_size_t, [P(DistillLoss)]),
     "cg_distill_loss_forward": (
         c_int32, [P(DistillLoss), c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p],
     ),

@@ -124,7 +124,7 @@ struct RowScalars {
 
 // top, rest_top: the row's largest entry, and the largest outside R; rest: the sum outside, from rest_top.
 __device__ __forceinline__ RowScalars row_scalars(const DistillArgs &a, int64_t r, float weight, float top, float rest_top,
-                                                  double rest, const TopSums &t, bool good, double scale) {
+                                                  double rest, const TopSums &t, bool good) {
   RowScalars o;
   const double gap = rest > 0 ? (double(rest_top) - double(top)) * a.inverse : 0.0;
   const double lower = rest > 0 ? exp_of(gap) : 0.0;
@@ -149,16 +149,12 @@ __device__ __forceinline__ RowScalars row_scalars(const DistillArgs &a, int64_t 
     mass = t.q > 0 ? 1 : t.q;
     o.pull = inv;
   }
-  const double f = double(weight) * scale * a.inverse;
+  const double f = double(weight) * (a.upstream ? double(*a.upstream) : 1.0) / read(a.normalizer) * a.inverse;
   o.inner = f * mass * reciprocal(s);
   o.pull *= f;
   o.outer = o.live ? float(o.inner * lower - f * outer) : 0.f;
   o.value = double(weight) * o.kl;
   return o;
-}
-
-__device__ __forceinline__ double scale_of(const DistillArgs &a) {
-  return (a.upstream ? double(*a.upstream) : 1.0) / read(a.normalizer);
 }
 
 template <int G>
@@ -169,11 +165,11 @@ struct Slots {
 };
 
 // From a row's entries outside R to its numbers and its gradient: what every kernel does with a row.
-// each(visit): visit(first entry, entries, inside) for this lane's vectors, those in R as -inf.
-template <int G, int V, typename T, typename Each>
+// each(visit): visit(first entry, entries, inside) for this lane's vectors, those in R as -inf.  pass(): between passes.
+template <int G, int V, typename T, typename Each, typename Pass>
 __device__ __forceinline__ void distill_row(const DistillArgs &a, int64_t r, int lane, float weight, bool good,
-                                            const T *logits, const uint8_t *legal, Slots<G> &slots, double scale,
-                                            bool in, const Each &each, double &value) {
+                                            const T *logits, const uint8_t *legal, Slots<G> &slots, bool in,
+                                            const Each &each, const Pass &pass, double &value) {
   float tops[3] = {-INFINITY, -INFINITY, -INFINITY};  // of z outside R, in it, and of log q
   if (weight != 0) {
     each([&](int, const auto &z, bool) {
@@ -186,6 +182,7 @@ __device__ __forceinline__ void distill_row(const DistillArgs &a, int64_t r, int
     });
   }
   join<G>(tops, slots.tops, Most{});
+  pass();
   const float rest_top = tops[0] > -INFINITY ? tops[0] : 0.f;
   const float most = fmaxf(tops[0], tops[1]), top = most > -INFINITY ? most : 0.f;
   // Without q_r, only the differences of the log q count.
@@ -209,8 +206,9 @@ __device__ __forceinline__ void distill_row(const DistillArgs &a, int64_t r, int
   }
   sums[5] = good ? 0 : 1;
   join<G>(sums, slots.sums, Add{});
+  pass();
   const RowScalars o = row_scalars(a, r, weight, top, rest_top, sums[0], TopSums{sums[1], sums[2], sums[3], sums[4]},
-                                   sums[5] == 0, scale);
+                                   sums[5] == 0);
   if (in && lane == 0 && a.kl) {
     if (o.live) value += o.value;
     a.kl[r] = o.live ? float(o.kl) : 0.f;
@@ -237,56 +235,55 @@ __device__ __forceinline__ void distill_row(const DistillArgs &a, int64_t r, int
   }
 }
 
-// ---- rows in registers: E entries a lane, G lanes a row, 256 / G rows a block at a time (one from 256 on) -----
+// ---- rows in registers: E entries a lane, G lanes a row, 256 / G rows a block (one from 256 on) -----------------
+//
+// A block takes its rows and ends: in a loop over rows the compiler keeps what is the same for all of them in registers,
+// which the row needs (bf16 4096 x 32768, 512 blocks in a loop: 311 us).
 
 // S: the type in which entries are kept (T, or float where rows are shorter than a load).
 template <typename T, int G, int E, typename S = T>
-__global__ __launch_bounds__((G > 256 ? G : 256)) void rows_kernel(const DistillArgs a) {
+__global__ __launch_bounds__((G > 256 ? G : 256), 4) void rows_kernel(const DistillArgs a) {
   constexpr int V = E == 1 ? 1 : VEC<T>, C = E / V, THREADS = G > 256 ? G : 256, ROWS = THREADS / G;
   if (done(a)) return;
   __shared__ Slots<G> slots;
   __shared__ Bits<G * E> bits[ROWS];
-  const double scale = scale_of(a);
   double value = 0;
   const int in_block = threadIdx.x / G, lane = threadIdx.x % G;
-  // every thread of the block takes every turn: lanes of rows past the end have nothing live
-  for (int64_t first = int64_t(blockIdx.x) * ROWS; first < a.rows; first += int64_t(gridDim.x) * ROWS) {
-    const bool in = first + in_block < a.rows;
-    const int64_t r = min(first + in_block, int64_t(a.rows) - 1);
-    const float weight = in ? a.weights ? a.weights[r] : 1.f : 0.f;
-    const T *logits = static_cast<const T *>(a.logits) + r * a.ld_logits;
-    const uint8_t *legal = a.mask ? a.mask + r * a.ld_mask : nullptr;
-    Entries<S, E> z;
-    bool good = true;
-    if (weight != 0) {  // rows without weight are not read
-      load_entries<G, C, V>(z.w, logits, legal, lane * V, a.width);
-    } else {
-      z.clear();
-    }
-    // (groups of a wave go through their barriers together, weight or not)
-    if (weight != 0 || G <= 64) good = mark<G>(a, r, lane, bits[in_block]) || weight == 0;
-    if (weight != 0) {
+  const int64_t first = int64_t(blockIdx.x) * ROWS + in_block;
+  const bool in = first < a.rows;  // (lanes of rows past the end have nothing live)
+  const int64_t r = in ? first : int64_t(a.rows) - 1;
+  const float weight = in ? a.weights ? a.weights[r] : 1.f : 0.f;
+  const T *logits = static_cast<const T *>(a.logits) + r * a.ld_logits;
+  const uint8_t *legal = a.mask ? a.mask + r * a.ld_mask : nullptr;
+  Entries<S, E> z;
+  bool good = true;
+  if (weight != 0) {  // rows without weight are not read
+    load_entries<G, C, V>(z.w, logits, legal, lane * V, a.width);
+  } else {
+    z.clear();
+  }
+  // (groups of a wave go through their barriers together, weight or not)
+  if (weight != 0 || G <= 64) good = mark<G>(a, r, lane, bits[in_block]) || weight == 0;
+  if (weight != 0) {
 #pragma unroll
-      for (int c = 0; c < C; ++c) {
-        const int at = V == 1 ? lane : min((c * G + lane) * V, a.width - V);
-        const uint32_t set = at < a.width ? bits[in_block].from(at) & ((1u << V) - 1) : 0;
-        if (set == 0) continue;
+    for (int c = 0; c < C; ++c) {
+      const int at = V == 1 ? lane : min((c * G + lane) * V, a.width - V);
+      const uint32_t set = at < a.width ? bits[in_block].from(at) & ((1u << V) - 1) : 0;
+      if (set == 0) continue;
 #pragma unroll
-        for (int k = 0; k < V; ++k) {
-          const uint32_t part = Entries<S, E>::PER == 1 ? ~0u : k % 2 ? 0xffff0000u : 0xffffu;
-          uint32_t &w = z.w[(c * V + k) / Entries<S, E>::PER];
-          if (set >> k & 1) w = (w & ~part) | (NEGATIVE_INFINITY<S> & part);
-        }
+      for (int k = 0; k < V; ++k) {
+        const uint32_t part = Entries<S, E>::PER == 1 ? ~0u : k % 2 ? 0xffff0000u : 0xffffu;
+        uint32_t &w = z.w[(c * V + k) / Entries<S, E>::PER];
+        if (set >> k & 1) w = (w & ~part) | (NEGATIVE_INFINITY<S> & part);
       }
     }
-    const auto each = [&](const auto &visit) {
-#pragma unroll
-      for (int c = 0; c < C; ++c)
-        visit((c * G + lane) * V, [&](int k) { return z[c * V + k]; }, (c + 1) * G * V <= a.width);
-    };
-    distill_row<G, V>(a, r, lane, weight, good, logits, legal, slots, scale, in, each, value);
-    group_sync<G>();  // (the bits and slots are written again)
   }
+  const auto each = [&](const auto &visit) {
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+      visit((c * G + lane) * V, [&](int k) { return z[c * V + k]; }, (c + 1) * G * V <= a.width);
+  };
+  distill_row<G, V>(a, r, lane, weight, good, logits, legal, slots, in, each, [&] { z.forget(); }, value);
   if (a.kl) block_loss(a, value);
 }
 
@@ -298,29 +295,26 @@ __global__ __launch_bounds__(1024) void long_rows_kernel(const DistillArgs a) {
   if (done(a)) return;
   __shared__ Slots<G> slots;
   __shared__ Bits<MAX_WIDTH> bits;
-  const double scale = scale_of(a);
   double value = 0;
   const int lane = threadIdx.x;
-  for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
-    const float weight = a.weights ? a.weights[r] : 1.f;
-    const T *logits = static_cast<const T *>(a.logits) + r * a.ld_logits;
-    const uint8_t *legal = a.mask ? a.mask + r * a.ld_mask : nullptr;
-    const bool good = weight != 0 ? mark<G>(a, r, lane, bits) : true;
-    const auto each = [&](const auto &visit) {
-      for (int i = lane * V; i < a.width; i += G * V) {
-        Entries<T, V> z;
-        z.clear();
-        uint32_t set = 0;
-        if (weight != 0) {
-          load_entries<1, 1, V>(z.w, logits, legal, i, a.width);
-          set = bits.from(min(i, a.width - V));
-        }
-        visit(i, [&](int k) { return set >> k & 1 ? -INFINITY : z[k]; }, false);
+  const int64_t r = blockIdx.x;
+  const float weight = a.weights ? a.weights[r] : 1.f;
+  const T *logits = static_cast<const T *>(a.logits) + r * a.ld_logits;
+  const uint8_t *legal = a.mask ? a.mask + r * a.ld_mask : nullptr;
+  const bool good = weight != 0 ? mark<G>(a, r, lane, bits) : true;
+  const auto each = [&](const auto &visit) {
+    for (int i = lane * V; i < a.width; i += G * V) {
+      Entries<T, V> z;
+      z.clear();
+      uint32_t set = 0;
+      if (weight != 0) {
+        load_entries<1, 1, V>(z.w, logits, legal, i, a.width);
+        set = bits.from(min(i, a.width - V));
       }
-    };
-    distill_row<G, V>(a, r, lane, weight, good, logits, legal, slots, scale, true, each, value);
-    __syncthreads();
-  }
+      visit(i, [&](int k) { return set >> k & 1 ? -INFINITY : z[k]; }, false);
+    }
+  };
+  distill_row<G, V>(a, r, lane, weight, good, logits, legal, slots, true, each, [] {}, value);
   if (a.kl) block_loss(a, value);
 }
 
@@ -328,7 +322,7 @@ __global__ __launch_bounds__(1024) void long_rows_kernel(const DistillArgs a) {
 
 struct Launch {
   void (*kernel)(DistillArgs);
-  int rows, threads;  // rows a block takes at a time
+  int rows, threads;  // rows a block takes
 };
 
 template <typename T, int G, int E, typename S = T>
@@ -354,15 +348,20 @@ Launch launch_of(int width) {
   return {long_rows_kernel<T>, 1, 1024};
 }
 
-// Returns the number of partial sums of the loss that are written (by one block for all rows: the loss itself).
-int launch_rows(const DistillArgs &a, int dtype, hipStream_t stream) {
-  const Launch l = dtype == CG_F32 ? launch_of<float>(a.width) : dtype == CG_BF16 ? launch_of<bf16>(a.width) : launch_of<f16>(a.width);
-  const int64_t blocks = (int64_t(a.rows) + l.rows - 1) / l.rows;
-  const int most = l.threads >= 512 ? 512 : MAX_BLOCKS;
-  const int grid = int(blocks < most ? blocks : most);
-  l.kernel<<<grid, l.threads, 0, stream>>>(a);
+Launch launch_of(const cg_policy_rows &p) {
+  return p.dtype == CG_F32 ? launch_of<float>(p.width) : p.dtype == CG_BF16 ? launch_of<bf16>(p.width) : launch_of<f16>(p.width);
+}
+
+// Each block's sum of the loss is a partial sum of it (one block's the loss itself).
+int64_t blocks_of(const cg_policy_rows &p) {
+  const Launch l = launch_of(p);
+  return (int64_t(p.rows) + l.rows - 1) / l.rows;
+}
+
+void launch_rows(const DistillArgs &a, const cg_policy_rows &p, hipStream_t stream) {
+  const Launch l = launch_of(p);
+  l.kernel<<<unsigned(blocks_of(p)), l.threads, 0, stream>>>(a);
   CG_LAUNCHED();
-  return grid;
 }
 
 DistillArgs args_of(const cg_distill_loss *loss) {
@@ -396,21 +395,23 @@ using namespace cg;
 
 extern "C" {
 
-size_t cg_distill_loss_workspace_size(void) { return MAX_BLOCKS * sizeof(double); }
+size_t cg_distill_loss_workspace_size(const cg_distill_loss *loss) {
+  return loss && loss->rows.rows > 0 && loss->rows.width > 0 ? blocks_of(loss->rows) * sizeof(double) : sizeof(double);
+}
 
 int cg_distill_loss_forward(const cg_distill_loss *loss, float *value, float *kl, void *grad, void *workspace,
                             size_t workspace_size, void *stream) {
   return guarded([&] {
     DistillArgs a = args_of(loss);
     CG_REQUIRE(value && workspace, CG_ERR_INVALID, "value and workspace are required");
-    CG_REQUIRE(workspace_size >= cg_distill_loss_workspace_size(), CG_ERR_INVALID, "workspace too small");
+    CG_REQUIRE(workspace_size >= cg_distill_loss_workspace_size(loss), CG_ERR_INVALID, "workspace too small");
     CG_REQUIRE(a.rows == 0 || kl, CG_ERR_INVALID, "kl is required");
     a.partials = static_cast<double *>(workspace);
     a.loss = value, a.kl = kl, a.grad = grad;
-    int sums = 0;
-    if (a.rows > 0) sums = launch_rows(a, loss->rows.dtype, as_stream(stream));
+    const int64_t sums = a.rows > 0 ? blocks_of(loss->rows) : 0;
+    if (sums > 0) launch_rows(a, loss->rows, as_stream(stream));
     if (sums != 1) {
-      loss_kernel<DistillArgs><<<1, 256, 0, as_stream(stream)>>>(a, sums);
+      loss_kernel<DistillArgs><<<1, 256, 0, as_stream(stream)>>>(a, int(sums));
       CG_LAUNCHED();
     }
   });
@@ -424,7 +425,7 @@ int cg_distill_loss_backward(const cg_distill_loss *loss, const float *upstream,
     if (a.rows == 0) return;
     CG_REQUIRE(grad, CG_ERR_INVALID, "grad is required");
     a.grad = grad, a.upstream = upstream, a.written = written;
-    launch_rows(a, loss->rows.dtype, as_stream(stream));
+    launch_rows(a, loss->rows, as_stream(stream));
   });
 }
 

@@ -57,7 +57,7 @@ class _Call:
     def forward(self, device: torch.device, grad: torch.Tensor | None) -> torch.Tensor:
         loss = torch.empty((), device=device)
         self.kl = torch.empty(self.descriptor.rows.rows, device=device)
-        size = nat.lib().cg_distill_loss_workspace_size()
+        size = nat.lib().cg_distill_loss_workspace_size(self.descriptor)
         workspace = torch.empty(size, device=device, dtype=torch.uint8)
         with _on(device):
             nat.call("cg_distill_loss_forward", self.descriptor, loss.data_ptr(), self.kl.data_ptr(),

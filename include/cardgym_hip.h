@@ -645,7 +645,7 @@ typedef struct {
 
 /* value[0], kl [rows] and, where grad is not NULL, the value's gradient [rows, width] dense, of the
  * logits' type.  workspace: 8-byte aligned, of this call alone until it has run. */
-size_t cg_distill_loss_workspace_size(void);
+size_t cg_distill_loss_workspace_size(const cg_distill_loss *loss);
 int cg_distill_loss_forward(const cg_distill_loss *loss, float *value, float *kl, void *grad, void *workspace,
                             size_t workspace_size, void *stream);
 /* grad = upstream[0] times the value's gradient, formed from the inputs and rounded once.  written != 0: grad

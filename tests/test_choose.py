@@ -221,6 +221,8 @@ def test_native_refusals():
             setattr(loss, name, x)
         if upstream is not None:
             return lib.cg_distill_loss_backward(ctypes.byref(loss), upstream or None, 0, grad, None)
+        if size < 0:  # short by that much
+            size += lib.cg_distill_loss_workspace_size(ctypes.byref(loss))
         return lib.cg_distill_loss_forward(ctypes.byref(loss), value, kl, None, workspace, size, None)
 
     for call in (sample, top, distill):
@@ -233,7 +235,7 @@ def test_native_refusals():
     for changes in ({"k": 0}, {"k": 257}, {"temperature": 0.0}, {"temperature": float("nan")}, {"log_probs": None},
                     {"indices": None}, {"log_rest": None}):
         assert top(rows(), **changes) == invalid, changes
-    for changes in ({"value": None}, {"kl": None}, {"workspace": None}, {"size": lib.cg_distill_loss_workspace_size() - 1},
+    for changes in ({"value": None}, {"kl": None}, {"workspace": None}, {"size": -1},
                     {"k": 0}, {"k": 257}, {"temperature": 0.0}, {"indices": None}, {"log_probs": None}, {"upstream": 0},
                     {"upstream": 16, "grad": None}):
         assert distill(rows(), **changes) == invalid, changes
