@@ -878,8 +878,14 @@ __device__ __forceinline__ void top_row(const ChooseArgs &a, int64_t r, Row &row
   }
   const float base = next > -INFINITY ? next : 0.f;
   const double c = 1.44269504088896340736 * inverse;
-  const float scale = float(c);
-  const auto weigh = [&](float z) { return __builtin_amdgcn_exp2f((z - base) * scale); };
+  // (the scale in two parts, both above 0: its rounding would be the same for all entries, and -inf stays -inf)
+  float fast = float(c);
+  if (double(fast) >= c) fast = __uint_as_float(__float_as_uint(fast) - 1);
+  const float slow = float(c - double(fast));
+  const auto weigh = [&](float z) {
+    const float d = z - base;
+    return __builtin_amdgcn_exp2f(fmaf(d, fast, d * slow));
+  };
   double sums[2] = {0, 0};  // of the others, and of the record
   row.each([&](int, const auto &z) {
     float sum = 0;

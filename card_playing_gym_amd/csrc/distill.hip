@@ -23,6 +23,10 @@ namespace {
 
 constexpr int MAX_WIDTH = 1 << 18;
 constexpr int MAX_TOP = 256;
+constexpr int64_t STREAM_BYTES = 512 << 20;
+#ifndef WV
+#define WV 4
+#endif
 
 struct DistillArgs {
   const void *logits;
@@ -33,7 +37,7 @@ struct DistillArgs {
   int64_t ld_logits, ld_mask;
   int32_t rows, width, k;
   double inverse;     // 1 / T
-  float fast, slow;   // log2(e) / T, and what that leaves out
+  float fast, slow;   // log2(e) / T rounded down, and the rest of it: both above 0, so that -inf stays -inf
   Scalar normalizer;
   float *kl;   // NULL in a backward call
   void *grad;  // NULL: none
@@ -41,13 +45,14 @@ struct DistillArgs {
   float *loss;
   const float *upstream;  // of a backward call
   int32_t written;        // the gradient for an upstream of 1 is in place
+  int32_t streams;        // the logits and their gradient go past the caches (rows of 512 lanes and more)
 };
 
-// e^((z - from) / T) for z <= from (-inf: 0), with what the rounding of the product cuts off.
+// e^((z - from) / T) for z <= from (-inf: 0).  The scale's second part keeps its rounding, which is the same for all
+// entries, out of their sum; what the rounding of the product leaves differs from one to the next.
 __device__ __forceinline__ float exp_from(const DistillArgs &a, float z, float from) {
-  const float d = z - from, t = d * a.fast, e = __builtin_amdgcn_exp2f(t);
-  const float cut = fmaf(d, a.slow, fmaf(d, a.fast, -t));
-  return t > -126.f ? fmaf(e, cut * 0.69314718f, e) : e;  // (below it: inf - inf)
+  const float d = z - from;
+  return __builtin_amdgcn_exp2f(fmaf(d, a.fast, d * a.slow));
 }
 
 // ---- the record's entries in a row -------------------------------------------------------------------------
@@ -74,39 +79,75 @@ __device__ __forceinline__ void group_sync() {
   }
 }
 
-// The entry's logit, -inf where it is not legal.
-template <typename T>
-__device__ __forceinline__ float logit_at(const T *row, const uint8_t *legal, int i) {
-  return !legal || legal[i] ? to_f32(row[i]) : -INFINITY;
-}
+// This lane's entries of R.  A group of 64 lanes or more loads them once, beside the row; in narrower ones, whose rows
+// have few words to wait for, they would take more registers than the row does.
+template <int G, typename T>
+struct Record {
+  static constexpr int N = G < 64 ? 0 : G < MAX_TOP ? MAX_TOP / G : 1;
+  const DistillArgs &a;
+  const int64_t *indices;
+  const float *top;
+  const T *logits;
+  const uint8_t *legal;
+  int lane, index[N > 0 ? N : 1];  // -1: none; -2: not of the row
+  float log_q[N > 0 ? N : 1], z[N > 0 ? N : 1];
 
-// visit(index, log q) for this lane's entries of R that are there.
-template <int G, typename Visit>
-__device__ __forceinline__ void each_top(const DistillArgs &a, int64_t r, int lane, const Visit &visit) {
-  for (int k = lane; k < a.k; k += G) {
-    const int64_t i = a.indices[r * a.k + k];
-    if (i != -1) visit(i, a.top[r * a.k + k]);
+  __device__ __forceinline__ Record(const DistillArgs &a, int64_t r, int lane, const T *logits, const uint8_t *legal, bool counts)
+      : a(a), indices(a.indices + r * a.k), top(a.top + r * a.k), logits(logits), legal(legal), lane(lane) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int k = lane + i * G;
+      index[i] = -1, log_q[i] = z[i] = -INFINITY;
+      if (!counts || k >= a.k) continue;
+      index[i] = in_row(indices[k]);
+      log_q[i] = top[k];
+    }
   }
-}
-
-// Marks R.  Returns whether its indices are in the row, and each there once.
-template <int G, typename B>
-__device__ __forceinline__ bool mark(const DistillArgs &a, int64_t r, int lane, B &bits) {
-  const int words = min((a.width >> 5) + 2, B::WORDS);  // (of vectors that begin before the row's end, and one more)
-  for (int i = lane; i < words; i += G) bits.w[i] = 0;
-  group_sync<G>();
-  bool good = true;
-  each_top<G>(a, r, lane, [&](int64_t i, float) {
-    if (i < 0 || i >= a.width) {
-      good = false;
+  __device__ __forceinline__ int in_row(int64_t i) const { return i >= 0 && i < a.width ? int(i) : i == -1 ? -1 : -2; }
+  // The entry's logit, -inf where it is not legal.
+  __device__ __forceinline__ float logit(int i) const { return !legal || legal[i] ? to_f32(logits[i]) : -INFINITY; }
+  __device__ __forceinline__ void load_logits() {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (index[i] >= 0) z[i] = logit(index[i]);
+  }
+  // visit(index, log q, logit) for those in the row.
+  template <typename Visit>
+  __device__ __forceinline__ void each(const Visit &visit) const {
+    if constexpr (N > 0) {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (index[i] >= 0) visit(index[i], log_q[i], z[i]);
     } else {
+      for (int k = lane; k < a.k; k += G) {
+        const int i = in_row(indices[k]);
+        if (i >= 0) visit(i, top[k], logit(i));
+      }
+    }
+  }
+  // Marks R.  Returns whether this lane's indices are in the row, and there once.
+  template <typename B>
+  __device__ __forceinline__ bool mark(B &bits) const {
+    const int words = min((a.width >> 5) + 2, B::WORDS);  // (of vectors that begin before the row's end, and one more)
+    for (int i = lane; i < words; i += G) bits.w[i] = 0;
+    group_sync<G>();
+    bool good = true;
+    const auto set = [&](int i) {
+      if (i == -2) good = false;
+      if (i < 0) return;
       const uint32_t bit = 1u << (i & 31);
       if (atomicOr(&bits.w[i >> 5], bit) & bit) good = false;
+    };
+    if constexpr (N > 0) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) set(index[i]);
+    } else {
+      for (int k = lane; k < a.k; k += G) set(in_row(indices[k]));
     }
-  });
-  group_sync<G>();
-  return good;
-}
+    group_sync<G>();
+    return good;
+  }
+};
 
 // ---- a row's scalars -----------------------------------------------------------------------------------------
 
@@ -168,16 +209,15 @@ struct Slots {
 // each(visit): visit(first entry, entries, inside) for this lane's vectors, those in R as -inf.  pass(): between passes.
 template <int G, int V, typename T, typename Each, typename Pass>
 __device__ __forceinline__ void distill_row(const DistillArgs &a, int64_t r, int lane, float weight, bool good,
-                                            const T *logits, const uint8_t *legal, Slots<G> &slots, bool in,
-                                            const Each &each, const Pass &pass, double &value) {
+                                            const Record<G, T> &record, Slots<G> &slots, bool in, const Each &each, const Pass &pass, double &value) {
   float tops[3] = {-INFINITY, -INFINITY, -INFINITY};  // of z outside R, in it, and of log q
   if (weight != 0) {
     each([&](int, const auto &z, bool) {
 #pragma unroll
       for (int k = 0; k < V; ++k) tops[0] = fmaxf(tops[0], z(k));
     });
-    each_top<G>(a, r, lane, [&](int64_t i, float log_q) {
-      if (i >= 0 && i < a.width) tops[1] = fmaxf(tops[1], logit_at(logits, legal, int(i)));
+    record.each([&](int, float log_q, float z) {
+      tops[1] = fmaxf(tops[1], z);
       tops[2] = fmaxf(tops[2], log_q);
     });
   }
@@ -195,9 +235,7 @@ __device__ __forceinline__ void distill_row(const DistillArgs &a, int64_t r, int
       for (int k = 0; k < V; ++k) s += exp_from(a, z(k), rest_top);
       sums[0] += s;
     });
-    each_top<G>(a, r, lane, [&](int64_t i, float log_q) {
-      if (i < 0 || i >= a.width) return;
-      const float z = logit_at(logits, legal, int(i));
+    record.each([&](int, float log_q, float z) {
       const double x = (double(z) - double(top)) * a.inverse, l = double(log_q) - double(base), q = exp_of(l);
       sums[1] += exp_of(x);
       sums[2] += q;
@@ -220,14 +258,12 @@ __device__ __forceinline__ void distill_row(const DistillArgs &a, int64_t r, int
       float g[V];
 #pragma unroll
       for (int k = 0; k < V; ++k) g[k] = o.outer * exp_from(a, z(k), rest_top);
-      store_entries<V>(grad, g, i, a.width, inside);
+      store_entries<V>(grad, g, i, a.width, inside, G >= 512 && a.streams);
     });
   }
   if constexpr (G > 64) __syncthreads();  // (the zeros just written at R's entries come first)
   if (in && o.live) {
-    each_top<G>(a, r, lane, [&](int64_t i, float log_q) {
-      if (i < 0 || i >= a.width) return;
-      const float z = logit_at(logits, legal, int(i));
+    record.each([&](int i, float log_q, float z) {
       if (z == -INFINITY) return;
       const double x = (double(z) - double(top)) * a.inverse;
       grad[i] = from_f32<T>(float(o.inner * exp_of(x) - o.pull * exp_of(double(log_q) - double(base))));
@@ -242,7 +278,7 @@ __device__ __forceinline__ void distill_row(const DistillArgs &a, int64_t r, int
 
 // S: the type in which entries are kept (T, or float where rows are shorter than a load).
 template <typename T, int G, int E, typename S = T>
-__global__ __launch_bounds__((G > 256 ? G : 256), 4) void rows_kernel(const DistillArgs a) {
+__global__ __launch_bounds__((G > 256 ? G : 256), (G >= 1024 ? 4 : G >= 64 ? WV : 4)) void rows_kernel(const DistillArgs a) {
   constexpr int V = E == 1 ? 1 : VEC<T>, C = E / V, THREADS = G > 256 ? G : 256, ROWS = THREADS / G;
   if (done(a)) return;
   __shared__ Slots<G> slots;
@@ -255,15 +291,17 @@ __global__ __launch_bounds__((G > 256 ? G : 256), 4) void rows_kernel(const Dist
   const float weight = in ? a.weights ? a.weights[r] : 1.f : 0.f;
   const T *logits = static_cast<const T *>(a.logits) + r * a.ld_logits;
   const uint8_t *legal = a.mask ? a.mask + r * a.ld_mask : nullptr;
+  Record<G, T> record(a, r, lane, logits, legal, weight != 0);
   Entries<S, E> z;
   bool good = true;
   if (weight != 0) {  // rows without weight are not read
-    load_entries<G, C, V>(z.w, logits, legal, lane * V, a.width);
+    load_entries<G, C, V>(z.w, logits, legal, lane * V, a.width, G >= 512 && a.streams);
   } else {
     z.clear();
   }
   // (groups of a wave go through their barriers together, weight or not)
-  if (weight != 0 || G <= 64) good = mark<G>(a, r, lane, bits[in_block]) || weight == 0;
+  record.load_logits();
+  if (weight != 0 || G <= 64) good = record.mark(bits[in_block]) || weight == 0;
   if (weight != 0) {
 #pragma unroll
     for (int c = 0; c < C; ++c) {
@@ -283,7 +321,7 @@ __global__ __launch_bounds__((G > 256 ? G : 256), 4) void rows_kernel(const Dist
     for (int c = 0; c < C; ++c)
       visit((c * G + lane) * V, [&](int k) { return z[c * V + k]; }, (c + 1) * G * V <= a.width);
   };
-  distill_row<G, V>(a, r, lane, weight, good, logits, legal, slots, in, each, [&] { z.forget(); }, value);
+  distill_row<G, V>(a, r, lane, weight, good, record, slots, in, each, [&] { z.forget(); }, value);
   if (a.kl) block_loss(a, value);
 }
 
@@ -301,7 +339,9 @@ __global__ __launch_bounds__(1024) void long_rows_kernel(const DistillArgs a) {
   const float weight = a.weights ? a.weights[r] : 1.f;
   const T *logits = static_cast<const T *>(a.logits) + r * a.ld_logits;
   const uint8_t *legal = a.mask ? a.mask + r * a.ld_mask : nullptr;
-  const bool good = weight != 0 ? mark<G>(a, r, lane, bits) : true;
+  Record<G, T> record(a, r, lane, logits, legal, weight != 0);
+  record.load_logits();
+  const bool good = weight != 0 ? record.mark(bits) : true;
   const auto each = [&](const auto &visit) {
     for (int i = lane * V; i < a.width; i += G * V) {
       Entries<T, V> z;
@@ -314,7 +354,7 @@ __global__ __launch_bounds__(1024) void long_rows_kernel(const DistillArgs a) {
       visit(i, [&](int k) { return set >> k & 1 ? -INFINITY : z[k]; }, false);
     }
   };
-  distill_row<G, V>(a, r, lane, weight, good, logits, legal, slots, true, each, [] {}, value);
+  distill_row<G, V>(a, r, lane, weight, good, record, slots, true, each, [] {}, value);
   if (a.kl) block_loss(a, value);
 }
 
@@ -383,8 +423,15 @@ DistillArgs args_of(const cg_distill_loss *loss) {
   a.rows = q.rows, a.width = q.width, a.k = p.k;
   a.inverse = 1 / p.temperature;
   const double c = 1.44269504088896340736 / p.temperature;
-  a.fast = float(c), a.slow = float(c - double(a.fast));
+  a.fast = float(c);
+  if (double(a.fast) >= c) a.fast = nextafterf(a.fast, 0.f);
+  a.slow = float(c - double(a.fast));
   a.normalizer = scalar(p.normalizer);
+#ifdef NOSTREAM
+  a.streams = 0;
+#else
+  a.streams = int64_t(q.rows) * q.width >= STREAM_BYTES / (2 * dtype_size(q.dtype));
+#endif
   return a;
 }
 
