@@ -195,22 +195,6 @@ struct InLds {
   __device__ __forceinline__ InLds(Vector *held, const T *row, const uint8_t *legal, int width)
       : held(held), width(width), vectors((width + V - 1) / V) {
     const int lane = threadIdx.x % G;
-    if (width < V) {
-      if (lane > 0) return;
-      Vector q;
-      for (int k = 0; k < 4; ++k) q.w[k] = NEGATIVE_INFINITY<T>;
-      for (int k = 0; k < V; ++k) {
-        if (k >= width || (legal && !legal[k])) continue;
-        if constexpr (sizeof(T) == 4) {
-          q.w[k] = __float_as_uint(row[k]);
-        } else {
-          const int shift = 16 * (k % 2);
-          q.w[k / 2] = (q.w[k / 2] & ~(0xffffu << shift)) | uint32_t(row[k].bits) << shift;
-        }
-      }
-      held[0] = q;
-      return;
-    }
     for (int first = lane; first < vectors; first += G * BATCH) {
       uint32_t w[BATCH][4];
 #pragma unroll
@@ -220,7 +204,7 @@ struct InLds {
         if (first + c * G < vectors) __builtin_memcpy(&held[first + c * G], w[c], 16);
     }
   }
-  __device__ __forceinline__ int at(int j) const { return max(min(j * V, width - V), 0); }
+  __device__ __forceinline__ int at(int j) const { return min(j * V, width - V); }
   template <typename Visit>
   __device__ __forceinline__ void each(const Visit &visit) const {
 #pragma unroll 1
@@ -685,15 +669,46 @@ __device__ __forceinline__ float below(float z) {
 template <int G>
 constexpr int SHORT = G == 64 ? 32 : Shared<G>::LIST / 2;
 
+// A row's controls.
+struct Controls {
+  double temperature, p, least, u;
+  int64_t most;
+  uint64_t one;  // the weight of 1
+  __device__ __forceinline__ Controls(const ChooseArgs &a, int64_t r)
+      : temperature(a.temperature.of(r)), p(a.top_p.of(r)), least(a.min_p.of(r)), u(a.uniforms[r]), most(a.top_k.of(r)),
+        one(uint64_t(1) << a.scale) {}
+  // min_p as the least weight that is kept: 1 without, the first entry's at most.
+  __device__ __forceinline__ uint64_t bound() const {
+    if (!(least > 0)) return 1;
+    const double x = ceil(least * double(one));
+    return x < double(one) ? uint64_t(x) : one;
+  }
+  // top_p as a sum: entries before which less than this is summed up are kept.
+  __device__ __forceinline__ uint64_t limit(uint64_t total) const {
+    const double x = ceil(p * double(total));
+    return x > 1 ? uint64_t(x) : 1;
+  }
+  // The running sum that the answer's is the first to reach: u of what is kept, and a unit more; the last one's for a u
+  // of 1 or NaN.
+  __device__ __forceinline__ uint64_t target(uint64_t kept) const {
+    const double x = u * double(kept);
+    const uint64_t place = x > 0 ? x < double(kept) ? uint64_t(x) : kept - 1 : u != u ? kept - 1 : 0;
+    return (place < kept ? place : kept - 1) + 1;
+  }
+  __device__ __forceinline__ float log_share(float z, float top, uint64_t kept, int scale) const {
+    return float((double(z) - double(top)) / temperature - log_of(__builtin_amdgcn_ldexp(double(kept), -scale)));  // (0 for the whole)
+  }
+};
+
 template <typename Row, int G>
 __device__ __forceinline__ void sample_row(const ChooseArgs &a, int64_t r, Row &row, Group<G> &group) {
   Shared<G> &s = group.shared;
-  const double temperature = a.temperature.of(r), p = a.top_p.of(r), least = a.min_p.of(r), u = a.uniforms[r];
-  const int64_t most = a.top_k.of(r);
+  const Controls c(a, r);
+  const int64_t most = c.most;
   float mine;
   const float top = row_top(row, group, mine);
   const auto answer = [&](int64_t action, float log_prob) { a.actions[r] = action, a.log_probs[r] = log_prob; };
-  if (top != top || !(temperature >= 0)) {
+  if (top != top || !(c.temperature >= 0)) {
     if (group.lane() == 0) answer(-1, NAN);
     return;
   }
@@ -701,41 +716,20 @@ __device__ __forceinline__ void sample_row(const ChooseArgs &a, int64_t r, Row &
     if (group.lane() == 0) answer(-1, 0);
     return;
   }
-  if (temperature == 0) {
+  if (c.temperature == 0) {
     const int first = first_index(row, group, top);
     if (group.lane() == 0) answer(first, 0);
     return;
   }
-  const Weights weight(top, temperature, a.scale);
-  const uint64_t one = uint64_t(1) << a.scale;
-  // min_p as the least weight that is kept (the first entry's at most)
-  uint64_t bound = 1;
-  if (least > 0) {
-    const double x = ceil(least * double(one));
-    bound = x < double(one) ? uint64_t(x) : one;
-  }
-  const auto limit_of = [&](uint64_t total) {  // top_p as a sum: entries before which less than this is summed up are kept
-    const double x = ceil(p * double(total));
-    return x > 1 ? uint64_t(x) : 1;
-  };
-  // The running sum that the answer's is the first to reach: u of what is kept, and a unit more.
-  const auto target = [&](uint64_t kept) {
-    const double x = u * double(kept);
-    const uint64_t place = x > 0 ? x < double(kept) ? uint64_t(x) : kept - 1 : u != u ? kept - 1 : 0;
-    return (place < kept ? place : kept - 1) + 1;
-  };
-  const auto log_share = [&](uint64_t place, uint64_t kept) {
-    return float((double(value_at(place)) - double(top)) / temperature -
-                 log_of(__builtin_amdgcn_ldexp(double(kept), -a.scale)));  // (0 for the whole of it)
-  };
+  const Weights weight(top, c.temperature, a.scale);
+  const uint64_t bound = c.bound();
   const bool limited = most > 0 && most < a.width;
-  if (limited ? most <= SHORT<G> : a.width <= 64) {
-    const float from = limited ? bound_of_top(group, top, mine, int(most)) : -INFINITY;
-    const float under = below(from);
+  if (limited && most <= SHORT<G>) {
+    const float under = below(bound_of_top(group, top, mine, int(most)));
     const int n = gather(row, group, [&](float z, int) { return z > under; });
     if (n <= Shared<G>::LIST) {
       const Mine<G> list(group, n, weight);
-      const int last = limited && most < n ? int(most) - 1 : n - 1;
+      const int last = most < n ? int(most) - 1 : n - 1;
       const auto each = [&](const auto &visit) {
 #pragma unroll
         for (int i = 0; i < Mine<G>::N; ++i)
@@ -746,8 +740,8 @@ __device__ __forceinline__ void sample_row(const ChooseArgs &a, int64_t r, Row &
       });
       group.sync();
       uint64_t kept = s.found[0];
-      if (p < 1) {
-        const uint64_t limit = limit_of(kept);
+      if (c.p < 1) {
+        const uint64_t limit = c.limit(kept);
         each([&](const Item &item, uint64_t before, int) {
           if (before < limit && limit <= before + item.weight) s.found[1] = before + item.weight;
         });
@@ -759,11 +753,11 @@ __device__ __forceinline__ void sample_row(const ChooseArgs &a, int64_t r, Row &
         each([&](const Item &item, uint64_t before, int) {
           if (item.weight >= bound) upto = Largest{}(upto, before + item.weight);
         });
-        kept = min(kept, least > 1 ? one : group.join(upto, Largest{}));
+        kept = min(kept, c.least > 1 ? c.one : group.join(upto, Largest{}));
       }
-      const uint64_t sum = target(kept);
+      const uint64_t sum = c.target(kept);
       each([&](const Item &item, uint64_t before, int) {
-        if (before < sum && sum <= before + item.weight) answer(index_at(item.key), log_share(item.key, kept));
+        if (before < sum && sum <= before + item.weight) answer(index_at(item.key), c.log_share(value_at(item.key), top, kept, a.scale));
       });
       return;
     }
@@ -788,13 +782,13 @@ __device__ __forceinline__ void sample_row(const ChooseArgs &a, int64_t r, Row &
   h.make(row, group, weight, top, fmaxf(end, lowest), lowest);
   uint64_t kept = h.total;
   if (after >= lowest && after < INFINITY) kept = h.above(row, group, weight, after) + ties * weight.near(after);
-  if (p < 1) {
-    const uint64_t limit = limit_of(kept);
+  if (c.p < 1) {
+    const uint64_t limit = c.limit(kept);
     if (limit < kept) kept = h.entry(row, group, weight, limit).upto;
   }
   if (bound > 1) {
     // The largest value whose weight is not kept, by halving, near where the logarithm says it is.
-    const uint32_t near = key_of(float(double(top) + log_of(least) * temperature));
+    const uint32_t near = key_of(float(double(top) + log_of(c.least) * c.temperature));
     uint32_t lo = key_of(lowest), hi = key_of(top);
     if (weight.near(lowest) < bound) {
       if (near - 4 > lo && near < hi && weight.near(of_key(near - 4)) < bound) lo = near - 4;
@@ -809,12 +803,28 @@ __device__ __forceinline__ void sample_row(const ChooseArgs &a, int64_t r, Row &
       kept = min(kept, h.above(row, group, weight, of_key(lo)));
     }
   }
-  if (least > 1) kept = one;
-  const uint64_t place = h.entry(row, group, weight, target(kept)).place;
-  if (group.lane() == 0) answer(index_at(place), log_share(place, kept));
+  if (c.least > 1) kept = c.one;
+  const uint64_t place = h.entry(row, group, weight, c.target(kept)).place;
+  if (group.lane() == 0) answer(index_at(place), c.log_share(value_at(place), top, kept, a.scale));
 }
 
 // ---- the record --------------------------------------------------------------------------------------------------
+
+// e^((z - base) / T) in float32, -inf's 0.  log2(e) / T in two parts, both above 0: its rounding would be the same for all
+// entries, and -inf stays -inf.
+struct Share {
+  float base, fast, slow;
+  __device__ __forceinline__ Share(float base, double inverse) : base(base) {
+    const double c = 1.44269504088896340736 * inverse;
+    fast = float(c);
+    if (double(fast) >= c) fast = __uint_as_float(__float_as_uint(fast) - 1);
+    slow = float(c - double(fast));
+  }
+  __device__ __forceinline__ float operator()(float z) const {
+    const float d = z - base;
+    return __builtin_amdgcn_exp2f(fmaf(d, fast, d * slow));
+  }
+};
 
 template <typename Row, int G>
 __device__ __forceinline__ void top_row(const ChooseArgs &a, int64_t r, Row &row, Group<G> &group) {
@@ -877,15 +887,7 @@ __device__ __forceinline__ void top_row(const ChooseArgs &a, int64_t r, Row &row
     next = group.join(next, Most{});
   }
   const float base = next > -INFINITY ? next : 0.f;
-  const double c = 1.44269504088896340736 * inverse;
-  // (the scale in two parts, both above 0: its rounding would be the same for all entries, and -inf stays -inf)
-  float fast = float(c);
-  if (double(fast) >= c) fast = __uint_as_float(__float_as_uint(fast) - 1);
-  const float slow = float(c - double(fast));
-  const auto weigh = [&](float z) {
-    const float d = z - base;
-    return __builtin_amdgcn_exp2f(fmaf(d, fast, d * slow));
-  };
+  const Share weigh(base, inverse);
   double sums[2] = {0, 0};  // of the others, and of the record
   row.each([&](int, const auto &z) {
     float sum = 0;
@@ -915,6 +917,112 @@ __device__ __forceinline__ void top_row(const ChooseArgs &a, int64_t r, Row &row
   }
   for (int i = held + lane; i < a.k; i += G) log_probs[i] = -INFINITY, indices[i] = -1;
   if (lane == 0) a.log_rest[r] = rest > 0 ? float(gap + log_of(rest) - log_total) : -INFINITY;
+}
+
+// ---- rows of up to 64 entries: a lane an entry, 64 / G rows a wave ---------------------------------------------
+//
+// A lane counts what stands before its entry, puts it there and takes the entry of its own place: from then on the lanes
+// are in the row's order, and its sums are those of the lanes before.  131072 rows of 32 float32 entries, a row a wave and
+// entry by entry over lists: 148 us.
+
+// Over the lanes of a group of G, its first one `base` in the wave.
+template <int G>
+struct Lanes {
+  int lane, base;
+  __device__ __forceinline__ Lanes() : lane(threadIdx.x % G), base((threadIdx.x & 63) / G * G) {}
+  template <typename X>
+  __device__ __forceinline__ X at(X x, int i) const {
+    return __shfl(x, base + i, 64);
+  }
+  __device__ __forceinline__ int count(bool is) const {
+    return __popcll(__ballot(is) >> base & (G == 64 ? ~0ull : (1ull << G % 64) - 1));
+  }
+  // The sum over the lanes up to and with this one.
+  __device__ __forceinline__ uint64_t running_sum(uint64_t x) const {
+    const auto add = [&](uint64_t y, int step) { x += G >= 16 || lane >= step ? y : 0; };
+    add(from_lower<0x111>(x), 1);
+    add(from_lower<0x112>(x), 2);
+    if constexpr (G > 4) add(from_lower<0x114>(x), 4);
+    if constexpr (G > 8) add(from_lower<0x118>(x), 8);
+    if constexpr (G > 16) x += from_lower<0x142, 0xa>(x);
+    if constexpr (G > 32) x += from_lower<0x143, 0xc>(x);
+    return x;
+  }
+};
+
+template <typename T, int G, bool RECORD>
+__global__ __launch_bounds__(256) void narrow_kernel(const ChooseArgs a) {
+  constexpr int ROWS = 256 / G, PITCH = G + 1;  // (rows side by side start in different banks)
+  __shared__ uint64_t places[ROWS * PITCH];
+  const Lanes<G> lanes;
+  const int lane = lanes.lane;
+  const int64_t first = int64_t(blockIdx.x) * ROWS + threadIdx.x / G;
+  const bool in = first < a.rows;  // (every lane takes part: rows past the end are the last one again)
+  const int64_t r = in ? first : int64_t(a.rows) - 1;
+  uint64_t *mine = places + threadIdx.x / G * PITCH;
+  float z = -INFINITY;
+  if (lane < a.width && (!a.mask || a.mask[r * a.ld_mask + lane]))
+    z = to_f32(static_cast<const T *>(a.logits)[r * a.ld_logits + lane]);
+  float top = lanes_join<G>(z, [](float x, float y) { return __builtin_elementwise_maximum(x, y); });
+  const bool nan = top != top, none = top == -INFINITY;
+  if (top == INFINITY) z = z == INFINITY ? 0.f : -INFINITY, top = 0;
+  if (nan || none) z = -INFINITY, top = 0;
+  // Into the row's order.
+  uint64_t place = place_of(z, lane);
+  mine[lane] = place;
+  const auto visible = [] {  // the wave's LDS writes to its own reads
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  };
+  visible();
+  int rank = 0;
+#pragma unroll 4
+  for (int j = 0; j < G; ++j) rank += mine[j] > place;  // (all different: an index is in each)
+  visible();
+  mine[rank] = place;
+  visible();
+  place = mine[lane];
+  z = value_at(place);
+  const int legal = lanes.count(z > -INFINITY);
+  if constexpr (RECORD) {
+    const double inverse = 1 / a.temperature.value;
+    const bool held = lane < a.k && lane < legal;
+    const float next = lanes.at(z, min(a.k, G - 1));  // the largest of the others, where there are any
+    const bool rest_there = a.k < legal;
+    const Share weigh(rest_there ? next : 0.f, inverse);
+    const double x = (double(z) - double(top)) * inverse;
+    const double rest = lanes_join<G>(lane >= a.k && lane < legal ? double(weigh(z)) : 0.0, Add{});
+    const double held_sum = lanes_join<G>(held ? exp_of(x) : 0.0, Add{});
+    const double gap = (double(weigh.base) - double(top)) * inverse;
+    const double log_total = log_of(held_sum + (rest_there ? rest * exp_of(gap) : 0.0));
+    const float absent = nan ? NAN : -INFINITY;
+    if (!in) return;
+    for (int i = lane; i < a.k; i += G) {  // (one turn where k is up to G: those behind are absent)
+      const bool there = i == lane && held;
+      a.log_probs[r * a.k + i] = there ? float(x - log_total) : absent;
+      a.indices[r * a.k + i] = there ? index_at(place) : -1;
+    }
+    if (lane == 0) a.log_rest[r] = rest_there ? float(gap + log_of(rest) - log_total) : absent;
+  } else {
+    const Controls c(a, r);
+    const bool bad = nan || !(c.temperature >= 0), greedy = c.temperature == 0;
+    const Weights weight(top, greedy || bad ? 1.0 : c.temperature, a.scale);
+    const uint64_t w = weight(z), upto = lanes.running_sum(w), before = upto - w;
+    uint64_t kept = lanes.at(upto, (c.most > 0 && c.most < G ? int(c.most) : G) - 1);
+    if (c.p < 1) {
+      const uint64_t limit = c.limit(kept);
+      kept = min(kept, lanes.at(upto, max(lanes.count(before < limit), 1) - 1));
+    }
+    const uint64_t bound = c.bound();
+    if (bound > 1) kept = min(kept, lanes.at(upto, max(lanes.count(w >= bound), 1) - 1));
+    if (c.least > 1) kept = c.one;
+    const uint64_t sum = c.target(kept);
+    const bool chosen = bad || none || greedy ? lane == 0 : before < sum && sum <= upto;
+    if (!in || !chosen) return;
+    a.actions[r] = bad || none ? -1 : index_at(place);
+    a.log_probs[r] = bad ? NAN : none || greedy ? 0.f : c.log_share(z, top, kept, a.scale);
+  }
 }
 
 // ---- kernels -------------------------------------------------------------------------------------------------------
@@ -955,8 +1063,18 @@ Launch launch_as() {
   return {choose_kernel<T, G, BYTES, RECORD>, G > 256 ? 1 : 256 / G, G > 256 ? G : 256};
 }
 
+template <typename T, int G, bool RECORD>
+Launch narrow_as() {
+  return {narrow_kernel<T, G, RECORD>, 256 / G, 256};
+}
+
 template <typename T, bool RECORD>
 Launch launch_of(int width) {
+  if (width <= 4) return narrow_as<T, 4, RECORD>();
+  if (width <= 8) return narrow_as<T, 8, RECORD>();
+  if (width <= 16) return narrow_as<T, 16, RECORD>();
+  if (width <= 32) return narrow_as<T, 32, RECORD>();
+  if (width <= 64) return narrow_as<T, 64, RECORD>();
   const int bytes = width * int(sizeof(T));
   if (bytes <= 2048) return launch_as<T, 64, 2048, RECORD>();
   if (bytes <= 16384) return launch_as<T, 256, 16384, RECORD>();
