@@ -501,7 +501,7 @@ struct Bins {
     low = -INFINITY, high = INFINITY;
     if (scale == 0) return;
     const float near = float(b) * width, far = float(b + 1) * width;
-    const float slack = 9 * 0x1p-24f * (fabsf(from) + far);
+    const float slack = 9 * 0x1p-24f * (fabsf(from) + far) + 0x1p-146f;
     high = from - near + slack;
     if (float(b) < last) low = from - far - slack;
   }
@@ -866,16 +866,20 @@ __device__ __forceinline__ void top_row(const ChooseArgs &a, int64_t r, Row &row
     n = gather(row, group, [&](float z, int i) { return z > under || (z == under && i <= index); });
     if (index >= 0) under = below(under);
   }
-  const Mine<G> list(group, n, one);
+  // Into the order, whatever the order in which they came: sums go by it.
+  {
+    const Mine<G> list(group, n, one);
+    group.sync();
+#pragma unroll
+    for (int i = 0; i < Mine<G>::N; ++i)
+      if (list.in[i]) s.list[list.rank[i]] = list.item[i];
+    group.sync();
+  }
   const int held = min(n, a.k);
   // The others: those behind in the list, those not in it, and ties; `next` is their largest.
   float next;
   if (n > a.k) {
-#pragma unroll
-    for (int i = 0; i < Mine<G>::N; ++i)
-      if (list.in[i] && list.rank[i] == a.k) s.found[0] = list.item[i].key;
-    group.sync();
-    next = value_at(s.found[0]);
+    next = value_at(s.list[a.k].key);
   } else if (ties > 0) {
     next = of_key(key_of(under) + 1);
   } else {
@@ -886,36 +890,30 @@ __device__ __forceinline__ void top_row(const ChooseArgs &a, int64_t r, Row &row
     });
     next = group.join(next, Most{});
   }
-  const float base = next > -INFINITY ? next : 0.f;
-  const Share weigh(base, inverse);
-  double sums[2] = {0, 0};  // of the others, and of the record
+  const Share weigh(next > -INFINITY ? next : 0.f, inverse);
+  double others = 0, record = 0;
   row.each([&](int, const auto &z) {
     float sum = 0;
 #pragma unroll
     for (int k = 0; k < Row::V; ++k) sum += z(k) <= under ? weigh(z(k)) : 0.f;
-    sums[0] += sum;
+    others += sum;
   });
-  if (lane == 0) sums[0] += ties;  // (the largest of the others, where there are any)
-#pragma unroll
-  for (int i = 0; i < Mine<G>::N; ++i) {
-    if (!list.in[i]) continue;
-    const float z = value_at(list.item[i].key);
-    if (list.rank[i] < a.k)
-      sums[1] += exp_of((double(z) - double(top)) * inverse);
+  if (lane == 0) others += ties;  // (the largest of the others, where there are any)
+  for (int i = lane; i < n; i += G) {
+    const float z = value_at(s.list[i].key);
+    if (i < a.k)
+      record += exp_of((double(z) - double(top)) * inverse);
     else
-      sums[0] += weigh(z);
+      others += weigh(z);
   }
-  const double rest = group.join(sums[0], Add{}), held_sum = group.join(sums[1], Add{});
-  const double gap = (double(base) - double(top)) * inverse;
+  const double rest = group.join(others, Add{}), held_sum = group.join(record, Add{});
+  const double gap = (double(weigh.base) - double(top)) * inverse;
   const double log_total = log_of(held_sum + (rest > 0 ? rest * exp_of(gap) : 0.0));
-#pragma unroll
-  for (int i = 0; i < Mine<G>::N; ++i) {
-    if (!list.in[i] || list.rank[i] >= a.k) continue;
-    const float z = value_at(list.item[i].key);
-    log_probs[list.rank[i]] = float((double(z) - double(top)) * inverse - log_total);
-    indices[list.rank[i]] = index_at(list.item[i].key);
+  for (int i = lane; i < a.k; i += G) {
+    const uint64_t place = i < held ? s.list[i].key : 0;
+    log_probs[i] = i < held ? float((double(value_at(place)) - double(top)) * inverse - log_total) : -INFINITY;
+    indices[i] = i < held ? index_at(place) : -1;
   }
-  for (int i = held + lane; i < a.k; i += G) log_probs[i] = -INFINITY, indices[i] = -1;
   if (lane == 0) a.log_rest[r] = rest > 0 ? float(gap + log_of(rest) - log_total) : -INFINITY;
 }
 
@@ -1088,7 +1086,9 @@ void launch(const ChooseArgs &a, int dtype, hipStream_t stream) {
   const Launch l = dtype == CG_F32    ? launch_of<float, RECORD>(a.width)
                    : dtype == CG_BF16 ? launch_of<bf16, RECORD>(a.width)
                                       : launch_of<f16, RECORD>(a.width);
-  l.kernel<<<unsigned((int64_t(a.rows) + l.rows - 1) / l.rows), l.threads, 0, stream>>>(a);
+  const int64_t blocks = (int64_t(a.rows) + l.rows - 1) / l.rows;
+  CG_REQUIRE(blocks * l.threads < int64_t(1) << 32, CG_ERR_UNSUPPORTED, "more rows than a launch has threads for");
+  l.kernel<<<unsigned(blocks), l.threads, 0, stream>>>(a);
   CG_LAUNCHED();
 }
 

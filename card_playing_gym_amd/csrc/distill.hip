@@ -23,10 +23,10 @@ namespace {
 
 constexpr int MAX_WIDTH = 1 << 18;
 constexpr int MAX_TOP = 256;
+// Logits and gradient of this many bytes go past the caches (256 MB of Infinity Cache); below, whatever made the logits
+// or takes the gradient may find them there.  us kept and past them: fp32 2048 x 32768 163 and 139, bf16 4096 x 32768, whose
+// time is arithmetic, even.
 constexpr int64_t STREAM_BYTES = 512 << 20;
-#ifndef WV
-#define WV 4
-#endif
 
 struct DistillArgs {
   const void *logits;
@@ -261,7 +261,7 @@ __device__ __forceinline__ void distill_row(const DistillArgs &a, int64_t r, int
       store_entries<V>(grad, g, i, a.width, inside, G >= 512 && a.streams);
     });
   }
-  if constexpr (G > 64) __syncthreads();  // (the zeros just written at R's entries come first)
+  group_sync<G>();  // (the zeros just written at R's entries come first)
   if (in && o.live) {
     record.each([&](int i, float log_q, float z) {
       if (z == -INFINITY) return;
@@ -278,7 +278,7 @@ __device__ __forceinline__ void distill_row(const DistillArgs &a, int64_t r, int
 
 // S: the type in which entries are kept (T, or float where rows are shorter than a load).
 template <typename T, int G, int E, typename S = T>
-__global__ __launch_bounds__((G > 256 ? G : 256), (G >= 1024 ? 4 : G >= 64 ? WV : 4)) void rows_kernel(const DistillArgs a) {
+__global__ __launch_bounds__((G > 256 ? G : 256), 4) void rows_kernel(const DistillArgs a) {
   constexpr int V = E == 1 ? 1 : VEC<T>, C = E / V, THREADS = G > 256 ? G : 256, ROWS = THREADS / G;
   if (done(a)) return;
   __shared__ Slots<G> slots;
@@ -400,7 +400,9 @@ int64_t blocks_of(const cg_policy_rows &p) {
 
 void launch_rows(const DistillArgs &a, const cg_policy_rows &p, hipStream_t stream) {
   const Launch l = launch_of(p);
-  l.kernel<<<unsigned(blocks_of(p)), l.threads, 0, stream>>>(a);
+  const int64_t blocks = blocks_of(p);
+  CG_REQUIRE(blocks * l.threads < int64_t(1) << 32, CG_ERR_UNSUPPORTED, "more rows than a launch has threads for");
+  l.kernel<<<unsigned(blocks), l.threads, 0, stream>>>(a);
   CG_LAUNCHED();
 }
 
@@ -427,11 +429,7 @@ DistillArgs args_of(const cg_distill_loss *loss) {
   if (double(a.fast) >= c) a.fast = nextafterf(a.fast, 0.f);
   a.slow = float(c - double(a.fast));
   a.normalizer = scalar(p.normalizer);
-#ifdef NOSTREAM
-  a.streams = 0;
-#else
   a.streams = int64_t(q.rows) * q.width >= STREAM_BYTES / (2 * dtype_size(q.dtype));
-#endif
   return a;
 }
 

@@ -265,3 +265,42 @@ def test_sampled_shares_are_the_policys(device):
     also = share(sample_rows(p.repeat(n, 1), mask.repeat(n, 1), u))
     # an entry's share of n evenly spread uniforms is off by one of them at most
     assert ((got - p[0].double()).abs() <= 1.0 / n + 40 * U).all() and ((also - p[0].double()).abs() <= 1.0 / n + 40 * U).all()
+
+
+def test_more_entries_than_32_bits_count(device):
+    """The last rows of a table of more than 2^31 entries are those of a table of their own."""
+
+    rows, width = 70000, 31000
+    logits = torch.empty(rows, width, dtype=torch.bfloat16, device=device)
+    for first in range(0, rows, 10000):
+        logits[first : first + 10000].normal_()
+    u = torch.rand(rows, dtype=torch.float64, device=device)
+    out, record = sample_logits(logits, u, top_p=0.9), top_logits(logits, 10)
+    for few in (slice(0, 5), slice(rows - 5, rows)):
+        want, held = sample_logits(logits[few].clone(), u[few], top_p=0.9), top_logits(logits[few].clone(), 10)
+        assert torch.equal(out.actions[few], want.actions) and torch.equal(out.log_probs[few], want.log_probs)
+        assert all(torch.equal(a[few], b) for a, b in zip(record, held))
+
+
+@pytest.mark.parametrize("width", [30, 400, 3000, 40000, 80000])
+def test_records_are_the_same_every_time(device, width):
+    """Entries come into a list in any order; the sums go by their order in the row."""
+
+    logits = torch.randn(64, width, device=device)
+    first = top_logits(logits, 50)
+    for _ in range(20):
+        assert all(torch.equal(a, b) for a, b in zip(top_logits(logits, 50), first))
+
+
+@pytest.mark.parametrize("width", [9, 300, 20000])
+def test_temperatures_without_end(device, width):
+    """An infinite temperature is uniform over what is legal, the least above 0 the largest entry."""
+
+    logits, mask, u = make(device, 40, width, torch.float32, 21)
+    hot = sample_logits(logits, u, mask=mask, temperature=torch.full((40,), float("inf"), device=device))
+    order = torch.sort(logits.masked_fill(~mask, -float("inf")), dim=1, descending=True, stable=True).indices
+    n = mask.sum(1)
+    assert torch.equal(hot.actions, order.gather(1, (u * n).long()[:, None])[:, 0])
+    torch.testing.assert_close(hot.log_probs.double(), -n.double().log(), rtol=U, atol=1e-9)
+    cold = sample_logits(logits, u, mask=mask, temperature=torch.full((40,), 2.0**-149, device=device))
+    assert torch.equal(cold.actions, order[:, 0]) and (cold.log_probs == 0).all()

@@ -386,3 +386,17 @@ def test_a_policy_learns_another_through_its_record(device):
     (learned.loss + acted.loss).backward()
     optimizer.step()
     assert all(p.grad is not None and p.grad.isfinite().all() for p in [*trunk.parameters(), *head.parameters()])
+
+
+def test_more_entries_than_32_bits_count(device):
+    rows, width = 70000, 31000
+    logits = torch.empty(rows, width, dtype=torch.bfloat16, device=device)
+    for first in range(0, rows, 10000):
+        logits[first : first + 10000].normal_()
+    indices = torch.arange(8, device=device).expand(rows, 8) * 3000 + torch.arange(rows, device=device)[:, None] % 3000
+    log_probs = torch.full((rows, 8), -3.0, device=device)
+    log_rest = torch.full((rows,), -0.5, device=device)
+    out, grad = run(logits, indices, log_probs, {"log_rest": log_rest, "normalizer": 1.0})
+    few = slice(rows - 5, rows)
+    want, want_grad = run(logits[few].clone(), indices[few], log_probs[few], {"log_rest": log_rest[few], "normalizer": 1.0})
+    assert torch.equal(out.kl[few], want.kl) and torch.equal(grad[few], want_grad)
