@@ -96,11 +96,15 @@ struct Item {
 template <int G>
 struct Shared {
   static constexpr int W = G > 64 ? G / 64 : 1;
-  static constexpr int BINS = G > 64 ? 1024 : 256, LIST = G > 64 ? 512 : 256;
+  static constexpr int BINS = G > 64 ? 1024 : 256, LIST = G > 64 ? 512 : 256, JOINED = G > 256 ? LIST : 0;
   uint64_t slots[2][W];
   union {  // (the bins are in registers when a list is made)
     uint64_t bins[BINS];
-    Item list[LIST];
+    struct {
+      Item list[LIST];
+      uint64_t before[JOINED > 0 ? JOINED : 1];
+      int rank[JOINED > 0 ? JOINED : 1];
+    };
   };
   uint64_t found[2];
   int count;
@@ -169,9 +173,21 @@ struct Group {
 
 // The vector from entry i on, -inf for those that are not legal; a row's last one is its last V entries, of which those
 // that the one before has count as -inf.
-template <typename T, int V = VEC<T>>
-__device__ __forceinline__ void load_vector(uint32_t (&w)[4], const T *row, const uint8_t *legal, int i, int width) {
-  if (i + V <= width) {
+template <typename T, int V>
+__device__ __forceinline__ void load_vector(uint32_t *w, const T *row, const uint8_t *legal, int i, int width) {
+  if constexpr (V == 2) {
+    const int at = min(i, width - 2);
+    const bool first = at == i && (!legal || legal[at]), second = !legal || legal[at + 1];
+    __builtin_memcpy(w, row + at, 2 * sizeof(T));
+    constexpr uint32_t NONE = NEGATIVE_INFINITY<T>;
+    if constexpr (sizeof(T) == 4) {
+      w[0] = first ? w[0] : NONE;
+      w[1] = second ? w[1] : NONE;
+    } else {
+      w[0] = first ? w[0] : (w[0] & 0xffff0000u) | (NONE & 0xffffu);
+      w[0] = second ? w[0] : (w[0] & 0xffffu) | (NONE & 0xffff0000u);
+    }
+  } else if (i + V <= width) {
     __builtin_memcpy(w, row + i, 16);
     if (legal) {
       uint32_t b[V / 4];
@@ -184,11 +200,14 @@ __device__ __forceinline__ void load_vector(uint32_t (&w)[4], const T *row, cons
   }
 }
 
+// Vectors are 16 bytes, or two entries where rows have fewer bytes than 16 for each lane: us a pass with either, bf16
+// 32768 x 256 (the 32 largest) 163 and 54, 65536 x 77 (top_p) 121 and 107, but 16384 x 1000 (masked) 37 and 57.
 template <typename T, int G, int BYTES>
 struct InLds {
-  static constexpr int V = VEC<T>, VECTORS = BYTES / 16, BATCH = VECTORS / G < 8 ? VECTORS / G : 8;
-  struct alignas(16) Vector {
-    uint32_t w[4];
+  static constexpr int V = BYTES > 16 * G ? VEC<T> : 2, SIZE = V * int(sizeof(T)), VECTORS = BYTES / SIZE;
+  static constexpr int BATCH = VECTORS / G < 8 ? VECTORS / G : 8;
+  struct alignas(SIZE) Vector {
+    uint32_t w[SIZE / 4];
   };
   Vector *held;
   int width, vectors;
@@ -196,12 +215,12 @@ struct InLds {
       : held(held), width(width), vectors((width + V - 1) / V) {
     const int lane = threadIdx.x % G;
     for (int first = lane; first < vectors; first += G * BATCH) {
-      uint32_t w[BATCH][4];
+      uint32_t w[BATCH][SIZE / 4];
 #pragma unroll
-      for (int c = 0; c < BATCH; ++c) load_vector(w[c], row, legal, min(first + c * G, vectors - 1) * V, width);
+      for (int c = 0; c < BATCH; ++c) load_vector<T, V>(w[c], row, legal, min(first + c * G, vectors - 1) * V, width);
 #pragma unroll
       for (int c = 0; c < BATCH; ++c)
-        if (first + c * G < vectors) __builtin_memcpy(&held[first + c * G], w[c], 16);
+        if (first + c * G < vectors) __builtin_memcpy(&held[first + c * G], w[c], SIZE);
     }
   }
   __device__ __forceinline__ int at(int j) const { return min(j * V, width - V); }
@@ -210,7 +229,7 @@ struct InLds {
 #pragma unroll 1
     for (int j = threadIdx.x % G; j < vectors; j += G) {
       Entries<T, V> q;
-      __builtin_memcpy(q.w, &held[j], 16);
+      __builtin_memcpy(q.w, &held[j], SIZE);
       visit(at(j), [&](int k) { return q[k]; });
     }
   }
@@ -218,14 +237,14 @@ struct InLds {
   __device__ __forceinline__ void unbounded() {
     for (int j = threadIdx.x % G; j < vectors; j += G) {
       Entries<T, V> q;
-      __builtin_memcpy(q.w, &held[j], 16);
+      __builtin_memcpy(q.w, &held[j], SIZE);
 #pragma unroll
       for (int k = 0; k < V; ++k) {
         const uint32_t part = sizeof(T) == 4 ? ~0u : k % 2 ? 0xffff0000u : 0xffffu;
         uint32_t &w = q.w[k / Entries<T, V>::PER];
         w = (w & ~part) | (q[k] == INFINITY ? 0u : NEGATIVE_INFINITY<T> & part);
       }
-      __builtin_memcpy(&held[j], q.w, 16);
+      __builtin_memcpy(&held[j], q.w, SIZE);
     }
   }
 };
@@ -244,7 +263,7 @@ struct Read {
     for (int first = threadIdx.x % G; first < vectors; first += G * BATCH) {
       Entries<T, V> q[BATCH];
 #pragma unroll
-      for (int c = 0; c < BATCH; ++c) load_vector(q[c].w, row, legal, min(first + c * G, vectors - 1) * V, width);
+      for (int c = 0; c < BATCH; ++c) load_vector<T, V>(q[c].w, row, legal, min(first + c * G, vectors - 1) * V, width);
 #pragma unroll
       for (int c = 0; c < BATCH; ++c)
         if (first + c * G < vectors) {
@@ -418,6 +437,21 @@ __device__ __forceinline__ float bound_of_top(Group<G> &group, float top, float 
 template <typename Row, int G, typename In>
 __device__ __forceinline__ int gather(const Row &row, Group<G> &group, const In &in) {
   Shared<G> &s = group.shared;
+  if constexpr (G == 64) {  // (a wave counts for itself)
+    int n = 0;
+    row.each([&](int at, const auto &z) {
+#pragma unroll
+      for (int k = 0; k < Row::V; ++k) {
+        const bool is = in(z(k), at + k);
+        const uint64_t all = __ballot(is);
+        const int slot = n + __builtin_amdgcn_mbcnt_hi(uint32_t(all >> 32), __builtin_amdgcn_mbcnt_lo(uint32_t(all), 0));
+        if (is && slot < Shared<G>::LIST) s.list[slot].key = place_of(z(k), at + k);
+        n += __popcll(all);
+      }
+    });
+    group.sync();
+    return __builtin_amdgcn_readfirstlane(n);  // (lane 0 takes every turn that any takes)
+  }
   if (group.lane() == 0) s.count = 0;
   group.sync();
   row.each([&](int at, const auto &z) {
@@ -432,7 +466,9 @@ __device__ __forceinline__ int gather(const Row &row, Group<G> &group, const In 
   return s.count;
 }
 
-// This lane's items of a list, their weights (weight(z)), and what stands before each.
+// This lane's items of a list, their weights (weight(z)), and what stands before each.  In blocks of 512 lanes and more
+// every wave adds up a part of the list for all of its items: the one or two waves that have them would be waited for
+// (bf16 4096 x 32768 by top_p 216 and 207 us).  In narrower ones the room that the joining takes is worth more.
 template <int G>
 struct Mine {
   static constexpr int N = Shared<G>::LIST / G > 0 ? Shared<G>::LIST / G : 1;
@@ -453,27 +489,49 @@ struct Mine {
       if (in[i]) {
         item[i].key = s.list[at].key;
         s.list[at].weight = item[i].weight = weight(value_at(item[i].key));
+        if constexpr (Shared<G>::JOINED > 0) s.before[at] = 0, s.rank[at] = 0;
       }
     }
     group.sync();
-    if (n <= G)
-      add_up<1>(s, n);
-    else if (n <= 2 * G)
-      add_up<(N < 2 ? N : 2)>(s, n);
-    else
-      add_up<N>(s, n);
+    if constexpr (Shared<G>::JOINED > 0) {
+      constexpr int W = G / 64;
+      const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), first = n * wave / W, last = n * (wave + 1) / W;
+      for (int at = threadIdx.x & 63; at < n; at += 64) {
+        const uint64_t key[1] = {s.list[at].key};
+        uint64_t sum[1] = {0};
+        int ahead[1] = {0};
+        add_up<1>(s, key, first, last, sum, ahead);
+        atomicAdd(reinterpret_cast<unsigned long long *>(&s.before[at]), sum[0]);
+        atomicAdd(&s.rank[at], ahead[0]);
+      }
+      group.sync();
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (in[i]) before[i] = s.before[group.lane() + i * G], rank[i] = s.rank[group.lane() + i * G];
+    } else {
+      if (int(threadIdx.x % G) / 64 * 64 >= n) return;  // (waves without items)
+      uint64_t key[N];
+#pragma unroll
+      for (int i = 0; i < N; ++i) key[i] = item[i].key;
+      if (n <= G)
+        add_up<1>(s, key, 0, n, before, rank);
+      else if (n <= 2 * G)
+        add_up<(N < 2 ? N : 2)>(s, key, 0, n, before, rank);
+      else
+        add_up<N>(s, key, 0, n, before, rank);
+    }
   }
   template <int USED>
-  __device__ __forceinline__ void add_up(const Shared<G> &s, int n) {
-    if (int(threadIdx.x % G) / 64 * 64 >= n) return;  // (waves without items)
+  static __device__ __forceinline__ void add_up(const Shared<G> &s, const uint64_t *key, int first, int last, uint64_t *sum,
+                                                int *count) {
 #pragma unroll 4
-    for (int j = 0; j < n; ++j) {
+    for (int j = first; j < last; ++j) {
       const Item other = s.list[j];
 #pragma unroll
       for (int i = 0; i < USED; ++i) {
-        const bool ahead = other.key > item[i].key;
-        before[i] += ahead ? other.weight : 0;
-        rank[i] += ahead;
+        const bool ahead = other.key > key[i];
+        sum[i] += ahead ? other.weight : 0;
+        count[i] += ahead;
       }
     }
   }
@@ -1074,6 +1132,7 @@ Launch launch_of(int width) {
   if (width <= 32) return narrow_as<T, 32, RECORD>();
   if (width <= 64) return narrow_as<T, 64, RECORD>();
   const int bytes = width * int(sizeof(T));
+  if (bytes < 1024) return launch_as<T, 64, 1024, RECORD>();
   if (bytes <= 2048) return launch_as<T, 64, 2048, RECORD>();
   if (bytes <= 16384) return launch_as<T, 256, 16384, RECORD>();
   if (bytes <= 65536) return launch_as<T, 512, 65536, RECORD>();

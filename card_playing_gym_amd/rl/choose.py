@@ -50,17 +50,17 @@ def _policy_rows(logits: torch.Tensor, mask: torch.Tensor | None) -> tuple[nat.P
         raise ValueError("logits must be [rows, width] with at least one entry a row")
     require_device(logits)
     dtype = dtype_code(logits.dtype)
-    rows, width = logits.shape
+    rows, width = shape = logits.shape
     if rows >= 2**31 or width > MAX_WIDTH:
         raise ValueError(f"logits may have up to 2^31 - 1 rows of up to {MAX_WIDTH} entries")
     logits = _entries(logits)
-    if mask is not None:
-        if mask.shape != logits.shape or mask.dtype != torch.bool or mask.device != logits.device:
-            raise ValueError("mask must be bool [rows, width] on the logits' device")
-        mask = _entries(mask)
-    descriptor = nat.PolicyRows(logits.data_ptr(), None if mask is None else mask.data_ptr(), logits.stride(0),
-                                0 if mask is None else mask.stride(0), rows, width, dtype)
-    return descriptor, (logits, mask)
+    if mask is None:
+        return nat.PolicyRows(logits.data_ptr(), None, logits.stride(0), 0, rows, width, dtype), (logits, None)
+    if mask.shape != shape or mask.dtype != torch.bool or mask.device != logits.device:
+        raise ValueError("mask must be bool [rows, width] on the logits' device")
+    mask = _entries(mask)
+    return (nat.PolicyRows(logits.data_ptr(), mask.data_ptr(), logits.stride(0), mask.stride(0), rows, width, dtype),
+            (logits, mask))
 
 
 def _control(x, name: str, none, dtype: torch.dtype, rows: int, device) -> tuple:
