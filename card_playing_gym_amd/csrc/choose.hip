@@ -17,7 +17,8 @@
 // Finding that entry, or the k-th: a histogram of the row's weights (or of ones) in LDS, over bins of equal width in z, says
 // which bin the place falls into and what is summed up before it.  The entries of that bin, a few dozen, go into a
 // list, where each one adds up what stands before it.  A bin of more entries than the list has room for is cut into
-// bins again, between its least and its largest entry; one of equal entries is decided by halving the range of their indices.
+// bins again, between its least and its largest entry; one of equal entries is decided by halving the range of their indices
+// (and one of entries that differ by less than 1e-38 by halving the range of their values before).
 // The first k of a row with k up to the lanes of its group need no histogram: at least k entries are as large as the k-th
 // largest of the lanes' own maxima, and not many more, so these are the list.
 //
@@ -214,13 +215,19 @@ struct InLds {
   __device__ __forceinline__ InLds(Vector *held, const T *row, const uint8_t *legal, int width)
       : held(held), width(width), vectors((width + V - 1) / V) {
     const int lane = threadIdx.x % G;
-    for (int first = lane; first < vectors; first += G * BATCH) {
+    for (int first = 0; first < vectors; first += G * BATCH) {
       uint32_t w[BATCH][SIZE / 4];
 #pragma unroll
-      for (int c = 0; c < BATCH; ++c) load_vector<T, V>(w[c], row, legal, min(first + c * G, vectors - 1) * V, width);
+      for (int c = 0; c < BATCH; ++c) {
+        const int from = first + c * G;  // (the same for all lanes, as is whether all of theirs are whole)
+        if (!legal && (from + G) * V <= width)
+          __builtin_memcpy(w[c], row + int64_t(from) * V + lane * V, SIZE);
+        else
+          load_vector<T, V>(w[c], row, legal, min(from + lane, vectors - 1) * V, width);
+      }
 #pragma unroll
       for (int c = 0; c < BATCH; ++c)
-        if (first + c * G < vectors) __builtin_memcpy(&held[first + c * G], w[c], SIZE);
+        if (first + c * G + lane < vectors) __builtin_memcpy(&held[first + c * G + lane], w[c], SIZE);
     }
   }
   __device__ __forceinline__ int at(int j) const { return min(j * V, width - V); }
@@ -540,7 +547,7 @@ struct Mine {
 // ---- the entry at a place of the running sum over the order ------------------------------------------------------
 
 // Bins of equal width from `from` downwards, the last one for all below (and what float32 cannot tell from there).  A
-// range of one value is one bin; of any other, its ends are in different ones.
+// range of one value is one bin; of any other, its ends are in different ones, unless it is shorter than 1 / 1e38.
 struct Bins {
   float from, scale, last, width;
   Bins() = default;
@@ -691,9 +698,29 @@ struct Histogram {
       });
       lowest = group.join(lowest, Least{});
       largest = group.join(largest, Largest{});
-      if (lowest == largest) {  // equal entries
-        const uint64_t w = weight.near(lowest), r = (sum - 1 - ahead) / w;
-        return Entry{place_of(lowest, tie(row, group, lowest, int(r))), ahead + (r + 1) * w};
+      if (Bins(largest, lowest, Shared<G>::BINS).at(lowest) < 1) {
+        // Equal entries, or closer to each other than float32's reciprocals reach (numbers below its least normal one):
+        // the value by halving its range, `over` the sum of those above, then the entry by halving the indices.
+        uint32_t lo = key_of(lowest), hi = key_of(largest);
+        uint64_t over = 0;
+        while (lo < hi) {
+          const uint32_t mid = hi - (hi - lo) / 2;
+          uint64_t x = 0;
+          row.each([&](int, const auto &z) {
+#pragma unroll
+            for (int k = 0; k < Row::V; ++k)
+              if (z(k) <= largest && key_of(z(k)) >= mid) x += weight.near(z(k));
+          });
+          x = group.join(x, Plus{});
+          if (x >= sum - ahead)
+            lo = mid;
+          else
+            hi = mid - 1, over = x;
+        }
+        ahead += over;
+        const float v = of_key(lo);
+        const uint64_t w = weight.near(v), r = (sum - 1 - ahead) / w;
+        return Entry{place_of(v, tie(row, group, v, int(r))), ahead + (r + 1) * w};
       }
       h.template make<true>(row, group, weight, largest, lowest, lowest);
     }

@@ -189,6 +189,26 @@ def test_top_of_rows_that_crowd(device, width, how):
             check_sample(logits, torch.tensor([0.111, 0.5234, 0.901], dtype=torch.float64, device=device), None, **controls)
 
 
+@pytest.mark.parametrize("width", [300, 3000, 33000, 70000])
+@pytest.mark.parametrize("step", [2.0**-149, 2.0**-137])
+def test_entries_that_differ_by_less_than_normal_numbers(device, width, step):
+    """More of them than a list holds, closer to each other than bins can be; of one weight, or (a temperature of
+    their size) of different ones."""
+
+    rng = np.random.default_rng(width)
+    z = torch.from_numpy(rng.integers(-300, 300, (3, width)) * step).float().to(device)
+    # (equal weights: borders between actions are whole multiples of 1 / width, which no root is)
+    u = torch.tensor([0.013, 0.27, 0.83], dtype=torch.float64, device=device).sqrt()
+    for high in (False, True):  # (alone, or behind some that are far above)
+        logits = z.clone()
+        if high:
+            logits[:, 3:8] = 5.0
+        for k in (20, 100, 256):
+            check_top(logits, k, None)
+        for controls in ({}, {"top_k": 280}, {"top_p": 0.38**0.5}, {"top_k": 290, "temperature": 100 * step}):
+            check_sample(logits, u, None, **controls)
+
+
 def test_a_rest_far_below_one_keeps_its_digits(device):
     logits = torch.tensor([[0.0, -80.0, -81.0, 0.5]], device=device)
     out = top_logits(logits, 2, temperature=0.25)
