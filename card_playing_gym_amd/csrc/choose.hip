@@ -440,9 +440,9 @@ __device__ __forceinline__ float bound_of_top(Group<G> &group, float top, float 
 }
 
 // The entries for which in(z, index) holds into the list.  Returns how many there are, of which those past the list's
-// room are not in it.
-template <typename Row, int G, typename In>
-__device__ __forceinline__ int gather(const Row &row, Group<G> &group, const In &in) {
+// room are not in it.  after(): behind each of this lane's vectors.
+template <typename Row, int G, typename In, typename After>
+__device__ __forceinline__ int gather(const Row &row, Group<G> &group, const In &in, const After &after) {
   Shared<G> &s = group.shared;
   if constexpr (G == 64) {  // (a wave counts for itself)
     int n = 0;
@@ -455,6 +455,7 @@ __device__ __forceinline__ int gather(const Row &row, Group<G> &group, const In 
         if (is && slot < Shared<G>::LIST) s.list[slot].key = place_of(z(k), at + k);
         n += __popcll(all);
       }
+      after();
     });
     group.sync();
     return __builtin_amdgcn_readfirstlane(n);  // (lane 0 takes every turn that any takes)
@@ -468,9 +469,14 @@ __device__ __forceinline__ int gather(const Row &row, Group<G> &group, const In 
       const int slot = atomicAdd(&s.count, 1);
       if (slot < Shared<G>::LIST) s.list[slot].key = place_of(z(k), at + k);
     }
+    after();
   });
   group.sync();
   return s.count;
+}
+template <typename Row, int G, typename In>
+__device__ __forceinline__ int gather(const Row &row, Group<G> &group, const In &in) {
+  return gather(row, group, in, [] {});
 }
 
 // This lane's items of a list, their weights (weight(z)), and what stands before each.  In blocks of 512 lanes and more
@@ -929,10 +935,20 @@ __device__ __forceinline__ void top_row(const ChooseArgs &a, int64_t r, Row &row
   const One one;
   float under = -INFINITY;
   int index = -1, n = Shared<G>::LIST + 1;
+  double low = 0;  // those not in the list, from `under`
   if (a.k >= a.width || a.k <= SHORT<G>) {
     // (one more, where the lanes suffice: the largest of the others)
     if (a.k < a.width) under = below(bound_of_top(group, top, mine, min(a.k + 1, G)));
-    n = gather(row, group, [&](float z, int) { return z > under; });
+    const Share weigh(under > -INFINITY ? under : 0.f, inverse);
+    float sum = 0;
+    n = gather(
+        row, group,
+        [&](float z, int) {
+          const bool is = z > under;
+          sum += is ? 0.f : weigh(z);
+          return is;
+        },
+        [&] { low += sum, sum = 0; });
   }
   int ties = 0;  // of the others, those equal to the k-th
   if (n > Shared<G>::LIST) {
@@ -961,7 +977,9 @@ __device__ __forceinline__ void top_row(const ChooseArgs &a, int64_t r, Row &row
     group.sync();
   }
   const int held = min(n, a.k);
-  // The others: those behind in the list, those not in it, and ties; `next` is their largest.
+  // The others: those behind in the list, those not in it, and ties; `next` is their largest.  Where it is in the list,
+  // those not in it were summed up while it was made, measured from `under`: one that is lost so far below is nothing beside
+  // `next`.
   float next;
   if (n > a.k) {
     next = value_at(s.list[a.k].key);
@@ -977,12 +995,16 @@ __device__ __forceinline__ void top_row(const ChooseArgs &a, int64_t r, Row &row
   }
   const Share weigh(next > -INFINITY ? next : 0.f, inverse);
   double others = 0, record = 0;
-  row.each([&](int, const auto &z) {
-    float sum = 0;
+  if (n > a.k) {
+    others = low > 0 ? low * exp_of((double(under) - double(next)) * inverse) : 0;
+  } else {
+    row.each([&](int, const auto &z) {
+      float sum = 0;
 #pragma unroll
-    for (int k = 0; k < Row::V; ++k) sum += z(k) <= under ? weigh(z(k)) : 0.f;
-    others += sum;
-  });
+      for (int k = 0; k < Row::V; ++k) sum += z(k) <= under ? weigh(z(k)) : 0.f;
+      others += sum;
+    });
+  }
   if (lane == 0) others += ties;  // (the largest of the others, where there are any)
   for (int i = lane; i < n; i += G) {
     const float z = value_at(s.list[i].key);
@@ -1151,6 +1173,12 @@ Launch narrow_as() {
   return {narrow_kernel<T, G, RECORD>, 256 / G, 256};
 }
 
+// The fewest lanes and the least LDS that a row fits: us as chosen and by the next one (no filter, top_p, the 8 largest),
+//   131072 x 4 bf16       7.6   8.2   9.0 and  11.8  12.6  11.2     32768 x 1024 bf16  70  93  56 and 189 236 166
+//   131072 x 16 fp32       21    22    23 and    40    42    43      8192 x 4096 fp32  70  88  47 and 123 154 130
+//   131072 x 64 bf16       92    95    98 and   164   207   164      1024 x 32768 bf16 52  64  35 and  72  86  67
+//    65536 x 256 bf16      87   114    83 and   100   129    89       910 x 36864 fp32 84 101  67 and  95 119  76
+// Rows of 640 bytes to 1 KB have two entries a lane no longer: 65536 x 160 fp32 so 87 111 81, with them 90 116 86.
 template <typename T, bool RECORD>
 Launch launch_of(int width) {
   if (width <= 4) return narrow_as<T, 4, RECORD>();
@@ -1159,7 +1187,7 @@ Launch launch_of(int width) {
   if (width <= 32) return narrow_as<T, 32, RECORD>();
   if (width <= 64) return narrow_as<T, 64, RECORD>();
   const int bytes = width * int(sizeof(T));
-  if (bytes < 1024) return launch_as<T, 64, 1024, RECORD>();
+  if (bytes < 640) return launch_as<T, 64, 640, RECORD>();
   if (bytes <= 2048) return launch_as<T, 64, 2048, RECORD>();
   if (bytes <= 16384) return launch_as<T, 256, 16384, RECORD>();
   if (bytes <= 65536) return launch_as<T, 512, 65536, RECORD>();

@@ -370,6 +370,12 @@ Launch launch_as() {
   return {rows_kernel<T, G, E, S>, G > 256 ? 1 : 256 / G, G > 256 ? G : 256};
 }
 
+// The fewest lanes that hold a row: more have less to do each in the row's joins and its record, and rows wait for both.
+// us of forward and backward as chosen and with the next more lanes, k 16 and k 32:
+//   65536 x 32 bf16  27  40 and  41  48     16384 x 2048 bf16  58  59 and 156 (k 32)     2048 x 16384 fp32 65 and 118
+//   65536 x 128 bf16 44  51 and  73  74      4096 x 8192 bf16      55 and  85            1024 x 32768 bf16 47 and  83
+//   65536 x 512 bf16 81  82 and 125 125      2048 x 16384 bf16     53 and  72             512 x 65536 bf16 54 and  60
+// (Records of nearly all of a narrow row would have more: 131072 x 32 fp32, k 32, 193 and 79.)
 template <typename T>
 Launch launch_of(int width) {
   if (width < VEC<T>) return launch_as<T, 8, 1, float>();

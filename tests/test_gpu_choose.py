@@ -61,6 +61,16 @@ def test_sample_is_the_definition(device, width):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("width", [65, 159, 160, 161, 319, 320, 321])
+def test_both_sides_of_640_bytes(device, width, dtype):
+    logits, mask, u = make(device, 21, width, dtype, width)
+    for controls in CONTROLS:
+        check_sample(logits, u, mask, **controls)
+        check_sample(logits, u, None, **controls)
+    check_top(logits, 40, mask)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("width", [6, 300, 5000, 66000])
 def test_every_row_has_its_own_controls(device, width, dtype):
     rows = 24
