@@ -463,13 +463,17 @@ __device__ __forceinline__ int gather(const Row &row, Group<G> &group, const In 
   if (group.lane() == 0) s.count = 0;
   group.sync();
   row.each([&](int at, const auto &z) {
+    bool is[Row::V], any = false;
+#pragma unroll
+    for (int k = 0; k < Row::V; ++k) any |= is[k] = in(z(k), at + k);
+    after();
+    if (!any) return;
 #pragma unroll
     for (int k = 0; k < Row::V; ++k) {
-      if (!in(z(k), at + k)) continue;
+      if (!is[k]) continue;
       const int slot = atomicAdd(&s.count, 1);
       if (slot < Shared<G>::LIST) s.list[slot].key = place_of(z(k), at + k);
     }
-    after();
   });
   group.sync();
   return s.count;
@@ -1132,9 +1136,10 @@ __global__ __launch_bounds__(256) void narrow_kernel(const ChooseArgs a) {
 
 // ---- kernels -------------------------------------------------------------------------------------------------------
 
-// BYTES: of LDS for a row; 0: it is read again for each pass.
+// BYTES: of LDS for a row; 0: it is read again for each pass.  The record's blocks of 256 lanes fit a SIMD six times with two
+// registers less than they would take (8192 x 2048 bf16, the 8 and 128 largest: 49 82 us, so 44 75); sampling's would spill.
 template <typename T, int G, int BYTES, bool RECORD>
-__global__ __launch_bounds__((G > 256 ? G : 256), 4) void choose_kernel(const ChooseArgs a) {
+__global__ __launch_bounds__((G > 256 ? G : 256), RECORD && G == 256 ? 6 : 4) void choose_kernel(const ChooseArgs a) {
   constexpr int ROWS = G > 256 ? 1 : 256 / G;
   __shared__ Shared<G> shared[ROWS];
   const int in_block = G < 256 ? __builtin_amdgcn_readfirstlane(threadIdx.x / G) : 0;
