@@ -239,6 +239,10 @@ def test_native_refusals():
                     {"k": 0}, {"k": 257}, {"temperature": 0.0}, {"indices": None}, {"log_probs": None}, {"upstream": 0},
                     {"upstream": 16, "grad": None}):
         assert distill(rows(), **changes) == invalid, changes
+    # A launch has fewer than 2^32 threads.
+    many = {"rows": 2**31 - 1, "width": 9000}
+    assert sample(rows(**many)) == top(rows(**many)) == distill(rows(**many), upstream=16) == unsupported
+    assert distill(rows(**many), size=1 << 40) == unsupported
     assert lib.cg_sample_logits(None, 16, None, 16, 16, None) == invalid
     assert lib.cg_sample_logits(ctypes.byref(rows()), 16, None, 16, 16, None) == invalid
     assert lib.cg_top_logits(None, 3, 1.0, 16, 16, 16, None) == invalid
