@@ -128,8 +128,8 @@ def distill_loss(
     those with weight for their mean.  It may be a float32 device scalar, which a captured loss reads at every replay.
     A backward captured in a graph of its own follows one replay of its forward's each time.
 
-    Index -1 stands for no entry.  An index outside the row, or twice in it, makes its row, and the loss, NaN.  An
-    entry with a q above 0 that is not legal here makes its row's KL infinite.  A row of weight 0 (padding) is not
+    Index -1 stands for no entry.  An index outside the row, or twice in it, makes its row, and the loss, NaN, as does
+    a legal entry that is NaN or +inf.  An entry with a q above 0 that is not legal here makes its row's KL infinite.  A row of weight 0 (padding) is not
     read: like a row without a legal entry, or (without ``log_rest``) without a record, it adds nothing, has a
     zero gradient and reports 0."""
 

@@ -627,11 +627,12 @@ int cg_policy_loss_backward(const cg_policy_loss *loss, const float *upstream, i
  * logits / temperature over a row's legal entries, q_k = exp(log_probs) over the record R and q_r =
  * exp(log_rest), p_r being p's mass outside R,
  *   KL = sum_R q_k (log q_k - log p_k) + q_r (log q_r - log p_r);
- * without log_rest, q is made to sum to 1 over R (logits / temperature will do for log_probs) and the second term is not
- * there.  The value is
- * sum_i w_i KL_i / normalizer.  Index -1: no entry.  An index outside the row, or twice in it, makes the row NaN; an entry that
- * is not legal but has a q above 0 makes its KL infinite.  A row of weight 0 is not read; it and a row without a
- * legal entry add nothing, have a zero gradient and report 0, as does, without log_rest, one whose record is empty. */
+ * without log_rest, q is made to sum to 1 over R (logits / temperature will do for log_probs) and the
+ * second term is not there.  The value is sum_i w_i KL_i / normalizer.  Index -1: no entry.  An index outside
+ * the row, or twice in it, makes the row NaN, as does a legal entry that is NaN or +inf; an entry that is
+ * not legal but has a q above 0 makes its KL infinite.  A row of weight 0 is not read; it and a row without a
+ * legal entry add nothing, have a zero gradient and report 0, as does, without log_rest, one whose record
+ * is empty. */
 typedef struct {
   cg_policy_rows rows;
   const int64_t *indices;  /* [rows, k] dense */

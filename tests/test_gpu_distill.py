@@ -184,6 +184,24 @@ def test_rows_that_do_not_count(device, width):
           {"mask": mask[good], "weights": weights[good], "log_rest": log_rest[good].nan_to_num(), "temperature": 1.0})
 
 
+@pytest.mark.parametrize("width", [5, 60, 500, 3000, 20000, 70000])
+@pytest.mark.parametrize("value", [float("inf"), float("nan")])
+def test_legal_entries_that_are_not_finite(device, width, value):
+    """In the record or outside it, they make their row NaN, and no other; in masked places they are not there."""
+
+    logits = torch.randn(4, width, device=device)
+    logits[0, 1] = logits[1, 3] = logits[2, 0] = logits[2, 4] = value
+    mask = torch.ones(4, width, dtype=torch.bool, device=device)
+    mask[2, 0] = mask[2, 4] = False
+    indices = torch.tensor([2, 1], device=device).repeat(4, 1)  # (row 0: in the record, row 1: outside)
+    log_probs, log_rest = torch.full((4, 2), -1.5, device=device), torch.full((4,), -0.6, device=device)
+    for options in ({"log_rest": log_rest}, {}):
+        out, _ = run(logits, indices, log_probs, {"mask": mask, **options})
+        assert out.kl[:2].isnan().all() and out.kl[2:].isfinite().all() and out.loss.isnan()
+        _, grad = run(logits[2:], indices[2:], log_probs[2:], {"mask": mask[2:], **{n: x[2:] for n, x in options.items()}})
+        assert grad.isfinite().all() and (grad[0, [0, 4]] == 0).all()
+
+
 def test_records_without_entries(device):
     logits = torch.randn(3, 50, device=device)
     indices = torch.full((3, 4), -1, device=device)
