@@ -172,6 +172,19 @@ struct Group {
 // each(visit): visit(index of entry 0, z) for this lane's vectors, z(k) the k-th logit, -inf where it is not legal.  A
 // lane reads what it has written: no barrier stands between.
 
+// NaN where one is.
+__device__ __forceinline__ float larger(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+
+template <typename Row>
+__device__ __forceinline__ float largest_of(const Row &row) {
+  float most = -INFINITY;
+  row.each([&](int, const auto &z) {
+#pragma unroll
+    for (int k = 0; k < Row::V; ++k) most = larger(most, z(k));
+  });
+  return most;
+}
+
 // The vector from entry i on, -inf for those that are not legal; a row's last one is its last V entries, of which those
 // that the one before has count as -inf.
 template <typename T, int V>
@@ -212,24 +225,30 @@ struct InLds {
   };
   Vector *held;
   int width, vectors;
+  float most = -INFINITY;  // of this lane's entries, as they came
   __device__ __forceinline__ InLds(Vector *held, const T *row, const uint8_t *legal, int width)
       : held(held), width(width), vectors((width + V - 1) / V) {
     const int lane = threadIdx.x % G;
     for (int first = 0; first < vectors; first += G * BATCH) {
-      uint32_t w[BATCH][SIZE / 4];
+      Entries<T, V> q[BATCH];
 #pragma unroll
       for (int c = 0; c < BATCH; ++c) {
         const int from = first + c * G;  // (the same for all lanes, as is whether all of theirs are whole)
         if (!legal && (from + G) * V <= width)
-          __builtin_memcpy(w[c], row + int64_t(from) * V + lane * V, SIZE);
+          __builtin_memcpy(q[c].w, row + int64_t(from) * V + lane * V, SIZE);
         else
-          load_vector<T, V>(w[c], row, legal, min(from + lane, vectors - 1) * V, width);
+          load_vector<T, V>(q[c].w, row, legal, min(from + lane, vectors - 1) * V, width);
       }
 #pragma unroll
       for (int c = 0; c < BATCH; ++c)
-        if (first + c * G + lane < vectors) __builtin_memcpy(&held[first + c * G + lane], w[c], SIZE);
+        if (first + c * G + lane < vectors) {
+          __builtin_memcpy(&held[first + c * G + lane], q[c].w, SIZE);
+#pragma unroll
+          for (int k = 0; k < V; ++k) most = larger(most, q[c][k]);
+        }
     }
   }
+  __device__ __forceinline__ float largest() const { return most; }
   __device__ __forceinline__ int at(int j) const { return min(j * V, width - V); }
   template <typename Visit>
   __device__ __forceinline__ void each(const Visit &visit) const {
@@ -279,6 +298,7 @@ struct Read {
         }
     }
   }
+  __device__ __forceinline__ float largest() const { return largest_of(*this); }
   __device__ __forceinline__ void unbounded() { infinite = true; }
 };
 
@@ -351,19 +371,12 @@ __device__ __forceinline__ int index_at(uint64_t place) { return int(~uint32_t(p
 // A row's largest entry, -inf where none is legal and NaN where one of them is; of this lane's entries: `mine`.
 template <typename Row, int G>
 __device__ __forceinline__ float row_top(Row &row, Group<G> &group, float &mine) {
-  const auto pass = [&] {
-    const auto larger = [](float a, float b) { return __builtin_elementwise_maximum(a, b); };  // (NaN where one is)
-    mine = -INFINITY;
-    row.each([&](int, const auto &z) {
-#pragma unroll
-      for (int k = 0; k < Row::V; ++k) mine = larger(mine, z(k));
-    });
-    return group.join(mine, larger);
-  };
-  float top = pass();
+  mine = row.largest();
+  float top = group.join(mine, larger);
   if (top == INFINITY) {
     row.unbounded();
-    top = pass();
+    mine = largest_of(row);
+    top = group.join(mine, larger);
   }
   return top;
 }
@@ -1072,7 +1085,7 @@ __global__ __launch_bounds__(256) void narrow_kernel(const ChooseArgs a) {
   float z = -INFINITY;
   if (lane < a.width && (!a.mask || a.mask[r * a.ld_mask + lane]))
     z = to_f32(static_cast<const T *>(a.logits)[r * a.ld_logits + lane]);
-  float top = lanes_join<G>(z, [](float x, float y) { return __builtin_elementwise_maximum(x, y); });
+  float top = lanes_join<G>(z, larger);
   const bool nan = top != top, none = top == -INFINITY;
   if (top == INFINITY) z = z == INFINITY ? 0.f : -INFINITY, top = 0;
   if (nan || none) z = -INFINITY, top = 0;
