@@ -38,6 +38,7 @@ struct DistillArgs {
   int32_t rows, width, k;
   double inverse;     // 1 / T
   float fast, slow;   // log2(e) / T rounded down, and the rest of it: both above 0, so that -inf stays -inf
+  float scale;        // log2(e) / T to the nearest
   Scalar normalizer;
   float *kl;   // NULL in a backward call
   void *grad;  // NULL: none
@@ -53,6 +54,13 @@ struct DistillArgs {
 __device__ __forceinline__ float exp_from(const DistillArgs &a, float z, float from) {
   const float d = z - from;
   return __builtin_amdgcn_exp2f(fmaf(d, a.fast, d * a.slow));
+}
+
+// For a gradient of 16 bits, whose own rounding is 2^-8 or 2^-11 of it: the scale's rounding, |x| 2^-24 of the exponential
+// (x = (z - from) / T), is below that until the exponential is 0.  One instruction less of five: 4096 x 32768 bf16 143 and
+// 140 us.
+__device__ __forceinline__ float exp_near(const DistillArgs &a, float z, float from) {
+  return __builtin_amdgcn_exp2f((z - from) * a.scale);
 }
 
 // ---- the record's entries in a row -------------------------------------------------------------------------
@@ -257,7 +265,7 @@ __device__ __forceinline__ void distill_row(const DistillArgs &a, int64_t r, int
     each([&](int i, const auto &z, bool inside) {
       float g[V];
 #pragma unroll
-      for (int k = 0; k < V; ++k) g[k] = o.outer * exp_from(a, z(k), rest_top);
+      for (int k = 0; k < V; ++k) g[k] = o.outer * (sizeof(T) == 2 ? exp_near(a, z(k), rest_top) : exp_from(a, z(k), rest_top));
       store_entries<V>(grad, g, i, a.width, inside, G >= 512 && a.streams);
     });
   }
@@ -434,6 +442,7 @@ DistillArgs args_of(const cg_distill_loss *loss) {
   a.fast = float(c);
   if (double(a.fast) >= c) a.fast = nextafterf(a.fast, 0.f);
   a.slow = float(c - double(a.fast));
+  a.scale = float(c);
   a.normalizer = scalar(p.normalizer);
   a.streams = int64_t(q.rows) * q.width >= STREAM_BYTES / (2 * dtype_size(q.dtype));
   return a;
