@@ -22,10 +22,11 @@
 // The first k of a row with k up to the lanes of its group need no histogram: at least k entries are as large as the k-th
 // largest of the lanes' own maxima, and not many more, so these are the list.
 //
-// A row is read from HBM once (what its bytes take: bf16 4096 x 32768 53 us) and looked through in LDS, so wide rows are bound by
-// VALU instructions: 8 an entry for its load and the maximum, 25 for its weight and the histogram, up to 9 for each entry
-// that is looked for.  us there: greedy 43, the record of 64 entries 101 to 113, no filter 159, top_p 198 to 206.  Few rows are bound
-// by the latency of passes and barriers (256 x 32768 with every filter 38), rows of up to 64 entries by their scalars.
+// A row is read from HBM once (what its bytes take: bf16 4096 x 32768 53 us) and looked through in LDS, so wide rows
+// are bound by VALU instructions: 8 an entry for its load and the maximum, 25 for its weight and the histogram, up to
+// 9 for each entry that is looked for.  us there: greedy 43, the record of 64 entries 101 to 113, no filter 159,
+// top_p 198 to 206.  Few rows are bound by the latency of passes and barriers (256 x 32768 with every filter 38),
+// rows of up to 64 entries by their scalars.
 #include "rows.h"
 
 namespace cg {

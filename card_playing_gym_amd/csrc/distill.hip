@@ -13,10 +13,11 @@
 // R has; and the gradient outside R is e^((z - m_r) / T) times one number a row, whose two terms nearly cancel where the policies
 // agree and are therefore subtracted in fp64.
 //
-// Every logit (mask byte) is read once and every gradient written once; a row stays in registers between
-// its maximum, its sum and its gradient.  Wide rows are bound by VALU instructions beside HBM (29.5 an entry of 16 bits, two of them
-// exponentials; bf16 4096 x 32768 140 us, its bytes 107), narrow ones by the record's terms and the row's scalars.  The forward writes the gradient for an upstream of 1; a backward with another
-// one forms it again from the inputs, so it is rounded once whatever the scale.
+// Every logit (mask byte) is read once and every gradient written once; a row stays in registers between its maximum,
+// its sum and its gradient.  Wide rows are bound by VALU instructions beside HBM (29.5 an entry of 16 bits, two of
+// them exponentials; bf16 4096 x 32768 140 us, its bytes 107), narrow ones by the record's terms and the row's
+// scalars.  The forward writes the gradient for an upstream of 1; a backward with another one forms it again from the
+// inputs, so it is rounded once whatever the scale.
 #include "rows.h"
 
 namespace cg {
