@@ -181,7 +181,8 @@ __device__ __forceinline__ RowScalars row_scalars(const DistillArgs &a, int64_t 
   const double lower = rest > 0 ? exp_of(gap) : 0.0;
   double s = t.s + (rest > 0 ? rest * lower : rest);  // (rest: NaN stays)
   if (!good) s = NAN;
-  o.live = weight != 0 && s != 0;
+  // (without q_r the largest q counts as 1: they sum to 0 where the record has nothing, and the row has no term whatever its logits)
+  o.live = weight != 0 && s != 0 && (a.rest || t.q != 0 || !good);
   const double log_s = log_of(s);
   double mass = t.q, outer = 0;
   if (a.rest) {
@@ -196,14 +197,14 @@ __device__ __forceinline__ RowScalars row_scalars(const DistillArgs &a, int64_t 
     o.pull = 1;
   } else {
     const double inv = t.q > 0 ? reciprocal(t.q) : 0;
-    o.kl = t.q > 0 ? (t.own - t.cross) * inv - log_of(t.q) + log_s : t.q;
-    mass = t.q > 0 ? 1 : t.q;
+    o.kl = t.q > 0 ? (t.own - t.cross) * inv - log_of(t.q) + log_s : NAN;
+    mass = t.q > 0 ? 1 : NAN;
     o.pull = inv;
   }
   const double f = double(weight) * (a.upstream ? double(*a.upstream) : 1.0) / read(a.normalizer) * a.inverse;
   o.inner = f * mass * reciprocal(s);
   o.pull *= f;
-  o.outer = o.live ? float(o.inner * lower - f * outer) : 0.f;
+  o.outer = float(o.inner * lower - f * outer);
   o.value = double(weight) * o.kl;
   return o;
 }
@@ -263,13 +264,16 @@ __device__ __forceinline__ void distill_row(const DistillArgs &a, int64_t r, int
   }
   if (!a.grad) return;
   T *grad = static_cast<T *>(a.grad) + r * int64_t(a.width);
-  if (in) {
+  if (in && o.live) {
     each([&](int i, const auto &z, bool inside) {
       float g[V];
 #pragma unroll
       for (int k = 0; k < V; ++k) g[k] = o.outer * (sizeof(T) == 2 ? exp_near(a, z(k), rest_top) : exp_from(a, z(k), rest_top));
       store_entries<V>(grad, g, i, a.width, inside, G >= 512 && a.streams);
     });
+  } else if (in) {  // (their logits may be NaN: no product with them is 0)
+    const float zeros[V] = {};
+    each([&](int i, const auto &, bool inside) { store_entries<V>(grad, zeros, i, a.width, inside, G >= 512 && a.streams); });
   }
   group_sync<G>();  // (the zeros just written at R's entries come first)
   if (in && o.live) {

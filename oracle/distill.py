@@ -20,9 +20,12 @@ def distill(logits, indices, log_probs, log_rest=None, mask=None, weights=None, 
         legal = (np.ones(width, dtype=bool) if mask is None else mask[r]) & ~(z == -np.inf)
         there = indices[r] != -1
         at, logq = indices[r][there], log_probs[r][there].astype(np.float64)
-        if weights[r] == 0 or not legal.any() or (log_rest is None and not (logq > -np.inf).any()):
+        if weights[r] == 0 or not legal.any():
             continue
-        if ((at < 0) | (at >= width)).any() or len(set(at)) < len(at) or np.isnan(z[legal]).any():
+        astray = ((at < 0) | (at >= width)).any() or len(set(at)) < len(at)
+        if log_rest is None and not astray and (logq == -np.inf).all():
+            continue
+        if astray or np.isnan(z[legal]).any() or (z[legal] == np.inf).any():
             out["kl"][r], out["grad"][r] = np.nan, np.nan
             continue
         logp = np.where(legal, z - log_sum_exp(z[legal]), -np.inf)

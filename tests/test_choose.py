@@ -87,6 +87,21 @@ def test_distillation_is_autograds(masked, rest):
         assert abs((up - down) / (2 * step) - got["grad"][r, j]) < 1e-8
 
 
+def test_rows_of_the_distillation_oracle_that_do_not_count():
+    logits = np.zeros((6, 4))
+    logits[0, 1], logits[1, 2] = np.nan, np.inf
+    indices = np.array([[-1, -1], [0, -1], [1, 1], [4, -1], [0, -2], [0, 1]])
+    log_probs = np.full((6, 2), -1.0)
+    log_probs[:5] = -np.inf
+    out = ref_distill.distill(logits, indices, log_probs)
+    assert (out["kl"][:2] == 0).all() and (out["grad"][:2] == 0).all()  # no record
+    assert np.isnan(out["kl"][2:5]).all() and np.isnan(out["grad"][2:5]).all()  # one out of order
+    assert np.isfinite(out["kl"][5])
+    assert np.isnan(ref_distill.distill(logits, indices, log_probs, np.zeros(6))["kl"][:5]).all()
+    nothing = ref_distill.distill(logits, indices, log_probs, mask=np.zeros((6, 4), dtype=bool))
+    assert (nothing["kl"] == 0).all() and (nothing["grad"] == 0).all()
+
+
 # ---- refusals --------------------------------------------------------------------------------------------------------
 
 

@@ -418,3 +418,21 @@ def test_more_entries_than_32_bits_count(device):
     few = slice(rows - 5, rows)
     want, want_grad = run(logits[few].clone(), indices[few], log_probs[few], {"log_rest": log_rest[few], "normalizer": 1.0})
     assert torch.equal(out.kl[few], want.kl) and torch.equal(grad[few], want_grad)
+
+
+@pytest.mark.parametrize("width", [5, 60, 500, 3000, 20000, 70000])
+def test_records_without_mass_and_without_a_rest(device, width):
+    """Without a rest, a record that is out of order makes its row NaN though none of its entries weighs anything; one that
+    is in order and weighs nothing is no record, whatever the row's logits are."""
+
+    logits = torch.randn(7, width, device=device)
+    indices = torch.tensor([[width, -1], [-2, 10**12], [2, 2], [-1, -1], [3, -1], [-1, 1], [0, 3]], device=device)
+    log_probs = torch.full((7, 2), -1.5, device=device)
+    log_probs[2] = log_probs[4] = log_probs[5] = -float("inf")
+    logits[3, 1], logits[4, 0], logits[5, 2] = float("nan"), float("inf"), float("nan")
+    out, grad = run(logits, indices, log_probs, {})
+    assert out.kl[:3].isnan().all() and grad[:3].isnan().all() and out.loss.isnan()
+    assert (out.kl[3:6] == 0).all() and (grad[3:6] == 0).all()
+    out, grad = run(logits[3:], indices[3:], log_probs[3:], {})
+    assert (out.kl[:3] == 0).all() and (grad[:3] == 0).all() and out.loss == out.kl[3] / 4
+    check(logits[6:], indices[6:], log_probs[6:], {"temperature": 1.0})
