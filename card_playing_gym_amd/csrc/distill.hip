@@ -180,9 +180,10 @@ __device__ __forceinline__ RowScalars row_scalars(const DistillArgs &a, int64_t 
   const double gap = rest > 0 ? (double(rest_top) - double(top)) * a.inverse : 0.0;
   const double lower = rest > 0 ? exp_of(gap) : 0.0;
   double s = t.s + (rest > 0 ? rest * lower : rest);  // (rest: NaN stays)
-  if (!good) s = NAN;
-  // (without q_r the largest q counts as 1: they sum to 0 where the record has nothing, and the row has no term whatever its logits)
+  // s is 0 where nothing is legal.  (Without q_r the largest q counts as 1: they sum to 0 where the record has nothing, and
+  // the row has no term whatever its logits.)
   o.live = weight != 0 && s != 0 && (a.rest || t.q != 0 || !good);
+  if (!good) s = NAN;
   const double log_s = log_of(s);
   double mass = t.q, outer = 0;
   if (a.rest) {

@@ -631,7 +631,7 @@ int cg_policy_loss_backward(const cg_policy_loss *loss, const float *upstream, i
  * second term is not there.  The value is sum_i w_i KL_i / normalizer.  Index -1: no entry.  An index outside
  * the row, or twice in it, makes the row NaN, as does a legal entry that is NaN or +inf; an entry that is
  * not legal but has a q above 0 makes its KL infinite.  A row of weight 0 is not read; it and a row without a
- * legal entry add nothing, have a zero gradient and report 0.  So does, without log_rest, one whose record is
+ * legal entry, whatever its record, add nothing, have a zero gradient and report 0.  So does, without log_rest, one whose record is
  * empty or has no q above 0, whatever its logits are; not where an index is outside the row or twice in it. */
 typedef struct {
   cg_policy_rows rows;

@@ -436,3 +436,21 @@ def test_records_without_mass_and_without_a_rest(device, width):
     out, grad = run(logits[3:], indices[3:], log_probs[3:], {})
     assert (out.kl[:3] == 0).all() and (grad[:3] == 0).all() and out.loss == out.kl[3] / 4
     check(logits[6:], indices[6:], log_probs[6:], {"temperature": 1.0})
+
+
+@pytest.mark.parametrize("width", [5, 60, 500, 3000, 20000, 70000])
+@pytest.mark.parametrize("rest", [False, True])
+def test_rows_with_nothing_legal_and_a_record_out_of_order(device, width, rest):
+    """Padding by an all-false mask over records filled with zeros: nothing legal, so nothing counts."""
+
+    logits = torch.randn(5, width, device=device)
+    mask = torch.ones(5, width, dtype=torch.bool, device=device)
+    mask[:3] = False
+    logits[3] = -float("inf")
+    indices = torch.tensor([[0, 0, 0], [0, width, 1], [-2, 1, 2], [1, 1, 0], [2, 0, 1]], device=device)
+    log_probs = torch.full((5, 3), -1.5, device=device)
+    options = {"mask": mask} | ({"log_rest": torch.full((5,), -1.1, device=device)} if rest else {})
+    out, grad = run(logits, indices, log_probs, options)
+    assert (out.kl[:4] == 0).all() and (grad[:4] == 0).all()
+    assert out.loss.isfinite() and out.kl[4] > 0 and grad[4].isfinite().all()
+    check(logits[3:], indices[3:], log_probs[3:], {n: x[3:] for n, x in options.items()} | {"temperature": 1.0})
