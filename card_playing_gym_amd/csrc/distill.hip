@@ -135,9 +135,9 @@ struct Record {
       }
     }
   }
-  // Marks R.  Returns whether this lane's indices are in the row, and there once.
+  // Marks R, of a row that counts.  Returns whether this lane's indices are in the row, and there once.
   template <typename B>
-  __device__ __forceinline__ bool mark(B &bits) const {
+  __device__ __forceinline__ bool mark(B &bits, bool counts) const {
     const int words = min((a.width >> 5) + 2, B::WORDS);  // (of vectors that begin before the row's end, and one more)
     for (int i = lane; i < words; i += G) bits.w[i] = 0;
     group_sync<G>();
@@ -151,7 +151,7 @@ struct Record {
     if constexpr (N > 0) {
 #pragma unroll
       for (int i = 0; i < N; ++i) set(index[i]);
-    } else {
+    } else if (counts) {
       for (int k = lane; k < a.k; k += G) set(in_row(indices[k]));
     }
     group_sync<G>();
@@ -187,7 +187,7 @@ __device__ __forceinline__ RowScalars row_scalars(const DistillArgs &a, int64_t 
   const double log_s = log_of(s);
   double mass = t.q, outer = 0;
   if (a.rest) {
-    const double log_q = a.rest[r], q = exp_of(log_q);
+    const double log_q = weight != 0 ? a.rest[r] : -INFINITY, q = exp_of(log_q);
     mass += q;
     o.kl = t.own - t.cross + t.q * log_s;
     if (!(q <= 0)) {
@@ -316,7 +316,7 @@ __global__ __launch_bounds__((G > 256 ? G : 256), 4) void rows_kernel(const Dist
   }
   // (groups of a wave go through their barriers together, weight or not)
   record.load_logits();
-  if (weight != 0 || G <= 64) good = record.mark(bits[in_block]) || weight == 0;
+  if (weight != 0 || G <= 64) good = record.mark(bits[in_block], weight != 0);
   if (weight != 0) {
 #pragma unroll
     for (int c = 0; c < C; ++c) {
@@ -356,7 +356,7 @@ __global__ __launch_bounds__(1024) void long_rows_kernel(const DistillArgs a) {
   const uint8_t *legal = a.mask ? a.mask + r * a.ld_mask : nullptr;
   Record<G, T> record(a, r, lane, logits, legal, weight != 0);
   record.load_logits();
-  const bool good = weight != 0 ? record.mark(bits) : true;
+  const bool good = weight != 0 ? record.mark(bits, true) : true;
   const auto each = [&](const auto &visit) {
     for (int i = lane * V; i < a.width; i += G * V) {
       Entries<T, V> z;

@@ -132,8 +132,8 @@ def distill_loss(
     a legal entry that is NaN or +inf.  An entry with a q above 0 that is not legal here makes its row's KL infinite.
 
     A row of weight 0 (padding) is not read: like a row without a legal entry, whatever its record, it adds nothing, has a
-    zero gradient and reports 0.  So does, without ``log_rest``, a row whose record is empty or has no q above 0, whatever its logits are; an
-    index outside the row, or twice in it, still makes it NaN."""
+    zero gradient and reports 0.  So does, without ``log_rest``, a row whose record is empty or has no q above 0, whatever
+    its logits are; an index outside the row, or twice in it, still makes it NaN."""
 
     descriptor, (entries, mask) = _policy_rows(logits, mask)
     _no_tangents(logits, log_probs, log_rest, weights, normalizer, name="distill_loss")
