@@ -478,7 +478,8 @@ int cg_distill_loss_forward(const cg_distill_loss *loss, float *value, float *kl
     const int64_t sums = a.rows > 0 ? blocks_of(loss->rows) : 0;
     if (sums > 0) launch_rows(a, loss->rows, as_stream(stream));
     if (sums != 1) {
-      loss_kernel<DistillArgs><<<1, 256, 0, as_stream(stream)>>>(a, int(sums));
+      // (us of 256 lanes a load at a time, and of these: 4096 sums 6.3 and 4.8, 32768 33 and 6.4, 262144 355 and 45)
+      loss_kernel<DistillArgs, 1024><<<1, 1024, 0, as_stream(stream)>>>(a, int(sums));
       CG_LAUNCHED();
     }
   });

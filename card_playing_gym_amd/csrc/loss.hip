@@ -30,6 +30,7 @@ namespace {
 // logits or takes the gradient may find them there.  us kept and past them: fp32 4096 x 16384 (512 MB) 102 and 98,
 // 8192 x 16384 205 and 201; bf16, whose time is arithmetic, 4096 x 32768 128-133 and 127-129.
 constexpr int64_t STREAM_BYTES = 512 << 20;
+constexpr int MAX_BLOCKS = 2048;  // and partial sums of the loss
 // The least x = z - top that p = e^x is multiplied by: e^x is 0 from -104 on.  No lower, so that the coefficient
 // of x may be as large as 2^120 before the product is infinite, which times p = 0 is NaN.
 constexpr float LOWEST = -128.f;

@@ -277,8 +277,6 @@ __device__ __forceinline__ void store_entries(T *row, const float *g, int i, int
 
 // ---- a loss over rows: its scalars, its partial sums ------------------------------------------------------
 
-constexpr int MAX_BLOCKS = 2048;  // and partial sums of the loss
-
 struct Scalar {
   float value;
   const float *at;  // NULL: value
@@ -303,10 +301,12 @@ __device__ __forceinline__ void block_loss(const Args &a, double value) {
     a.partials[blockIdx.x] = s;
 }
 
-template <typename Args>
-__global__ __launch_bounds__(256) void loss_kernel(const Args a, int count) {
+// The loss of all blocks, in a fixed order: one block, whose threads each add up every THREADS-th partial sum.
+template <typename Args, int THREADS = 256>
+__global__ __launch_bounds__(THREADS) void loss_kernel(const Args a, int count) {
   double s = 0;
-  for (int k = threadIdx.x; k < count; k += 256) s += a.partials[k];
+#pragma unroll 8
+  for (int k = threadIdx.x; k < count; k += THREADS) s += a.partials[k];
   block_loss(a, s);  // (of one block)
 }
 

@@ -482,3 +482,17 @@ def test_records_of_rows_without_weight_are_not_read(device, width):
         return min(times)
 
     assert least(256) - least(1) < 67
+
+
+@pytest.mark.parametrize("rows, width", [(5003, 2100), (70001, 66), (9000, 8193)])
+def test_the_loss_of_many_blocks(device, rows, width):
+    """The value is the rows' sum, whose terms are reported rounded once, by half a step of each."""
+
+    logits = torch.randn(rows, width, device=device).bfloat16()
+    record = top_logits(logits.float() + 0.5 * torch.randn(rows, width, device=device), 4)
+    weights = torch.rand(rows, device=device)
+    first = distill_loss(logits, record.indices, record.log_probs, log_rest=record.log_rest, weights=weights)
+    terms = weights.double() * first.kl.double()
+    assert abs(first.loss.item() - terms.sum().item() / rows) <= (terms.abs().sum().item() / rows + abs(first.loss.item())) * U
+    again = distill_loss(logits, record.indices, record.log_probs, log_rest=record.log_rest, weights=weights)
+    assert torch.equal(first.loss, again.loss)
