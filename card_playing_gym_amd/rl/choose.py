@@ -17,6 +17,7 @@ import torch
 from .. import _native as nat
 from ..nn.kv_cache import dtype_code, require_device, stream_handle
 from ..nn.optim import _on
+from .policy import _no_tangents
 
 MAX_WIDTH = 2**18
 MAX_TOP = 256
@@ -102,9 +103,11 @@ def sample_logits(
 
     A row without a legal entry has action -1 and log-probability 0.  One with a NaN among its legal entries
     (or a negative or NaN temperature of its own) has action -1 and NaN.  Entries at +inf share everything.
-    The actions are the same whatever the launch: a row's sums are exact."""
+    The actions are the same whatever the launch: a row's sums are exact.  Nothing here is differentiable: ``log_probs``
+    carry no gradient (``policy_loss`` forms its own from the logits), and forward-mode tangents are refused."""
 
     descriptor, held = _policy_rows(logits, mask)
+    _no_tangents(logits, uniforms, temperature, top_p, min_p, name="sample_logits")
     rows, device = descriptor.rows, logits.device
     if uniforms.shape != (rows,) or uniforms.dtype != torch.float64 or uniforms.device != device:
         raise ValueError("uniforms must be float64 [rows] on the logits' device")
@@ -143,9 +146,11 @@ def top_logits(
 
     Where a row has fewer than k legal entries the places behind them hold -inf and index -1, and ``log_rest``
     is -inf, as ``distill_loss`` takes them.  A row with a NaN among its legal entries reports NaN and
-    indices -1.  Entries at +inf share everything."""
+    indices -1.  Entries at +inf share everything.  The record is a constant: it carries no gradient of the logits, and
+    forward-mode tangents are refused."""
 
     descriptor, held = _policy_rows(logits, mask)
+    _no_tangents(logits, name="top_logits")
     rows, device = descriptor.rows, logits.device
     if not 1 <= k <= MAX_TOP:
         raise ValueError(f"k must be from 1 to {MAX_TOP}")

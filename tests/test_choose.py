@@ -207,6 +207,21 @@ def test_forward_derivatives_are_refused(anywhere, name):
             _distill(**{name: forward_ad.make_dual(torch.ones(shape), torch.ones(shape))})
 
 
+@pytest.mark.parametrize("name", ["logits", "uniforms", "temperature", "top_p", "min_p"])
+def test_forward_derivatives_of_answers_are_refused(anywhere, name):
+    from torch.autograd import forward_ad
+
+    dtype = torch.float64 if name == "uniforms" else torch.float32
+    x = torch.ones((4, 6) if name == "logits" else (4,), dtype=dtype)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        with pytest.raises(RuntimeError, match="sample_logits has no forward"):
+            _sample(**{name: dual})
+        if name == "logits":
+            with pytest.raises(RuntimeError, match="top_logits has no forward"):
+                top_logits(dual, 3)
+
+
 def test_native_refusals():
     """Fake addresses: every check comes before a launch."""
 

@@ -334,3 +334,10 @@ def test_temperatures_without_end(device, width):
     torch.testing.assert_close(hot.log_probs.double(), -n.double().log(), rtol=U, atol=1e-9)
     cold = sample_logits(logits, u, mask=mask, temperature=torch.full((40,), 2.0**-149, device=device))
     assert torch.equal(cold.actions, order[:, 0]) and (cold.log_probs == 0).all()
+
+
+def test_answers_carry_no_gradient(device):
+    logits = torch.randn(4, 50, device=device, requires_grad=True)
+    u = torch.rand(4, device=device, dtype=torch.float64)
+    for given in (logits, logits * 2, (logits * 2).t().contiguous().t()):
+        assert not any(t.requires_grad for t in (*sample_logits(given, u), *top_logits(given, 5)))
