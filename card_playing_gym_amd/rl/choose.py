@@ -122,6 +122,8 @@ def sample_logits(
         raise ValueError("top_p must not be negative")
     if not m <= 1:
         raise ValueError("min_p may be 1 at most")
+    if k % 1 != 0:  # (a share of the entries, say, would be cut to 0: all of them)
+        raise ValueError("top_k must be a whole number")
     controls = nat.SampleControls(t, p, m, min(max(int(k), 0), MAX_WIDTH), *(None if x is None else x.data_ptr()
                                                                              for x in (ts, ps, ms, ks)))
     actions = torch.empty(rows, device=device, dtype=torch.int64)

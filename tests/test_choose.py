@@ -207,6 +207,12 @@ def test_forward_derivatives_are_refused(anywhere, name):
             _distill(**{name: forward_ad.make_dual(torch.ones(shape), torch.ones(shape))})
 
 
+@pytest.mark.parametrize("k", [0.5, 2.7, float("nan"), float("inf"), -0.5])
+def test_a_top_k_that_is_no_whole_number_is_refused(anywhere, k):
+    with pytest.raises(ValueError, match="top_k must be a whole number"):
+        _sample(top_k=k)
+
+
 @pytest.mark.parametrize("name", ["logits", "uniforms", "temperature", "top_p", "min_p"])
 def test_forward_derivatives_of_answers_are_refused(anywhere, name):
     from torch.autograd import forward_ad
