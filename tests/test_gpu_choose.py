@@ -341,3 +341,122 @@ def test_answers_carry_no_gradient(device):
     u = torch.rand(4, device=device, dtype=torch.float64)
     for given in (logits, logits * 2, (logits * 2).t().contiguous().t()):
         assert not any(t.requires_grad for t in (*sample_logits(given, u), *top_logits(given, 5)))
+
+
+# ---- rows that are read again for each pass, in every type -----------------------------------------------------------
+
+
+# Both sides of 147456 bytes in 4 and in 2 bytes an entry, an odd width beyond, and the widest.
+WIDE = [36864, 36865, 73728, 73729, 131071, 2**18]
+
+
+def check_wide_sample(logits, uniforms, mask, **controls):
+    """As check_sample, with the weights' error in full.  An entry's weight is off by 2^-44 of it and by half a unit of
+    2^-min(50, 62 - log2 width): the sum S' of what is kept by e = 2^-44 + n 2^-s / (2 S') of itself, a running sum over it by
+    2 e, and its logarithm by e; a logarithm and a distance add 2^-50 of themselves, their float32 half a step."""
+
+    rows, width = logits.shape
+    out = sample_logits(logits, uniforms, mask=mask, **controls)
+    z, legal = numpy_of(logits), np.ones((rows, width), dtype=bool) if mask is None else numpy_of(mask)
+    actions, log_probs, margin = ref.sample(z, numpy_of(uniforms), numpy_of(mask), **controls)
+    unit = 2.0 ** -min(50, 62 - int(np.ceil(np.log2(width))))
+    if controls.get("temperature", 1.0) > 0:
+        total = np.array([ref.kept_weights(z[r], legal[r], **controls)[1].sum() for r in range(rows)])
+        e = 2.0**-44 + width * unit / 2 / total
+        assert (margin > 2 * e).all()  # (of the inputs, not of the kernel)
+    else:
+        e = np.zeros(rows)
+    np.testing.assert_array_equal(out.actions.cpu().numpy(), actions)
+    assert (np.abs(numpy_of(out.log_probs) - log_probs) <= np.abs(log_probs) * U + e + 2.0**-49 * (1 + np.abs(log_probs))).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("width", WIDE)
+def test_wide_samples_are_the_definition(device, width, dtype):
+    for i, controls in enumerate(CONTROLS):
+        logits, mask, u = make(device, 2, width, dtype, width + i, masked=(i + DTYPES.index(dtype)) % 2 == 0)
+        check_wide_sample(logits, u, mask, **controls)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("width", WIDE)
+def test_wide_records_are_the_definition(device, width, dtype):
+    for i, (k, temperature) in enumerate(((1, 1.0), (64, 2.0), (256, 0.5))):
+        logits, mask, _ = make(device, 2, width, dtype, width + i, masked=(i + DTYPES.index(dtype)) % 2 == 1)
+        check_top(logits, k, mask, temperature)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("width", [80001, 2**18])
+def test_wide_equal_entries_go_by_their_index(device, width, dtype):
+    test_equal_entries_go_by_their_index(device, width, dtype)
+
+
+@pytest.mark.parametrize("how", ["few_values", "falling", "rising", "one_vector"])
+def test_top_of_wide_rows_that_crowd(device, how):
+    test_top_of_rows_that_crowd(device, 90001, how)
+
+
+def test_wide_strides(device):
+    test_strides(device, 90001)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("width", [4, 40, 600, 20000, 90001])
+def test_rows_with_nothing_to_choose_in_16_bits(device, width, dtype):
+    rows = 6
+    logits = torch.randn(rows, width, device=device).to(dtype)
+    mask = torch.ones(rows, width, dtype=torch.bool, device=device)
+    mask[0] = False
+    logits[1] = -float("inf")
+    logits[2, width - 1] = float("nan")
+    logits[3, width - 1], mask[3, width - 1] = float("nan"), False  # not legal: not read as one
+    logits[4, [0, width // 2, width - 1]] = float("inf")
+    logits[5, width - 2], mask[5, width - 2] = float("inf"), False
+    out = sample_logits(logits, torch.full((rows,), 0.5, dtype=torch.float64, device=device), mask=mask)
+    assert out.actions[:3].tolist() == [-1, -1, -1] and out.actions[4] == width // 2
+    assert out.log_probs[:2].tolist() == [0, 0] and out.log_probs[2].isnan()
+    assert abs(out.log_probs[4] + np.log(3)) < 1e-6
+    for r, barred in ((3, width - 1), (5, width - 2)):
+        assert 0 <= out.actions[r] != barred and out.log_probs[r].isfinite()
+    top = top_logits(logits, 4, mask=mask)
+    assert (top.indices[:3] == -1).all() and (top.log_probs[:2] == -float("inf")).all() and top.log_probs[2].isnan().all()
+    assert (top.log_rest[:2] == -float("inf")).all() and top.log_rest[2].isnan() and not top.log_probs[[3, 5]].isnan().any()
+    assert top.indices[4].tolist()[:3] == [0, width // 2, width - 1] and top.log_rest[4] == -float("inf")
+    assert (top.indices[3] != width - 1).all() and (top.indices[5] != width - 2).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("width", [400, 6000, 40000, 90001])
+def test_records_in_16_bits_are_the_same_every_time(device, width, dtype):
+    logits = torch.randn(64, width, device=device).to(dtype)
+    first = top_logits(logits, 50)
+    for _ in range(20):
+        assert all(torch.equal(a, b) for a, b in zip(top_logits(logits, 50), first))
+
+
+@pytest.mark.parametrize("width", [6, 300, 5000, 66000])
+def test_controls_that_only_a_row_of_its_own_may_have(device, width):
+    """What is refused as a number for all: as the definition has it, NaN being no filter, an infinite temperature uniform."""
+
+    nan, inf = float("nan"), float("inf")
+    rows = [{"top_p": nan}, {"min_p": nan}, {"top_p": -0.5}, {"top_p": -inf}, {"min_p": 1.5}, {"min_p": inf}, {"min_p": -inf},
+            {"top_p": inf}, {"temperature": inf}, {"temperature": -0.0}]
+    logits = torch.randn(1, width, device=device).expand(len(rows), width).clone()
+    best = logits[0].argmax().item()
+    logits[:, (best + 1) % width] = logits[0, best]  # (equal to the largest)
+    u = torch.full((len(rows),), 0.4219, dtype=torch.float64, device=device)
+    controls = {name: torch.tensor([r.get(name, free) for r in rows], device=device)
+                for name, free in (("temperature", 1.0), ("top_p", 1.0), ("min_p", 0.0))}
+    out = sample_logits(logits, u, **controls)
+    plain = sample_logits(logits, u)
+    for i, row in enumerate(rows):
+        if row.get("top_p", 1) < 0 or row.get("min_p", 0) > 1 or row.get("temperature") == 0:
+            assert out.actions[i] == min(best, (best + 1) % width) and out.log_probs[i] == 0, row
+        elif row.get("temperature") == inf:
+            order = torch.sort(logits[i], descending=True, stable=True).indices
+            assert out.actions[i] == order[int(0.4219 * width)] and abs(out.log_probs[i].item() + np.log(width)) < 1e-6 * np.log(width)
+        else:
+            assert out.actions[i] == plain.actions[i] and out.log_probs[i] == plain.log_probs[i], row
+    bad = sample_logits(logits[:2], u[:2], temperature=torch.tensor([-1.0, -inf], device=device))
+    assert bad.actions.tolist() == [-1, -1] and bad.log_probs.isnan().all()

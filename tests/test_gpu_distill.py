@@ -496,3 +496,41 @@ def test_the_loss_of_many_blocks(device, rows, width):
     assert abs(first.loss.item() - terms.sum().item() / rows) <= (terms.abs().sum().item() / rows + abs(first.loss.item())) * U
     again = distill_loss(logits, record.indices, record.log_probs, log_rest=record.log_rest, weights=weights)
     assert torch.equal(first.loss, again.loss)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+@pytest.mark.parametrize("width", [20, 500, 3000, 40000, 80001])
+@pytest.mark.parametrize("upstream", [float(np.float32(0.1)), -3.0])
+def test_upstream_gradients_in_every_type(device, width, upstream, dtype):
+    check(*make(device, 7, width, dtype, 6, 16, weighted=True), upstream=upstream)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("width", [40000, 80001])
+def test_a_factor_in_the_normalizer_is_one_on_the_loss(device, width, dtype):
+    logits, indices, log_probs, options = make(device, 4, width, dtype, 15, 16)
+    out, grad = check(logits, indices, log_probs, options | {"normalizer": 4 / 0.125})
+    scaled, scaled_grad = run(logits, indices, log_probs, options, 0.125)
+    assert torch.equal(out.loss, scaled.loss * 0.125) and torch.equal(grad, scaled_grad)  # (a power of two)
+
+
+@pytest.mark.parametrize("width", [5, 500, 20000])
+def test_a_rest_that_this_policy_does_not_have(device, width):
+    """The teacher has mass outside the record and this policy nothing there: an infinite KL, the gradient of what is finite."""
+
+    logits = torch.randn(2, width, device=device)
+    mask = torch.zeros(2, width, dtype=torch.bool, device=device)
+    mask[:, 1:3] = True
+    indices, log_probs = torch.tensor([[2, 1]] * 2, device=device), torch.full((2, 2), -1.5, device=device)
+    log_rest = torch.tensor([-0.6, -float("inf")], device=device)
+    out, grad = run(logits, indices, log_probs, {"mask": mask, "log_rest": log_rest})
+    assert out.kl[0] == float("inf") and out.kl[1].isfinite() and out.loss == float("inf")
+    want = ref.distill(numpy_of(logits), numpy_of(indices), numpy_of(log_probs), numpy_of(log_rest), numpy_of(mask))
+    assert (np.abs(numpy_of(grad) - want["grad"]) <= 1e-12 + np.abs(want["grad"]) * U).all() and (grad[~mask] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("width", [131071, 2**18])
+def test_the_widest_rows(device, width, dtype):
+    masked = dtype != torch.bfloat16
+    check(*make(device, 2, width, dtype, 16, 256, masked=masked, rest=width % 2 == 0, weighted=masked, temperature=0.7))
