@@ -99,10 +99,15 @@ def sample_logits(
     the first entry always.  The action is the first entry of the order at which the running sum over what is
     kept exceeds uniform times all of it; ``log_probs`` is the log of its share.  A temperature of 0 takes the first entry.
 
-    Each control is a number, or a tensor [rows] (float32; ``top_k`` int64) with every row's own.
+    Each control is a number, or a tensor [rows] (float32; ``top_k`` int64) with every row's own.  A number is looked at: a
+    temperature that is negative, infinite or NaN, a ``top_p`` below 0 or NaN, a ``min_p`` above 1 or NaN is refused.
+    A row's own, which is on the device, is taken as it stands: an infinite temperature weighs all legal entries alike, a
+    ``top_p`` below 0 and a ``min_p`` above 1 leave the first entry, and a NaN in either is no filter.
 
     A row without a legal entry has action -1 and log-probability 0.  One with a NaN among its legal entries
     (or a negative or NaN temperature of its own) has action -1 and NaN.  Entries at +inf share everything.
+    Weights are whole multiples of a unit, 2^-50 of the largest in rows of up to 4096 entries and up to 2^-44 in wider
+    ones: an entry of less than half a unit is never drawn.
     The actions are the same whatever the launch: a row's sums are exact.  Nothing here is differentiable: ``log_probs``
     carry no gradient (``policy_loss`` forms its own from the logits), and forward-mode tangents are refused."""
 

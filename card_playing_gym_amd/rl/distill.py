@@ -126,10 +126,13 @@ def distill_loss(
 
     ``weights``: float32 [rows] (ones).  ``normalizer``: the number of rows, padding among them; pass the count of
     those with weight for their mean.  It may be a float32 device scalar, which a captured loss reads at every replay.
+    A factor of the loss belongs in it too (n / 0.1 for a tenth): the forward writes the gradient for an arriving 1, and
+    for another one, as ``0.1 * out.loss`` sends, the backward forms it again.
     A backward captured in a graph of its own follows one replay of its forward's each time.
 
     Index -1 stands for no entry.  An index outside the row, or twice in it, makes its row, and the loss, NaN, as does
-    a legal entry that is NaN or +inf.  An entry with a q above 0 that is not legal here makes its row's KL infinite.
+    a legal entry that is NaN or +inf.  An entry with a q above 0 that is not legal here makes its row's KL infinite, as
+    does a ``log_rest`` above -inf where nothing outside the record is legal; the gradient stays finite.
 
     A row of weight 0 (padding) is not read: like a row without a legal entry, whatever its record, it adds nothing, has a
     zero gradient and reports 0.  So does, without ``log_rest``, a row whose record is empty or has no q above 0, whatever

@@ -567,7 +567,10 @@ typedef struct {
  * (all: 0 or less); the first entry always.  actions[row] is the first of the order whose running sum over the
  * kept, S' in all, exceeds uniforms[row] S' (the last kept for a uniform of 1 or more, or NaN), and
  * log_probs[row] = d - log S'.  Temperature 0: the first of the order, with 0.  A row without a legal entry
- * has action -1 and 0; one with a NaN among them, or a temperature that is negative or NaN, -1 and NaN. */
+ * has action -1 and 0; one with a NaN among them, or a temperature that is negative or NaN, -1 and NaN.
+ * A temperature for all has to be finite; a row's own may be +inf (all legal entries alike).  A NaN in top_p or
+ * min_p is no filter.  A weight is a whole multiple of 2^-50 (of 2^-62 times the power of two that `width` fits, beyond
+ * 4096): entries below half of that are never drawn. */
 int cg_sample_logits(const cg_policy_rows *rows, const double *uniforms, const cg_sample_controls *controls,
                      int64_t *actions, float *log_probs, void *stream);
 
@@ -630,9 +633,10 @@ int cg_policy_loss_backward(const cg_policy_loss *loss, const float *upstream, i
  * without log_rest, q is made to sum to 1 over R (logits / temperature will do for log_probs) and the
  * second term is not there.  The value is sum_i w_i KL_i / normalizer.  Index -1: no entry.  An index outside
  * the row, or twice in it, makes the row NaN, as does a legal entry that is NaN or +inf; an entry that is
- * not legal but has a q above 0 makes its KL infinite.  A row of weight 0 is not read; it and a row without a
- * legal entry, whatever its record, add nothing, have a zero gradient and report 0.  So does, without log_rest, one whose record is
- * empty or has no q above 0, whatever its logits are; not where an index is outside the row or twice in it. */
+ * not legal but has a q above 0 makes its KL infinite, as does a q_r above 0 with nothing legal outside R.
+ * A row of weight 0 is not read; it and a row without a legal entry, whatever its record, add nothing, have a
+ * zero gradient and report 0.  So does, without log_rest, one whose record is empty or has no q above 0, whatever
+ * its logits are; not where an index is outside the row or twice in it. */
 typedef struct {
   cg_policy_rows rows;
   const int64_t *indices;  /* [rows, k] dense */
