@@ -123,15 +123,7 @@ struct Group {
   __device__ __forceinline__ explicit Group(Shared<G> &s) : shared(s) {}
   static __device__ __forceinline__ int lane() { return threadIdx.x % G; }
 
-  __device__ __forceinline__ void sync() const {
-    if constexpr (G > 64) {
-      __syncthreads();
-    } else {  // the wave's LDS writes to its own reads
-      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-      __builtin_amdgcn_wave_barrier();
-      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-    }
-  }
+  __device__ __forceinline__ void sync() const { group_sync<G>(); }
   // Joins x over the group, the result in every lane.  Slots are used in turn: one is written again only behind the
   // next join's barrier, which every wave reaches after its reads.
   template <typename X, typename Op>
@@ -1097,18 +1089,13 @@ __global__ __launch_bounds__(256) void narrow_kernel(const ChooseArgs a) {
   // Into the row's order.
   uint64_t place = place_of(z, lane);
   mine[lane] = place;
-  const auto visible = [] {  // the wave's LDS writes to its own reads
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-  };
-  visible();
+  wave_sync();
   int rank = 0;
 #pragma unroll 4
   for (int j = 0; j < G; ++j) rank += mine[j] > place;  // (all different: an index is in each)
-  visible();
+  wave_sync();
   mine[rank] = place;
-  visible();
+  wave_sync();
   place = mine[lane];
   z = value_at(place);
   const int legal = lanes.count(z > -INFINITY);

@@ -78,17 +78,6 @@ struct Bits {
   }
 };
 
-template <int G>
-__device__ __forceinline__ void group_sync() {
-  if constexpr (G > 64) {
-    __syncthreads();
-  } else {  // the wave's LDS writes to its own reads
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-  }
-}
-
 // This lane's entries of R.  A group of 64 lanes or more loads them once, beside the row; in narrower ones, whose rows
 // have few words to wait for, they would take more registers than the row does.
 template <int G, typename T>

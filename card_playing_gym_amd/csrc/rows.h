@@ -42,6 +42,21 @@ struct Most {
   __device__ __forceinline__ float operator()(float a, float b) const { return fmaxf(a, b); }
 };
 
+// A wave's LDS writes, visible to its own reads.
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+// The same over a group.
+template <int G>
+__device__ __forceinline__ void group_sync() {
+  if constexpr (G > 64)
+    __syncthreads();
+  else
+    wave_sync();
+}
+
 // Within a wave: the lane's neighbour, the pair's, the quad's (mirrored halves of eight), the other eight
 // of the row of 16, the other rows.
 template <int G, typename X, typename Op>
