@@ -10,7 +10,10 @@
 //
 // An action is decided at borders between running sums, so it must not depend on the order or the rounding of
 // additions.  A weight is an integer, 2^scale e^d to the nearest from a polynomial within 2^-44 of e^d, and sums of a
-// row are exact 64-bit integers (scale + log2 width <= 62): the same whatever lanes and waves add up.  Every filter
+// row are exact 64-bit integers (scale + log2 width <= 62): the same whatever lanes and waves add up.  That is chosen
+// over float64 weights, whose sums would go by the order of the atomics: an entry is off by 2^-44 of its weight and by half
+// of 2^-scale of the largest, 2^-51 in rows of up to 4096 entries and 2^-45 in the widest, where a uniform number of
+// 2^-53 steps would meet an entry of less (which is never drawn) once in 2^45 draws.  Every filter
 // keeps a beginning of the order, so S' is the least of their sums, and sampling comes down to
 // finding the entry at a given place in the order's running sum.
 //
@@ -26,7 +29,9 @@
 // are bound by VALU instructions: 8 an entry for its load and the maximum, 25 for its weight and the histogram, up to
 // 9 for each entry that is looked for.  us there: greedy 43, the record of 64 entries 101 to 113, no filter 159,
 // top_p 198 to 206.  Few rows are bound by the latency of passes and barriers (256 x 32768 with every filter 38),
-// rows of up to 64 entries by their scalars.
+// rows of up to 64 entries by their scalars.  These are of normal logits.  Where many entries have few values, atomics to
+// the same bin wait for each other and a bin has more entries than the list: with all entries equal no filter takes 818 us
+// there, top_p 1230 and the record 988 (16 values 757, 1143 and 946); at 4096 x 512 22, 25 and 26 (normal 12, 15 and 17).
 #include "rows.h"
 
 namespace cg {
@@ -954,7 +959,7 @@ __device__ __forceinline__ void top_row(const ChooseArgs &a, int64_t r, Row &row
     // (one more, where the lanes suffice: the largest of the others)
     if (a.k < a.width) under = below(bound_of_top(group, top, mine, min(a.k + 1, G)));
     const Share weigh(under > -INFINITY ? under : 0.f, inverse);
-    float sum = 0;
+    float sum = 0;  // (of a vector's 2 to 8, each off by (3 |d| + 4) 2^-24: 8 roundings more, then float64)
     n = gather(
         row, group,
         [&](float z, int) {
@@ -1141,8 +1146,10 @@ __global__ __launch_bounds__(256) void narrow_kernel(const ChooseArgs a) {
 
 // ---- kernels -------------------------------------------------------------------------------------------------------
 
-// BYTES: of LDS for a row; 0: it is read again for each pass.  The record's blocks of 256 lanes fit a SIMD six times with two
-// registers less than they would take (8192 x 2048 bf16, the 8 and 128 largest: 49 82 us, so 44 75); sampling's would spill.
+// BYTES: of LDS for a row; 0: it is read again for each pass.  The record's blocks of 256 lanes fit a SIMD six times with a
+// few registers less than they would take; fp16's then spill 9, and gain as much.  us with four and six waves, the 8 and the
+// 128 largest: 8192 x 2048 bf16 48 80 and 44 73, fp16 48 81 and 43 74, fp32 47 80 and 43 74; 32768 x 1500 fp16 179 338 and
+// 160 309.  Sampling's would spill 69.
 template <typename T, int G, int BYTES, bool RECORD>
 __global__ __launch_bounds__((G > 256 ? G : 256), RECORD && G == 256 ? 6 : 4) void choose_kernel(const ChooseArgs a) {
   constexpr int ROWS = G > 256 ? 1 : 256 / G;
@@ -1189,6 +1196,8 @@ Launch narrow_as() {
 //   131072 x 64 bf16       92    95    98 and   164   207   164      1024 x 32768 bf16 52  64  35 and  72  86  67
 //    65536 x 256 bf16      87   114    83 and   100   129    89       910 x 36864 fp32 84 101  67 and  95 119  76
 // Rows of 640 bytes to 1 KB have two entries a lane no longer: 65536 x 160 fp32 so 87 111 81, with them 90 116 86.
+// fp16 goes as bf16: 131072 x 64 88 93 95 and 146 193 156, 32768 x 1024 68 90 53 and 191 238 146, 8192 x 8192 96 123 57 and
+// 146 190 137, 1024 x 32768 52 63 32 and 71 86 59; 910 x 73728 119 150 80 and, read again, 133 171 78.
 template <typename T, bool RECORD>
 Launch launch_of(int width) {
   if (width <= 4) return narrow_as<T, 4, RECORD>();

@@ -59,8 +59,8 @@ __device__ __forceinline__ float exp_from(const DistillArgs &a, float z, float f
 }
 
 // For a gradient of 16 bits, whose own rounding is 2^-8 or 2^-11 of it: the scale's rounding, |x| 2^-24 of the exponential
-// (x = (z - from) / T), is below that until the exponential is 0.  One instruction less of five: 4096 x 32768 bf16 143 and
-// 140 us.
+// (x = (z - from) / T, 104 at most before it is 0), is a 79th of fp16's at most.  One instruction less of five:
+// 4096 x 32768 bf16 143 and 140 us.  Values and sums have exp_from in every type.
 __device__ __forceinline__ float exp_near(const DistillArgs &a, float z, float from) {
   return __builtin_amdgcn_exp2f((z - from) * a.scale);
 }
@@ -231,7 +231,7 @@ __device__ __forceinline__ void distill_row(const DistillArgs &a, int64_t r, int
   double sums[6] = {};  // the rest, then TopSums, then whether the record is in order
   if (weight != 0) {
     each([&](int, const auto &z, bool) {
-      float s = 0;
+      float s = 0;  // (of a vector's 4 or 8, each off by (3 |x| + 4) 2^-24: 8 roundings more, then float64)
 #pragma unroll
       for (int k = 0; k < V; ++k) s += exp_from(a, z(k), rest_top);
       sums[0] += s;
@@ -379,6 +379,8 @@ Launch launch_as() {
 //   65536 x 32 bf16  27  40 and  41  48     16384 x 2048 bf16  58  59 and 156 (k 32)     2048 x 16384 fp32 65 and 118
 //   65536 x 128 bf16 44  51 and  73  74      4096 x 8192 bf16      55 and  85            1024 x 32768 bf16 47 and  83
 //   65536 x 512 bf16 81  82 and 125 125      2048 x 16384 bf16     53 and  72             512 x 65536 bf16 54 and  60
+// fp16, k 16: 26 and 38, 40 and 73, 74 and 153, 52 and 141; 4096 x 8192 50 and 82, 2048 x 16384 50 and 68, 1024 x 32768
+// 44 and 79, 512 x 65536 51 and 59.
 // (Records of nearly all of a narrow row would have more: 131072 x 32 fp32, k 32, 193 and 79.)
 template <typename T>
 Launch launch_of(int width) {
