@@ -3,7 +3,7 @@
 
     record = top_logits(teacher_logits, 64, mask=legal, temperature=2.0)
     out = distill_loss(logits, record.indices, record.log_probs, log_rest=record.log_rest, mask=legal, temperature=2.0)
-    (policy_loss.loss + out.loss).backward()
+    (policy.loss + out.loss).backward()
 
 A record of k entries takes 12 k + 4 bytes a row where the logits would take 2 or 4 bytes for every entry.
 """
@@ -125,9 +125,9 @@ def distill_loss(
     will then do for ``log_probs``.
 
     ``weights``: float32 [rows] (ones).  ``normalizer``: the number of rows, padding among them; pass the count of
-    those with weight for their mean.  It may be a float32 device scalar, which a captured loss reads at every replay.
-    A factor of the loss belongs in it too (n / 0.1 for a tenth): the forward writes the gradient for an arriving 1, and
-    for another one, as ``0.1 * out.loss`` sends, the backward forms it again.
+    those with weight (1 at least: nothing over 0 is NaN) for their mean.  It may be a float32 device scalar, which a
+    captured loss reads at every replay.  A factor of the loss belongs in it too (n / 0.1 for a tenth): the forward
+    writes the gradient for an arriving 1, and for another one, as ``0.1 * out.loss`` sends, the backward forms it again.
     A backward captured in a graph of its own follows one replay of its forward's each time.
 
     Index -1 stands for no entry.  An index outside the row, or twice in it, makes its row, and the loss, NaN, as does
