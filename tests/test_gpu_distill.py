@@ -534,3 +534,42 @@ def test_a_rest_that_this_policy_does_not_have(device, width):
 def test_the_widest_rows(device, width, dtype):
     masked = dtype != torch.bfloat16
     check(*make(device, 2, width, dtype, 16, 256, masked=masked, rest=width % 2 == 0, weighted=masked, temperature=0.7))
+
+
+@pytest.mark.parametrize("upstream", [1.0, 0.25])
+def test_saved_inputs_that_come_back_elsewhere(device, upstream):
+    """Hooks that keep what is saved on the host bring it back dense: with other addresses and row strides."""
+
+    logits, indices, log_probs, options = make(device, 9, 300, torch.float16, 17, 12, weighted=True)
+    _, want = run(logits, indices, log_probs, options, upstream)
+    wide = torch.zeros(9, 311, dtype=torch.float16, device=device)
+    wide[:, 3:303] = logits
+    legal = torch.zeros(9, 305, dtype=torch.bool, device=device)
+    legal[:, :300] = options["mask"]
+    leaf = wide[:, 3:303].detach().requires_grad_()
+    with torch.autograd.graph.save_on_cpu():
+        loss = distill_loss(leaf, indices, log_probs, **(options | {"mask": legal[:, :300]})).loss
+    (grad,) = torch.autograd.grad(loss * upstream, leaf)
+    assert torch.equal(grad, want)
+
+
+def test_two_graphs_of_one_pool(device):
+    """Replayed in any order, each leaves its own loss and gradient."""
+
+    sets = [make(device, rows, 500, torch.bfloat16, 18 + rows, 16, weighted=True) for rows in (40, 25)]
+    wants = [run(*s) for s in sets]
+    pool, graphs, outs = torch.cuda.graph_pool_handle(), [], []
+    for logits, indices, log_probs, options in sets:
+        leaf = logits.clone().requires_grad_()
+        graph = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph, pool=pool):
+            out = distill_loss(leaf, indices, log_probs, **options)
+            (grad,) = torch.autograd.grad(out.loss, leaf)
+        graphs.append(graph)
+        outs.append((out, grad))
+    for at in (0, 1, 1, 0, 1, 0):
+        graphs[at].replay()
+        torch.cuda.synchronize()
+        (out, grad), (want, want_grad) = outs[at], wants[at]
+        assert torch.equal(out.loss, want.loss) and torch.equal(out.kl, want.kl) and torch.equal(grad, want_grad)
